@@ -671,6 +671,111 @@ int vkml_attend_step_noalloc(const vkml_attend_step_params* p, const float* d_qk
 
 
 /* ---------------------------------------------------------------------- */
+/* Several sequences over one paged KV cache. The reference decodes one    */
+/* sequence over contiguous caches (llama.cpp:238-285 there); these have   */
+/* no counterpart in it.                                                   */
+/*                                                                        */
+/* The pools k and v hold `pages` pages [kv_heads, page_size, head_dim] of */
+/* kv_type, page_stride elements apart (0: no gap). Key p of sequence s is */
+/* row p % page_size of page d_table[s * table_stride + p / page_size]. A  */
+/* page may be in several sequences' rows of the table: they share its     */
+/* keys. A table entry outside 0 .. pages - 1 (-1, say) is no page: its    */
+/* keys are neither read nor written.                                      */
+/*                                                                        */
+/* A call's new tokens are the rows of q (or qkv), a sequence's one after  */
+/* another: d_starts[s] .. d_starts[s + 1] are sequence s's (seqs + 1      */
+/* entries from 0 .. tokens that do not decrease; NULL: token s is         */
+/* sequence s's only one, and tokens = seqs). d_lengths[s] are its keys,   */
+/* the new tokens' last among them: of n new tokens, token i stands at     */
+/* position d_lengths[s] - n + i. Rows of no sequence are left as they     */
+/* were. These arrays are device memory, read when the launch runs, so a   */
+/* captured graph follows them. Values that break these rules give         */
+/* unspecified results, but nothing outside the arrays named here is       */
+/* touched.                                                                */
+/* ---------------------------------------------------------------------- */
+
+/* softmax(q k^T scale) v of each new token over its sequence's keys up to
+ * its own position (f32 attention within f32 rounding, as vkml_attend_fast;
+ * with f32 caches on the f32 matrix instructions). d_q and d_out
+ * [tokens, heads, head_dim] f32. softcap: 0 for none. A token without keys
+ * gets zeros. head_dim 64 or 128; at most 128 query heads a KV head.
+ *
+ * groups > 0: sequences d_group_starts[g] .. d_group_starts[g + 1] (groups +
+ * 1 entries that do not decrease; sequences outside every group share
+ * nothing) have their first d_group_keys[g] keys in common: these are read
+ * once for all of the group's tokens, through its first sequence's row of
+ * the table, and only the rest through each one's own. d_group_keys[g] is at
+ * most the keys that each of them has before its new tokens; it need not
+ * fill whole pages.
+ *
+ * d_workspace: vkml_attend_pages_workspace_bytes(p) bytes, 16-byte aligned,
+ * of any content; calls that overlap need one each. */
+typedef struct vkml_attend_pages_params {
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t kv_type;
+    uint32_t page_size;    /* keys a page: a power of two, 16 to 1024 */
+    uint32_t pages;
+    uint32_t seqs;         /* at most 65536 */
+    uint32_t tokens;
+    uint32_t table_stride; /* table entries a sequence */
+    uint32_t groups;
+    uint64_t page_stride;
+    float scale;
+    float softcap;
+} vkml_attend_pages_params;
+uint64_t vkml_attend_pages_workspace_bytes(const vkml_attend_pages_params* p);
+int vkml_attend_pages(const vkml_attend_pages_params* p, const float* d_q, const void* d_k_pages, const void* d_v_pages,
+                      const int32_t* d_table, const int32_t* d_lengths, const int32_t* d_starts,
+                      const int32_t* d_group_starts, const int32_t* d_group_keys, void* d_workspace, float* d_out);
+
+/* The new tokens' q | k | v (rows of d_qkv, row_stride floats apart): q and
+ * k rotated at the token's position (or d_positions[token], if non-NULL) by
+ * d_rope_table [positions, rotary_dim / 2, 2] (cos, sin; vkml::rope_table,
+ * scaled for long contexts or not), q into d_q [tokens, heads, head_dim]
+ * f32, k and v rounded to the cache type and written at the token's position
+ * of its sequence's pages. style 0: pairs (2 i, 2 i + 1); 1: (i, i +
+ * rotary_dim / 2); dims from rotary_dim on are left unturned. A token whose
+ * position the table does not hold gets NaN for its turned dims. */
+typedef struct vkml_rope_kv_pages_params {
+    uint32_t heads;
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t kv_type;
+    uint32_t page_size;
+    uint32_t pages;
+    uint32_t seqs;
+    uint32_t tokens;
+    uint32_t table_stride;
+    uint32_t row_stride;
+    uint64_t page_stride;
+    uint32_t rotary_dim; /* 0: nothing is turned, and d_rope_table may be NULL */
+    uint32_t style;
+    uint32_t positions;  /* rows of d_rope_table */
+} vkml_rope_kv_pages_params;
+int vkml_rope_kv_pages(const vkml_rope_kv_pages_params* p, const float* d_qkv, const float* d_rope_table,
+                       const int32_t* d_table, const int32_t* d_lengths, const int32_t* d_starts,
+                       const int32_t* d_positions, float* d_q, void* d_k_pages, void* d_v_pages);
+
+/* Copies page src[i] to page dst[i] of both pools, in every layer: what a
+ * fork (of a part-filled page) and a compaction need. src and dst are host
+ * arrays, read before the call returns; a captured graph keeps them. No page
+ * may be a destination twice, or a source and a destination. page_stride and
+ * layer_stride (0: no gap) are bytes, multiples of 16 as page_bytes is. */
+typedef struct vkml_copy_pages_params {
+    uint32_t pages;
+    uint32_t layers;
+    uint32_t count;
+    uint64_t page_bytes;   /* kv_heads * page_size * head_dim elements */
+    uint64_t page_stride;
+    uint64_t layer_stride; /* from one layer's pool to the next's */
+} vkml_copy_pages_params;
+int vkml_copy_pages(const vkml_copy_pages_params* p, const int32_t* src, const int32_t* dst, void* d_k_pages,
+                    void* d_v_pages);
+
+
+/* ---------------------------------------------------------------------- */
 /* Fused decode-step kernels (no single reference counterpart: each       */
 /* replaces a sequence of the reference's dispatches, cited).             */
 /* ---------------------------------------------------------------------- */

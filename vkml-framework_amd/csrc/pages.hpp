@@ -1,0 +1,129 @@
+// pages.hpp -- the paged KV cache of several sequences: what a call's
+// parameters must be, and which rows, keys and shared prefix the sequences of
+// a batch have. Code without HIP's runtime, so that the checks can be tested
+// on any machine.
+#pragma once
+
+#include <cstdint>
+
+#include "../../include/vkml_hip.h"
+
+#if defined(__HIPCC__)
+#define VKML_HD __host__ __device__ __forceinline__
+#else
+#define VKML_HD inline
+#endif
+
+namespace vkml::pages {
+
+constexpr uint32_t kMaxGroup = 128;       // query heads a KV head
+constexpr uint32_t kMaxSeqs = 1u << 16;   // sequences a batch
+constexpr uint32_t kMaxTokens = 1u << 22;  // new tokens a batch
+
+VKML_HD int32_t clamp_to(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// The batch as the device reads it. Its values are device memory, so the host
+// cannot check them: every read here clamps what it finds, so that no value
+// leads outside q, the table or the pools.
+struct Batch {
+    const int32_t* lengths;
+    const int32_t* starts;        // null: token s is sequence s's
+    const int32_t* group_starts;  // groups + 1
+    const int32_t* group_keys;
+    int32_t seqs, tokens, groups, table_keys;
+
+    VKML_HD int32_t start(int32_t s) const { return starts ? clamp_to(starts[s], 0, tokens) : s < tokens ? s : tokens; }
+    // New tokens of sequence s from start(s) on.
+    VKML_HD int32_t count(int32_t s) const {
+        const int32_t n = start(s + 1) - start(s);
+        return n > 0 ? n : 0;
+    }
+    VKML_HD int32_t length(int32_t s) const { return clamp_to(lengths[s], 0, table_keys); }
+    VKML_HD int32_t group_start(int32_t g) const { return clamp_to(group_starts[g], 0, seqs); }
+    // Keys that the sequences of group g share; a group of one shares none.
+    VKML_HD int32_t group_shared(int32_t g) const {
+        return group_start(g + 1) - group_start(g) > 1 ? clamp_to(group_keys[g], 0, table_keys) : 0;
+    }
+    // The group that sequence s is in, -1 for none.
+    VKML_HD int32_t group_of(int32_t s) const {
+        int32_t lo = 0, hi = groups;  // group_start(lo) <= s < group_start(hi), if s is in any
+        while (hi - lo > 1) {
+            const int32_t mid = (lo + hi) / 2;
+            if (group_start(mid) <= s) lo = mid;
+            else hi = mid;
+        }
+        return groups > 0 && group_start(lo) <= s && s < group_start(lo + 1) ? lo : -1;
+    }
+};
+
+// ---------------------------------------------------------------- checks
+
+inline const char* check_cache(uint32_t kv_heads, uint32_t head_dim, uint32_t kv_type, uint32_t page_size, uint32_t pages, uint64_t page_stride) {
+    if (kv_type != VKML_F16 && kv_type != VKML_F32) return "caches must be f16 or f32";
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1))) return "page_size must be a power of two from 16 to 1024";
+    if (pages == 0 || pages > 0x7FFFFFFFu) return "the pools must hold 1 to 2^31 - 1 pages";
+    if (page_stride && page_stride < static_cast<uint64_t>(kv_heads) * page_size * head_dim) return "pages overlap";
+    if (page_stride % 8) return "page_stride must be a multiple of 8";
+    return nullptr;
+}
+
+inline const char* check_batch(uint32_t seqs, uint32_t tokens, uint32_t table_stride, uint32_t page_size) {
+    if (seqs > kMaxSeqs) return "more than 65536 sequences";
+    if (tokens > kMaxTokens) return "more than 2^22 new tokens";
+    if (table_stride == 0 || static_cast<uint64_t>(table_stride) * page_size > 0x7FFFFFFFu) return "a table row must hold 1 to 2^31 - 1 keys";
+    return nullptr;
+}
+
+inline const char* check(const vkml_attend_pages_params& p) {
+    if (p.kv_heads == 0 || p.heads == 0 || p.heads % p.kv_heads) return "heads must be a multiple of kv_heads";
+    if (p.heads / p.kv_heads > kMaxGroup) return "more than 128 query heads a KV head";
+    if (static_cast<uint64_t>(p.heads) * p.tokens > 0x7FFFFFFFu) return "too many rows";
+    if (p.head_dim != 64 && p.head_dim != 128) return "head_dim must be 64 or 128";
+    if (const char* why = check_cache(p.kv_heads, p.head_dim, p.kv_type, p.page_size, p.pages, p.page_stride)) return why;
+    if (const char* why = check_batch(p.seqs, p.tokens, p.table_stride, p.page_size)) return why;
+    if (p.groups > p.seqs) return "more groups than sequences";
+    if (!(p.softcap >= 0.0f)) return "softcap must not be negative";
+    return nullptr;
+}
+
+inline const char* check(const vkml_rope_kv_pages_params& p) {
+    if (p.kv_heads == 0 || p.heads == 0 || p.head_dim == 0 || p.head_dim % 2 || p.head_dim > 1024 || p.heads > 4096 || p.kv_heads > 4096) return "bad head layout";
+    if (const char* why = check_cache(p.kv_heads, p.head_dim, p.kv_type, p.page_size, p.pages, p.page_stride)) return why;
+    if (const char* why = check_batch(p.seqs, p.tokens, p.table_stride, p.page_size)) return why;
+    if (p.rotary_dim % 2 || p.rotary_dim > p.head_dim) return "rotary_dim must be even and at most head_dim";
+    if (p.style > 1) return "style must be 0 (interleaved pairs) or 1 (rotate-half)";
+    if (p.row_stride < static_cast<uint64_t>(p.heads + 2 * p.kv_heads) * p.head_dim) return "rows overlap";
+    return nullptr;
+}
+
+inline const char* check(const vkml_copy_pages_params& p) {
+    if (p.pages == 0 || p.pages > (1u << 24)) return "the pools must hold 1 to 2^24 pages";
+    if (p.page_bytes == 0 || p.page_bytes % 16 || p.page_stride % 16 || p.layer_stride % 16) return "page_bytes and the strides must be multiples of 16";
+    if (p.page_bytes > (1u << 30)) return "a page must have at most 2^30 bytes";
+    if (p.page_stride && p.page_stride < p.page_bytes) return "pages overlap";
+    const uint64_t stride = p.page_stride ? p.page_stride : p.page_bytes;
+    if (stride > (1ull << 40)) return "page_stride is too large";
+    if (p.layer_stride && p.layer_stride < (p.pages - 1) * stride + p.page_bytes) return "layers overlap";
+    if (p.layers == 0 || p.layers > 65535) return "1 to 65535 layers";
+    return nullptr;
+}
+
+// The copy list of vkml_copy_pages: every page in the pools, no destination
+// twice, and none that is also a source, so that the copies may run in any
+// order. marks: (pages + 63) / 64 words, zeroed.
+inline const char* check_copies(uint32_t pages, uint32_t count, const int32_t* src, const int32_t* dst, uint64_t* marks) {
+    for (uint32_t i = 0; i < count; ++i) {
+        const uint32_t d = static_cast<uint32_t>(dst[i]);
+        if (d >= pages) return "a destination is outside the pools";
+        if (marks[d / 64] >> (d % 64) & 1) return "a page is a destination twice";
+        marks[d / 64] |= 1ull << (d % 64);
+    }
+    for (uint32_t i = 0; i < count; ++i) {
+        const uint32_t s = static_cast<uint32_t>(src[i]);
+        if (s >= pages) return "a source is outside the pools";
+        if (marks[s / 64] >> (s % 64) & 1) return "a page is both a source and a destination";
+    }
+    return nullptr;
+}
+
+}  // namespace vkml::pages

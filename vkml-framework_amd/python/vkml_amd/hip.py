@@ -74,6 +74,16 @@ AttendPromptParams = _struct("AttendPromptParams", [("heads", u32), ("kv_heads",
 GemvRopeParams = _struct("GemvRopeParams", [("n", u32), ("k", u32), ("b_type", u32), ("scale_type", u32), ("eps", f32),
                                             ("row0", u32), ("heads", u32), ("kv_heads", u32), ("head_dim", u32),
                                             ("capacity", u32), ("kv_type", u32), ("rotate", u32)])
+AttendPagesParams = _struct("AttendPagesParams", [("heads", u32), ("kv_heads", u32), ("head_dim", u32), ("kv_type", u32),
+                                                  ("page_size", u32), ("pages", u32), ("seqs", u32), ("tokens", u32),
+                                                  ("table_stride", u32), ("groups", u32), ("page_stride", u64),
+                                                  ("scale", f32), ("softcap", f32)])
+RopeKvPagesParams = _struct("RopeKvPagesParams", [("heads", u32), ("kv_heads", u32), ("head_dim", u32), ("kv_type", u32),
+                                                  ("page_size", u32), ("pages", u32), ("seqs", u32), ("tokens", u32),
+                                                  ("table_stride", u32), ("row_stride", u32), ("page_stride", u64),
+                                                  ("rotary_dim", u32), ("style", u32), ("positions", u32)])
+CopyPagesParams = _struct("CopyPagesParams", [("pages", u32), ("layers", u32), ("count", u32), ("page_bytes", u64),
+                                              ("page_stride", u64), ("layer_stride", u64)])
 
 P = C.POINTER
 # name -> argtypes (all return int status unless noted)
@@ -148,6 +158,10 @@ SIGNATURES = {
     "vkml_attend_step_fast": [P(AttendStepParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, P(GemvDotParams), vp, vp, vp, vp, u32, u32],
     "vkml_attend_step_fast_supported": [P(AttendStepParams), P(GemvDotParams)],
     "vkml_attend_step_noalloc": [P(AttendStepParams), vp, vp, vp, vp, vp, vp, vp, vp],
+    "vkml_attend_pages_workspace_bytes": [P(AttendPagesParams)],
+    "vkml_attend_pages": [P(AttendPagesParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp],
+    "vkml_rope_kv_pages": [P(RopeKvPagesParams), vp, vp, vp, vp, vp, vp, vp, vp, vp],
+    "vkml_copy_pages": [P(CopyPagesParams), vp, vp, vp, vp],
     "vkml_attend_o_sync_bytes": [],
     "vkml_state_set": [vp, i32, i32, i32],
     "vkml_embedding_state": [P(EmbeddingParams), vp, vp, vp, vp],
@@ -176,6 +190,7 @@ def lib() -> C.CDLL:
         _lib.vkml_stream.restype = C.c_void_p
         _lib.vkml_attend_o_sync_bytes.restype = C.c_uint64
         _lib.vkml_attend_fused_sync_bytes.restype = C.c_uint64
+        _lib.vkml_attend_pages_workspace_bytes.restype = C.c_uint64
     return _lib
 
 
