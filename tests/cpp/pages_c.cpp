@@ -22,3 +22,58 @@ extern "C" void batch_c(const Batch* b, int32_t* out) {
         out[5 * s + 4] = g < 0 ? 0 : b->group_shared(g);
     }
 }
+
+// The whole work of a call as its workgroups cut it, a piece a row: workgroup,
+// KV head, segment, tile, first key, last key + 1, slot, few, whole, pieces of
+// the tile (as its first piece says). Returns the number of pieces.
+extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int32_t workgroups, int32_t block, int64_t* out, int64_t most) {
+    const int32_t segments = b->groups + b->seqs;
+    int64_t per_head = 0, few_per_head = 0, tiles_per_head = 0, n = 0;
+    for (int32_t i = 0; i < segments; ++i) {
+        const Segment s = segment(*b, group, i);
+        per_head += s.cost();
+        (s.few ? few_per_head : tiles_per_head) += s.tiles;
+    }
+    const int64_t cost = per_head * kv_heads;
+    if (cost == 0) return 0;
+    const int32_t w_all = parts(cost, workgroups);
+    for (int32_t w = 0; w < w_all; ++w) {
+        const int64_t u0 = part_start(cost, w_all, w), u1 = part_start(cost, w_all, w + 1);
+        int64_t off = 0, few = 0, tiles = 0;
+        for (int32_t h = 0; h < kv_heads; ++h)
+            for (int32_t i = 0; i < segments; ++i) {
+                const Segment s = segment(*b, group, i);
+                if (off + s.cost() > u0 && off < u1 && s.tiles) {
+                    for (int32_t t = u0 > off ? s.tile_at(u0 - off) : 0; t < s.tiles; ++t) {
+                        const int64_t at = off + s.before(t);
+                        if (at >= u1) break;
+                        const int64_t c = kOverhead + s.keys(t);
+                        if (n >= most) return -1;
+                        int64_t* o = out + 10 * n++;
+                        o[0] = w, o[1] = h, o[2] = i, o[3] = t;
+                        o[4] = u0 > at ? cut(u0 - at, s.keys(t), block) : 0;
+                        o[5] = u1 >= at + c ? s.keys(t) : cut(u1 - at, s.keys(t), block);
+                        o[6] = w + (s.few ? few : tiles + t);
+                        o[7] = s.few;
+                        o[8] = u0 <= at && u1 >= at + c;
+                        o[9] = at >= u0 ? part_of(cost, w_all, at + c - 1) - w + 1 : -1;
+                    }
+                }
+                off += s.cost();
+                (s.few ? few : tiles) += s.tiles;
+            }
+    }
+    return n;
+}
+
+// {few, tile} slots, then a segment's token0, n, lo, from, keys of its last tile, tiles, step, row, shared
+extern "C" void slots_c(int64_t kv_heads, int64_t group, int64_t seqs, int64_t groups, int64_t tokens, int64_t workgroups, int64_t* out) {
+    const Slots s = slots(kv_heads, group, seqs, groups, tokens, workgroups);
+    out[0] = s.few, out[1] = s.tile;
+}
+extern "C" void segment_c(const Batch* b, int32_t group, int32_t i, int32_t* out) {
+    const Segment s = segment(*b, group, i);
+    const int32_t v[] = {s.token0, s.n, s.lo, s.from, s.tiles ? s.keys(s.tiles - 1) : 0, s.tiles, s.step, s.row, s.shared};
+    for (int k = 0; k < 9; ++k) out[k] = v[k];
+}
+extern "C" int32_t limit_c(const Batch* b, int32_t group, int32_t i, int32_t token) { return segment(*b, group, i).limit(token); }

@@ -142,3 +142,114 @@ def test_a_batch_that_breaks_the_rules_stays_in_bounds(pages):
         for first, count, length, group, shared in rows(pages, pick(n), pick(n + 1), pick(g + 1), pick(g), 20, 64):
             assert 0 <= first <= 20 and 0 <= count and first + count <= 20
             assert 0 <= length <= 64 and -1 <= group < max(g, 1) and 0 <= shared <= 64
+
+
+# ---------------------------------------------------------------- the work of a call, cut into parts
+
+def pieces(pages, b, kv_heads, group, workgroups=512, block=64):
+    out = np.zeros((200000, 10), np.int64)
+    n = pages.pieces_c(C.byref(b), kv_heads, group, workgroups, block, out.ctypes.data_as(C.c_void_p), C.c_int64(len(out)))
+    assert n >= 0
+    return out[:n]
+
+
+def segments(pages, b, group):
+    out = np.zeros((b.groups + b.seqs, 9), np.int32)
+    for i in range(len(out)):
+        pages.segment_c(C.byref(b), group, i, out[i].ctypes.data_as(C.c_void_p))
+    return out
+
+
+def check_cut(pages, lengths, new, group_starts, group_keys, kv_heads, group, workgroups, block, table_keys=1 << 20):
+    starts = np.concatenate([[0], np.cumsum(new)])
+    b, keep = batch(lengths, starts, group_starts, group_keys, int(starts[-1]), table_keys)
+    got, seg = pieces(pages, b, kv_heads, group, workgroups, block), segments(pages, b, group)
+    few, tile = np.zeros(2, np.int64)
+    s = np.zeros(2, np.int64)
+    pages.slots_c(*[C.c_int64(int(x)) for x in (kv_heads, group, len(lengths), b.groups, starts[-1], workgroups)], s.ctypes.data_as(C.c_void_p))
+    # every key of every token is in exactly one tile of one of its segments
+    seen = {}
+    for i, (token0, n, lo, first, keys, tiles, step, row, shared) in enumerate(seg):
+        assert lo % 16 == 0 and lo <= first < lo + 16 and n <= max(1, tiles) * step
+        assert tiles == 0 or (tiles - 1) * step < n
+        for k in range(n):
+            t, end = token0 + k, pages.limit_c(C.byref(b), group, i, int(k))
+            seen.setdefault(t, []).append((first, max(first, end)))
+            assert end <= lo + keys or end <= first
+    for q, (length, n) in enumerate(zip(lengths, new)):
+        for k in range(n):
+            parts = sorted(x for x in seen[starts[q] + k] if x[1] > x[0])
+            end = 0
+            for a, z in parts:
+                assert a == end
+                end = z
+            assert end == max(0, length - n + k + 1)
+    # the pieces of a tile follow one another and cover it; the first one knows how many there are
+    used, tiles = {0: set(), 1: set()}, {}
+    for w, h, i, t, k0, k1, slot, is_few, whole, count in got.tolist():
+        assert 0 <= slot < s[0 if is_few else 1] and slot not in used[is_few]
+        used[is_few].add(slot)
+        tiles.setdefault((h, i, t), []).append((w, k0, k1, slot, whole, count))
+        assert k0 % block == 0 or k0 == k1
+    assert len(tiles) == kv_heads * sum(x[5] for x in seg)
+    for (h, i, t), p in tiles.items():
+        token0, n, lo, first, keys, count, step, row, shared = seg[i]
+        assert [x[0] for x in p] == list(range(p[0][0], p[0][0] + len(p))) and [x[3] for x in p] == list(range(p[0][3], p[0][3] + len(p)))
+        assert p[0][5] == len(p) and all(x[5] == -1 for x in p[1:])
+        assert (len(p) == 1) == bool(p[0][4]) and p[0][1] == 0
+        for x, y in zip(p, p[1:]):
+            assert x[2] == y[1]
+        if t == count - 1:
+            assert p[-1][2] == keys
+    return got
+
+
+@pytest.mark.parametrize("block", [32, 64, 128])
+@pytest.mark.parametrize("workgroups", [8, 512])
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (2, 4), (8, 4), (2, 3), (1, 16), (1, 128)])
+def test_the_parts_cover_the_work(pages, kv_heads, group, workgroups, block):
+    rng = np.random.default_rng(1)
+    for k in range(12):
+        n = int(rng.integers(1, 12))
+        new = rng.integers(0, [2, 5, 200][k % 3], n)
+        own = new + rng.integers(0, [1, 40, 3000][k // 3 % 3], n)
+        if k % 2:
+            shared = int(rng.integers(1, 2000))
+            check_cut(pages, own + shared, new, [0, n], [shared if n > 1 else 0], kv_heads, group, workgroups, block)
+        else:
+            check_cut(pages, own, new, None, None, kv_heads, group, workgroups, block)
+    cuts = sorted(int(x) for x in rng.integers(0, 10, 4))
+    keys = [int(x) for x in rng.integers(1, 700, 3)]
+    total = np.full(10, 700) + rng.integers(1, 50, 10)
+    check_cut(pages, total, np.ones(10, int), cuts, keys, kv_heads, group, workgroups, block)
+
+
+def test_a_large_prompt_is_cut_evenly(pages):
+    got = check_cut(pages, [4096, 33], [4096, 1], None, None, 8, 4, 512, 64)
+    load = np.zeros(512)
+    for w, _, _, _, k0, k1, *_ in got.tolist():
+        load[w] += k1 - k0 + 64
+    assert load.max() < 1.1 * load.mean()
+
+
+def test_parts_of_long_batches_fit_64_bits(pages):
+    n = 2 ** 22
+    b, keep = batch([n], [0, n], None, None, n, 2 ** 31 - 1)
+    out = np.zeros(9, np.int32)
+    pages.segment_c(C.byref(b), 128, 0, out.ctypes.data_as(C.c_void_p))
+    assert out[4:7].tolist() == [n, n, 1]  # a tile a token
+
+
+def test_the_work_of_a_batch_that_breaks_the_rules_is_finite(pages):
+    rng = np.random.default_rng(2)
+    edge = [-2 ** 31, -1, 0, 1, 5, 64, 65, 1000, 2 ** 31 - 1]
+    for _ in range(100):
+        n = int(rng.integers(1, 9))
+        pick = lambda k: rng.choice(edge, k)  # noqa: E731
+        g = int(rng.integers(0, n + 1))
+        b, keep = batch(pick(n), pick(n + 1), pick(g + 1), pick(g), 20, 640)
+        for token0, rows, lo, first, keys, tiles, step, row, shared in segments(pages, b, 4).tolist():
+            assert 0 <= token0 and token0 + rows <= 20 and 0 <= lo <= first <= 640 and 0 <= keys and lo + keys <= 640 + 20 and 0 <= tiles <= 20
+            assert tiles == 0 or 0 <= row < n
+        for w, h, i, t, k0, k1, slot, few, whole, count in pieces(pages, b, 2, 4).tolist():
+            assert 0 <= k0 <= k1 <= 660 and slot >= 0

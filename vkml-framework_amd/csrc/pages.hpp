@@ -22,6 +22,16 @@ constexpr uint32_t kMaxTokens = 1u << 22;  // new tokens a batch
 
 VKML_HD int32_t clamp_to(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
+// An element of a call's arrays, which no launch that reads them writes: for
+// an index that a workgroup's threads share, through the scalar unit.
+VKML_HD int32_t element(const int32_t* p, int32_t i) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(p + i));
+#else
+    return p[i];
+#endif
+}
+
 // The batch as the device reads it. Its values are device memory, so the host
 // cannot check them: every read here clamps what it finds, so that no value
 // leads outside q, the table or the pools.
@@ -32,17 +42,17 @@ struct Batch {
     const int32_t* group_keys;
     int32_t seqs, tokens, groups, table_keys;
 
-    VKML_HD int32_t start(int32_t s) const { return starts ? clamp_to(starts[s], 0, tokens) : s < tokens ? s : tokens; }
+    VKML_HD int32_t start(int32_t s) const { return starts ? clamp_to(element(starts, s), 0, tokens) : s < tokens ? s : tokens; }
     // New tokens of sequence s from start(s) on.
     VKML_HD int32_t count(int32_t s) const {
         const int32_t n = start(s + 1) - start(s);
         return n > 0 ? n : 0;
     }
-    VKML_HD int32_t length(int32_t s) const { return clamp_to(lengths[s], 0, table_keys); }
-    VKML_HD int32_t group_start(int32_t g) const { return clamp_to(group_starts[g], 0, seqs); }
+    VKML_HD int32_t length(int32_t s) const { return clamp_to(element(lengths, s), 0, table_keys); }
+    VKML_HD int32_t group_start(int32_t g) const { return clamp_to(element(group_starts, g), 0, seqs); }
     // Keys that the sequences of group g share; a group of one shares none.
     VKML_HD int32_t group_shared(int32_t g) const {
-        return group_start(g + 1) - group_start(g) > 1 ? clamp_to(group_keys[g], 0, table_keys) : 0;
+        return group_start(g + 1) - group_start(g) > 1 ? clamp_to(element(group_keys, g), 0, table_keys) : 0;
     }
     // The group that sequence s is in, -1 for none.
     VKML_HD int32_t group_of(int32_t s) const {
@@ -55,6 +65,128 @@ struct Batch {
         return groups > 0 && group_start(lo) <= s && s < group_start(lo + 1) ? lo : -1;
     }
 };
+
+// ---------------------------------------------------------------- the work of vkml_attend_pages
+
+// A KV head's work is a list of segments: for each group its shared keys by
+// all of its tokens, then for each sequence its own keys by its tokens. A
+// segment's tokens go in tiles: all of them where they are at most kFewRows
+// rows (token, query head), else kTileRows / (query heads a KV head) at a time.
+// A tile costs the keys it reads and kOverhead more (its queries, its joining
+// and storing), and the whole of all KV heads' tiles, laid end to end, is cut
+// into equal parts, one a workgroup: what a workgroup takes of a tile is a
+// piece.
+constexpr int32_t kFewRows = 16;
+constexpr int32_t kTileRows = 128;
+constexpr int32_t kOverhead = 64;
+constexpr int32_t kMinPart = 128;  // keys below which work is not cut further
+
+VKML_HD int32_t tile_tokens(int32_t group) { return kTileRows / group > 1 ? kTileRows / group : 1; }
+
+struct Segment {
+    int32_t row = 0;     // the sequence whose table holds the keys
+    int32_t token0 = 0;  // the first token
+    int32_t n = 0;       // tokens
+    int32_t lo = 0;      // the first key read, a multiple of 16
+    int32_t from = 0;    // the first key that counts
+    int32_t base = 0;    // own keys: those from lo on before the first token's; shared ones: all
+    int32_t tiles = 0, step = 1;
+    bool few = false, shared = false;
+
+    // Keys from lo on that tile i's tokens see.
+    VKML_HD int32_t keys(int32_t i) const {
+        if (shared) return base;
+        if (base < 0) return base + n > 0 ? base + n : 0;
+        const int32_t tokens = (i + 1) * step < n ? (i + 1) * step : n;
+        return base + tokens;
+    }
+    // The cost of the tiles before tile i.
+    VKML_HD int64_t before(int32_t i) const {
+        const int64_t k = i;
+        if (shared || base < 0) return k * (kOverhead + keys(0));
+        return k * (kOverhead + base) + step * k * (k + 1) / 2;
+    }
+    VKML_HD int64_t cost() const { return tiles ? before(tiles - 1) + kOverhead + keys(tiles - 1) : 0; }
+    // The tile that holds unit u of the segment, 0 <= u < cost().
+    VKML_HD int32_t tile_at(int64_t u) const {
+        int32_t lo_tile = 0, hi = tiles;
+        while (hi - lo_tile > 1) {
+            const int32_t mid = lo_tile + (hi - lo_tile) / 2;
+            if (before(mid) <= u) lo_tile = mid;
+            else hi = mid;
+        }
+        return lo_tile;
+    }
+    // The last key position (+ 1) that token i of the segment sees.
+    VKML_HD int32_t limit(int32_t i) const { return shared ? base : lo + base + i + 1; }
+    VKML_HD int32_t tile_n(int32_t i) const { return n - i * step < step ? n - i * step : step; }
+};
+
+// Segment i of a batch: groups 0 .. groups - 1, then the sequences.
+VKML_HD Segment segment(const Batch& b, int32_t group, int32_t i) {
+    Segment s;
+    if (i < b.groups) {
+        const int32_t first = b.group_start(i), last = b.group_start(i + 1);
+        s.row = first;
+        s.base = b.group_shared(i);
+        s.shared = true;
+        if (s.base == 0) return s;
+        s.token0 = b.start(first);
+        s.n = b.start(last) - s.token0;
+    } else {
+        s.row = i - b.groups;
+        const int32_t g = b.group_of(s.row);
+        s.from = g < 0 ? 0 : b.group_shared(g);
+        s.lo = s.from & ~15;
+        s.token0 = b.start(s.row);
+        s.n = b.count(s.row);
+        s.base = b.length(s.row) - s.n - s.lo;
+    }
+    if (s.n <= 0) {
+        s.n = 0;
+        return s;
+    }
+    s.few = s.n <= kFewRows && s.n * group <= kFewRows;
+    s.step = s.few ? s.n : tile_tokens(group);
+    s.tiles = (s.n + s.step - 1) / s.step;
+    return s;
+}
+
+// Workgroups that share a cost: all of them, in eights for the eight XCDs,
+// unless a part would be less than kMinPart.
+VKML_HD int32_t parts(int64_t cost, int32_t workgroups) {
+    int64_t n = cost / kMinPart / 8 * 8;
+    if (n < 8) n = 8;
+    return n < workgroups ? static_cast<int32_t>(n) : workgroups;
+}
+// The first unit of part w, and the part that unit u is in.
+VKML_HD int64_t part_start(int64_t cost, int32_t n, int32_t w) { return static_cast<int64_t>(static_cast<uint64_t>(cost) * static_cast<uint32_t>(w) / static_cast<uint32_t>(n)); }
+VKML_HD int32_t part_of(int64_t cost, int32_t n, int64_t u) {
+    return static_cast<int32_t>((static_cast<uint64_t>(u + 1) * static_cast<uint32_t>(n) - 1) / static_cast<uint64_t>(cost));
+}
+// Keys of a tile of `keys` that units before x of it stand for: whole blocks
+// (but the last), so that every part cuts at the same places.
+VKML_HD int32_t cut(int64_t x, int32_t keys, int32_t block) {
+    const int64_t k = x - kOverhead;
+    if (k <= 0) return 0;
+    const int64_t up = (k + block - 1) / block * block;
+    return up < keys ? static_cast<int32_t>(up) : keys;
+}
+
+// What a call keeps of unfinished rows: slots of kFewRows or kTileRows rows,
+// for each piece of a tile that is not the whole of its rows' work. Piece (w,
+// i), workgroup w's of the i-th tile of its kind, takes slot w + i: the next
+// piece has a larger w, a larger i or both.
+struct Slots {
+    int64_t few, tile;  // of each kind
+    VKML_HD int64_t rows() const { return few * kFewRows + tile * kTileRows; }
+};
+VKML_HD Slots slots(int64_t kv_heads, int64_t group, int64_t seqs, int64_t groups, int64_t tokens, int64_t workgroups) {
+    const int64_t many = tokens * group / (kFewRows + 1);  // segments of each kind with more than kFewRows rows, at most
+    const int64_t step = tile_tokens(static_cast<int32_t>(group));
+    const int64_t tiles = 2 * (tokens / step) + (seqs < many ? seqs : many) + (groups < many ? groups : many);
+    return {workgroups + kv_heads * (seqs + groups), workgroups + kv_heads * tiles};
+}
 
 // ---------------------------------------------------------------- checks
 
