@@ -26,37 +26,32 @@ extern "C" void batch_c(const Batch* b, int32_t* out) {
 // The whole work of a call as its workgroups cut it, a piece a row: workgroup,
 // KV head, segment, tile, first key, last key + 1, slot, few, whole, pieces of
 // the tile (as its first piece says). Returns the number of pieces.
-extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int32_t workgroups, int32_t block, int64_t* out, int64_t most) {
+extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int32_t workgroups_log2, int32_t block, int64_t* out, int64_t most) {
     const int32_t segments = b->groups + b->seqs;
-    int64_t per_head = 0, few_per_head = 0, tiles_per_head = 0, n = 0;
-    for (int32_t i = 0; i < segments; ++i) {
-        const Segment s = segment(*b, group, i);
-        per_head += s.cost();
-        (s.few ? few_per_head : tiles_per_head) += s.tiles;
-    }
+    int64_t per_head = 0, n = 0;
+    for (int32_t i = 0; i < segments; ++i) per_head += segment(*b, group, i).cost();
     const int64_t cost = per_head * kv_heads;
     if (cost == 0) return 0;
-    const int32_t w_all = parts(cost, workgroups);
-    for (int32_t w = 0; w < w_all; ++w) {
-        const int64_t u0 = part_start(cost, w_all, w), u1 = part_start(cost, w_all, w + 1);
+    const int32_t w_log2 = parts_log2(cost, workgroups_log2);
+    for (int32_t w = 0; w < 1 << w_log2; ++w) {
+        const int64_t u0 = part_start(cost, w_log2, w), u1 = part_start(cost, w_log2, w + 1);
         int64_t off = 0, few = 0, tiles = 0;
         for (int32_t h = 0; h < kv_heads; ++h)
             for (int32_t i = 0; i < segments; ++i) {
                 const Segment s = segment(*b, group, i);
                 if (off + s.cost() > u0 && off < u1 && s.tiles) {
                     for (int32_t t = u0 > off ? s.tile_at(u0 - off) : 0; t < s.tiles; ++t) {
-                        const int64_t at = off + s.before(t);
+                        const int64_t at = off + s.before(t), end = at + s.tile_cost(t);
                         if (at >= u1) break;
-                        const int64_t c = kOverhead + s.keys(t);
                         if (n >= most) return -1;
                         int64_t* o = out + 10 * n++;
                         o[0] = w, o[1] = h, o[2] = i, o[3] = t;
-                        o[4] = u0 > at ? cut(u0 - at, s.keys(t), block) : 0;
-                        o[5] = u1 >= at + c ? s.keys(t) : cut(u1 - at, s.keys(t), block);
+                        o[4] = u0 > at ? cut(u0 - at, s.key_cost(), s.keys(t), block) : 0;
+                        o[5] = u1 >= end ? s.keys(t) : cut(u1 - at, s.key_cost(), s.keys(t), block);
                         o[6] = w + (s.few ? few : tiles + t);
                         o[7] = s.few;
-                        o[8] = u0 <= at && u1 >= at + c;
-                        o[9] = at >= u0 ? part_of(cost, w_all, at + c - 1) - w + 1 : -1;
+                        o[8] = u0 <= at && u1 >= end;
+                        o[9] = at >= u0 ? part_of(cost, w_log2, end - 1) - w + 1 : -1;
                     }
                 }
                 off += s.cost();
@@ -66,14 +61,20 @@ extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int
     return n;
 }
 
-// {few, tile} slots, then a segment's token0, n, lo, from, keys of its last tile, tiles, step, row, shared
+// The KV head that part w of the work of kv_heads equal ones begins in, found by division, and by shift.
+extern "C" int32_t first_head_c(int64_t per_head, int32_t kv_heads, int32_t w_log2, int32_t w) {
+    return static_cast<int32_t>(part_start(per_head * kv_heads, w_log2, w) / per_head) - (kv_heads * w >> w_log2);
+}
+
+// {few, tile} slots
 extern "C" void slots_c(int64_t kv_heads, int64_t group, int64_t seqs, int64_t groups, int64_t tokens, int64_t workgroups, int64_t* out) {
     const Slots s = slots(kv_heads, group, seqs, groups, tokens, workgroups);
     out[0] = s.few, out[1] = s.tile;
 }
+// A segment's token0, n, lo, from, keys of its last tile, tiles, step, row, shared, lead, lead_row, lead_span
 extern "C" void segment_c(const Batch* b, int32_t group, int32_t i, int32_t* out) {
     const Segment s = segment(*b, group, i);
-    const int32_t v[] = {s.token0, s.n, s.lo, s.from, s.tiles ? s.keys(s.tiles - 1) : 0, s.tiles, s.step, s.row, s.shared};
-    for (int k = 0; k < 9; ++k) out[k] = v[k];
+    const int32_t v[] = {s.token0, s.n, s.lo, s.from, s.tiles ? s.keys(s.tiles - 1) : 0, s.tiles, s.step, s.row, s.shared, s.lead, s.lead_row, s.lead_span()};
+    for (int k = 0; k < 12; ++k) out[k] = v[k];
 }
 extern "C" int32_t limit_c(const Batch* b, int32_t group, int32_t i, int32_t token) { return segment(*b, group, i).limit(token); }

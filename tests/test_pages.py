@@ -31,7 +31,7 @@ BAD_ATTEND = [
     (dict(kv_type=H.Q8_0), "f16 or f32"), (dict(page_size=0), "power of two"), (dict(page_size=8), "power of two"), (dict(page_size=48), "power of two"),
     (dict(page_size=2048), "power of two"), (dict(pages=0), "pages"), (dict(pages=2 ** 31), "pages"), (dict(page_stride=16 * 2 * 128 - 8), "overlap"),
     (dict(page_stride=16 * 2 * 128 + 4), "multiple of 8"), (dict(seqs=65537), "65536"), (dict(tokens=2 ** 22 + 1), "2^22"), (dict(table_stride=0), "table row"),
-    (dict(table_stride=2 ** 27), "table row"), (dict(groups=5), "groups"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
+    (dict(table_stride=2 ** 26 + 1), "table row"), (dict(groups=5), "groups"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
     (dict(heads=2 ** 10, kv_heads=8, tokens=2 ** 22), "too many rows"),
 ]
 
@@ -45,7 +45,7 @@ def test_attend_refuses(pages, change, why):
 
 def test_attend_takes_the_whole_range(pages):
     for change in (dict(heads=2, kv_heads=2), dict(heads=256), dict(head_dim=64), dict(kv_type=H.F32), dict(page_size=1024), dict(page_stride=16 * 2 * 128 + 8),
-                   dict(seqs=65536), dict(table_stride=2 ** 27 - 1), dict(groups=0), dict(groups=4), dict(seqs=0, tokens=0, groups=0), dict(softcap=50.0),
+                   dict(seqs=65536), dict(table_stride=2 ** 26), dict(groups=0), dict(groups=4), dict(seqs=0, tokens=0, groups=0), dict(softcap=50.0),
                    dict(pages=2 ** 31 - 1)):
         assert pages.check_attend_c(C.byref(H.AttendPagesParams(**{**ATTEND, **change}))) is None, change
 
@@ -146,41 +146,40 @@ def test_a_batch_that_breaks_the_rules_stays_in_bounds(pages):
 
 # ---------------------------------------------------------------- the work of a call, cut into parts
 
-def pieces(pages, b, kv_heads, group, workgroups=512, block=64):
+def pieces(pages, b, kv_heads, group, workgroups_log2=9, block=64):
     out = np.zeros((200000, 10), np.int64)
-    n = pages.pieces_c(C.byref(b), kv_heads, group, workgroups, block, out.ctypes.data_as(C.c_void_p), C.c_int64(len(out)))
+    n = pages.pieces_c(C.byref(b), kv_heads, group, workgroups_log2, block, out.ctypes.data_as(C.c_void_p), C.c_int64(len(out)))
     assert n >= 0
     return out[:n]
 
 
 def segments(pages, b, group):
-    out = np.zeros((b.groups + b.seqs, 9), np.int32)
+    out = np.zeros((b.groups + b.seqs, 12), np.int32)
     for i in range(len(out)):
         pages.segment_c(C.byref(b), group, i, out[i].ctypes.data_as(C.c_void_p))
     return out
 
 
-def check_cut(pages, lengths, new, group_starts, group_keys, kv_heads, group, workgroups, block, table_keys=1 << 20):
+def check_cut(pages, lengths, new, group_starts, group_keys, kv_heads, group, workgroups_log2, block, table_keys=1 << 20):
     starts = np.concatenate([[0], np.cumsum(new)])
     b, keep = batch(lengths, starts, group_starts, group_keys, int(starts[-1]), table_keys)
-    got, seg = pieces(pages, b, kv_heads, group, workgroups, block), segments(pages, b, group)
-    few, tile = np.zeros(2, np.int64)
+    got, seg = pieces(pages, b, kv_heads, group, workgroups_log2, block), segments(pages, b, group)
     s = np.zeros(2, np.int64)
-    pages.slots_c(*[C.c_int64(int(x)) for x in (kv_heads, group, len(lengths), b.groups, starts[-1], workgroups)], s.ctypes.data_as(C.c_void_p))
-    # every key of every token is in exactly one tile of one of its segments
+    pages.slots_c(*[C.c_int64(int(x)) for x in (kv_heads, group, len(lengths), b.groups, starts[-1], 1 << workgroups_log2)], s.ctypes.data_as(C.c_void_p))
+    # every key of every token is in exactly one of its segments, or in the lead of one
     seen = {}
-    for i, (token0, n, lo, first, keys, tiles, step, row, shared) in enumerate(seg):
-        assert lo % 16 == 0 and lo <= first < lo + 16 and n <= max(1, tiles) * step
+    for i, (token0, n, lo, first, keys, tiles, step, row, shared, lead, lead_row, span) in enumerate(seg):
+        assert lo % 16 == 0 and lo <= first < lo + 16 and n <= max(1, tiles) * step and span % 128 == 0 and lead <= span < lead + 128
         assert tiles == 0 or (tiles - 1) * step < n
+        assert lead in (0, first)
         for k in range(n):
             t, end = token0 + k, pages.limit_c(C.byref(b), group, i, int(k))
-            seen.setdefault(t, []).append((first, max(first, end)))
-            assert end <= lo + keys or end <= first
+            seen.setdefault(t, []).extend([(0, lead), (first, max(first, end))])
+            assert end - lo <= keys - span or end <= first
     for q, (length, n) in enumerate(zip(lengths, new)):
         for k in range(n):
-            parts = sorted(x for x in seen[starts[q] + k] if x[1] > x[0])
             end = 0
-            for a, z in parts:
+            for a, z in sorted(x for x in seen[starts[q] + k] if x[1] > x[0]):
                 assert a == end
                 end = z
             assert end == max(0, length - n + k + 1)
@@ -193,7 +192,7 @@ def check_cut(pages, lengths, new, group_starts, group_keys, kv_heads, group, wo
         assert k0 % block == 0 or k0 == k1
     assert len(tiles) == kv_heads * sum(x[5] for x in seg)
     for (h, i, t), p in tiles.items():
-        token0, n, lo, first, keys, count, step, row, shared = seg[i]
+        keys, count = seg[i][4:6]
         assert [x[0] for x in p] == list(range(p[0][0], p[0][0] + len(p))) and [x[3] for x in p] == list(range(p[0][3], p[0][3] + len(p)))
         assert p[0][5] == len(p) and all(x[5] == -1 for x in p[1:])
         assert (len(p) == 1) == bool(p[0][4]) and p[0][1] == 0
@@ -205,9 +204,9 @@ def check_cut(pages, lengths, new, group_starts, group_keys, kv_heads, group, wo
 
 
 @pytest.mark.parametrize("block", [32, 64, 128])
-@pytest.mark.parametrize("workgroups", [8, 512])
+@pytest.mark.parametrize("workgroups_log2", [3, 9])
 @pytest.mark.parametrize("kv_heads,group", [(1, 1), (2, 4), (8, 4), (2, 3), (1, 16), (1, 128)])
-def test_the_parts_cover_the_work(pages, kv_heads, group, workgroups, block):
+def test_the_parts_cover_the_work(pages, kv_heads, group, workgroups_log2, block):
     rng = np.random.default_rng(1)
     for k in range(12):
         n = int(rng.integers(1, 12))
@@ -215,27 +214,48 @@ def test_the_parts_cover_the_work(pages, kv_heads, group, workgroups, block):
         own = new + rng.integers(0, [1, 40, 3000][k // 3 % 3], n)
         if k % 2:
             shared = int(rng.integers(1, 2000))
-            check_cut(pages, own + shared, new, [0, n], [shared if n > 1 else 0], kv_heads, group, workgroups, block)
+            check_cut(pages, own + shared, new, [0, n], [shared if n > 1 else 0], kv_heads, group, workgroups_log2, block)
         else:
-            check_cut(pages, own, new, None, None, kv_heads, group, workgroups, block)
+            check_cut(pages, own, new, None, None, kv_heads, group, workgroups_log2, block)
     cuts = sorted(int(x) for x in rng.integers(0, 10, 4))
     keys = [int(x) for x in rng.integers(1, 700, 3)]
     total = np.full(10, 700) + rng.integers(1, 50, 10)
-    check_cut(pages, total, np.ones(10, int), cuts, keys, kv_heads, group, workgroups, block)
+    check_cut(pages, total, np.ones(10, int), cuts, keys, kv_heads, group, workgroups_log2, block)
+
+
+def test_shared_keys_are_a_segment_where_tokens_are_few(pages):
+    def lead(new, group):
+        n = len(new)
+        b, keep = batch([500 + x for x in new], np.concatenate([[0], np.cumsum(new)]), [0, n], [500], sum(new), 4096)
+        s = segments(pages, b, group)
+        assert (s[0][5] > 0) == all(x[9] == 0 for x in s[1:])
+        return [int(x[9]) for x in s[1:]]
+    assert lead([1] * 8, 4) == [0] * 8
+    assert lead([1, 31], 4) == [0, 0]  # 32 tokens of 128 rows a tile
+    assert lead([1, 32], 4) == [500, 500]
+    assert lead([1] * 5, 64) == [0] * 5
+    assert lead([1] * 5, 65) == [500] * 5  # a tile a token either way
 
 
 def test_a_large_prompt_is_cut_evenly(pages):
-    got = check_cut(pages, [4096, 33], [4096, 1], None, None, 8, 4, 512, 64)
+    got = check_cut(pages, [4096, 33], [4096, 1], None, None, 8, 4, 9, 64)
     load = np.zeros(512)
     for w, _, _, _, k0, k1, *_ in got.tolist():
-        load[w] += k1 - k0 + 64
+        load[w] += k1 - k0 + 43
     assert load.max() < 1.1 * load.mean()
+
+
+def test_the_first_head_of_a_part(pages):
+    for per_head in (1, 7, 129, 1000003, 2 ** 40 + 5):
+        for kv_heads in (1, 2, 3, 8, 96):
+            for w_log2 in (3, 9):
+                assert not any(pages.first_head_c(C.c_int64(per_head), kv_heads, w_log2, w) for w in range(1 << w_log2))
 
 
 def test_parts_of_long_batches_fit_64_bits(pages):
     n = 2 ** 22
     b, keep = batch([n], [0, n], None, None, n, 2 ** 31 - 1)
-    out = np.zeros(9, np.int32)
+    out = np.zeros(12, np.int32)
     pages.segment_c(C.byref(b), 128, 0, out.ctypes.data_as(C.c_void_p))
     assert out[4:7].tolist() == [n, n, 1]  # a tile a token
 
@@ -248,8 +268,8 @@ def test_the_work_of_a_batch_that_breaks_the_rules_is_finite(pages):
         pick = lambda k: rng.choice(edge, k)  # noqa: E731
         g = int(rng.integers(0, n + 1))
         b, keep = batch(pick(n), pick(n + 1), pick(g + 1), pick(g), 20, 640)
-        for token0, rows, lo, first, keys, tiles, step, row, shared in segments(pages, b, 4).tolist():
-            assert 0 <= token0 and token0 + rows <= 20 and 0 <= lo <= first <= 640 and 0 <= keys and lo + keys <= 640 + 20 and 0 <= tiles <= 20
-            assert tiles == 0 or 0 <= row < n
+        for token0, rows, lo, first, keys, tiles, step, row, shared, lead, lead_row, span in segments(pages, b, 4).tolist():
+            assert 0 <= token0 and token0 + rows <= 20 and 0 <= lo <= first <= 640 and lo + keys - span <= 660 and 0 <= tiles <= 20
+            assert 0 <= lead <= 640 and 0 <= lead_row < n and (tiles == 0 or 0 <= row < n)
         for w, h, i, t, k0, k1, slot, few, whole, count in pieces(pages, b, 2, 4).tolist():
-            assert 0 <= k0 <= k1 <= 660 and slot >= 0
+            assert 0 <= k0 <= k1 <= 660 + 768 and slot >= 0

@@ -73,7 +73,8 @@ struct PagesArgs {
     Batch batch;
     uint64_t page_bytes;  // from a page to the next
     int64_t few_slots, tile_slots;
-    uint32_t heads, kv_heads, group, page_shift, pages, table_stride, workgroups;
+    uint32_t heads, kv_heads, group, page_shift, pages, table_stride;
+    int32_t workgroups_log2;
     float scale, softcap;
 };
 
@@ -104,25 +105,37 @@ struct Buffer {
     alignas(16) uint8_t v[16384];
 };
 
-// The pages that a wave's N loads of a block from key0 on read, 16 keys or
-// less each, and a bit for each of the block's tiles that is in no page.
+// Where the keys of a tile are (pages.hpp's axis: the lead, then its own).
+struct Tile {
+    const int32_t* lead_table;  // the table row that the lead is read through
+    const int32_t* table;       // and the other keys
+    int32_t span, lead;         // the axis' part that the lead takes, its keys
+    int32_t lo, from, end;      // of the others: the first read, the first and past the last that count
+    uint32_t kvh;
+};
+
+// A block's keys: positions key0 on through a table row, those that count.
+struct Keys {
+    const int32_t* table;
+    int32_t key0, from, end;
+    bool lead;
+};
+__device__ __forceinline__ Keys keys_at(const Tile& t, int32_t x) {
+    const bool lead = x < t.span;
+    return {lead ? t.lead_table : t.table, lead ? x : t.lo + x - t.span, lead ? 0 : t.from, lead ? t.lead : t.end, lead};
+}
+__device__ __forceinline__ int32_t page_id(const PagesArgs& a, const Keys& k, int32_t key) {
+    return key < k.end ? ld_scalar_i32(k.table + (key >> a.page_shift)) : -1;
+}
+
+// A block, its pages as a wave's N loads of it read them, 16 keys or less
+// each, and a bit for each of its 16-key tiles that is in no page.
 template <int N>
 struct Pages {
+    Keys keys;
     int32_t id[N];
-    int32_t key0;
     uint32_t dead;
 };
-
-// What a tile's pieces have in common.
-struct Tile {
-    const int32_t* table;  // its sequence's row
-    uint32_t kvh;
-    int32_t from, end;     // the keys that count
-};
-
-__device__ __forceinline__ int32_t page_id(const PagesArgs& a, const Tile& t, int32_t key) {
-    return key < t.end ? ld_scalar_i32(t.table + (key >> a.page_shift)) : -1;
-}
 
 // 16 keys of a block: where their first row is, and whether all of them count.
 struct Rows {
@@ -132,11 +145,11 @@ struct Rows {
     int32_t first, last;  // the rows that count
 };
 template <uint32_t ROW>
-__device__ __forceinline__ Rows rows_at(const PagesArgs& a, const Tile& t, int32_t id, int32_t key) {
+__device__ __forceinline__ Rows rows_at(const PagesArgs& a, uint32_t kvh, const Keys& k, int32_t id, int32_t key) {
     const bool held = static_cast<uint32_t>(id) < a.pages;
     const uint64_t at = static_cast<uint64_t>(held ? id : 0) * a.page_bytes +
-                        ((static_cast<uint64_t>(t.kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * ROW;
-    Rows r{a.k + at, a.v + at, false, held ? max(t.from - key, 0) : 16, min(t.end - key, 16)};
+                        ((static_cast<uint64_t>(kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * ROW;
+    Rows r{a.k + at, a.v + at, false, held ? max(k.from - key, 0) : 16, min(k.end - key, 16)};
     r.whole = r.first == 0 && r.last == 16;
     return r;
 }
@@ -150,41 +163,53 @@ __device__ __forceinline__ const uint8_t* piece_at(const uint8_t* base, const Ro
 
 // RT tiles of 16 rows of q as the matrix instructions take them: lane (j, g)
 // has row j's pieces 4 s + g. c[rt]: what turns a product with them into a
-// score in log2 units (with a soft cap: into a score).
+// score in log2 units (with a soft cap: into a score), not negative; the
+// scale's sign is in q.
 template <typename T, int HD, int RT>
 struct Queries;
+
+// A row as loaded, in the order of the keys' 16-byte pieces.
+template <typename T, int HD>
+struct RawRow {
+    static constexpr int N = HD / 16;
+    float4 x[N];
+    __device__ __forceinline__ void load(const float* row, uint32_t g) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t at = sizeof(T) == 2 ? 32 * (i / 2) + 8 * g + 4 * (i % 2) : 16 * i + 4 * g;
+            x[i] = ldg(reinterpret_cast<const float4*>(row + at));
+        }
+    }
+};
 
 template <int HD, int RT>
 struct Queries<_Float16, HD, RT> {
     half8 hi[RT][HD / 32], lo[RT][HD / 32];
     float c[RT];
-    __device__ __forceinline__ void load(int rt, const float* row, uint32_t g, float scale) {
-        float x[HD / 32][8], most = 0.0f;
+    __device__ __forceinline__ void take(int rt, const RawRow<_Float16, HD>& raw, float scale) {
+        float most = 0.0f;
 #pragma unroll
-        for (int s = 0; s < HD / 32; ++s) {
-            const float4 a = ldg(reinterpret_cast<const float4*>(row + 32 * s + 8 * g)), b = ldg(reinterpret_cast<const float4*>(row + 32 * s + 8 * g + 4));
-            const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[s][e] = y[e];
-                most = fmaxf(most, fabsf(y[e]));
-            }
-        }
+        for (int i = 0; i < raw.N; ++i)
+            most = fmaxf(most, fmaxf(fmaxf(fabsf(raw.x[i].x), fabsf(raw.x[i].y)), fmaxf(fabsf(raw.x[i].z), fabsf(raw.x[i].w))));
         const uint2 r16 = swap_rows<16>(__float_as_uint(most));
         most = fmaxf(__uint_as_float(r16.x), __uint_as_float(r16.y));
         const uint2 r32 = swap_rows<32>(__float_as_uint(most));
         most = fmaxf(__uint_as_float(r32.x), __uint_as_float(r32.y));
         // The row's largest value to [1/2, 1): neither term leaves f16's range.
         const int e2 = __builtin_amdgcn_frexp_expf(most);
+        const float sign = scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
-        for (int s = 0; s < HD / 32; ++s)
+        for (int s = 0; s < HD / 32; ++s) {
+            const float4 a = raw.x[2 * s], b = raw.x[2 * s + 1];
+            const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float y = __builtin_amdgcn_ldexpf(x[s][e], -e2);
-                hi[rt][s][e] = static_cast<_Float16>(y);
-                lo[rt][s][e] = static_cast<_Float16>(y - static_cast<float>(hi[rt][s][e]));
+                const float z = __builtin_amdgcn_ldexpf(y[e] * sign, -e2);
+                hi[rt][s][e] = static_cast<_Float16>(z);
+                lo[rt][s][e] = static_cast<_Float16>(z - static_cast<float>(hi[rt][s][e]));
             }
-        c[rt] = __builtin_amdgcn_ldexpf(scale, e2);
+        }
+        c[rt] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale), e2), __FLT_MIN__);
     }
     // The products of step s with the keys' tiles, in turn, so that an
     // instruction does not wait for the one before it.
@@ -204,10 +229,11 @@ template <int HD, int RT>
 struct Queries<float, HD, RT> {
     float4 x[RT][HD / 16];
     float c[RT];
-    __device__ __forceinline__ void load(int rt, const float* row, uint32_t g, float scale) {
+    __device__ __forceinline__ void take(int rt, const RawRow<float, HD>& raw, float scale) {
+        const float sign = scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s) x[rt][s] = ldg(reinterpret_cast<const float4*>(row + 16 * s + 4 * g));
-        c[rt] = scale;
+        for (int i = 0; i < raw.N; ++i) x[rt][i] = make_float4(raw.x[i].x * sign, raw.x[i].y * sign, raw.x[i].z * sign, raw.x[i].w * sign);
+        c[rt] = fmaxf(fabsf(scale), __FLT_MIN__);
     }
     template <int TT>
     __device__ __forceinline__ void score(int s, const uint4 (&k)[TT], f32x4 (&acc)[RT][TT]) const {
@@ -243,13 +269,12 @@ struct Running {
     }
 };
 
-// The rows' own limits: row j of tile rt sees keys below limit[rt]. low: the
-// least of the piece's tile; mixed: they differ.
+// The rows' own limits: row j of tile rt sees positions below limit[rt], of
+// the lead all. low: the least of them.
 template <int RT>
 struct Limits {
     int32_t limit[RT];
     int32_t low;
-    bool mixed;
 };
 
 // Zeros for the infinities and NaN among a block's V values; whether there
@@ -276,16 +301,17 @@ __device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t bytes, uint
     return found;
 }
 
-// The infinities and NaN of V at keys [k0, k1) for the rows that see them: a
-// row's output there is their sum, whatever its finite values are.
+// The infinities and NaN of V at positions [k0, k1) for the rows that see
+// them: a row's output there is their sum, whatever its finite values are.
 template <typename T, int HD, int RT>
 __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Tile& t, const Limits<RT>& lim, int32_t k0, int32_t k1, Running<HD, RT>& run) {
     const uint32_t g = threadIdx.x % kWave / 16;
+    const Keys keys{t.table, 0, t.from, t.end, false};
 #pragma unroll 1
     for (int32_t key = k0; key < k1; ++key) {
-        const int32_t id = ld_scalar_i32(t.table + (key >> a.page_shift));
+        const int32_t id = page_id(a, keys, key);
         if (static_cast<uint32_t>(id) >= a.pages || key < t.from) continue;
-        const Rows at = rows_at<Block<T, HD>::kRow>(a, t, id, key);
+        const Rows at = rows_at<Block<T, HD>::kRow>(a, t.kvh, keys, id, key);
         const T* row = reinterpret_cast<const T*>(at.v) + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < HD / 16; ++dt)
@@ -299,12 +325,28 @@ __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Tile& t,
     }
 }
 
-// One block: TT tiles of 16 keys from key0, K in the lane's registers (REGS)
-// or as swizzled rows in the LDS, V's rows in the LDS. dead: a bit for each
-// tile that is in no page.
-template <typename T, int HD, int RT, int TT, bool REGS>
-__device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const Limits<RT>& lim, const Tile& tile, int32_t key0, uint32_t dead,
-                                             float softcap, const uint4 (*k_regs)[Block<T, HD>::kSteps], const uint8_t* k, const uint8_t* v,
+// Eight f32 values as two f16 terms each, two at a time; the remainder is an
+// fma that takes the f16 term as it is.
+__device__ __forceinline__ void split(f32x4 a, f32x4 b, half8& hi, half8& lo) {
+    typedef float float2v __attribute__((ext_vector_type(2)));
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2v x = i < 2 ? float2v{a[2 * i], a[2 * i + 1]} : float2v{b[2 * i - 4], b[2 * i - 3]};
+        const half2v h = __builtin_convertvector(x, half2v);
+        const float2v r = {__builtin_fmaf(static_cast<float>(h[0]), -1.0f, x[0]), __builtin_fmaf(static_cast<float>(h[1]), -1.0f, x[1])};
+        const half2v l = __builtin_convertvector(r, half2v);
+        hi[2 * i] = h[0], hi[2 * i + 1] = h[1];
+        lo[2 * i] = l[0], lo[2 * i + 1] = l[1];
+    }
+}
+
+// One block of TT tiles of 16 keys, K in the lane's registers (REGS) or as
+// swizzled rows in the LDS, V's rows in the LDS. dead: a bit for each tile
+// that is in no page.
+template <typename T, int HD, int RT, int TT, bool REGS, bool CAP>
+__device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const Limits<RT>& lim, const Keys& keys, uint32_t dead, float softcap,
+                                             const uint4 (*k_regs)[Block<T, HD>::kSteps], const uint8_t* k, const uint8_t* v,
                                              Running<HD, RT>& run) {
     using B = Block<T, HD>;
     const uint32_t l = threadIdx.x % kWave, j = l % 16, g = l / 16;
@@ -324,28 +366,26 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         }
         q.score(st, kk, s);
     }
-    const bool masked = key0 < tile.from || key0 + 16 * TT > lim.low || dead;
+    const bool masked = keys.key0 < keys.from || keys.key0 + 16 * TT > (keys.lead ? keys.end : lim.low) || dead;
     constexpr float kShift = B::kF16 ? 14.0f : 0.0f;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float c = q.c[rt];
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[rt][tt][e] *= c;
-        if (softcap > 0.0f) {
+        float c = q.c[rt];
+        if constexpr (CAP) {
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[rt][tt][e] = softcap * tanhf(s[rt][tt][e] / softcap) * kLog2e;
+                for (int e = 0; e < 4; ++e) s[rt][tt][e] = softcap * tanhf(s[rt][tt][e] * c / softcap);
+            c = kLog2e;
         }
         if (masked) {
+            const int32_t limit = keys.lead ? keys.end : lim.limit[rt];
 #pragma unroll
             for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int32_t key = key0 + 16 * tt + 4 * static_cast<int32_t>(g) + e;
-                    if (key < tile.from || key >= lim.limit[rt] || (dead >> tt & 1)) s[rt][tt][e] = -__builtin_inff();
+                    const int32_t key = keys.key0 + 16 * tt + 4 * static_cast<int32_t>(g) + e;
+                    if (key < keys.from || key >= limit || (dead >> tt & 1)) s[rt][tt][e] = -__builtin_inff();
                 }
         }
         float bm = -__builtin_inff();
@@ -357,13 +397,13 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         bm = fmaxf(__uint_as_float(a16.x), __uint_as_float(a16.y));
         const uint2 a32 = swap_rows<32>(__float_as_uint(bm));
         bm = fmaxf(__uint_as_float(a32.x), __uint_as_float(a32.y));
-        const float mn = fmaxf(run.m[rt], bm), factor = __builtin_amdgcn_exp2f(run.m[rt] - mn), mm = mn - kShift;
+        const float mn = fmaxf(run.m[rt], bm * c), factor = __builtin_amdgcn_exp2f(run.m[rt] - mn), mm = mn - kShift;
         float bs = 0.0f;
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = __builtin_amdgcn_exp2f(s[rt][tt][e] - mm);
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][tt][e], c, -mm));
                 s[rt][tt][e] = p;
                 bs += p;
             }
@@ -389,13 +429,7 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         for (int u = 0; u < TT / 2; ++u) {
             half8 ph[RT], pl[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float p = s[rt][2 * u + e / 4][e % 4];
-                    ph[rt][e] = static_cast<_Float16>(p);
-                    pl[rt][e] = static_cast<_Float16>(p - static_cast<float>(ph[rt][e]));
-                }
+            for (int rt = 0; rt < RT; ++rt) split(s[rt][2 * u], s[rt][2 * u + 1], ph[rt], pl[rt]);
 #pragma unroll
             for (int d0 = 0; d0 < HD / 16; d0 += D) {
                 half8 vv[D];
@@ -435,29 +469,42 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
 
 // ---------------------------------------------------------------- pieces
 
-// A piece of a tile: keys [k0, k1) of rows `rows` from token0 on.
+// A piece of a tile: [x0, x1) of its keys' axis, rows from token0 on.
 struct Piece {
     Tile tile;
-    int32_t k0, k1;
+    int32_t x0, x1;
     int32_t token0, tokens;
-    int32_t limit0;   // the keys below which the first token sees
-    bool causal;      // and each further token one more
-    bool whole;       // all of its rows' work: the output itself
+    int32_t limit0;    // the position below which the first token sees
+    bool causal;       // and each further token one more
+    bool whole;        // all of its rows' work: the output itself
     int64_t slot_row;  // else the rows of the workspace, -1 for none
 };
 
+// The LDS of the workgroup's waves is theirs together from here on: what they
+// wrote there is there, and what they read is read (unlike __syncthreads(),
+// stores to memory need not have arrived).
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+__device__ __forceinline__ float lanes_sum(float v) {  // over a row's four lanes
+    const uint2 l16 = swap_rows<16>(__float_as_uint(v));
+    v = __uint_as_float(l16.x) + __uint_as_float(l16.y);
+    const uint2 l32 = swap_rows<32>(__float_as_uint(v));
+    return __uint_as_float(l32.x) + __uint_as_float(l32.y);
+}
+
 template <typename T, int HD, int RT>
-__device__ __forceinline__ void load_rows(const PagesArgs& a, const Piece& p, uint32_t first_row, Queries<T, HD, RT>& q, Limits<RT>& lim) {
+__device__ __forceinline__ void load_rows(const PagesArgs& a, const Piece& p, uint32_t first_row, RawRow<T, HD> (&raw)[RT], Limits<RT>& lim) {
     const uint32_t l = threadIdx.x % kWave, j = l % 16, g = l / 16, rows = p.tokens * a.group;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const uint32_t r = min(first_row + 16 * rt + j, rows - 1), t = r / a.group;
-        const float* row = a.q + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r % a.group) * HD;
-        q.load(rt, row, g, a.softcap > 0.0f ? a.scale : a.scale * kLog2e);
+        raw[rt].load(a.q + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r % a.group) * HD, g);
         lim.limit[rt] = p.causal ? p.limit0 + static_cast<int32_t>(t) : p.limit0;
     }
-    lim.low = p.limit0;
-    lim.mixed = p.causal && p.tokens > 1;
 }
 
 // dims of a row, 4 a lane, to the output or the workspace
@@ -475,26 +522,25 @@ __device__ __forceinline__ void store_row(const PagesArgs& a, const Piece& p, ui
 }
 
 // At most 16 rows: each wave by itself over blocks of kWaveKeys keys in turn.
-template <typename T, int HD>
+template <typename T, int HD, bool CAP>
 __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buffer* buf) {
     using B = Block<T, HD>;
     constexpr int TT = B::kWaveTiles, N = TT;
-    const uint32_t w = threadIdx.x / kWave, l = threadIdx.x % kWave, j = l % 16, g = l / 16;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave, j = l % 16, g = l / 16;
     Queries<T, HD, 1> q;
-    Limits<1> lim;
+    Limits<1> lim{{p.limit0}, p.limit0};
     Running<HD, 1> run;
     run.clear();
     uint8_t* v = reinterpret_cast<uint8_t*>(buf) + 8192 * w;  // and as far into the second buffer
-    const int32_t step = kWaves * B::kWaveKeys;
-    int32_t key = p.k0 + static_cast<int32_t>(w * B::kWaveKeys);
-    key = __builtin_amdgcn_readfirstlane(key);
-    const int32_t first = key;
-    const auto issue = [&](const Pages<N>& ids, uint4 (&k)[TT][B::kSteps], uint8_t* to) {
+    constexpr int32_t kStep = kWaves * B::kWaveKeys, kSpan = B::kWaveKeys;
+    const int32_t first = p.x0 + static_cast<int32_t>(w) * kSpan;
+    int32_t x = first;
+    const auto issue = [&](const Pages<N>& at, uint4 (&k)[TT][B::kSteps], uint8_t* to) {
         Rows rows[N];
         bool whole = true;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            rows[i] = rows_at<B::kRow>(a, p.tile, ids.id[i], ids.key0 + 16 * i);
+            rows[i] = rows_at<B::kRow>(a, p.tile.kvh, at.keys, at.id[i], at.keys.key0 + 16 * i);
             whole &= rows[i].whole;
         }
         const auto loads = [&](auto piece) {
@@ -506,70 +552,69 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
                 const uint32_t u = 64 * i + l, row = u / B::kPieces, r = row % 16;
-                const Rows& at = rows[64 * i / B::kPieces / 16];
-                load_to_lds16(piece(at.v, at, r, r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row))), to + 1024 * i);
+                const Rows& from = rows[64 * i / B::kPieces / 16];
+                load_to_lds16(piece(from.v, from, r, r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row))), to + 1024 * i);
             }
         };
         if (whole) loads([](const uint8_t* base, const Rows&, uint32_t, uint32_t offset) { return base + offset; });
         else loads(piece_at);
     };
-    uint4 k[TT][B::kSteps];
-    const auto pages_at = [&](int32_t key0) {
-        Pages<N> r{{}, key0, 0};
+    const auto pages_at = [&](int32_t at) {
+        Pages<N> r{keys_at(p.tile, at), {}, 0};
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            r.id[i] = page_id(a, p.tile, key0 + 16 * i);
+            r.id[i] = page_id(a, r.keys, r.keys.key0 + 16 * i);
             r.dead |= static_cast<uint32_t>(r.id[i]) < a.pages ? 0u : 1u << i;
         }
         return r;
     };
-    Pages<N> cur = pages_at(key), nxt = pages_at(key + step);
+    uint4 k[TT][B::kSteps];
+    Pages<N> cur = pages_at(x), nxt = pages_at(x + kStep);
     // Values that are not finite in blocks that some rows see less of than
     // others are left out of the product and added at the end.
+    const bool mixed = p.causal && p.tokens > 1;
     bool unbounded = false;
     // The buffers don't overlap. Said so (__restrict__), and with both's loads
     // issued in here, the reads of one do not wait for the loads into the other.
     const auto block = [&](uint8_t* __restrict__ here, uint8_t* __restrict__ there) {
-        if (key == first) {
+        if (x == first) {
+            RawRow<T, HD> raw[1];
+            load_rows(a, p, 0, raw, lim);
             issue(cur, k, here);
-            load_rows(a, p, 0, q, lim);
+            q.take(0, raw[0], CAP ? a.scale : a.scale * kLog2e);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this block has landed
         uint4 k_next[TT][B::kSteps] = {};
-        if (key + step < p.k1) issue(nxt, k_next, there);
-        const Pages<N> after = pages_at(key + 2 * step);
-        if (lim.mixed && key + static_cast<int32_t>(B::kWaveKeys) > lim.low) unbounded |= clear_unbounded<T>(here, 8192, l, kWave);
-        attend_block<T, HD, 1, TT, true>(q, lim, p.tile, key, cur.dead, a.softcap, k, nullptr, here, run);
+        if (x + kStep < p.x1) issue(nxt, k_next, there);
+        const Pages<N> after = pages_at(x + 2 * kStep);
+        if (mixed && !cur.keys.lead && cur.keys.key0 + kSpan > lim.low) unbounded |= clear_unbounded<T>(here, 8192, l, kWave);
+        attend_block<T, HD, 1, TT, true, CAP>(q, lim, cur.keys, cur.dead, a.softcap, k, nullptr, here, run);
         cur = nxt;
         nxt = after;
-        key += step;
+        x += kStep;
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int s = 0; s < static_cast<int>(B::kSteps); ++s) k[tt][s] = k_next[tt][s];
     };
-    for (uint32_t n = 0; key < p.k1; n ^= sizeof(Buffer)) block(v + n, v + (n ^ sizeof(Buffer)));
+    for (uint32_t n = 0; x < p.x1; n ^= sizeof(Buffer)) block(v + n, v + (n ^ sizeof(Buffer)));
     if (__any(unbounded)) {
-        for (int32_t k = p.k0 + static_cast<int32_t>(w * B::kWaveKeys); k < p.k1; k += step) {
-            const int32_t end = min(k + static_cast<int32_t>(B::kWaveKeys), p.k1);
-            if (k + static_cast<int32_t>(B::kWaveKeys) > lim.low)
-                add_unbounded<T, HD, 1>(a, p.tile, lim, __builtin_amdgcn_readfirstlane(k), __builtin_amdgcn_readfirstlane(end), run);
+        for (int32_t at = first; at < p.x1; at += kStep) {
+            const Keys keys = keys_at(p.tile, at);
+            if (!keys.lead && keys.key0 + kSpan > lim.low) add_unbounded<T, HD, 1>(a, p.tile, lim, keys.key0, min(keys.key0 + kSpan, p.tile.end), run);
         }
     }
     // The waves' parts join in the LDS, rows HD + 4 floats apart.
-    const uint2 l16 = swap_rows<16>(__float_as_uint(run.l[0]));
-    float sum = __uint_as_float(l16.x) + __uint_as_float(l16.y);
-    const uint2 l32 = swap_rows<32>(__float_as_uint(sum));
-    sum = __uint_as_float(l32.x) + __uint_as_float(l32.y);
+    const float sum = lanes_sum(run.l[0]);
     constexpr uint32_t kStride = HD + 4;
     float* part = reinterpret_cast<float*>(buf);  // [waves][16][kStride], then [waves][16] of (m, l)
     float2* ml = reinterpret_cast<float2*>(part + kWaves * 16 * kStride);
-    __syncthreads();
+    lds_barrier();
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt)
         *reinterpret_cast<f32x4*>(part + (16 * w + j) * kStride + 16 * dt + 4 * g) = run.o[0][dt];
     if (g == 0) ml[16 * w + j] = make_float2(run.m[0], sum);
-    __syncthreads();
+    lds_barrier();
     const uint32_t r = threadIdx.x / 16;
     if (r < p.tokens * a.group) {
         float m = kLowest, f[kWaves], lsum = 0.0f;
@@ -586,21 +631,21 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (uint32_t i = 0; i < kWaves; ++i) {
-                const f32x4 x = *reinterpret_cast<const f32x4*>(part + (16 * i + r) * kStride + dim);
+                const f32x4 y = *reinterpret_cast<const f32x4*>(part + (16 * i + r) * kStride + dim);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] += f[i] * x[e];
+                for (int e = 0; e < 4; ++e) o[e] += f[i] * y[e];
             }
             store_row<HD>(a, p, r, dim, o, m, lsum);
         }
     }
-    __syncthreads();  // the next piece loads into this memory
 }
 
 // Many rows: RT tiles of 16 a wave, the blocks shared.
-template <typename T, int HD, int RT>
+template <typename T, int HD, int RT, bool CAP>
 __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Buffer* buf) {
     using B = Block<T, HD>;
     constexpr int TT = B::kTiles, N = 4;
+    constexpr int32_t kSpan = B::kKeys;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave, j = l % 16, g = l / 16;
     const uint32_t rows = p.tokens * a.group, first = 16 * RT * w;
     Queries<T, HD, RT> q;
@@ -609,80 +654,138 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
     run.clear();
     // The first of the 16 keys that the wave's i-th load is in.
     const auto part_of_load = [&](int i) { return static_cast<int32_t>((i * kThreads + w * kWave) / B::kPieces / 16 * 16); };
-    const auto issue = [&](const Pages<N>& ids, uint8_t* k_all, uint8_t* v_all) {
+    const auto issue = [&](const Pages<N>& at, uint8_t* k_all, uint8_t* v_all) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t u = i * kThreads + threadIdx.x, row = u / B::kPieces, r = row % 16;
-            const Rows at = rows_at<B::kRow>(a, p.tile, ids.id[i], ids.key0 + part_of_load(i));
+            const Rows from = rows_at<B::kRow>(a, p.tile.kvh, at.keys, at.id[i], at.keys.key0 + part_of_load(i));
             const uint32_t k_offset = r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row));
             const uint32_t v_offset = r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row));
             uint8_t* k_to = k_all + 16 * (i * kThreads + w * kWave);
             uint8_t* v_to = v_all + 16 * (i * kThreads + w * kWave);
-            if (at.whole) {
-                load_to_lds16(at.k + k_offset, k_to);
-                load_to_lds16(at.v + v_offset, v_to);
+            if (from.whole) {
+                load_to_lds16(from.k + k_offset, k_to);
+                load_to_lds16(from.v + v_offset, v_to);
             } else {
-                load_to_lds16(piece_at(at.k, at, r, k_offset), k_to);
-                load_to_lds16(piece_at(at.v, at, r, v_offset), v_to);
+                load_to_lds16(piece_at(from.k, from, r, k_offset), k_to);
+                load_to_lds16(piece_at(from.v, from, r, v_offset), v_to);
             }
         }
     };
-    int32_t key = p.k0;
-    const auto pages_at = [&](int32_t key0) {
-        Pages<N> r{{}, key0, 0};
+    const auto pages_at = [&](int32_t at) {
+        Pages<N> r{keys_at(p.tile, at), {}, 0};
 #pragma unroll
-        for (int i = 0; i < N; ++i) r.id[i] = page_id(a, p.tile, key0 + part_of_load(i));
+        for (int i = 0; i < N; ++i) r.id[i] = page_id(a, r.keys, r.keys.key0 + part_of_load(i));
 #pragma unroll
-        for (int i = 0; i < TT; ++i) r.dead |= static_cast<uint32_t>(page_id(a, p.tile, key0 + 16 * i)) < a.pages ? 0u : 1u << i;
+        for (int i = 0; i < TT; ++i) r.dead |= static_cast<uint32_t>(page_id(a, r.keys, r.keys.key0 + 16 * i)) < a.pages ? 0u : 1u << i;
         return r;
     };
-    Pages<N> cur = pages_at(key), nxt = pages_at(key + B::kKeys);
+    int32_t x = p.x0;
+    Pages<N> cur = pages_at(x), nxt = pages_at(x + kSpan);
     // The wave's rows that are none of the tile's take no part; nor do blocks
     // past all that the wave's rows see.
     const int32_t last_row = static_cast<int32_t>(min(first + 16 * RT, rows)) - 1;
-    const int32_t wave_end = first >= rows ? 0 : p.causal ? p.limit0 + last_row / static_cast<int32_t>(a.group) : p.limit0;
+    const int32_t wave_end = p.causal ? p.limit0 + last_row / static_cast<int32_t>(a.group) : p.limit0;
+    const bool idle = first >= rows, mixed = p.causal && p.tokens > 1;
+    lim.low = p.causal ? p.limit0 + static_cast<int32_t>(first / a.group) : p.limit0;
     bool unbounded = false;  // as in few_rows
     const auto block = [&](uint8_t* __restrict__ k, uint8_t* __restrict__ v, uint8_t* __restrict__ k_next, uint8_t* __restrict__ v_next) {
-        if (key == p.k0) {
+        if (x == p.x0) {
+            RawRow<T, HD> raw[RT];
+            load_rows(a, p, first, raw, lim);
             issue(cur, k, v);
-            load_rows(a, p, first, q, lim);
-            lim.low = p.causal ? p.limit0 + static_cast<int32_t>(first / a.group) : p.limit0;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) q.take(rt, raw[rt], CAP ? a.scale : a.scale * kLog2e);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // every wave's loads have landed, and the other buffer is read no more
-        if (key + static_cast<int32_t>(B::kKeys) < p.k1) issue(nxt, k_next, v_next);
-        const Pages<N> after = pages_at(key + 2 * B::kKeys);
-        if (lim.mixed && key + static_cast<int32_t>(B::kKeys) > p.limit0) {
+        lds_barrier();  // every wave's loads have landed, and the other buffer is read no more
+        if (x + kSpan < p.x1) issue(nxt, k_next, v_next);
+        const Pages<N> after = pages_at(x + 2 * kSpan);
+        if (mixed && !cur.keys.lead && cur.keys.key0 + kSpan > p.limit0) {
             unbounded |= clear_unbounded<T>(v, sizeof buf[0].v, threadIdx.x, kThreads);
-            __syncthreads();
+            lds_barrier();
         }
-        if (key < wave_end) attend_block<T, HD, RT, TT, false>(q, lim, p.tile, key, cur.dead, a.softcap, nullptr, k, v, run);
+        if (!idle && (cur.keys.lead || cur.keys.key0 < wave_end))
+            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, cur.dead, a.softcap, nullptr, k, v, run);
         cur = nxt;
         nxt = after;
-        key += B::kKeys;
+        x += kSpan;
     };
-    for (uint32_t n = 0; key < p.k1; n ^= 1) block(buf[n].k, buf[n].v, buf[n ^ 1].k, buf[n ^ 1].v);
-    if (p.causal && p.tokens > 1 && __syncthreads_or(unbounded)) {
-        // the blocks from the one that holds the first limit on
-        const int32_t first_block = max(p.limit0 - p.k0, 0) / static_cast<int32_t>(B::kKeys) * static_cast<int32_t>(B::kKeys);
-        add_unbounded<T, HD, RT>(a, p.tile, lim, p.k0 + first_block, p.k1, run);
+    for (uint32_t n = 0; x < p.x1; n ^= 1) block(buf[n].k, buf[n].v, buf[n ^ 1].k, buf[n ^ 1].v);
+    if (mixed && __syncthreads_or(unbounded)) {
+        // the blocks that reach past the first limit
+        for (int32_t at = p.x0; at < p.x1; at += kSpan) {
+            const Keys keys = keys_at(p.tile, at);
+            if (!keys.lead && keys.key0 + kSpan > p.limit0) add_unbounded<T, HD, RT>(a, p.tile, lim, keys.key0, min(keys.key0 + kSpan, p.tile.end), run);
+        }
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const uint2 l16 = swap_rows<16>(__float_as_uint(run.l[rt]));
-        float sum = __uint_as_float(l16.x) + __uint_as_float(l16.y);
-        const uint2 l32 = swap_rows<32>(__float_as_uint(sum));
-        sum = __uint_as_float(l32.x) + __uint_as_float(l32.y);
+        const float sum = lanes_sum(run.l[rt]);
         const uint32_t r = first + 16 * rt + j;
         if (r < rows) {
 #pragma unroll
             for (int dt = 0; dt < HD / 16; ++dt) store_row<HD>(a, p, r, 16 * dt + 4 * g, run.o[rt][dt], run.m[rt], sum);
         }
     }
-    __syncthreads();  // the next piece loads into this memory
 }
 
 // ---------------------------------------------------------------- the launch
+
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int32_t>(x >> 32)))) << 32 |
+                                static_cast<uint32_t>(uniform(static_cast<int32_t>(x))));
+}
+
+// v of lane i - n (DPP's row shifts and broadcasts), 0 where there is none:
+// the steps of an inclusive sum over the wave.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t shifted(int64_t v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, true);
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
+}
+__device__ __forceinline__ int64_t inclusive_sum(int64_t v) {
+    v += shifted<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8: within 16 lanes
+    v += shifted<0x112, 0xF>(v);
+    v += shifted<0x114, 0xF>(v);
+    v += shifted<0x118, 0xF>(v);
+    v += shifted<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    v += shifted<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
+// Segments as the workgroup keeps them, the first kThreads of a batch.
+struct Kept {
+    int32_t v[10];
+};
+__device__ __forceinline__ Kept kept(const Segment& s) {
+    return {{s.row, s.lead_row, s.lead, s.token0, s.n, s.from, s.base, s.tiles, s.step, (s.few ? 1 : 0) + (s.shared ? 2 : 0)}};
+}
+__device__ __forceinline__ Segment taken(const Kept& k) {
+    Segment s;
+    s.row = uniform(k.v[0]);
+    s.lead_row = uniform(k.v[1]);
+    s.lead = uniform(k.v[2]);
+    s.token0 = uniform(k.v[3]);
+    s.n = uniform(k.v[4]);
+    s.from = uniform(k.v[5]);
+    s.base = uniform(k.v[6]);
+    s.tiles = uniform(k.v[7]);
+    s.step = uniform(k.v[8]);
+    const int32_t flags = uniform(k.v[9]);
+    s.few = flags & 1;
+    s.shared = flags & 2;
+    s.lo = s.from & ~15;
+    return s;
+}
+
+struct Scratch {
+    int64_t cost[kThreads];    // inclusive sums of a wave
+    int64_t counts[kThreads];  // of tiles: few rows' in the low half, others' in the high
+    Kept segments[kThreads];
+};
 
 // Where a workgroup's part begins, and the whole of the work.
 struct Place {
@@ -690,136 +793,122 @@ struct Place {
     int64_t off;           // the cost before the segment
     int32_t kvh, segment;  // the first that the part has work of
     int32_t few, tiles;    // tiles of each kind before the segment
-    int32_t part, parts;
+    int32_t part, parts_log2;
 };
 
-// Every thread sums its run of segments; the workgroup's exclusive sums then
-// place them, and the thread whose run holds the part's first unit finds it.
-__device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, uint8_t* lds) {
-    const int32_t n = a.batch.groups + a.batch.seqs, each = (n + kThreads - 1) / kThreads;
-    const int32_t i0 = min(static_cast<int32_t>(threadIdx.x) * each, n), i1 = min(i0 + each, n);
-    int64_t cost = 0;
-    int32_t few = 0, tiles = 0;
+// Every thread sums its run of segments (one, up to kThreads of them), and the
+// waves' sums place the part's first unit among them.
+__device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scratch& lds) {
+    const int32_t n = a.batch.groups + a.batch.seqs, each = n <= static_cast<int32_t>(kThreads) ? 1 : (n + kThreads - 1) / kThreads;
+    const int32_t t = static_cast<int32_t>(threadIdx.x), i0 = t * each, i1 = min(i0 + each, n);
+    int64_t cost = 0, counts = 0;
     for (int32_t i = i0; i < i1; ++i) {
         const Segment s = segment(a.batch, a.group, i);
+        if (each == 1) lds.segments[t] = kept(s);
         cost += s.cost();
-        (s.few ? few : tiles) += s.tiles;
+        counts += s.few ? static_cast<int64_t>(s.tiles) : static_cast<int64_t>(s.tiles) << 32;
     }
-    int64_t* costs = reinterpret_cast<int64_t*>(lds);
-    int32_t* fews = reinterpret_cast<int32_t*>(costs + kThreads);
-    int32_t* tile_sums = fews + kThreads;
-    Place* place = reinterpret_cast<Place*>(tile_sums + kThreads);
-    // inclusive sums in the wave, then across the waves
-    const uint32_t l = threadIdx.x % kWave, w = threadIdx.x / kWave;
-    int64_t c = cost;
-    int32_t f = few, t = tiles;
-#pragma unroll
-    for (uint32_t d = 1; d < kWave; d *= 2) {
-        const int64_t cc = __shfl_up(static_cast<long long>(c), d, kWave);
-        const int32_t ff = __shfl_up(f, d, kWave), tt = __shfl_up(t, d, kWave);
-        if (l >= d) c += cc, f += ff, t += tt;
-    }
-    if (l == kWave - 1) costs[w] = c, fews[w] = f, tile_sums[w] = t;
-    __syncthreads();
-    int64_t per_head = 0;
-    int32_t few_head = 0, tiles_head = 0;
+    lds.cost[t] = inclusive_sum(cost);
+    lds.counts[t] = inclusive_sum(counts);
+    lds_barrier();
+    const uint32_t l = threadIdx.x % kWave;
+    int64_t sums[kWaves], per_head = 0, counts_head = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kWaves; ++i) {
-        if (i < w) c += costs[i], f += fews[i], t += tile_sums[i];
-        per_head += costs[i], few_head += fews[i], tiles_head += tile_sums[i];
+        sums[i] = uniform(lds.cost[kWave * i + kWave - 1]);
+        per_head += sums[i];
+        counts_head += uniform(lds.counts[kWave * i + kWave - 1]);
     }
-    const int64_t all = per_head * a.kv_heads;
-    const int32_t n_parts = parts(all, a.workgroups);
-    // dealt to the XCDs round-robin: part p is with its neighbours on one
+    out.cost = per_head * a.kv_heads;
+    out.parts_log2 = parts_log2(out.cost, a.workgroups_log2);
+    // dealt to the XCDs round-robin: the parts of one are neighbours
     const int32_t b = static_cast<int32_t>(blockIdx.x);
-    if (all == 0 || b >= n_parts) return false;
-    const int32_t part = b % 8 * (n_parts / 8) + b / 8;
-    const int64_t u0 = part_start(all, n_parts, part);
-    const int32_t kvh = static_cast<int32_t>(u0 / per_head);
-    const int64_t rem = u0 - kvh * per_head;
-    int64_t off = c - cost;
-    f -= few, t -= tiles;
-    if (rem >= off && rem < c) {
-        for (int32_t i = i0; i < i1; ++i) {
-            const Segment s = segment(a.batch, a.group, i);
-            if (rem < off + s.cost()) {
-                place->cost = all;
-                place->off = kvh * per_head + off;
-                place->kvh = kvh;
-                place->segment = i;
-                place->few = kvh * few_head + f;
-                place->tiles = kvh * tiles_head + t;
-                place->part = part;
-                place->parts = n_parts;
-                break;
-            }
-            off += s.cost();
-            (s.few ? f : t) += s.tiles;
+    if (out.cost == 0 || b >> out.parts_log2) return false;
+    out.part = (b % 8 << (out.parts_log2 - 3)) + b / 8;
+    out.kvh = static_cast<int32_t>(static_cast<int64_t>(a.kv_heads) * out.part >> out.parts_log2);
+    const int64_t unit = part_start(out.cost, out.parts_log2, out.part) - out.kvh * per_head;
+    int64_t off = 0, before = 0;  // of the wave whose segments hold the unit
+    uint32_t w = 0;
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < kWaves; ++i)
+        if (w == i && unit >= off + sums[i]) {
+            off += sums[i];
+            before += uniform(lds.counts[kWave * i + kWave - 1]);
+            ++w;
         }
+    const int64_t mine = lds.cost[kWave * w + l], my_counts = lds.counts[kWave * w + l];
+    const uint32_t lane = static_cast<uint32_t>(__builtin_ctzll(__ballot(off + mine > unit)));
+    if (lane > 0) {
+        const auto from_lane = [&](int64_t v) {
+            return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane - 1))) << 32 |
+                                        static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane - 1)));
+        };
+        off += from_lane(mine);
+        before += from_lane(my_counts);
     }
-    __syncthreads();
-    // the workgroup's, in scalar registers
-    const auto whole = [](int32_t x) { return __builtin_amdgcn_readfirstlane(x); };
-    const auto whole64 = [&](int64_t x) {
-        return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(whole(static_cast<int32_t>(x >> 32)))) << 32 |
-                                    static_cast<uint32_t>(whole(static_cast<int32_t>(x))));
-    };
-    out.cost = whole64(place->cost);
-    out.off = whole64(place->off);
-    out.kvh = whole(place->kvh);
-    out.segment = whole(place->segment);
-    out.few = whole(place->few);
-    out.tiles = whole(place->tiles);
-    out.part = whole(place->part);
-    out.parts = whole(place->parts);
-    __syncthreads();
+    int32_t i = static_cast<int32_t>(kWave * w + lane) * each;
+    for (; each > 1; ++i) {
+        const Segment s = segment(a.batch, a.group, i);
+        if (unit < off + s.cost()) break;
+        off += s.cost();
+        before += s.few ? static_cast<int64_t>(s.tiles) : static_cast<int64_t>(s.tiles) << 32;
+    }
+    out.segment = i;
+    out.off = out.kvh * per_head + off;
+    out.few = static_cast<int32_t>(before) + out.kvh * static_cast<int32_t>(counts_head);
+    out.tiles = static_cast<int32_t>(before >> 32) + out.kvh * static_cast<int32_t>(counts_head >> 32);
     return true;
 }
 
-template <typename T, int HD>
+template <typename T, int HD, bool CAP>
 __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     using B = Block<T, HD>;
     __shared__ Buffer buf[2];
+    __shared__ Scratch scratch;
     Place at;
-    if (!find_place(a, at, buf[0].k)) return;
-    const int64_t u0 = part_start(at.cost, at.parts, at.part), u1 = part_start(at.cost, at.parts, at.part + 1);
+    if (!find_place(a, at, scratch)) return;
+    const int64_t u0 = part_start(at.cost, at.parts_log2, at.part), u1 = part_start(at.cost, at.parts_log2, at.part + 1);
     const int32_t segments = a.batch.groups + a.batch.seqs;
     int32_t kvh = at.kvh, i = at.segment, few = at.few, tiles = at.tiles;
     int64_t off = at.off;
+    bool again = false;
     while (off < u1 && kvh < static_cast<int32_t>(a.kv_heads)) {
-        const Segment s = segment(a.batch, a.group, i);
-        for (int32_t t = s.tiles && u0 > off ? s.tile_at(u0 - off) : 0; t < s.tiles; ++t) {
-            const int64_t start = off + s.before(t);
+        const Segment s = segments <= static_cast<int32_t>(kThreads) ? taken(scratch.segments[i]) : segment(a.batch, a.group, i);
+        for (int32_t t = s.tiles > 1 && u0 > off ? s.tile_at(u0 - off) : 0; t < s.tiles; ++t) {
+            const int64_t start = off + s.before(t), end = start + s.tile_cost(t);
             if (start >= u1) break;
             const int32_t keys = s.keys(t);
-            const int64_t end = start + kOverhead + keys;
             Piece p;
-            p.tile = {a.table + static_cast<uint64_t>(s.row) * a.table_stride, static_cast<uint32_t>(kvh), s.from, s.lo + keys};
-            p.k0 = s.lo + (u0 > start ? cut(u0 - start, keys, B::kKeys) : 0);
-            p.k1 = s.lo + (u1 >= end ? keys : cut(u1 - start, keys, B::kKeys));
+            p.tile = {a.table + static_cast<uint64_t>(s.lead_row) * a.table_stride, a.table + static_cast<uint64_t>(s.row) * a.table_stride,
+                      s.lead_span(), s.lead, s.lo, s.from, s.lo + keys - s.lead_span(), static_cast<uint32_t>(kvh)};
+            p.x0 = u0 > start ? cut(u0 - start, s.key_cost(), keys, B::kKeys) : 0;
+            p.x1 = u1 >= end ? keys : cut(u1 - start, s.key_cost(), keys, B::kKeys);
             p.token0 = s.token0 + t * s.step;
             p.tokens = s.tile_n(t);
             p.limit0 = s.limit(t * s.step);
             p.causal = !s.shared;
-            const bool alone = u0 <= start && u1 >= end;
-            p.whole = alone && !s.shared && s.from == 0;
+            // the rows' own keys are all there is, but for a shared segment's
+            const bool all = !s.shared && s.from == s.lead;
+            p.whole = all && u0 <= start && u1 >= end;
             const int32_t slot = at.part + (s.few ? few : tiles + t);
             p.slot_row = s.few ? (slot < a.few_slots ? static_cast<int64_t>(slot) * kFewRows : -1)
                                : (slot < a.tile_slots ? a.few_slots * kFewRows + static_cast<int64_t>(slot) * kTileRows : -1);
-            // The tile's first piece tells the merge where they all are; of
-            // tokens without shared keys also that those have none.
+            // The tile's first piece tells the merge where they all are, and
+            // where there is no shared segment, that there is none.
             if (start >= u0) {
-                const uint32_t count = p.whole || p.slot_row < 0 ? 0 : part_of(at.cost, at.parts, end - 1) - at.part + 1;
+                const uint32_t count = p.whole || p.slot_row < 0 ? 0 : part_of(at.cost, at.parts_log2, end - 1) - at.part + 1;
                 for (uint32_t k = threadIdx.x; k < static_cast<uint32_t>(p.tokens); k += kThreads) {
                     Parts* to = a.parts + (static_cast<uint64_t>(kvh) * a.batch.tokens + p.token0 + k) * 2;
-                    const Parts mine = {static_cast<uint32_t>(p.slot_row + k * a.group), 2 * count + (s.few ? 0u : 1u)};
-                    stg(reinterpret_cast<uint2*>(to + (s.shared ? 0 : 1)), make_uint2(mine.row, mine.count));
-                    if (!s.shared && s.from == 0) stg(reinterpret_cast<uint2*>(to), make_uint2(0, 0));
+                    const uint2 mine = make_uint2(static_cast<uint32_t>(p.slot_row + k * a.group), 2 * count + (s.few ? 0u : 1u));
+                    if (all) stg(reinterpret_cast<uint4*>(to), make_uint4(0, 0, mine.x, mine.y));
+                    else stg(reinterpret_cast<uint2*>(to + (s.shared ? 0 : 1)), mine);
                 }
             }
-            if (s.few) few_rows<T, HD>(a, p, buf);
-            else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1>(a, p, buf);
-            else many_rows<T, HD, 2>(a, p, buf);
+            if (again) lds_barrier();  // the last piece's LDS
+            again = true;
+            if (s.few) few_rows<T, HD, CAP>(a, p, buf);
+            else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1, CAP>(a, p, buf);
+            else many_rows<T, HD, 2, CAP>(a, p, buf);
         }
         off += s.cost();
         (s.few ? few : tiles) += s.tiles;
@@ -827,57 +916,88 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     }
 }
 
-// Joins the pieces of the rows that are in several: a wave a row, the pieces'
-// (m, l) a lane each, then their o, HD / 64 dims a lane.
-template <int HD>
+// Joins the pieces of the rows that are in several: W waves a row, the
+// pieces' (m, l) a lane each, then each wave its share of their o, HD / 64
+// dims a lane, kFlight pieces in flight.
+template <int HD, int W>
 __global__ void __launch_bounds__(kThreads) k_attend_pages_merge(PagesArgs a, int64_t ws_rows) {
-    constexpr int N = HD / 64;
-    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t l = threadIdx.x % kWave;
+    constexpr int N = HD / 64, kFlight = 8;
+    __shared__ float s_o[kWaves][HD];
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
+    const uint64_t row = static_cast<uint64_t>(blockIdx.x) * (kWaves / W) + w / W;
     if (row >= static_cast<uint64_t>(a.batch.tokens) * a.heads) return;
     const int32_t t = static_cast<int32_t>(row / a.heads);
-    if (t < a.batch.start(0) || t >= a.batch.start(a.batch.seqs)) return;
     const uint32_t h = static_cast<uint32_t>(row % a.heads), kvh = h / a.group;
     const uint4 both = ldg(reinterpret_cast<const uint4*>(a.parts + (static_cast<uint64_t>(kvh) * a.batch.tokens + t) * 2));
-    const uint32_t n0 = both.y / 2, n1 = both.w / 2, n = n0 + n1;
+    if (t < a.batch.start(0) || t >= a.batch.start(a.batch.seqs)) return;
+    const uint32_t n0 = both.y / 2, n1 = both.w / 2, n = n0 + n1, in_group = h % a.group;
+    const uint32_t step0 = both.y & 1 ? kTileRows : kFewRows, step1 = both.w & 1 ? kTileRows : kFewRows;
     if (n == 0) return;
-    const auto row_of = [&](uint32_t p) -> int64_t {
-        const bool own = p >= n0;
-        const uint32_t kind = own ? both.w : both.y;
-        return static_cast<int64_t>(own ? both.z : both.x) + h % a.group + static_cast<int64_t>(own ? p - n0 : p) * (kind & 1 ? kTileRows : kFewRows);
+    const auto row_of = [&](uint32_t p) {
+        return p < n0 ? static_cast<int64_t>(both.x) + in_group + static_cast<int64_t>(p) * step0
+                      : static_cast<int64_t>(both.z) + in_group + static_cast<int64_t>(p - n0) * step1;
     };
     if (row_of(n - 1) >= ws_rows || (n0 && row_of(n0 - 1) >= ws_rows)) return;
     float m = kLowest, lsum = 0.0f, o[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = 0.0f;
     for (uint32_t p0 = 0; p0 < n; p0 += kWave) {
-        const uint32_t p = p0 + l;
-        const float2 ml = p < n ? ldg(a.stats + row_of(p)) : make_float2(kLowest, 0.0f);
+        const uint32_t many = min(n - p0, static_cast<uint32_t>(kWave));
+        const float2 ml = l < many ? ldg(a.stats + row_of(p0 + l)) : make_float2(kLowest, 0.0f);
         const float mn = fmaxf(m, wave_max(ml.x)), factor = __builtin_amdgcn_exp2f(m - mn), weight = __builtin_amdgcn_exp2f(ml.x - mn);
-        lsum = lsum * factor + wave_sum(p < n ? weight * ml.y : 0.0f);
+        lsum = lsum * factor + wave_sum(l < many ? weight * ml.y : 0.0f);
         m = mn;
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] *= factor;
-        const uint32_t many = min(n - p0, static_cast<uint32_t>(kWave));
-#pragma unroll 8
-        for (uint32_t k = 0; k < many; ++k) {
-            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), k));
-            const float* from = a.o + row_of(p0 + k) * HD + N * l;
+        for (uint32_t k0 = w % W; k0 < many; k0 += W * kFlight) {
+            float x[kFlight][N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) o[i] += f * ldg(from + i);
+            for (uint32_t k = 0; k < kFlight; ++k) {  // past the last: its o again, with no weight
+                const float* from = a.o + row_of(p0 + min(k0 + W * k, many - 1)) * HD + N * l;
+                if constexpr (N == 2) {
+                    const float2 y = ldg(reinterpret_cast<const float2*>(from));
+                    x[k][0] = y.x, x[k][1] = y.y;
+                } else {
+                    x[k][0] = ldg(from);
+                }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kFlight; ++k) {
+                if (k0 + W * k >= many) break;
+                const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), k0 + W * k));
+#pragma unroll
+                for (int i = 0; i < N; ++i) o[i] += f * x[k][i];
+            }
         }
     }
     const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+    if constexpr (W > 1) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) stg(a.out + row * HD + N * l + i, o[i] * inv);
+        for (int i = 0; i < N; ++i) s_o[w][N * l + i] = o[i];
+        __syncthreads();
+        if (threadIdx.x < HD) {
+            float x = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) x += s_o[i][threadIdx.x];
+            stg(a.out + row * HD + threadIdx.x, x * inv);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) stg(a.out + row * HD + N * l + i, o[i] * inv);
+    }
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-uint32_t workgroups() { return std::max(8u, 2 * vkml::abi::compute_units() / 8 * 8); }
+// Two workgroups a compute unit, or the power of two below.
+int32_t workgroups_log2() {
+    int32_t n = 3;
+    while ((2u << n) <= 2 * vkml::abi::compute_units()) ++n;
+    return n;
+}
 
 Slots slots_of(const vkml_attend_pages_params& p) {
-    return slots(p.kv_heads, p.heads / p.kv_heads, p.seqs, p.groups, p.tokens, workgroups());
+    return slots(p.kv_heads, p.heads / p.kv_heads, p.seqs, p.groups, p.tokens, int64_t{1} << workgroups_log2());
 }
 
 uint64_t up16(uint64_t bytes) { return (bytes + 15) / 16 * 16; }
@@ -929,17 +1049,27 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     a.page_shift = static_cast<uint32_t>(__builtin_ctz(p->page_size));
     a.pages = p->pages;
     a.table_stride = p->table_stride;
-    a.workgroups = workgroups();
+    a.workgroups_log2 = workgroups_log2();
     a.scale = p->scale;
     a.softcap = p->softcap;
     vkml::abi::ProfileScope prof("attend_pages");
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(a.workgroups), dim3(kThreads), 0, vkml::abi::stream(), a); };
-    if (p->kv_type == VKML_F16) p->head_dim == 128 ? go(k_attend_pages<_Float16, 128>) : go(k_attend_pages<_Float16, 64>);
-    else p->head_dim == 128 ? go(k_attend_pages<float, 128>) : go(k_attend_pages<float, 64>);
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(1u << a.workgroups_log2), dim3(kThreads), 0, vkml::abi::stream(), a); };
+    const bool wide = p->head_dim == 128;
+    if (p->kv_type == VKML_F16) {
+        if (p->softcap > 0.0f) wide ? go(k_attend_pages<_Float16, 128, true>) : go(k_attend_pages<_Float16, 64, true>);
+        else wide ? go(k_attend_pages<_Float16, 128, false>) : go(k_attend_pages<_Float16, 64, false>);
+    } else {
+        if (p->softcap > 0.0f) wide ? go(k_attend_pages<float, 128, true>) : go(k_attend_pages<float, 64, true>);
+        else wide ? go(k_attend_pages<float, 128, false>) : go(k_attend_pages<float, 64, false>);
+    }
     if (const int r = vkml::abi::check_launch("attend_pages")) return r;
-    const dim3 merge(static_cast<uint32_t>((static_cast<uint64_t>(p->tokens) * p->heads + kWaves - 1) / kWaves));
-    if (p->head_dim == 128) hipLaunchKernelGGL(k_attend_pages_merge<128>, merge, dim3(kThreads), 0, vkml::abi::stream(), a, s.rows());
-    else hipLaunchKernelGGL(k_attend_pages_merge<64>, merge, dim3(kThreads), 0, vkml::abi::stream(), a, s.rows());
+    const uint32_t rows = p->tokens * p->heads;
+    const auto merge = [&](auto kernel, uint32_t workgroups) {
+        hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kThreads), 0, vkml::abi::stream(), a, s.rows());
+    };
+    // Few rows in many pieces: a workgroup a row; many, most of them in one: a wave.
+    if (rows <= 4096) wide ? merge(k_attend_pages_merge<128, kWaves>, rows) : merge(k_attend_pages_merge<64, kWaves>, rows);
+    else wide ? merge(k_attend_pages_merge<128, 1>, (rows + kWaves - 1) / kWaves) : merge(k_attend_pages_merge<64, 1>, (rows + kWaves - 1) / kWaves);
     return vkml::abi::check_launch("attend_pages: merge");
 }
 

@@ -69,7 +69,7 @@ struct Batch {
 // ---------------------------------------------------------------- the work of vkml_attend_pages
 
 // A KV head's work is a list of segments: for each group its shared keys by
-// all of its tokens, then for each sequence its own keys by its tokens. A
+// all of its tokens, then for each sequence its other keys by its tokens. A
 // segment's tokens go in tiles: all of them where they are at most kFewRows
 // rows (token, query head), else kTileRows / (query heads a KV head) at a time.
 // A tile costs the keys it reads and kOverhead more (its queries, its joining
@@ -78,65 +78,88 @@ struct Batch {
 // piece.
 constexpr int32_t kFewRows = 16;
 constexpr int32_t kTileRows = 128;
-constexpr int32_t kOverhead = 64;
-constexpr int32_t kMinPart = 128;  // keys below which work is not cut further
+// What a key costs a tile of few rows, and another, and a tile by itself.
+constexpr int32_t kFewCost = 2, kTileCost = 3, kOverhead = 128;
+constexpr int32_t kMinPart = 256;  // the cost below which work is not cut further
+constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
 
 VKML_HD int32_t tile_tokens(int32_t group) { return kTileRows / group > 1 ? kTileRows / group : 1; }
 
+// The keys of a segment lie on one axis: first the `lead` keys that its tokens
+// read through the table row of their group's first sequence, filled up to a
+// multiple of kLeadStep, then those from position lo on, of its own row.
 struct Segment {
-    int32_t row = 0;     // the sequence whose table holds the keys
+    int32_t row = 0;       // the sequence whose table holds the keys from lo on
+    int32_t lead_row = 0;  // and the `lead` keys
+    int32_t lead = 0;
     int32_t token0 = 0;  // the first token
     int32_t n = 0;       // tokens
-    int32_t lo = 0;      // the first key read, a multiple of 16
-    int32_t from = 0;    // the first key that counts
-    int32_t base = 0;    // own keys: those from lo on before the first token's; shared ones: all
+    int32_t lo = 0;      // the first position read, a multiple of 16
+    int32_t from = 0;    // the first that counts
+    int32_t base = 0;    // positions from lo on before the first token's; shared keys: all
     int32_t tiles = 0, step = 1;
     bool few = false, shared = false;
 
-    // Keys from lo on that tile i's tokens see.
+    VKML_HD int32_t lead_span() const { return (lead + kLeadStep - 1) / kLeadStep * kLeadStep; }
+    // The axis' length for tile i's tokens.
     VKML_HD int32_t keys(int32_t i) const {
-        if (shared) return base;
-        if (base < 0) return base + n > 0 ? base + n : 0;
-        const int32_t tokens = (i + 1) * step < n ? (i + 1) * step : n;
-        return base + tokens;
+        int32_t own = base;
+        if (!shared) {
+            own += base < 0 || (i + 1) * step > n ? n : (i + 1) * step;
+            own = own > 0 ? own : 0;
+        }
+        return lead_span() + own;
     }
+    VKML_HD int32_t key_cost() const { return few ? kFewCost : kTileCost; }
+    VKML_HD int64_t tile_cost(int32_t i) const { return kOverhead + static_cast<int64_t>(key_cost()) * keys(i); }
     // The cost of the tiles before tile i.
     VKML_HD int64_t before(int32_t i) const {
-        const int64_t k = i;
-        if (shared || base < 0) return k * (kOverhead + keys(0));
-        return k * (kOverhead + base) + step * k * (k + 1) / 2;
+        const int64_t k = i, each = kOverhead + static_cast<int64_t>(key_cost()) * (shared || base < 0 ? keys(0) : lead_span() + base);
+        return shared || base < 0 ? k * each : k * each + key_cost() * (step * (k * (k + 1) / 2));
     }
-    VKML_HD int64_t cost() const { return tiles ? before(tiles - 1) + kOverhead + keys(tiles - 1) : 0; }
+    VKML_HD int64_t cost() const { return tiles ? before(tiles - 1) + tile_cost(tiles - 1) : 0; }
     // The tile that holds unit u of the segment, 0 <= u < cost().
     VKML_HD int32_t tile_at(int64_t u) const {
-        int32_t lo_tile = 0, hi = tiles;
-        while (hi - lo_tile > 1) {
-            const int32_t mid = lo_tile + (hi - lo_tile) / 2;
-            if (before(mid) <= u) lo_tile = mid;
+        int32_t first = 0, hi = tiles;
+        while (hi - first > 1) {
+            const int32_t mid = first + (hi - first) / 2;
+            if (before(mid) <= u) first = mid;
             else hi = mid;
         }
-        return lo_tile;
+        return first;
     }
-    // The last key position (+ 1) that token i of the segment sees.
+    // The position past the last that token i of the segment sees.
     VKML_HD int32_t limit(int32_t i) const { return shared ? base : lo + base + i + 1; }
     VKML_HD int32_t tile_n(int32_t i) const { return n - i * step < step ? n - i * step : step; }
 };
+
+// Whether group g's shared keys are a segment of their own. Where its
+// sequences have half a tile of tokens or more on average, their own tiles
+// read few blocks more than the group's would, and no rows are in two parts.
+VKML_HD bool shares(const Batch& b, int32_t group, int32_t g) {
+    const int32_t first = b.group_start(g), last = b.group_start(g + 1);
+    const int64_t tokens = static_cast<int64_t>(b.start(last)) - b.start(first);
+    return tokens > 0 && 2 * tokens <= static_cast<int64_t>(last - first) * tile_tokens(group);
+}
 
 // Segment i of a batch: groups 0 .. groups - 1, then the sequences.
 VKML_HD Segment segment(const Batch& b, int32_t group, int32_t i) {
     Segment s;
     if (i < b.groups) {
-        const int32_t first = b.group_start(i), last = b.group_start(i + 1);
-        s.row = first;
         s.base = b.group_shared(i);
         s.shared = true;
-        if (s.base == 0) return s;
-        s.token0 = b.start(first);
-        s.n = b.start(last) - s.token0;
+        if (s.base == 0 || !shares(b, group, i)) return s;
+        s.row = b.group_start(i);
+        s.token0 = b.start(s.row);
+        s.n = b.start(b.group_start(i + 1)) - s.token0;
     } else {
         s.row = i - b.groups;
         const int32_t g = b.group_of(s.row);
         s.from = g < 0 ? 0 : b.group_shared(g);
+        if (s.from > 0 && !shares(b, group, g)) {
+            s.lead = s.from;
+            s.lead_row = b.group_start(g);
+        }
         s.lo = s.from & ~15;
         s.token0 = b.start(s.row);
         s.n = b.count(s.row);
@@ -152,25 +175,30 @@ VKML_HD Segment segment(const Batch& b, int32_t group, int32_t i) {
     return s;
 }
 
-// Workgroups that share a cost: all of them, in eights for the eight XCDs,
-// unless a part would be less than kMinPart.
-VKML_HD int32_t parts(int64_t cost, int32_t workgroups) {
-    int64_t n = cost / kMinPart / 8 * 8;
-    if (n < 8) n = 8;
-    return n < workgroups ? static_cast<int32_t>(n) : workgroups;
+// The parts of a cost, as a power of two: one a workgroup, at least one an
+// XCD, and fewer where a part would be less than kMinPart.
+VKML_HD int32_t parts_log2(int64_t cost, int32_t workgroups_log2) {
+    int32_t n = 3;
+    while (n < workgroups_log2 && cost >> n >= 2 * kMinPart) ++n;
+    return n;
 }
-// The first unit of part w, and the part that unit u is in.
-VKML_HD int64_t part_start(int64_t cost, int32_t n, int32_t w) { return static_cast<int64_t>(static_cast<uint64_t>(cost) * static_cast<uint32_t>(w) / static_cast<uint32_t>(n)); }
-VKML_HD int32_t part_of(int64_t cost, int32_t n, int64_t u) {
-    return static_cast<int32_t>((static_cast<uint64_t>(u + 1) * static_cast<uint32_t>(n) - 1) / static_cast<uint64_t>(cost));
+// The first unit of part w, and the part that unit u is in (the quotient,
+// found in f32 and set right).
+VKML_HD int64_t part_start(int64_t cost, int32_t n_log2, int32_t w) { return cost * w >> n_log2; }
+VKML_HD int32_t part_of(int64_t cost, int32_t n_log2, int64_t u) {
+    int32_t w = static_cast<int32_t>(static_cast<float>(u) / static_cast<float>(cost) * static_cast<float>(1 << n_log2));
+    while (part_start(cost, n_log2, w) > u) --w;
+    while (part_start(cost, n_log2, w + 1) <= u) ++w;
+    return w;
 }
 // Keys of a tile of `keys` that units before x of it stand for: whole blocks
 // (but the last), so that every part cuts at the same places.
-VKML_HD int32_t cut(int64_t x, int32_t keys, int32_t block) {
-    const int64_t k = x - kOverhead;
-    if (k <= 0) return 0;
-    const int64_t up = (k + block - 1) / block * block;
-    return up < keys ? static_cast<int32_t>(up) : keys;
+VKML_HD int32_t cut(int64_t x, int32_t key_cost, int32_t keys, int32_t block) {
+    if (x <= kOverhead) return 0;
+    const int64_t k = (x - kOverhead) / key_cost;
+    if (k >= keys) return keys;
+    const int32_t up = (static_cast<int32_t>(k) + block - 1) / block * block;
+    return up < keys ? up : keys;
 }
 
 // What a call keeps of unfinished rows: slots of kFewRows or kTileRows rows,
@@ -202,7 +230,7 @@ inline const char* check_cache(uint32_t kv_heads, uint32_t head_dim, uint32_t kv
 inline const char* check_batch(uint32_t seqs, uint32_t tokens, uint32_t table_stride, uint32_t page_size) {
     if (seqs > kMaxSeqs) return "more than 65536 sequences";
     if (tokens > kMaxTokens) return "more than 2^22 new tokens";
-    if (table_stride == 0 || static_cast<uint64_t>(table_stride) * page_size > 0x7FFFFFFFu) return "a table row must hold 1 to 2^31 - 1 keys";
+    if (table_stride == 0 || static_cast<uint64_t>(table_stride) * page_size > (1u << 30)) return "a table row must hold 1 to 2^30 keys";
     return nullptr;
 }
 
