@@ -75,7 +75,7 @@ struct PagesArgs {
     int64_t few_slots, tile_slots;
     uint32_t heads, kv_heads, group, page_shift, pages, table_stride;
     int32_t workgroups_log2;
-    float scale, softcap;
+    float scale, softcap, group_inverse;
 };
 
 // 16 bytes of zeros that the rows without a key are read from.
@@ -305,7 +305,7 @@ __device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t bytes, uint
 // them: a row's output there is their sum, whatever its finite values are.
 template <typename T, int HD, int RT>
 __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Tile& t, const Limits<RT>& lim, int32_t k0, int32_t k1, Running<HD, RT>& run) {
-    const uint32_t g = threadIdx.x % kWave / 16;
+    const uint32_t g = thread_index() % kWave / 16;
     const Keys keys{t.table, 0, t.from, t.end, false};
 #pragma unroll 1
     for (int32_t key = k0; key < k1; ++key) {
@@ -325,20 +325,23 @@ __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Tile& t,
     }
 }
 
-// Eight f32 values as two f16 terms each, two at a time; the remainder is an
-// fma that takes the f16 term as it is.
+// Eight f32 values as two f16 terms each, two at a time, the remainder by an
+// fma that widens the f16 term itself.
 __device__ __forceinline__ void split(f32x4 a, f32x4 b, half8& hi, half8& lo) {
     typedef float float2v __attribute__((ext_vector_type(2)));
     typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    uint32_t h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2v x = i < 2 ? float2v{a[2 * i], a[2 * i + 1]} : float2v{b[2 * i - 4], b[2 * i - 3]};
-        const half2v h = __builtin_convertvector(x, half2v);
-        const float2v r = {__builtin_fmaf(static_cast<float>(h[0]), -1.0f, x[0]), __builtin_fmaf(static_cast<float>(h[1]), -1.0f, x[1])};
-        const half2v l = __builtin_convertvector(r, half2v);
-        hi[2 * i] = h[0], hi[2 * i + 1] = h[1];
-        lo[2 * i] = l[0], lo[2 * i + 1] = l[1];
+        h[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, half2v));
+        float2v r;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(h[i]), "v"(x[0]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(h[i]), "v"(x[1]));
+        l[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, half2v));
     }
+    hi = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
+    lo = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
 }
 
 // One block of TT tiles of 16 keys, K in the lane's registers (REGS) or as
@@ -349,7 +352,9 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
                                              const uint4 (*k_regs)[Block<T, HD>::kSteps], const uint8_t* k, const uint8_t* v,
                                              Running<HD, RT>& run) {
     using B = Block<T, HD>;
-    const uint32_t l = threadIdx.x % kWave, j = l % 16, g = l / 16;
+    // (from a fresh thread index, so that the addresses are not kept in
+    // registers from one block to the next)
+    const uint32_t l = thread_index() % kWave, j = l % 16, g = l / 16;
     const uint32_t k_at = j * B::kRow + 16 * (g ^ B::swizzle_k(j));
     f32x4 s[RT][TT];
 #pragma unroll
@@ -496,13 +501,17 @@ __device__ __forceinline__ float lanes_sum(float v) {  // over a row's four lane
     return __uint_as_float(l32.x) + __uint_as_float(l32.y);
 }
 
+// The token of row r < 128 of a tile: r / group, (r + 1/2) / group being at
+// least 1/256 from a whole number.
+__device__ __forceinline__ uint32_t token_of(const PagesArgs& a, uint32_t r) { return static_cast<uint32_t>((static_cast<float>(r) + 0.5f) * a.group_inverse); }
+
 template <typename T, int HD, int RT>
 __device__ __forceinline__ void load_rows(const PagesArgs& a, const Piece& p, uint32_t first_row, RawRow<T, HD> (&raw)[RT], Limits<RT>& lim) {
-    const uint32_t l = threadIdx.x % kWave, j = l % 16, g = l / 16, rows = p.tokens * a.group;
+    const uint32_t l = thread_index() % kWave, j = l % 16, g = l / 16, rows = p.tokens * a.group;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const uint32_t r = min(first_row + 16 * rt + j, rows - 1), t = r / a.group;
-        raw[rt].load(a.q + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r % a.group) * HD, g);
+        const uint32_t r = min(first_row + 16 * rt + j, rows - 1), t = token_of(a, r);
+        raw[rt].load(a.q + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r - t * a.group) * HD, g);
         lim.limit[rt] = p.causal ? p.limit0 + static_cast<int32_t>(t) : p.limit0;
     }
 }
@@ -511,8 +520,8 @@ __device__ __forceinline__ void load_rows(const PagesArgs& a, const Piece& p, ui
 template <int HD>
 __device__ __forceinline__ void store_row(const PagesArgs& a, const Piece& p, uint32_t r, uint32_t dim, f32x4 o, float m, float l) {
     if (p.whole) {
-        const uint32_t t = r / a.group;
-        float* to = a.out + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r % a.group) * HD + dim;
+        const uint32_t t = token_of(a, r);
+        float* to = a.out + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r - t * a.group) * HD + dim;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         stg(reinterpret_cast<float4*>(to), make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
     } else if (p.slot_row >= 0) {
@@ -526,7 +535,7 @@ template <typename T, int HD, bool CAP>
 __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buffer* buf) {
     using B = Block<T, HD>;
     constexpr int TT = B::kWaveTiles, N = TT;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave, j = l % 16, g = l / 16;
+    const uint32_t thread = thread_index(), w = __builtin_amdgcn_readfirstlane(thread / kWave), l = thread % kWave, j = l % 16, g = l / 16;
     Queries<T, HD, 1> q;
     Limits<1> lim{{p.limit0}, p.limit0};
     Running<HD, 1> run;
@@ -615,7 +624,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
         *reinterpret_cast<f32x4*>(part + (16 * w + j) * kStride + 16 * dt + 4 * g) = run.o[0][dt];
     if (g == 0) ml[16 * w + j] = make_float2(run.m[0], sum);
     lds_barrier();
-    const uint32_t r = threadIdx.x / 16;
+    const uint32_t r = thread / 16;
     if (r < p.tokens * a.group) {
         float m = kLowest, f[kWaves], lsum = 0.0f;
 #pragma unroll
@@ -627,7 +636,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
         }
 #pragma unroll
         for (uint32_t d = 0; d < HD / 64; ++d) {
-            const uint32_t dim = 64 * d + 4 * (threadIdx.x % 16);
+            const uint32_t dim = 64 * d + 4 * (thread % 16);
             f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (uint32_t i = 0; i < kWaves; ++i) {
@@ -646,7 +655,7 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
     using B = Block<T, HD>;
     constexpr int TT = B::kTiles, N = 4;
     constexpr int32_t kSpan = B::kKeys;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave, j = l % 16, g = l / 16;
+    const uint32_t thread = thread_index(), w = __builtin_amdgcn_readfirstlane(thread / kWave), l = thread % kWave, j = l % 16, g = l / 16;
     const uint32_t rows = p.tokens * a.group, first = 16 * RT * w;
     Queries<T, HD, RT> q;
     Limits<RT> lim;
@@ -654,15 +663,15 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
     run.clear();
     // The first of the 16 keys that the wave's i-th load is in.
     const auto part_of_load = [&](int i) { return static_cast<int32_t>((i * kThreads + w * kWave) / B::kPieces / 16 * 16); };
-    const auto issue = [&](const Pages<N>& at, uint8_t* k_all, uint8_t* v_all) {
+    const auto issue = [&](const Pages<N>& at, uint8_t* to) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t u = i * kThreads + threadIdx.x, row = u / B::kPieces, r = row % 16;
+            const uint32_t u = i * kThreads + thread, row = u / B::kPieces, r = row % 16;
             const Rows from = rows_at<B::kRow>(a, p.tile.kvh, at.keys, at.id[i], at.keys.key0 + part_of_load(i));
             const uint32_t k_offset = r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row));
             const uint32_t v_offset = r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row));
-            uint8_t* k_to = k_all + 16 * (i * kThreads + w * kWave);
-            uint8_t* v_to = v_all + 16 * (i * kThreads + w * kWave);
+            uint8_t* k_to = to + 16 * (i * kThreads + w * kWave);
+            uint8_t* v_to = k_to + sizeof buf[0].k;
             if (from.whole) {
                 load_to_lds16(from.k + k_offset, k_to);
                 load_to_lds16(from.v + v_offset, v_to);
@@ -685,33 +694,33 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
     // The wave's rows that are none of the tile's take no part; nor do blocks
     // past all that the wave's rows see.
     const int32_t last_row = static_cast<int32_t>(min(first + 16 * RT, rows)) - 1;
-    const int32_t wave_end = p.causal ? p.limit0 + last_row / static_cast<int32_t>(a.group) : p.limit0;
+    const int32_t wave_end = p.causal ? p.limit0 + static_cast<int32_t>(token_of(a, last_row)) : p.limit0;
     const bool idle = first >= rows, mixed = p.causal && p.tokens > 1;
-    lim.low = p.causal ? p.limit0 + static_cast<int32_t>(first / a.group) : p.limit0;
+    lim.low = p.causal ? p.limit0 + static_cast<int32_t>(token_of(a, first)) : p.limit0;
     bool unbounded = false;  // as in few_rows
-    const auto block = [&](uint8_t* __restrict__ k, uint8_t* __restrict__ v, uint8_t* __restrict__ k_next, uint8_t* __restrict__ v_next) {
+    const auto block = [&](uint8_t* __restrict__ here, uint8_t* __restrict__ there) {
         if (x == p.x0) {
             RawRow<T, HD> raw[RT];
             load_rows(a, p, first, raw, lim);
-            issue(cur, k, v);
+            issue(cur, here);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) q.take(rt, raw[rt], CAP ? a.scale : a.scale * kLog2e);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();  // every wave's loads have landed, and the other buffer is read no more
-        if (x + kSpan < p.x1) issue(nxt, k_next, v_next);
+        if (x + kSpan < p.x1) issue(nxt, there);
         const Pages<N> after = pages_at(x + 2 * kSpan);
         if (mixed && !cur.keys.lead && cur.keys.key0 + kSpan > p.limit0) {
-            unbounded |= clear_unbounded<T>(v, sizeof buf[0].v, threadIdx.x, kThreads);
+            unbounded |= clear_unbounded<T>(here + sizeof buf[0].k, sizeof buf[0].v, thread, kThreads);
             lds_barrier();
         }
         if (!idle && (cur.keys.lead || cur.keys.key0 < wave_end))
-            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, cur.dead, a.softcap, nullptr, k, v, run);
+            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, cur.dead, a.softcap, nullptr, here, here + sizeof buf[0].k, run);
         cur = nxt;
         nxt = after;
         x += kSpan;
     };
-    for (uint32_t n = 0; x < p.x1; n ^= 1) block(buf[n].k, buf[n].v, buf[n ^ 1].k, buf[n ^ 1].v);
+    for (uint32_t n = 0; x < p.x1; n ^= 1) block(buf[n].k, buf[n ^ 1].k);
     if (mixed && __syncthreads_or(unbounded)) {
         // the blocks that reach past the first limit
         for (int32_t at = p.x0; at < p.x1; at += kSpan) {
@@ -881,8 +890,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             Piece p;
             p.tile = {a.table + static_cast<uint64_t>(s.lead_row) * a.table_stride, a.table + static_cast<uint64_t>(s.row) * a.table_stride,
                       s.lead_span(), s.lead, s.lo, s.from, s.lo + keys - s.lead_span(), static_cast<uint32_t>(kvh)};
-            p.x0 = u0 > start ? cut(u0 - start, s.key_cost(), keys, B::kKeys) : 0;
-            p.x1 = u1 >= end ? keys : cut(u1 - start, s.key_cost(), keys, B::kKeys);
+            p.x0 = u0 > start ? cut(u0 - start, s.few, keys, B::kKeys) : 0;
+            p.x1 = u1 >= end ? keys : cut(u1 - start, s.few, keys, B::kKeys);
             p.token0 = s.token0 + t * s.step;
             p.tokens = s.tile_n(t);
             p.limit0 = s.limit(t * s.step);
@@ -1052,6 +1061,7 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     a.workgroups_log2 = workgroups_log2();
     a.scale = p->scale;
     a.softcap = p->softcap;
+    a.group_inverse = 1.0f / static_cast<float>(a.group);
     vkml::abi::ProfileScope prof("attend_pages");
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(1u << a.workgroups_log2), dim3(kThreads), 0, vkml::abi::stream(), a); };
     const bool wide = p->head_dim == 128;

@@ -114,6 +114,7 @@ struct Segment {
     VKML_HD int64_t tile_cost(int32_t i) const { return kOverhead + static_cast<int64_t>(key_cost()) * keys(i); }
     // The cost of the tiles before tile i.
     VKML_HD int64_t before(int32_t i) const {
+        if (i == 0) return 0;
         const int64_t k = i, each = kOverhead + static_cast<int64_t>(key_cost()) * (shared || base < 0 ? keys(0) : lead_span() + base);
         return shared || base < 0 ? k * each : k * each + key_cost() * (step * (k * (k + 1) / 2));
     }
@@ -193,11 +194,12 @@ VKML_HD int32_t part_of(int64_t cost, int32_t n_log2, int64_t u) {
 }
 // Keys of a tile of `keys` that units before x of it stand for: whole blocks
 // (but the last), so that every part cuts at the same places.
-VKML_HD int32_t cut(int64_t x, int32_t key_cost, int32_t keys, int32_t block) {
+VKML_HD int32_t cut(int64_t x, bool few, int32_t keys, int32_t block) {
     if (x <= kOverhead) return 0;
-    const int64_t k = (x - kOverhead) / key_cost;
+    const uint32_t cost = static_cast<uint32_t>(x - kOverhead);  // a tile's: at most kTileCost * (2^30 + kLeadStep)
+    const int32_t k = static_cast<int32_t>(few ? cost / kFewCost : cost / kTileCost);
     if (k >= keys) return keys;
-    const int32_t up = (static_cast<int32_t>(k) + block - 1) / block * block;
+    const int32_t up = (k + block - 1) / block * block;
     return up < keys ? up : keys;
 }
 
