@@ -46,8 +46,8 @@ extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int
                         if (n >= most) return -1;
                         int64_t* o = out + 10 * n++;
                         o[0] = w, o[1] = h, o[2] = i, o[3] = t;
-                        o[4] = u0 > at ? cut(u0 - at, s.few, s.keys(t), block) : 0;
-                        o[5] = u1 >= end ? s.keys(t) : cut(u1 - at, s.few, s.keys(t), block);
+                        o[4] = u0 > at ? cut(u0 - at, s.overhead(), s.keys(t), block) : 0;
+                        o[5] = u1 >= end ? s.keys(t) : cut(u1 - at, s.overhead(), s.keys(t), block);
                         o[6] = w + (s.few ? few : tiles + t);
                         o[7] = s.few;
                         o[8] = u0 <= at && u1 >= end;

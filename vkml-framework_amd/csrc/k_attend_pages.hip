@@ -30,8 +30,11 @@
 // rows of V. f16: every product is exact, q (scaled by a power of two a row to
 // [1, 2)) and the weights (times 2^14) split in two f16 terms, sums in f32.
 //
-// Rows of a block past the sequence's keys, below the first that counts or in
-// no page are read as zeros, so that what lies there, NaN included, has no part.
+// Rows of a block that hold no key that counts (past the sequence's keys, below
+// the first that counts, in no page) are read from where they would be, within
+// the pools; their scores are masked, and what is not finite in their V is
+// cleared in the LDS before the product. So are infinities and NaN of keys that
+// some rows see and others don't, which are added to those rows at the end.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -71,15 +74,12 @@ struct PagesArgs {
     float2* stats;  // [rows]: m, l
     float* o;       // [rows, hd]
     Batch batch;
-    uint64_t page_bytes;  // from a page to the next
+    uint32_t page_units;  // 16 bytes each, from a page to the next
     int64_t few_slots, tile_slots;
     uint32_t heads, kv_heads, group, page_shift, pages, table_stride;
     int32_t workgroups_log2;
     float scale, softcap, group_inverse;
 };
-
-// 16 bytes of zeros that the rows without a key are read from.
-__device__ const uint4 g_zeros = {0, 0, 0, 0};
 
 // The blocks: 16 KiB each of K and V for a workgroup, 8 KiB for a wave alone.
 template <typename T, int HD>
@@ -124,42 +124,77 @@ __device__ __forceinline__ Keys keys_at(const Tile& t, int32_t x) {
     const bool lead = x < t.span;
     return {lead ? t.lead_table : t.table, lead ? x : t.lo + x - t.span, lead ? 0 : t.from, lead ? t.lead : t.end, lead};
 }
-__device__ __forceinline__ int32_t page_id(const PagesArgs& a, const Keys& k, int32_t key) {
-    return key < k.end ? ld_scalar_i32(k.table + (key >> a.page_shift)) : -1;
-}
-
-// A block, its pages as a wave's N loads of it read them, 16 keys or less
-// each, and a bit for each of its 16-key tiles that is in no page.
-template <int N>
+// A block's keys and the pages that hold them: lane i has the page of the table
+// row's entry first + i, -1 past the keys. Neighbouring blocks share a window.
 struct Pages {
     Keys keys;
-    int32_t id[N];
-    uint32_t dead;
+    int32_t ids, first;
 };
-
-// 16 keys of a block: where their first row is, and whether all of them count.
-struct Rows {
-    const uint8_t* k;
-    const uint8_t* v;
-    bool whole;
-    int32_t first, last;  // the rows that count
-};
-template <uint32_t ROW>
-__device__ __forceinline__ Rows rows_at(const PagesArgs& a, uint32_t kvh, const Keys& k, int32_t id, int32_t key) {
-    const bool held = static_cast<uint32_t>(id) < a.pages;
-    const uint64_t at = static_cast<uint64_t>(held ? id : 0) * a.page_bytes +
-                        ((static_cast<uint64_t>(kvh) << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * ROW;
-    Rows r{a.k + at, a.v + at, false, held ? max(k.from - key, 0) : 16, min(k.end - key, 16)};
-    r.whole = r.first == 0 && r.last == 16;
-    return r;
+__device__ __forceinline__ void load_window(const PagesArgs& a, Pages& p) {
+    p.first = p.keys.key0 >> a.page_shift;
+    const int32_t i = p.first + static_cast<int32_t>(thread_index() % kWave);
+    p.ids = -1;
+    if (i < (p.keys.end + (1 << a.page_shift) - 1) >> a.page_shift) p.ids = ldg(p.keys.table + i);
 }
-
-// The bytes at `offset`, in row r of 16 rows, or zeros where the row holds no key.
-__device__ __forceinline__ const uint8_t* piece_at(const uint8_t* base, const Rows& rows, uint32_t r, uint32_t offset) {
-    return static_cast<int32_t>(r) >= rows.first && static_cast<int32_t>(r) < rows.last ? base + offset : reinterpret_cast<const uint8_t*>(&g_zeros);
+__device__ __forceinline__ Pages pages_at(const PagesArgs& a, const Tile& t, int32_t x) {
+    Pages p{keys_at(t, x), 0, 0};
+    load_window(a, p);
+    return p;
+}
+// The block at x, `span` keys, whose predecessor is p's.
+__device__ __forceinline__ Pages pages_after(const PagesArgs& a, const Tile& t, const Pages& p, int32_t x, int32_t span) {
+    Pages n{keys_at(t, x), p.ids, p.first};
+    if (n.keys.lead != p.keys.lead || ((n.keys.key0 + span - 1) >> a.page_shift) - n.first >= static_cast<int32_t>(kWave)) load_window(a, n);
+    return n;
+}
+__device__ __forceinline__ int32_t page_of(const PagesArgs& a, const Pages& p, int32_t key) {
+    return __builtin_amdgcn_readlane(p.ids, (key >> a.page_shift) - p.first);
+}
+// A bit for each of the block's 16-key tiles that is in no page.
+template <int TT>
+__device__ __forceinline__ uint32_t dead_tiles(const PagesArgs& a, const Pages& p) {
+    uint32_t dead = 0;
+#pragma unroll
+    for (int i = 0; i < TT; ++i) dead |= static_cast<uint32_t>(page_of(a, p, p.keys.key0 + 16 * i)) < a.pages ? 0u : 1u << i;
+    return dead;
+}
+// Where the 16 keys from `key` on of page id are (page 0's for none), from a
+// pool's first on.
+template <uint32_t ROW>
+__device__ __forceinline__ uint64_t offset_of(const PagesArgs& a, uint32_t kvh, int32_t id, int32_t key) {
+    const uint32_t held = static_cast<uint32_t>(id) < a.pages ? static_cast<uint32_t>(id) : 0u;
+    const uint32_t row = (kvh << a.page_shift) + (static_cast<uint32_t>(key) & ((1u << a.page_shift) - 1));
+    return (static_cast<uint64_t>(held) * a.page_units + row * (ROW / 16)) * 16;
+}
+// pool + offset, in scalar registers as one: the lanes' offsets are added by
+// the loads, not to the pool ahead of a loop, where their sums would take two
+// registers each.
+__device__ __forceinline__ const uint8_t* at_offset(const uint8_t* pool, uint64_t offset) {
+    uint64_t p = reinterpret_cast<uint64_t>(pool) + offset;
+    asm volatile("" : "+s"(p));
+    return reinterpret_cast<const uint8_t*>(p);
 }
 
 // ---------------------------------------------------------------- q
+
+// Eight f32 values as two f16 terms each, two at a time, the remainder by an
+// fma that widens the f16 term itself.
+__device__ __forceinline__ void split(f32x4 a, f32x4 b, half8& hi, half8& lo) {
+    typedef float float2v __attribute__((ext_vector_type(2)));
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2v x = i < 2 ? float2v{a[2 * i], a[2 * i + 1]} : float2v{b[2 * i - 4], b[2 * i - 3]};
+        h[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, half2v));
+        float2v r;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(h[i]), "v"(x[0]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(h[i]), "v"(x[1]));
+        l[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, half2v));
+    }
+    hi = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
+    lo = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
+}
 
 // RT tiles of 16 rows of q as the matrix instructions take them: lane (j, g)
 // has row j's pieces 4 s + g. c[rt]: what turns a product with them into a
@@ -195,19 +230,14 @@ struct Queries<_Float16, HD, RT> {
         most = fmaxf(__uint_as_float(r16.x), __uint_as_float(r16.y));
         const uint2 r32 = swap_rows<32>(__float_as_uint(most));
         most = fmaxf(__uint_as_float(r32.x), __uint_as_float(r32.y));
-        // The row's largest value to [1/2, 1): neither term leaves f16's range.
-        const int e2 = __builtin_amdgcn_frexp_expf(most);
-        const float sign = scale < 0.0f ? -1.0f : 1.0f;
+        // The row's largest value to [1/2, 1), by a power of two that f32 holds:
+        // neither term leaves f16's range.
+        const int e2 = max(__builtin_amdgcn_frexp_expf(most), -100);
+        const float f = __builtin_amdgcn_ldexpf(scale < 0.0f ? -1.0f : 1.0f, -e2);
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s) {
-            const float4 a = raw.x[2 * s], b = raw.x[2 * s + 1];
-            const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float z = __builtin_amdgcn_ldexpf(y[e] * sign, -e2);
-                hi[rt][s][e] = static_cast<_Float16>(z);
-                lo[rt][s][e] = static_cast<_Float16>(z - static_cast<float>(hi[rt][s][e]));
-            }
+            const float4 x = raw.x[2 * s], y = raw.x[2 * s + 1];
+            split(f32x4{x.x * f, x.y * f, x.z * f, x.w * f}, f32x4{y.x * f, y.y * f, y.z * f, y.w * f}, hi[rt][s], lo[rt][s]);
         }
         c[rt] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale), e2), __FLT_MIN__);
     }
@@ -270,17 +300,16 @@ struct Running {
 };
 
 // The rows' own limits: row j of tile rt sees positions below limit[rt], of
-// the lead all. low: the least of them.
+// the lead all.
 template <int RT>
 struct Limits {
     int32_t limit[RT];
-    int32_t low;
 };
 
-// Zeros for the infinities and NaN among a block's V values; whether there
-// were any among the thread's.
-template <typename T>
-__device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t bytes, uint32_t thread, uint32_t threads) {
+// Zeros for the infinities and NaN among a masked block's V values; whether
+// any of the thread's were those of keys that count.
+template <typename T, uint32_t ROW>
+__device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t bytes, uint32_t thread, uint32_t threads, const Keys& keys, uint32_t dead) {
     bool found = false;
 #pragma unroll 1
     for (uint32_t i = 16 * thread; i < bytes; i += 16 * threads) {
@@ -296,59 +325,17 @@ __device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t bytes, uint
             y[e] &= keep;
         }
         if (here) *reinterpret_cast<uint4*>(v + i) = make_uint4(y[0], y[1], y[2], y[3]);
-        found |= here;
+        const int32_t row = static_cast<int32_t>(i / ROW), key = keys.key0 + row;
+        found |= here && key >= keys.from && key < keys.end && !(dead >> (row / 16) & 1);
     }
     return found;
 }
 
-// The infinities and NaN of V at positions [k0, k1) for the rows that see
-// them: a row's output there is their sum, whatever its finite values are.
-template <typename T, int HD, int RT>
-__device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Tile& t, const Limits<RT>& lim, int32_t k0, int32_t k1, Running<HD, RT>& run) {
-    const uint32_t g = thread_index() % kWave / 16;
-    const Keys keys{t.table, 0, t.from, t.end, false};
-#pragma unroll 1
-    for (int32_t key = k0; key < k1; ++key) {
-        const int32_t id = page_id(a, keys, key);
-        if (static_cast<uint32_t>(id) >= a.pages || key < t.from) continue;
-        const Rows at = rows_at<Block<T, HD>::kRow>(a, t.kvh, keys, id, key);
-        const T* row = reinterpret_cast<const T*>(at.v) + 4 * g;
-#pragma unroll
-        for (int dt = 0; dt < HD / 16; ++dt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = static_cast<float>(row[16 * dt + e]);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    if (key < lim.limit[rt] && !(fabsf(x) <= __FLT_MAX__)) run.o[rt][dt][e] += x;
-            }
-    }
-}
-
-// Eight f32 values as two f16 terms each, two at a time, the remainder by an
-// fma that widens the f16 term itself.
-__device__ __forceinline__ void split(f32x4 a, f32x4 b, half8& hi, half8& lo) {
-    typedef float float2v __attribute__((ext_vector_type(2)));
-    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2v x = i < 2 ? float2v{a[2 * i], a[2 * i + 1]} : float2v{b[2 * i - 4], b[2 * i - 3]};
-        h[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, half2v));
-        float2v r;
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(h[i]), "v"(x[0]));
-        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(h[i]), "v"(x[1]));
-        l[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, half2v));
-    }
-    hi = __builtin_bit_cast(half8, make_uint4(h[0], h[1], h[2], h[3]));
-    lo = __builtin_bit_cast(half8, make_uint4(l[0], l[1], l[2], l[3]));
-}
-
 // One block of TT tiles of 16 keys, K in the lane's registers (REGS) or as
-// swizzled rows in the LDS, V's rows in the LDS. dead: a bit for each tile
-// that is in no page.
+// swizzled rows in the LDS, V's rows in the LDS. masked: some rows don't see
+// all of its keys. dead: a bit for each tile that is in no page.
 template <typename T, int HD, int RT, int TT, bool REGS, bool CAP>
-__device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const Limits<RT>& lim, const Keys& keys, uint32_t dead, float softcap,
+__device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const Limits<RT>& lim, const Keys& keys, bool masked, uint32_t dead, float softcap,
                                              const uint4 (*k_regs)[Block<T, HD>::kSteps], const uint8_t* k, const uint8_t* v,
                                              Running<HD, RT>& run) {
     using B = Block<T, HD>;
@@ -371,7 +358,6 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         }
         q.score(st, kk, s);
     }
-    const bool masked = keys.key0 < keys.from || keys.key0 + 16 * TT > (keys.lead ? keys.end : lim.low) || dead;
     constexpr float kShift = B::kF16 ? 14.0f : 0.0f;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -474,6 +460,12 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
 
 // ---------------------------------------------------------------- pieces
 
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int32_t>(x >> 32)))) << 32 |
+                                static_cast<uint32_t>(uniform(static_cast<int32_t>(x))));
+}
+
 // A piece of a tile: [x0, x1) of its keys' axis, rows from token0 on.
 struct Piece {
     Tile tile;
@@ -530,58 +522,79 @@ __device__ __forceinline__ void store_row(const PagesArgs& a, const Piece& p, ui
     }
 }
 
+// Whether some of a tile's rows don't see all of a block of `span` keys.
+__device__ __forceinline__ bool is_masked(const Piece& p, const Keys& keys, int32_t span, uint32_t dead) {
+    return keys.key0 < keys.from || keys.key0 + span > (keys.lead ? keys.end : p.limit0) || dead;
+}
+
+// The infinities and NaN of V in a piece's masked blocks, which the products
+// have left out, for the rows that see them, where the workgroup has stored
+// those: a row's value there is their sum, whatever the finite ones are.
+template <typename T, int HD>
+__device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Piece& p) {
+    using B = Block<T, HD>;
+    if (!p.whole && p.slot_row < 0) return;
+    const uint32_t thread = thread_index(), dim = thread % HD, rows = p.tokens * a.group;
+    __syncthreads();  // the rows are stored
+    for (int32_t x = p.x0; x < p.x1; x += B::kKeys) {
+        const Pages at = pages_at(a, p.tile, x);
+        if (!is_masked(p, at.keys, B::kKeys, dead_tiles<B::kTiles>(a, at))) continue;
+#pragma unroll 1
+        for (int32_t key = max(at.keys.key0, at.keys.from); key < min(at.keys.key0 + static_cast<int32_t>(B::kKeys), at.keys.end); ++key) {
+            const int32_t id = ld_scalar_i32(at.keys.table + (key >> a.page_shift));
+            if (static_cast<uint32_t>(id) >= a.pages) continue;
+            const float v = static_cast<float>(reinterpret_cast<const T*>(a.v + offset_of<B::kRow>(a, p.tile.kvh, id, key))[dim]);
+            if (fabsf(v) <= __FLT_MAX__) continue;
+#pragma unroll 1
+            for (uint32_t r = thread / HD; r < rows; r += kThreads / HD) {
+                const uint32_t t = token_of(a, r);
+                if (!at.keys.lead && p.causal && key >= p.limit0 + static_cast<int32_t>(t)) continue;
+                float* to = p.whole ? a.out + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r - t * a.group) * HD + dim
+                                    : a.o + (p.slot_row + r) * HD + dim;
+                stg(to, ldg(to) + v);
+            }
+        }
+    }
+}
+
 // At most 16 rows: each wave by itself over blocks of kWaveKeys keys in turn.
 template <typename T, int HD, bool CAP>
 __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buffer* buf) {
     using B = Block<T, HD>;
-    constexpr int TT = B::kWaveTiles, N = TT;
+    constexpr int TT = B::kWaveTiles;
     const uint32_t thread = thread_index(), w = __builtin_amdgcn_readfirstlane(thread / kWave), l = thread % kWave, j = l % 16, g = l / 16;
     Queries<T, HD, 1> q;
-    Limits<1> lim{{p.limit0}, p.limit0};
+    Limits<1> lim{{p.limit0}};
     Running<HD, 1> run;
     run.clear();
     uint8_t* v = reinterpret_cast<uint8_t*>(buf) + 8192 * w;  // and as far into the second buffer
     constexpr int32_t kStep = kWaves * B::kWaveKeys, kSpan = B::kWaveKeys;
     const int32_t first = p.x0 + static_cast<int32_t>(w) * kSpan;
     int32_t x = first;
-    const auto issue = [&](const Pages<N>& at, uint4 (&k)[TT][B::kSteps], uint8_t* to) {
-        Rows rows[N];
-        bool whole = true;
+    const auto issue = [&](const Pages& at, uint4 (&k)[TT][B::kSteps], uint8_t* to) {
+        const uint8_t *k_part[TT], *v_part[TT];
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            rows[i] = rows_at<B::kRow>(a, p.tile.kvh, at.keys, at.id[i], at.keys.key0 + 16 * i);
-            whole &= rows[i].whole;
+        for (int i = 0; i < TT; ++i) {
+            const int32_t key = at.keys.key0 + 16 * i;
+            const uint64_t part = offset_of<B::kRow>(a, p.tile.kvh, page_of(a, at, key), key);
+            k_part[i] = at_offset(a.k, part);
+            v_part[i] = at_offset(a.v, part);
         }
-        const auto loads = [&](auto piece) {
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
+        for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
-                for (int s = 0; s < static_cast<int>(B::kSteps); ++s)
-                    k[tt][s] = ldg(reinterpret_cast<const uint4*>(piece(rows[tt].k, rows[tt], j, j * B::kRow + 64 * s + 16 * g)));
+            for (int s = 0; s < static_cast<int>(B::kSteps); ++s)
+                k[tt][s] = ldg(reinterpret_cast<const uint4*>(k_part[tt] + (j * B::kRow + 64 * s + 16 * g)));
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const uint32_t u = 64 * i + l, row = u / B::kPieces, r = row % 16;
-                const Rows& from = rows[64 * i / B::kPieces / 16];
-                load_to_lds16(piece(from.v, from, r, r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row))), to + 1024 * i);
-            }
-        };
-        if (whole) loads([](const uint8_t* base, const Rows&, uint32_t, uint32_t offset) { return base + offset; });
-        else loads(piece_at);
-    };
-    const auto pages_at = [&](int32_t at) {
-        Pages<N> r{keys_at(p.tile, at), {}, 0};
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            r.id[i] = page_id(a, r.keys, r.keys.key0 + 16 * i);
-            r.dead |= static_cast<uint32_t>(r.id[i]) < a.pages ? 0u : 1u << i;
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t u = 64 * i + l, row = u / B::kPieces;
+            load_to_lds16(v_part[64 * i / B::kPieces / 16] + (row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row))), to + 1024 * i);
         }
-        return r;
     };
     uint4 k[TT][B::kSteps];
-    Pages<N> cur = pages_at(x), nxt = pages_at(x + kStep);
-    // Values that are not finite in blocks that some rows see less of than
+    Pages cur = pages_at(a, p.tile, x), nxt = cur;
+    // Values of V that are not finite in blocks that some rows see less of than
     // others are left out of the product and added at the end.
-    const bool mixed = p.causal && p.tokens > 1;
     bool unbounded = false;
     // The buffers don't overlap. Said so (__restrict__), and with both's loads
     // issued in here, the reads of one do not wait for the loads into the other.
@@ -590,14 +603,17 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             RawRow<T, HD> raw[1];
             load_rows(a, p, 0, raw, lim);
             issue(cur, k, here);
+            nxt = pages_after(a, p.tile, cur, x + kStep, kSpan);
             q.take(0, raw[0], CAP ? a.scale : a.scale * kLog2e);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this block has landed
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this block and the next one's pages have landed
         uint4 k_next[TT][B::kSteps] = {};
+        const uint32_t dead = dead_tiles<TT>(a, cur);
         if (x + kStep < p.x1) issue(nxt, k_next, there);
-        const Pages<N> after = pages_at(x + 2 * kStep);
-        if (mixed && !cur.keys.lead && cur.keys.key0 + kSpan > lim.low) unbounded |= clear_unbounded<T>(here, 8192, l, kWave);
-        attend_block<T, HD, 1, TT, true, CAP>(q, lim, cur.keys, cur.dead, a.softcap, k, nullptr, here, run);
+        const Pages after = pages_after(a, p.tile, nxt, x + 2 * kStep, kSpan);
+        const bool masked = is_masked(p, cur.keys, kSpan, dead);
+        if (masked) unbounded |= clear_unbounded<T, B::kRow>(here, 8192, l, kWave, cur.keys, dead);
+        attend_block<T, HD, 1, TT, true, CAP>(q, lim, cur.keys, masked, dead, a.softcap, k, nullptr, here, run);
         cur = nxt;
         nxt = after;
         x += kStep;
@@ -607,22 +623,19 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             for (int s = 0; s < static_cast<int>(B::kSteps); ++s) k[tt][s] = k_next[tt][s];
     };
     for (uint32_t n = 0; x < p.x1; n ^= sizeof(Buffer)) block(v + n, v + (n ^ sizeof(Buffer)));
-    if (__any(unbounded)) {
-        for (int32_t at = first; at < p.x1; at += kStep) {
-            const Keys keys = keys_at(p.tile, at);
-            if (!keys.lead && keys.key0 + kSpan > lim.low) add_unbounded<T, HD, 1>(a, p.tile, lim, keys.key0, min(keys.key0 + kSpan, p.tile.end), run);
-        }
-    }
     // The waves' parts join in the LDS, rows HD + 4 floats apart.
     const float sum = lanes_sum(run.l[0]);
     constexpr uint32_t kStride = HD + 4;
     float* part = reinterpret_cast<float*>(buf);  // [waves][16][kStride], then [waves][16] of (m, l)
     float2* ml = reinterpret_cast<float2*>(part + kWaves * 16 * kStride);
+    uint32_t* found = reinterpret_cast<uint32_t*>(ml + kWaves * 16);  // [waves]
+    const bool mine = __any(unbounded);
     lds_barrier();
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt)
         *reinterpret_cast<f32x4*>(part + (16 * w + j) * kStride + 16 * dt + 4 * g) = run.o[0][dt];
     if (g == 0) ml[16 * w + j] = make_float2(run.m[0], sum);
+    if (l == 0) found[w] = mine;
     lds_barrier();
     const uint32_t r = thread / 16;
     if (r < p.tokens * a.group) {
@@ -647,13 +660,14 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             store_row<HD>(a, p, r, dim, o, m, lsum);
         }
     }
+    if (uniform(static_cast<int32_t>(found[0] | found[1] | found[2] | found[3]))) add_unbounded<T, HD>(a, p);
 }
 
 // Many rows: RT tiles of 16 a wave, the blocks shared.
 template <typename T, int HD, int RT, bool CAP>
 __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Buffer* buf) {
     using B = Block<T, HD>;
-    constexpr int TT = B::kTiles, N = 4;
+    constexpr int TT = B::kTiles;
     constexpr int32_t kSpan = B::kKeys;
     const uint32_t thread = thread_index(), w = __builtin_amdgcn_readfirstlane(thread / kWave), l = thread % kWave, j = l % 16, g = l / 16;
     const uint32_t rows = p.tokens * a.group, first = 16 * RT * w;
@@ -661,73 +675,53 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
     Limits<RT> lim;
     Running<HD, RT> run;
     run.clear();
-    // The first of the 16 keys that the wave's i-th load is in.
-    const auto part_of_load = [&](int i) { return static_cast<int32_t>((i * kThreads + w * kWave) / B::kPieces / 16 * 16); };
-    const auto issue = [&](const Pages<N>& at, uint8_t* to) {
+    const auto issue = [&](const Pages& at, uint8_t* to) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t u = i * kThreads + thread, row = u / B::kPieces, r = row % 16;
-            const Rows from = rows_at<B::kRow>(a, p.tile.kvh, at.keys, at.id[i], at.keys.key0 + part_of_load(i));
-            const uint32_t k_offset = r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row));
-            const uint32_t v_offset = r * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row));
+            const uint32_t u = i * kThreads + thread, row = u / B::kPieces;
+            // the first of the 16 keys that the wave's i-th load is in
+            const int32_t key = at.keys.key0 + static_cast<int32_t>((i * kThreads + w * kWave) / B::kPieces / 16 * 16);
+            const uint64_t part = offset_of<B::kRow>(a, p.tile.kvh, page_of(a, at, key), key);
             uint8_t* k_to = to + 16 * (i * kThreads + w * kWave);
-            uint8_t* v_to = k_to + sizeof buf[0].k;
-            if (from.whole) {
-                load_to_lds16(from.k + k_offset, k_to);
-                load_to_lds16(from.v + v_offset, v_to);
-            } else {
-                load_to_lds16(piece_at(from.k, from, r, k_offset), k_to);
-                load_to_lds16(piece_at(from.v, from, r, v_offset), v_to);
-            }
+            load_to_lds16(at_offset(a.k, part) + (row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row))), k_to);
+            load_to_lds16(at_offset(a.v, part) + (row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row))), k_to + sizeof buf[0].k);
         }
     };
-    const auto pages_at = [&](int32_t at) {
-        Pages<N> r{keys_at(p.tile, at), {}, 0};
-#pragma unroll
-        for (int i = 0; i < N; ++i) r.id[i] = page_id(a, r.keys, r.keys.key0 + part_of_load(i));
-#pragma unroll
-        for (int i = 0; i < TT; ++i) r.dead |= static_cast<uint32_t>(page_id(a, r.keys, r.keys.key0 + 16 * i)) < a.pages ? 0u : 1u << i;
-        return r;
-    };
     int32_t x = p.x0;
-    Pages<N> cur = pages_at(x), nxt = pages_at(x + kSpan);
+    Pages cur = pages_at(a, p.tile, x), nxt = cur;
     // The wave's rows that are none of the tile's take no part; nor do blocks
     // past all that the wave's rows see.
     const int32_t last_row = static_cast<int32_t>(min(first + 16 * RT, rows)) - 1;
     const int32_t wave_end = p.causal ? p.limit0 + static_cast<int32_t>(token_of(a, last_row)) : p.limit0;
-    const bool idle = first >= rows, mixed = p.causal && p.tokens > 1;
-    lim.low = p.causal ? p.limit0 + static_cast<int32_t>(token_of(a, first)) : p.limit0;
+    const bool idle = first >= rows;
     bool unbounded = false;  // as in few_rows
     const auto block = [&](uint8_t* __restrict__ here, uint8_t* __restrict__ there) {
         if (x == p.x0) {
             RawRow<T, HD> raw[RT];
             load_rows(a, p, first, raw, lim);
             issue(cur, here);
+            nxt = pages_after(a, p.tile, cur, x + kSpan, kSpan);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) q.take(rt, raw[rt], CAP ? a.scale : a.scale * kLog2e);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         lds_barrier();  // every wave's loads have landed, and the other buffer is read no more
+        const uint32_t dead = dead_tiles<TT>(a, cur);
         if (x + kSpan < p.x1) issue(nxt, there);
-        const Pages<N> after = pages_at(x + 2 * kSpan);
-        if (mixed && !cur.keys.lead && cur.keys.key0 + kSpan > p.limit0) {
-            unbounded |= clear_unbounded<T>(here + sizeof buf[0].k, sizeof buf[0].v, thread, kThreads);
+        const Pages after = pages_after(a, p.tile, nxt, x + 2 * kSpan, kSpan);
+        const bool masked = is_masked(p, cur.keys, kSpan, dead);
+        if (masked) {
+            unbounded |= clear_unbounded<T, B::kRow>(here + sizeof buf[0].k, sizeof buf[0].v, thread, kThreads, cur.keys, dead);
             lds_barrier();
         }
         if (!idle && (cur.keys.lead || cur.keys.key0 < wave_end))
-            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, cur.dead, a.softcap, nullptr, here, here + sizeof buf[0].k, run);
+            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, masked, dead, a.softcap, nullptr, here, here + sizeof buf[0].k, run);
         cur = nxt;
         nxt = after;
         x += kSpan;
     };
     for (uint32_t n = 0; x < p.x1; n ^= 1) block(buf[n].k, buf[n ^ 1].k);
-    if (mixed && __syncthreads_or(unbounded)) {
-        // the blocks that reach past the first limit
-        for (int32_t at = p.x0; at < p.x1; at += kSpan) {
-            const Keys keys = keys_at(p.tile, at);
-            if (!keys.lead && keys.key0 + kSpan > p.limit0) add_unbounded<T, HD, RT>(a, p.tile, lim, keys.key0, min(keys.key0 + kSpan, p.tile.end), run);
-        }
-    }
+    const bool found = __syncthreads_or(unbounded);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float sum = lanes_sum(run.l[rt]);
@@ -737,15 +731,10 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
             for (int dt = 0; dt < HD / 16; ++dt) store_row<HD>(a, p, r, 16 * dt + 4 * g, run.o[rt][dt], run.m[rt], sum);
         }
     }
+    if (found) add_unbounded<T, HD>(a, p);
 }
 
 // ---------------------------------------------------------------- the launch
-
-__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int32_t>(x >> 32)))) << 32 |
-                                static_cast<uint32_t>(uniform(static_cast<int32_t>(x))));
-}
 
 // v of lane i - n (DPP's row shifts and broadcasts), 0 where there is none:
 // the steps of an inclusive sum over the wave.
@@ -890,8 +879,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             Piece p;
             p.tile = {a.table + static_cast<uint64_t>(s.lead_row) * a.table_stride, a.table + static_cast<uint64_t>(s.row) * a.table_stride,
                       s.lead_span(), s.lead, s.lo, s.from, s.lo + keys - s.lead_span(), static_cast<uint32_t>(kvh)};
-            p.x0 = u0 > start ? cut(u0 - start, s.few, keys, B::kKeys) : 0;
-            p.x1 = u1 >= end ? keys : cut(u1 - start, s.few, keys, B::kKeys);
+            p.x0 = u0 > start ? cut(u0 - start, s.overhead(), keys, B::kKeys) : 0;
+            p.x1 = u1 >= end ? keys : cut(u1 - start, s.overhead(), keys, B::kKeys);
             p.token0 = s.token0 + t * s.step;
             p.tokens = s.tile_n(t);
             p.limit0 = s.limit(t * s.step);
@@ -1049,7 +1038,7 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     a.stats = reinterpret_cast<float2*>(at);
     a.o = reinterpret_cast<float*>(at + up16(s.rows() * sizeof(float2)));
     a.batch = batch;
-    a.page_bytes = stride * (p->kv_type == VKML_F16 ? 2 : 4);
+    a.page_units = static_cast<uint32_t>(stride * (p->kv_type == VKML_F16 ? 2 : 4) / 16);
     a.few_slots = s.few;
     a.tile_slots = s.tile;
     a.heads = p->heads;

@@ -72,15 +72,16 @@ struct Batch {
 // all of its tokens, then for each sequence its other keys by its tokens. A
 // segment's tokens go in tiles: all of them where they are at most kFewRows
 // rows (token, query head), else kTileRows / (query heads a KV head) at a time.
-// A tile costs the keys it reads and kOverhead more (its queries, its joining
-// and storing), and the whole of all KV heads' tiles, laid end to end, is cut
+// A tile costs the keys it reads and, for its queries, its first loads, its
+// joining and storing, as much as so many keys more; the whole of all KV heads' tiles, laid end to end, is cut
 // into equal parts, one a workgroup: what a workgroup takes of a tile is a
 // piece.
 constexpr int32_t kFewRows = 16;
 constexpr int32_t kTileRows = 128;
-// What a key costs a tile of few rows, and another, and a tile by itself.
-constexpr int32_t kFewCost = 2, kTileCost = 3, kOverhead = 128;
-constexpr int32_t kMinPart = 256;  // the cost below which work is not cut further
+// Measured (us): 64 keys of a tile of few rows 3.7, of another 3.3 (two
+// workgroups a compute unit, the first bound by memory); a piece by itself 5 and 7.
+constexpr int32_t kFewOverhead = 96, kTileOverhead = 128;
+constexpr int32_t kMinPart = 128;  // the cost below which work is not cut further
 constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
 
 VKML_HD int32_t tile_tokens(int32_t group) { return kTileRows / group > 1 ? kTileRows / group : 1; }
@@ -110,13 +111,13 @@ struct Segment {
         }
         return lead_span() + own;
     }
-    VKML_HD int32_t key_cost() const { return few ? kFewCost : kTileCost; }
-    VKML_HD int64_t tile_cost(int32_t i) const { return kOverhead + static_cast<int64_t>(key_cost()) * keys(i); }
+    VKML_HD int32_t overhead() const { return few ? kFewOverhead : kTileOverhead; }
+    VKML_HD int64_t tile_cost(int32_t i) const { return overhead() + keys(i); }
     // The cost of the tiles before tile i.
     VKML_HD int64_t before(int32_t i) const {
         if (i == 0) return 0;
-        const int64_t k = i, each = kOverhead + static_cast<int64_t>(key_cost()) * (shared || base < 0 ? keys(0) : lead_span() + base);
-        return shared || base < 0 ? k * each : k * each + key_cost() * (step * (k * (k + 1) / 2));
+        const int64_t k = i, each = overhead() + (shared || base < 0 ? keys(0) : lead_span() + base);
+        return shared || base < 0 ? k * each : k * each + step * (k * (k + 1) / 2);
     }
     VKML_HD int64_t cost() const { return tiles ? before(tiles - 1) + tile_cost(tiles - 1) : 0; }
     // The tile that holds unit u of the segment, 0 <= u < cost().
@@ -194,10 +195,9 @@ VKML_HD int32_t part_of(int64_t cost, int32_t n_log2, int64_t u) {
 }
 // Keys of a tile of `keys` that units before x of it stand for: whole blocks
 // (but the last), so that every part cuts at the same places.
-VKML_HD int32_t cut(int64_t x, bool few, int32_t keys, int32_t block) {
-    if (x <= kOverhead) return 0;
-    const uint32_t cost = static_cast<uint32_t>(x - kOverhead);  // a tile's: at most kTileCost * (2^30 + kLeadStep)
-    const int32_t k = static_cast<int32_t>(few ? cost / kFewCost : cost / kTileCost);
+VKML_HD int32_t cut(int64_t x, int32_t overhead, int32_t keys, int32_t block) {
+    if (x <= overhead) return 0;
+    const int32_t k = static_cast<int32_t>(x) - overhead;
     if (k >= keys) return keys;
     const int32_t up = (k + block - 1) / block * block;
     return up < keys ? up : keys;
@@ -226,6 +226,7 @@ inline const char* check_cache(uint32_t kv_heads, uint32_t head_dim, uint32_t kv
     if (pages == 0 || pages > 0x7FFFFFFFu) return "the pools must hold 1 to 2^31 - 1 pages";
     if (page_stride && page_stride < static_cast<uint64_t>(kv_heads) * page_size * head_dim) return "pages overlap";
     if (page_stride % 8) return "page_stride must be a multiple of 8";
+    if (page_stride > (1ull << 33) || static_cast<uint64_t>(kv_heads) * page_size * head_dim > (1ull << 33)) return "pages are too large";
     return nullptr;
 }
 
