@@ -719,7 +719,7 @@ typedef struct vkml_attend_pages_params {
     uint32_t pages;
     uint32_t seqs;         /* at most 65536 */
     uint32_t tokens;
-    uint32_t table_stride; /* table entries a sequence: at most 2^30 keys */
+    uint32_t table_stride; /* table entries a sequence: at most 2^26 keys */
     uint32_t groups;
     uint64_t page_stride;
     float scale;

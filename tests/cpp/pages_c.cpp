@@ -14,22 +14,23 @@ extern "C" const char* check_copies_c(uint32_t pages, uint32_t count, const int3
 // out [seqs, 5]: first row, rows, length, group, shared keys
 extern "C" void batch_c(const Batch* b, int32_t* out) {
     for (int32_t s = 0; s < b->seqs; ++s) {
-        const int32_t g = b->group_of(s);
+        const int32_t g = b->groups > 0 && b->group_start(b->group_near(s)) <= s && s < b->group_start(b->group_near(s) + 1) ? b->group_near(s) : -1;
         out[5 * s] = b->start(s);
         out[5 * s + 1] = b->count(s);
         out[5 * s + 2] = b->length(s);
         out[5 * s + 3] = g;
-        out[5 * s + 4] = g < 0 ? 0 : b->group_shared(g);
+        out[5 * s + 4] = g < 0 ? 0 : b->group_start(g + 1) - b->group_start(g) > 1 ? b->group_key(g) : 0;
     }
 }
 
 // The whole work of a call as its workgroups cut it, a piece a row: workgroup,
 // KV head, segment, tile, first key, last key + 1, slot, few, whole, pieces of
 // the tile (as its first piece says). Returns the number of pieces.
-extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int32_t workgroups_log2, int32_t block, int64_t* out, int64_t most) {
+extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int32_t head_dim, int32_t f16, int32_t workgroups_log2, int32_t block, int64_t* out, int64_t most) {
     const int32_t segments = b->groups + b->seqs;
+    const Costs cost_of = costs(head_dim, f16 != 0);
     int64_t per_head = 0, n = 0;
-    for (int32_t i = 0; i < segments; ++i) per_head += segment(*b, group, i).cost();
+    for (int32_t i = 0; i < segments; ++i) per_head += segment(*b, group, cost_of, i).cost();
     const int64_t cost = per_head * kv_heads;
     if (cost == 0) return 0;
     const int32_t w_log2 = parts_log2(cost, workgroups_log2);
@@ -38,7 +39,7 @@ extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int
         int64_t off = 0, few = 0, tiles = 0;
         for (int32_t h = 0; h < kv_heads; ++h)
             for (int32_t i = 0; i < segments; ++i) {
-                const Segment s = segment(*b, group, i);
+                const Segment s = segment(*b, group, cost_of, i);
                 if (off + s.cost() > u0 && off < u1 && s.tiles) {
                     for (int32_t t = u0 > off ? s.tile_at(u0 - off) : 0; t < s.tiles; ++t) {
                         const int64_t at = off + s.before(t), end = at + s.tile_cost(t);
@@ -46,8 +47,8 @@ extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int
                         if (n >= most) return -1;
                         int64_t* o = out + 10 * n++;
                         o[0] = w, o[1] = h, o[2] = i, o[3] = t;
-                        o[4] = u0 > at ? cut(u0 - at, s.overhead(), s.keys(t), block) : 0;
-                        o[5] = u1 >= end ? s.keys(t) : cut(u1 - at, s.overhead(), s.keys(t), block);
+                        o[4] = u0 > at ? cut(static_cast<int32_t>(u0 - at), s, s.keys(t), block) : 0;
+                        o[5] = u1 >= end ? s.keys(t) : cut(static_cast<int32_t>(u1 - at), s, s.keys(t), block);
                         o[6] = w + (s.few ? few : tiles + t);
                         o[7] = s.few;
                         o[8] = u0 <= at && u1 >= end;
@@ -73,8 +74,8 @@ extern "C" void slots_c(int64_t kv_heads, int64_t group, int64_t seqs, int64_t g
 }
 // A segment's token0, n, lo, from, keys of its last tile, tiles, step, row, shared, lead, lead_row, lead_span
 extern "C" void segment_c(const Batch* b, int32_t group, int32_t i, int32_t* out) {
-    const Segment s = segment(*b, group, i);
-    const int32_t v[] = {s.token0, s.n, s.lo, s.from, s.tiles ? s.keys(s.tiles - 1) : 0, s.tiles, s.step, s.row, s.shared, s.lead, s.lead_row, s.lead_span()};
+    const Segment s = segment(*b, group, costs(128, true), i);
+    const int32_t v[] = {s.token0, s.n, s.lo(), s.from, s.tiles ? s.keys(s.tiles - 1) : 0, s.tiles, s.step, s.row, s.shared, s.lead, s.lead_row, s.lead_span()};
     for (int k = 0; k < 12; ++k) out[k] = v[k];
 }
-extern "C" int32_t limit_c(const Batch* b, int32_t group, int32_t i, int32_t token) { return segment(*b, group, i).limit(token); }
+extern "C" int32_t limit_c(const Batch* b, int32_t group, int32_t i, int32_t token) { return segment(*b, group, costs(128, true), i).limit(token); }

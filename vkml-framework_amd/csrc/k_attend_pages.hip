@@ -79,6 +79,7 @@ struct PagesArgs {
     uint32_t heads, kv_heads, group, page_shift, pages, table_stride;
     int32_t workgroups_log2;
     float scale, softcap, group_inverse;
+    Costs costs;
 };
 
 // The blocks: 16 KiB each of K and V for a workgroup, 8 KiB for a wave alone.
@@ -508,18 +509,20 @@ __device__ __forceinline__ void load_rows(const PagesArgs& a, const Piece& p, ui
     }
 }
 
-// dims of a row, 4 a lane, to the output or the workspace
+// Where row r of a piece goes, and what its values are multiplied by there: the
+// output, divided by the sum of weights l, or the workspace, with (m, l) beside
+// it. null: nowhere.
 template <int HD>
-__device__ __forceinline__ void store_row(const PagesArgs& a, const Piece& p, uint32_t r, uint32_t dim, f32x4 o, float m, float l) {
+__device__ __forceinline__ float* row_to(const PagesArgs& a, const Piece& p, uint32_t r, bool first_lane, float m, float l, float& times) {
     if (p.whole) {
         const uint32_t t = token_of(a, r);
-        float* to = a.out + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r - t * a.group) * HD + dim;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        stg(reinterpret_cast<float4*>(to), make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv));
-    } else if (p.slot_row >= 0) {
-        stg(reinterpret_cast<float4*>(a.o + (p.slot_row + r) * HD + dim), make_float4(o[0], o[1], o[2], o[3]));
-        if (dim == 0) stg(a.stats + p.slot_row + r, make_float2(m, l));
+        times = l == 0.0f ? 0.0f : 1.0f / l;
+        return a.out + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r - t * a.group) * HD;
     }
+    times = 1.0f;
+    if (p.slot_row < 0) return nullptr;
+    if (first_lane) stg(a.stats + p.slot_row + r, make_float2(m, l));
+    return a.o + (p.slot_row + r) * HD;
 }
 
 // Whether some of a tile's rows don't see all of a block of `span` keys.
@@ -647,6 +650,8 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             f[i] = __builtin_amdgcn_exp2f(ml[16 * i + r].x - m);
             lsum += f[i] * ml[16 * i + r].y;
         }
+        float times;
+        float* to = row_to<HD>(a, p, r, thread % 16 == 0, m, lsum, times);
 #pragma unroll
         for (uint32_t d = 0; d < HD / 64; ++d) {
             const uint32_t dim = 64 * d + 4 * (thread % 16);
@@ -657,7 +662,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] += f[i] * y[e];
             }
-            store_row<HD>(a, p, r, dim, o, m, lsum);
+            if (to) stg(reinterpret_cast<float4*>(to + dim), make_float4(o[0] * times, o[1] * times, o[2] * times, o[3] * times));
         }
     }
     if (uniform(static_cast<int32_t>(found[0] | found[1] | found[2] | found[3]))) add_unbounded<T, HD>(a, p);
@@ -727,8 +732,15 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
         const float sum = lanes_sum(run.l[rt]);
         const uint32_t r = first + 16 * rt + j;
         if (r < rows) {
+            float times;
+            float* to = row_to<HD>(a, p, r, g == 0, run.m[rt], sum, times);
+            if (to) {
 #pragma unroll
-            for (int dt = 0; dt < HD / 16; ++dt) store_row<HD>(a, p, r, 16 * dt + 4 * g, run.o[rt][dt], run.m[rt], sum);
+                for (int dt = 0; dt < HD / 16; ++dt) {
+                    const f32x4 o = run.o[rt][dt];
+                    stg(reinterpret_cast<float4*>(to + 16 * dt + 4 * g), make_float4(o[0] * times, o[1] * times, o[2] * times, o[3] * times));
+                }
+            }
         }
     }
     if (found) add_unbounded<T, HD>(a, p);
@@ -761,7 +773,7 @@ struct Kept {
 __device__ __forceinline__ Kept kept(const Segment& s) {
     return {{s.row, s.lead_row, s.lead, s.token0, s.n, s.from, s.base, s.tiles, s.step, (s.few ? 1 : 0) + (s.shared ? 2 : 0)}};
 }
-__device__ __forceinline__ Segment taken(const Kept& k) {
+__device__ __forceinline__ Segment taken(const Kept& k, Costs costs) {
     Segment s;
     s.row = uniform(k.v[0]);
     s.lead_row = uniform(k.v[1]);
@@ -775,7 +787,7 @@ __device__ __forceinline__ Segment taken(const Kept& k) {
     const int32_t flags = uniform(k.v[9]);
     s.few = flags & 1;
     s.shared = flags & 2;
-    s.lo = s.from & ~15;
+    s.key_cost = s.few ? costs.few_key : costs.tile_key;
     return s;
 }
 
@@ -788,7 +800,7 @@ struct Scratch {
 // Where a workgroup's part begins, and the whole of the work.
 struct Place {
     int64_t cost;          // all KV heads'
-    int64_t off;           // the cost before the segment
+    int64_t unit;          // the part's first, from the segment's on
     int32_t kvh, segment;  // the first that the part has work of
     int32_t few, tiles;    // tiles of each kind before the segment
     int32_t part, parts_log2;
@@ -801,7 +813,7 @@ __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scrat
     const int32_t t = static_cast<int32_t>(threadIdx.x), i0 = t * each, i1 = min(i0 + each, n);
     int64_t cost = 0, counts = 0;
     for (int32_t i = i0; i < i1; ++i) {
-        const Segment s = segment(a.batch, a.group, i);
+        const Segment s = segment(a.batch, a.group, a.costs, i);
         if (each == 1) lds.segments[t] = kept(s);
         cost += s.cost();
         counts += s.few ? static_cast<int64_t>(s.tiles) : static_cast<int64_t>(s.tiles) << 32;
@@ -846,13 +858,13 @@ __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scrat
     }
     int32_t i = static_cast<int32_t>(kWave * w + lane) * each;
     for (; each > 1; ++i) {
-        const Segment s = segment(a.batch, a.group, i);
+        const Segment s = segment(a.batch, a.group, a.costs, i);
         if (unit < off + s.cost()) break;
         off += s.cost();
         before += s.few ? static_cast<int64_t>(s.tiles) : static_cast<int64_t>(s.tiles) << 32;
     }
     out.segment = i;
-    out.off = out.kvh * per_head + off;
+    out.unit = unit - off;
     out.few = static_cast<int32_t>(before) + out.kvh * static_cast<int32_t>(counts_head);
     out.tiles = static_cast<int32_t>(before >> 32) + out.kvh * static_cast<int32_t>(counts_head >> 32);
     return true;
@@ -865,36 +877,44 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     __shared__ Scratch scratch;
     Place at;
     if (!find_place(a, at, scratch)) return;
-    const int64_t u0 = part_start(at.cost, at.parts_log2, at.part), u1 = part_start(at.cost, at.parts_log2, at.part + 1);
+    const int64_t part_end = part_start(at.cost, at.parts_log2, at.part + 1);
     const int32_t segments = a.batch.groups + a.batch.seqs;
-    int32_t kvh = at.kvh, i = at.segment, few = at.few, tiles = at.tiles;
-    int64_t off = at.off;
+    int32_t kvh = at.kvh, i = at.segment, few = at.few, tiles = at.tiles, tile = 0;
+    int64_t left = part_end - part_start(at.cost, at.parts_log2, at.part);  // units of the part yet to do
+    int64_t unit = at.unit;  // the first of them, from the segment's on
     bool again = false;
-    while (off < u1 && kvh < static_cast<int32_t>(a.kv_heads)) {
-        const Segment s = segments <= static_cast<int32_t>(kThreads) ? taken(scratch.segments[i]) : segment(a.batch, a.group, i);
-        for (int32_t t = s.tiles > 1 && u0 > off ? s.tile_at(u0 - off) : 0; t < s.tiles; ++t) {
-            const int64_t start = off + s.before(t), end = start + s.tile_cost(t);
-            if (start >= u1) break;
-            const int32_t keys = s.keys(t);
+    for (;;) {
+        const Segment s = segments <= static_cast<int32_t>(kThreads) ? taken(scratch.segments[i], a.costs) : segment(a.batch, a.group, a.costs, i);
+        tile = 0;
+        if (unit > 0 && s.tiles > 1) {
+            tile = s.tile_at(unit);
+            unit -= s.before(tile);
+        }
+        int32_t skip = static_cast<int32_t>(unit);  // of the tile's units, those of parts before
+        unit = 0;
+        for (; tile < s.tiles; ++tile, skip = 0) {
+            const int32_t keys = s.keys(tile), cost = s.tile_cost(tile);
+            const bool ends = left >= cost - skip;
             Piece p;
+            p.x0 = skip ? cut(skip, s, keys, B::kKeys) : 0;
+            p.x1 = ends ? keys : cut(skip + static_cast<int32_t>(left), s, keys, B::kKeys);
             p.tile = {a.table + static_cast<uint64_t>(s.lead_row) * a.table_stride, a.table + static_cast<uint64_t>(s.row) * a.table_stride,
-                      s.lead_span(), s.lead, s.lo, s.from, s.lo + keys - s.lead_span(), static_cast<uint32_t>(kvh)};
-            p.x0 = u0 > start ? cut(u0 - start, s.overhead(), keys, B::kKeys) : 0;
-            p.x1 = u1 >= end ? keys : cut(u1 - start, s.overhead(), keys, B::kKeys);
-            p.token0 = s.token0 + t * s.step;
-            p.tokens = s.tile_n(t);
-            p.limit0 = s.limit(t * s.step);
+                      s.lead_span(), s.lead, s.lo(), s.from, s.lo() + keys - s.lead_span(), static_cast<uint32_t>(kvh)};
+            p.token0 = s.token0 + tile * s.step;
+            p.tokens = s.tile_n(tile);
+            p.limit0 = s.limit(tile * s.step);
             p.causal = !s.shared;
             // the rows' own keys are all there is, but for a shared segment's
             const bool all = !s.shared && s.from == s.lead;
-            p.whole = all && u0 <= start && u1 >= end;
-            const int32_t slot = at.part + (s.few ? few : tiles + t);
+            p.whole = all && ends && skip == 0;
+            const int32_t slot = at.part + (s.few ? few : tiles + tile);
             p.slot_row = s.few ? (slot < a.few_slots ? static_cast<int64_t>(slot) * kFewRows : -1)
                                : (slot < a.tile_slots ? a.few_slots * kFewRows + static_cast<int64_t>(slot) * kTileRows : -1);
             // The tile's first piece tells the merge where they all are, and
             // where there is no shared segment, that there is none.
-            if (start >= u0) {
-                const uint32_t count = p.whole || p.slot_row < 0 ? 0 : part_of(at.cost, at.parts_log2, end - 1) - at.part + 1;
+            if (skip == 0) {
+                uint32_t count = p.whole || p.slot_row < 0 ? 0 : 1;
+                if (count && !ends) count += part_of(at.cost, at.parts_log2, part_end + cost - left - 1) - at.part;
                 for (uint32_t k = threadIdx.x; k < static_cast<uint32_t>(p.tokens); k += kThreads) {
                     Parts* to = a.parts + (static_cast<uint64_t>(kvh) * a.batch.tokens + p.token0 + k) * 2;
                     const uint2 mine = make_uint2(static_cast<uint32_t>(p.slot_row + k * a.group), 2 * count + (s.few ? 0u : 1u));
@@ -907,10 +927,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             if (s.few) few_rows<T, HD, CAP>(a, p, buf);
             else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1, CAP>(a, p, buf);
             else many_rows<T, HD, 2, CAP>(a, p, buf);
+            left -= cost - skip;
+            if (left <= 0) return;
         }
-        off += s.cost();
         (s.few ? few : tiles) += s.tiles;
-        if (++i == segments) i = 0, ++kvh;
+        if (++i == segments) {
+            i = 0;
+            if (++kvh == static_cast<int32_t>(a.kv_heads)) return;
+        }
     }
 }
 
@@ -1050,6 +1074,7 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     a.workgroups_log2 = workgroups_log2();
     a.scale = p->scale;
     a.softcap = p->softcap;
+    a.costs = costs(p->head_dim, p->kv_type == VKML_F16);
     a.group_inverse = 1.0f / static_cast<float>(a.group);
     vkml::abi::ProfileScope prof("attend_pages");
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(1u << a.workgroups_log2), dim3(kThreads), 0, vkml::abi::stream(), a); };

@@ -50,19 +50,16 @@ struct Batch {
     }
     VKML_HD int32_t length(int32_t s) const { return clamp_to(element(lengths, s), 0, table_keys); }
     VKML_HD int32_t group_start(int32_t g) const { return clamp_to(element(group_starts, g), 0, seqs); }
-    // Keys that the sequences of group g share; a group of one shares none.
-    VKML_HD int32_t group_shared(int32_t g) const {
-        return group_start(g + 1) - group_start(g) > 1 ? clamp_to(element(group_keys, g), 0, table_keys) : 0;
-    }
-    // The group that sequence s is in, -1 for none.
-    VKML_HD int32_t group_of(int32_t s) const {
-        int32_t lo = 0, hi = groups;  // group_start(lo) <= s < group_start(hi), if s is in any
+    VKML_HD int32_t group_key(int32_t g) const { return clamp_to(element(group_keys, g), 0, table_keys); }
+    // The group that sequence s is in, if it is in any.
+    VKML_HD int32_t group_near(int32_t s) const {
+        int32_t lo = 0, hi = groups;
         while (hi - lo > 1) {
             const int32_t mid = (lo + hi) / 2;
             if (group_start(mid) <= s) lo = mid;
             else hi = mid;
         }
-        return groups > 0 && group_start(lo) <= s && s < group_start(lo + 1) ? lo : -1;
+        return lo;
     }
 };
 
@@ -72,17 +69,27 @@ struct Batch {
 // all of its tokens, then for each sequence its other keys by its tokens. A
 // segment's tokens go in tiles: all of them where they are at most kFewRows
 // rows (token, query head), else kTileRows / (query heads a KV head) at a time.
-// A tile costs the keys it reads and, for its queries, its first loads, its
-// joining and storing, as much as so many keys more; the whole of all KV heads' tiles, laid end to end, is cut
-// into equal parts, one a workgroup: what a workgroup takes of a tile is a
-// piece.
+// A tile has a cost, and the whole of all KV heads' tiles, laid end to end, is
+// cut into equal parts of it, one a workgroup: what a workgroup takes of a tile
+// is a piece.
 constexpr int32_t kFewRows = 16;
 constexpr int32_t kTileRows = 128;
-// Measured (us): 64 keys of a tile of few rows 3.7, of another 3.3 (two
-// workgroups a compute unit, the first bound by memory); a piece by itself 5 and 7.
-constexpr int32_t kFewOverhead = 96, kTileOverhead = 128;
-constexpr int32_t kMinPart = 128;  // the cost below which work is not cut further
 constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
+
+// A tile's cost: a key's times its keys, and one of its own for its queries,
+// its first loads, its joining and storing. Measured (us, f16, head_dim 128, two
+// workgroups a compute unit): 64 keys of a tile of few rows, which memory
+// bounds, 1.73 and of another 3.07; by itself the one 6.6, the other 9.0. f16 at
+// 64: 0.69, -, 3.2, -; f32 at 64: 1.81, 3.45, 1.8, 2.4.
+struct Costs {
+    int32_t few_key, tile_key;
+};
+constexpr int32_t kFewOverhead = 1600, kTileOverhead = 2400;
+constexpr int32_t kMinPart = 1024;  // the cost below which work is not cut further
+VKML_HD Costs costs(uint32_t head_dim, bool f16) {
+    const int32_t few = static_cast<int32_t>(head_dim / (f16 ? 16 : 8));
+    return {few, few + few * 3 / 4};
+}
 
 VKML_HD int32_t tile_tokens(int32_t group) { return kTileRows / group > 1 ? kTileRows / group : 1; }
 
@@ -93,14 +100,16 @@ struct Segment {
     int32_t row = 0;       // the sequence whose table holds the keys from lo on
     int32_t lead_row = 0;  // and the `lead` keys
     int32_t lead = 0;
-    int32_t token0 = 0;  // the first token
-    int32_t n = 0;       // tokens
-    int32_t lo = 0;      // the first position read, a multiple of 16
-    int32_t from = 0;    // the first that counts
-    int32_t base = 0;    // positions from lo on before the first token's; shared keys: all
+    int32_t token0 = 0;    // the first token
+    int32_t n = 0;         // tokens
+    int32_t from = 0;      // the first position that counts
+    int32_t base = 0;      // positions from lo() on before the first token's; shared keys: all
     int32_t tiles = 0, step = 1;
     bool few = false, shared = false;
+    int32_t key_cost = 0;
 
+    // The first position read, a multiple of 16.
+    VKML_HD int32_t lo() const { return from & ~15; }
     VKML_HD int32_t lead_span() const { return (lead + kLeadStep - 1) / kLeadStep * kLeadStep; }
     // The axis' length for tile i's tokens.
     VKML_HD int32_t keys(int32_t i) const {
@@ -112,12 +121,13 @@ struct Segment {
         return lead_span() + own;
     }
     VKML_HD int32_t overhead() const { return few ? kFewOverhead : kTileOverhead; }
-    VKML_HD int64_t tile_cost(int32_t i) const { return overhead() + keys(i); }
+    VKML_HD int32_t tile_cost(int32_t i) const { return overhead() + key_cost * keys(i); }  // (2^26 keys' fits)
     // The cost of the tiles before tile i.
     VKML_HD int64_t before(int32_t i) const {
         if (i == 0) return 0;
-        const int64_t k = i, each = overhead() + (shared || base < 0 ? keys(0) : lead_span() + base);
-        return shared || base < 0 ? k * each : k * each + step * (k * (k + 1) / 2);
+        const bool equal = shared || base < 0;
+        const int64_t k = i, each = overhead() + static_cast<int64_t>(key_cost) * (equal ? keys(0) : lead_span() + base);
+        return equal ? k * each : k * each + key_cost * (step * (k * (k + 1) / 2));
     }
     VKML_HD int64_t cost() const { return tiles ? before(tiles - 1) + tile_cost(tiles - 1) : 0; }
     // The tile that holds unit u of the segment, 0 <= u < cost().
@@ -131,49 +141,55 @@ struct Segment {
         return first;
     }
     // The position past the last that token i of the segment sees.
-    VKML_HD int32_t limit(int32_t i) const { return shared ? base : lo + base + i + 1; }
+    VKML_HD int32_t limit(int32_t i) const { return shared ? base : lo() + base + i + 1; }
     VKML_HD int32_t tile_n(int32_t i) const { return n - i * step < step ? n - i * step : step; }
 };
 
-// Whether group g's shared keys are a segment of their own. Where its
-// sequences have half a tile of tokens or more on average, their own tiles
-// read few blocks more than the group's would, and no rows are in two parts.
-VKML_HD bool shares(const Batch& b, int32_t group, int32_t g) {
-    const int32_t first = b.group_start(g), last = b.group_start(g + 1);
-    const int64_t tokens = static_cast<int64_t>(b.start(last)) - b.start(first);
-    return tokens > 0 && 2 * tokens <= static_cast<int64_t>(last - first) * tile_tokens(group);
-}
-
-// Segment i of a batch: groups 0 .. groups - 1, then the sequences.
-VKML_HD Segment segment(const Batch& b, int32_t group, int32_t i) {
-    Segment s;
-    if (i < b.groups) {
-        s.base = b.group_shared(i);
-        s.shared = true;
-        if (s.base == 0 || !shares(b, group, i)) return s;
-        s.row = b.group_start(i);
-        s.token0 = b.start(s.row);
-        s.n = b.start(b.group_start(i + 1)) - s.token0;
-    } else {
-        s.row = i - b.groups;
-        const int32_t g = b.group_of(s.row);
-        s.from = g < 0 ? 0 : b.group_shared(g);
-        if (s.from > 0 && !shares(b, group, g)) {
-            s.lead = s.from;
-            s.lead_row = b.group_start(g);
-        }
-        s.lo = s.from & ~15;
-        s.token0 = b.start(s.row);
-        s.n = b.count(s.row);
-        s.base = b.length(s.row) - s.n - s.lo;
+// Segment i of a batch: groups 0 .. groups - 1, then the sequences. (Loads that
+// don't depend on one another come before what branches on them.)
+//
+// A group's shared keys are a segment of their own unless its sequences have
+// half a tile of tokens or more on average: then their own tiles read few
+// blocks more than the group's would, and no rows are in two parts. A group of
+// one sequence shares nothing.
+VKML_HD Segment segment(const Batch& b, int32_t group, Costs costs, int32_t i) {
+    const bool of_group = i < b.groups;
+    const int32_t q = of_group ? 0 : i - b.groups;
+    const int32_t own0 = b.start(q), own1 = b.start(q + 1), length = b.length(q);
+    int32_t first = 0, last = 0, keys = 0;
+    if (b.groups > 0) {
+        const int32_t g = of_group ? i : b.group_near(q);
+        first = b.group_start(g);
+        last = b.group_start(g + 1);
+        keys = b.group_key(g);
+        if (last - first < 2 || !(of_group || (first <= q && q < last))) keys = 0;
     }
-    if (s.n <= 0) {
-        s.n = 0;
-        return s;
+    int32_t group0 = 0, group1 = 0;
+    if (keys > 0) {
+        group0 = b.start(first);
+        group1 = b.start(last);
+    }
+    const int64_t tokens = static_cast<int64_t>(group1) - group0;
+    const bool shares = keys > 0 && tokens > 0 && 2 * tokens <= static_cast<int64_t>(last - first) * tile_tokens(group);
+    Segment s;
+    if (of_group) {
+        s.row = first;
+        s.shared = true;
+        s.base = keys;
+        s.token0 = group0;
+        s.n = shares ? group1 - group0 : 0;
+    } else {
+        s.row = q;
+        s.from = keys;
+        if (!shares) s.lead = keys, s.lead_row = keys > 0 ? first : 0;
+        s.token0 = own0;
+        s.n = own1 > own0 ? own1 - own0 : 0;
+        s.base = length - s.n - s.lo();
     }
     s.few = s.n <= kFewRows && s.n * group <= kFewRows;
-    s.step = s.few ? s.n : tile_tokens(group);
-    s.tiles = (s.n + s.step - 1) / s.step;
+    s.step = s.few ? (s.n > 0 ? s.n : 1) : tile_tokens(group);
+    s.tiles = s.few ? (s.n > 0 ? 1 : 0) : (s.n + s.step - 1) / s.step;
+    s.key_cost = s.few ? costs.few_key : costs.tile_key;
     return s;
 }
 
@@ -186,20 +202,24 @@ VKML_HD int32_t parts_log2(int64_t cost, int32_t workgroups_log2) {
 }
 // The first unit of part w, and the part that unit u is in (the quotient,
 // found in f32 and set right).
-VKML_HD int64_t part_start(int64_t cost, int32_t n_log2, int32_t w) { return cost * w >> n_log2; }
+VKML_HD int64_t part_start(int64_t cost, int32_t n_log2, int32_t w) {
+    return (cost >> n_log2) * w + (static_cast<int64_t>(static_cast<uint32_t>(cost) & ((1u << n_log2) - 1)) * w >> n_log2);
+}
 VKML_HD int32_t part_of(int64_t cost, int32_t n_log2, int64_t u) {
     int32_t w = static_cast<int32_t>(static_cast<float>(u) / static_cast<float>(cost) * static_cast<float>(1 << n_log2));
     while (part_start(cost, n_log2, w) > u) --w;
     while (part_start(cost, n_log2, w + 1) <= u) ++w;
     return w;
 }
-// Keys of a tile of `keys` that units before x of it stand for: whole blocks
-// (but the last), so that every part cuts at the same places.
-VKML_HD int32_t cut(int64_t x, int32_t overhead, int32_t keys, int32_t block) {
-    if (x <= overhead) return 0;
-    const int32_t k = static_cast<int32_t>(x) - overhead;
-    if (k >= keys) return keys;
-    const int32_t up = (k + block - 1) / block * block;
+// Where on its keys' axis a tile is cut at unit x of it: at whole blocks (or
+// the end), so that every part cuts at the same places. f32's quotient is a
+// block off at most, for all parts alike.
+VKML_HD int32_t cut(int32_t x, const Segment& s, int32_t keys, int32_t block) {
+    if (x <= s.overhead()) return 0;
+    const float at = static_cast<float>(x - s.overhead()) / static_cast<float>(s.key_cost * block);
+    const int32_t blocks = (keys + block - 1) / block;
+    if (at >= static_cast<float>(blocks)) return keys;
+    const int32_t up = (static_cast<int32_t>(at) + 1) * block;
     return up < keys ? up : keys;
 }
 
@@ -233,7 +253,7 @@ inline const char* check_cache(uint32_t kv_heads, uint32_t head_dim, uint32_t kv
 inline const char* check_batch(uint32_t seqs, uint32_t tokens, uint32_t table_stride, uint32_t page_size) {
     if (seqs > kMaxSeqs) return "more than 65536 sequences";
     if (tokens > kMaxTokens) return "more than 2^22 new tokens";
-    if (table_stride == 0 || static_cast<uint64_t>(table_stride) * page_size > (1u << 30)) return "a table row must hold 1 to 2^30 keys";
+    if (table_stride == 0 || static_cast<uint64_t>(table_stride) * page_size > (1u << 26)) return "a table row must hold 1 to 2^26 keys";
     return nullptr;
 }
 
