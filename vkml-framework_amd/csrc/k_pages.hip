@@ -65,13 +65,32 @@ __device__ __forceinline__ void write(T* p, const Part<W>& r) {
     }
 }
 
-// Workgroup (x, y): kThreads units of token x, from unit y * kThreads on. A
-// unit is 2 W values of one head that one thread takes: W pairs of a turned
-// part, or 2 W consecutive dims of an unturned one (v, and q's and k's dims
-// from rotary_dim on).
-template <int W, typename T>
+// Workgroup (x, y): U kThreads units of token x. A unit is 2 W values of one
+// head that one thread takes: W pairs of a turned part, or 2 W consecutive dims
+// of an unturned one (v, and q's and k's dims from rotary_dim on). A thread's
+// values are loaded first; where its token stands is found meanwhile.
+template <int W, typename T, int U>
 __global__ void __launch_bounds__(kThreads) k_rope_kv_pages(RopeArgs a) {
     const int32_t t = static_cast<int32_t>(blockIdx.x);
+    const uint32_t hd = a.head_dim, r = a.rotary_dim, per_head = hd / (2 * W), turned = r / (2 * W), units = (a.heads + 2 * a.kv_heads) * per_head;
+    const float* row = a.qkv + static_cast<uint64_t>(t) * a.row_stride;
+    uint32_t head[U], e[U], ia[U], ib[U];
+    Part<W> x[U], y[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const uint32_t u = min((blockIdx.y * U + i) * kThreads + threadIdx.x, units - 1);  // the last again past it, not stored
+        head[i] = u / per_head;
+        e[i] = u % per_head;
+        if (head[i] >= a.heads + a.kv_heads) e[i] += turned;  // v: no part of it is turned
+        ia[i] = 2 * W * (e[i] - (head[i] >= a.heads + a.kv_heads ? turned : 0));
+        ib[i] = ia[i] + W;
+        if (e[i] < turned && a.style == 1) {
+            ia[i] = W * e[i];
+            ib[i] = r / 2 + W * e[i];
+        }
+        x[i] = read<W>(row + head[i] * hd + ia[i]);
+        y[i] = read<W>(row + head[i] * hd + ib[i]);
+    }
     int32_t s = t;
     if (a.batch.starts) {  // the sequences that end at or before the token
         s = 0;
@@ -82,67 +101,56 @@ __global__ void __launch_bounds__(kThreads) k_rope_kv_pages(RopeArgs a) {
     }
     if (s >= a.batch.seqs || t < a.batch.start(s)) return;
     const int32_t pos = a.batch.length(s) - a.batch.count(s) + t - a.batch.start(s);
-    const uint32_t hd = a.head_dim, r = a.rotary_dim;
-    const int32_t page = pos >= 0 && pos < a.batch.table_keys ? a.table[static_cast<uint64_t>(s) * a.table_stride + pos / a.page_size] : -1;
-    const bool kept = static_cast<uint32_t>(page) < a.pages;
     const int32_t turn = a.at ? a.at[t] : pos;
     const bool held = static_cast<uint32_t>(turn) < a.positions;
-    const uint32_t per_head = hd / (2 * W), turned = r / (2 * W), units = (a.heads + 2 * a.kv_heads) * per_head;
-    const float* row = a.qkv + static_cast<uint64_t>(t) * a.row_stride;
-    for (uint32_t u = blockIdx.y * kThreads + threadIdx.x; u < units; u += gridDim.y * kThreads) {
-        const uint32_t head = u / per_head, e = u % per_head;
-        const bool is_v = head >= a.heads + a.kv_heads;
-        uint32_t ia = 2 * W * e, ib = ia + W;
-        Part<W> x, y;
-        if (is_v || e >= turned) {
-            x = read<W>(row + head * hd + ia);
-            y = read<W>(row + head * hd + ib);
-        } else {
-            if (a.style == 1) ia = W * e, ib = r / 2 + W * e;
-            x = read<W>(row + head * hd + ia);
-            y = read<W>(row + head * hd + ib);
-            float c[W], d[W];
+    const int32_t page = pos >= 0 && pos < a.batch.table_keys ? a.table[static_cast<uint64_t>(s) * a.table_stride + pos / a.page_size] : -1;
+    const bool kept = static_cast<uint32_t>(page) < a.pages;
+    const float* angles = a.angles + static_cast<uint64_t>(held ? turn : 0) * r;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        if ((blockIdx.y * U + i) * kThreads + threadIdx.x >= units) break;
+        if (e[i] < turned) {
+            float c[W], d[W];  // cos and sin of the unit's pairs
+#pragma unroll
+            for (int j = 0; j < W; ++j) c[j] = d[j] = __builtin_nanf("");
             if (held) {
-                const float* cs = a.angles + static_cast<uint64_t>(turn) * r + 2 * W * e;
-                const Part<W> lo = read<W>(cs), hi = read<W>(cs + W);
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    c[i] = 2 * i < W ? lo.x[2 * i] : hi.x[2 * i - W];
-                    d[i] = 2 * i + 1 < W ? lo.x[2 * i + 1] : hi.x[2 * i + 1 - W];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < W; ++i) c[i] = d[i] = __builtin_nanf("");
-            }
-            // The pairs: (x[i], y[i]) in the split layout, the 2 W values' neighbours in the other.
-            Part<W> p = x, q = y;
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const int j = 2 * i, m = 2 * i + 1;
-                const float f = a.style == 1 ? x.x[i] : j < W ? x.x[j % W] : y.x[j % W];
-                const float g = a.style == 1 ? y.x[i] : m < W ? x.x[m % W] : y.x[m % W];
-                const float turned_f = f * c[i] - g * d[i], turned_g = f * d[i] + g * c[i];
-                if (a.style == 1) {
-                    p.x[i] = turned_f;
-                    q.x[i] = turned_g;
+                if constexpr (W == 4) {
+                    const Part<4> lo = read<4>(angles + 8 * e[i]), hi = read<4>(angles + 8 * e[i] + 4);
+                    c[0] = lo.x[0], d[0] = lo.x[1], c[1] = lo.x[2], d[1] = lo.x[3];
+                    c[2] = hi.x[0], d[2] = hi.x[1], c[3] = hi.x[2], d[3] = hi.x[3];
                 } else {
-                    (j < W ? p.x[j % W] : q.x[j % W]) = turned_f;
-                    (m < W ? p.x[m % W] : q.x[m % W]) = turned_g;
+                    c[0] = ldg(angles + 2 * e[i]);
+                    d[0] = ldg(angles + 2 * e[i] + 1);
                 }
             }
-            x = p;
-            y = q;
+            const Part<W> f = x[i], g = y[i];
+            if (W == 1 || a.style == 1) {  // the pairs are (f[j], g[j])
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    x[i].x[j] = f.x[j] * c[j] - g.x[j] * d[j];
+                    y[i].x[j] = f.x[j] * d[j] + g.x[j] * c[j];
+                }
+            } else {  // neighbours in the 2 W values
+#pragma unroll
+                for (int j = 0; j < W / 2; ++j) {
+                    x[i].x[2 * j] = f.x[2 * j] * c[j] - f.x[2 * j + 1] * d[j];
+                    x[i].x[2 * j + 1] = f.x[2 * j] * d[j] + f.x[2 * j + 1] * c[j];
+                    y[i].x[2 * j] = g.x[2 * j] * c[W / 2 + j] - g.x[2 * j + 1] * d[W / 2 + j];
+                    y[i].x[2 * j + 1] = g.x[2 * j] * d[W / 2 + j] + g.x[2 * j + 1] * c[W / 2 + j];
+                }
+            }
         }
-        if (head < a.heads) {
-            float* to = a.q + (static_cast<uint64_t>(t) * a.heads + head) * hd;
-            write<W>(to + ia, x);
-            write<W>(to + ib, y);
+        if (head[i] < a.heads) {
+            float* to = a.q + (static_cast<uint64_t>(t) * a.heads + head[i]) * hd;
+            write<W>(to + ia[i], x[i]);
+            write<W>(to + ib[i], y[i]);
         } else if (kept) {
-            const uint32_t kvh = head - a.heads - (is_v ? a.kv_heads : 0);
+            const bool is_v = head[i] >= a.heads + a.kv_heads;
+            const uint32_t kvh = head[i] - a.heads - (is_v ? a.kv_heads : 0);
             T* to = static_cast<T*>(is_v ? a.v : a.k) + static_cast<uint64_t>(page) * a.page_stride +
                     (static_cast<uint64_t>(kvh) * a.page_size + pos % a.page_size) * hd;
-            write<W>(to + ia, x);
-            write<W>(to + ib, y);
+            write<W>(to + ia[i], x[i]);
+            write<W>(to + ib[i], y[i]);
         }
     }
 }
@@ -200,11 +208,19 @@ int vkml_rope_kv_pages(const vkml_rope_kv_pages_params* p, const float* qkv, con
     const bool wide = p->head_dim % 8 == 0 && p->rotary_dim % 8 == 0 && p->row_stride % 4 == 0 && aligned16(qkv) && aligned16(rope_table) &&
                       aligned16(q) && aligned16(k_pages) && aligned16(v_pages);
     const uint32_t units = (p->heads + 2 * p->kv_heads) * (p->head_dim / (wide ? 8 : 2));
-    const dim3 grid(p->tokens, (units + kThreads - 1) / kThreads);
+    // Few tokens: as many workgroups as their units give; many: a thread has
+    // several units' loads in flight.
+    const uint32_t rounds = (units + kThreads - 1) / kThreads;
+    const uint32_t each = p->tokens * rounds <= 4 * vkml::abi::compute_units() || rounds < 2 ? 1 : rounds == 2 ? 2 : 3;
+    const dim3 grid(p->tokens, (rounds + each - 1) / each);
     vkml::abi::ProfileScope prof("rope_kv_pages");
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, vkml::abi::stream(), a); };
-    if (p->kv_type == VKML_F16) wide ? go(k_rope_kv_pages<4, _Float16>) : go(k_rope_kv_pages<1, _Float16>);
-    else wide ? go(k_rope_kv_pages<4, float>) : go(k_rope_kv_pages<1, float>);
+    const auto pick = [&](auto t) {
+        using T = decltype(t);
+        if (!wide) each == 1 ? go(k_rope_kv_pages<1, T, 1>) : each == 2 ? go(k_rope_kv_pages<1, T, 2>) : go(k_rope_kv_pages<1, T, 3>);
+        else each == 1 ? go(k_rope_kv_pages<4, T, 1>) : each == 2 ? go(k_rope_kv_pages<4, T, 2>) : go(k_rope_kv_pages<4, T, 3>);
+    };
+    p->kv_type == VKML_F16 ? pick(_Float16{}) : pick(0.0f);
     return vkml::abi::check_launch("rope_kv_pages");
 }
 
