@@ -40,20 +40,22 @@ extern "C" int64_t pieces_c(const Batch* b, int32_t kv_heads, int32_t group, int
         for (int32_t h = 0; h < kv_heads; ++h)
             for (int32_t i = 0; i < segments; ++i) {
                 const Segment s = segment(*b, group, cost_of, i);
-                if (off + s.cost() > u0 && off < u1 && s.tiles) {
-                    for (int32_t t = u0 > off ? s.tile_at(u0 - off) : 0; t < s.tiles; ++t) {
-                        const int64_t at = off + s.before(t), end = at + s.tile_cost(t);
-                        if (at >= u1) break;
-                        if (n >= most) return -1;
-                        int64_t* o = out + 10 * n++;
-                        o[0] = w, o[1] = h, o[2] = i, o[3] = t;
-                        o[4] = u0 > at ? cut(static_cast<int32_t>(u0 - at), s, s.keys(t), block) : 0;
-                        o[5] = u1 >= end ? s.keys(t) : cut(static_cast<int32_t>(u1 - at), s, s.keys(t), block);
-                        o[6] = w + (s.few ? few : tiles + t);
-                        o[7] = s.few;
-                        o[8] = u0 <= at && u1 >= end;
-                        o[9] = at >= u0 ? part_of(cost, w_log2, end - 1) - w + 1 : -1;
-                    }
+                for (int32_t t = 0; t < s.tiles; ++t) {
+                    const int64_t at = off + s.before(t);
+                    const int32_t c = s.tile_cost(t), keys = s.keys(t);
+                    // the part's range within the tile, as its workgroup finds it
+                    if (u0 >= at + c || u1 <= at) continue;
+                    const int32_t from = u0 > at ? snap(u0 - at, s, c) : 0, to = snap(u1 - at, s, c);
+                    if (from >= to) continue;
+                    if (n >= most) return -1;
+                    int64_t* o = out + 10 * n++;
+                    o[0] = w, o[1] = h, o[2] = i, o[3] = t;
+                    o[4] = cut(from, s, keys, block);
+                    o[5] = to == c ? keys : cut(to, s, keys, block);
+                    o[6] = w + (s.few ? few : tiles + t);
+                    o[7] = s.few;
+                    o[8] = from == 0 && to == c;
+                    o[9] = from == 0 ? (to == c ? 1 : pieces_of(cost, w_log2, s, at, c, w)) : -1;
                 }
                 off += s.cost();
                 (s.few ? few : tiles) += s.tiles;

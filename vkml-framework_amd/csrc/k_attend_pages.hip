@@ -82,6 +82,13 @@ struct PagesArgs {
     Costs costs;
 };
 
+// A value that a wave's lanes share, in a scalar register.
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int32_t>(x >> 32)))) << 32 |
+                                static_cast<uint32_t>(uniform(static_cast<int32_t>(x))));
+}
+
 // The blocks: 16 KiB each of K and V for a workgroup, 8 KiB for a wave alone.
 template <typename T, int HD>
 struct Block {
@@ -171,7 +178,7 @@ __device__ __forceinline__ uint64_t offset_of(const PagesArgs& a, uint32_t kvh, 
 // the loads, not to the pool ahead of a loop, where their sums would take two
 // registers each.
 __device__ __forceinline__ const uint8_t* at_offset(const uint8_t* pool, uint64_t offset) {
-    uint64_t p = reinterpret_cast<uint64_t>(pool) + offset;
+    uint64_t p = static_cast<uint64_t>(uniform(static_cast<int64_t>(reinterpret_cast<uint64_t>(pool) + offset)));
     asm volatile("" : "+s"(p));
     return reinterpret_cast<const uint8_t*>(p);
 }
@@ -345,6 +352,9 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
     const uint32_t l = thread_index() % kWave, j = l % 16, g = l / 16;
     const uint32_t k_at = j * B::kRow + 16 * (g ^ B::swizzle_k(j));
     f32x4 s[RT][TT];
+    // Where two waves share a SIMD's matrix unit (tiles of many rows), the one
+    // in its products goes first: 3 % of a prompt's time.
+    if constexpr (!REGS) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -359,6 +369,7 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         }
         q.score(st, kk, s);
     }
+    if constexpr (!REGS) __builtin_amdgcn_s_setprio(0);
     constexpr float kShift = B::kF16 ? 14.0f : 0.0f;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -417,6 +428,7 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         // j of the four rows.
         const uint32_t row = 4 * g + j / 4, at = row * B::kRow + 16 * ((j % 4 / 2) ^ B::swizzle_v(row)) + 8 * (j % 2);
         constexpr int D = RT == 1 && HD == 128 ? 8 : 4;  // tiles of dims read at a time
+        if constexpr (!REGS) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int u = 0; u < TT / 2; ++u) {
             half8 ph[RT], pl[RT];
@@ -442,6 +454,7 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
                             run.o[rt][d0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[i], term ? pl[rt] : ph[rt], run.o[rt][d0 + i], 0, 0, 0);
             }
         }
+        if constexpr (!REGS) __builtin_amdgcn_s_setprio(0);
     } else {
         // Instruction e of a tile takes keys 4 g + e: V's element of dim j.
 #pragma unroll
@@ -460,12 +473,6 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
 }
 
 // ---------------------------------------------------------------- pieces
-
-__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(uniform(static_cast<int32_t>(x >> 32)))) << 32 |
-                                static_cast<uint32_t>(uniform(static_cast<int32_t>(x))));
-}
 
 // A piece of a tile: [x0, x1) of its keys' axis, rows from token0 on.
 struct Piece {
@@ -788,6 +795,7 @@ __device__ __forceinline__ Segment taken(const Kept& k, Costs costs) {
     s.few = flags & 1;
     s.shared = flags & 2;
     s.key_cost = s.few ? costs.few_key : costs.tile_key;
+    s.own_cost = s.few ? costs.few_own : costs.tile_own;
     return s;
 }
 
@@ -880,24 +888,30 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     const int64_t part_end = part_start(at.cost, at.parts_log2, at.part + 1);
     const int32_t segments = a.batch.groups + a.batch.seqs;
     int32_t kvh = at.kvh, i = at.segment, few = at.few, tiles = at.tiles, tile = 0;
-    int64_t left = part_end - part_start(at.cost, at.parts_log2, at.part);  // units of the part yet to do
-    int64_t unit = at.unit;  // the first of them, from the segment's on
+    // The part's ends, from the segment's (then the tile's) first unit on.
+    int64_t begin = at.unit, end = begin + part_end - part_start(at.cost, at.parts_log2, at.part);
     bool again = false;
     for (;;) {
         const Segment s = segments <= static_cast<int32_t>(kThreads) ? taken(scratch.segments[i], a.costs) : segment(a.batch, a.group, a.costs, i);
         tile = 0;
-        if (unit > 0 && s.tiles > 1) {
-            tile = s.tile_at(unit);
-            unit -= s.before(tile);
+        if (begin > 0 && s.tiles > 1) {
+            tile = s.tile_at(begin);
+            const int64_t before = s.before(tile);
+            begin -= before;
+            end -= before;
         }
-        int32_t skip = static_cast<int32_t>(unit);  // of the tile's units, those of parts before
-        unit = 0;
-        for (; tile < s.tiles; ++tile, skip = 0) {
+        for (; tile < s.tiles; ++tile) {
             const int32_t keys = s.keys(tile), cost = s.tile_cost(tile);
-            const bool ends = left >= cost - skip;
+            const int32_t from = snap(begin, s, cost), to = snap(end, s, cost);
+            begin = 0;
+            if (to == 0) return;  // the next part's
+            const int64_t start = part_end - end;  // the tile's, in the whole
+            end -= cost;
+            if (from == cost) continue;  // the part before has taken the rest
+            const bool ends = to == cost;
             Piece p;
-            p.x0 = skip ? cut(skip, s, keys, B::kKeys) : 0;
-            p.x1 = ends ? keys : cut(skip + static_cast<int32_t>(left), s, keys, B::kKeys);
+            p.x0 = cut(from, s, keys, B::kKeys);
+            p.x1 = ends ? keys : cut(to, s, keys, B::kKeys);
             p.tile = {a.table + static_cast<uint64_t>(s.lead_row) * a.table_stride, a.table + static_cast<uint64_t>(s.row) * a.table_stride,
                       s.lead_span(), s.lead, s.lo(), s.from, s.lo() + keys - s.lead_span(), static_cast<uint32_t>(kvh)};
             p.token0 = s.token0 + tile * s.step;
@@ -906,15 +920,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             p.causal = !s.shared;
             // the rows' own keys are all there is, but for a shared segment's
             const bool all = !s.shared && s.from == s.lead;
-            p.whole = all && ends && skip == 0;
+            p.whole = all && ends && from == 0;
             const int32_t slot = at.part + (s.few ? few : tiles + tile);
             p.slot_row = s.few ? (slot < a.few_slots ? static_cast<int64_t>(slot) * kFewRows : -1)
                                : (slot < a.tile_slots ? a.few_slots * kFewRows + static_cast<int64_t>(slot) * kTileRows : -1);
             // The tile's first piece tells the merge where they all are, and
             // where there is no shared segment, that there is none.
-            if (skip == 0) {
-                uint32_t count = p.whole || p.slot_row < 0 ? 0 : 1;
-                if (count && !ends) count += part_of(at.cost, at.parts_log2, part_end + cost - left - 1) - at.part;
+            if (from == 0) {
+                const uint32_t count = p.whole || p.slot_row < 0 ? 0 : ends ? 1 : pieces_of(at.cost, at.parts_log2, s, start, cost, at.part);
                 for (uint32_t k = threadIdx.x; k < static_cast<uint32_t>(p.tokens); k += kThreads) {
                     Parts* to = a.parts + (static_cast<uint64_t>(kvh) * a.batch.tokens + p.token0 + k) * 2;
                     const uint2 mine = make_uint2(static_cast<uint32_t>(p.slot_row + k * a.group), 2 * count + (s.few ? 0u : 1u));
@@ -927,8 +940,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             if (s.few) few_rows<T, HD, CAP>(a, p, buf);
             else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1, CAP>(a, p, buf);
             else many_rows<T, HD, 2, CAP>(a, p, buf);
-            left -= cost - skip;
-            if (left <= 0) return;
+            if (end <= 0) return;
         }
         (s.few ? few : tiles) += s.tiles;
         if (++i == segments) {

@@ -71,24 +71,24 @@ struct Batch {
 // rows (token, query head), else kTileRows / (query heads a KV head) at a time.
 // A tile has a cost, and the whole of all KV heads' tiles, laid end to end, is
 // cut into equal parts of it, one a workgroup: what a workgroup takes of a tile
-// is a piece.
+// is a piece. A cut within a tile's own cost is made at its start instead, and one
+// near its end there: the rest would cost more by itself than it evens out.
 constexpr int32_t kFewRows = 16;
 constexpr int32_t kTileRows = 128;
 constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
 
 // A tile's cost: a key's times its keys, and one of its own for its queries,
-// its first loads, its joining and storing. Measured (us, f16, head_dim 128, two
-// workgroups a compute unit): 64 keys of a tile of few rows, which memory
-// bounds, 1.73 and of another 3.07; by itself the one 6.6, the other 9.0. f16 at
-// 64: 0.69, -, 3.2, -; f32 at 64: 1.81, 3.45, 1.8, 2.4.
+// its first loads, its joining and storing. Measured (us, two workgroups a
+// compute unit): f16, head_dim 128, 64 keys of a tile of few rows, which memory
+// bounds, 1.6 and of another 2.7, by itself the one 4.1, the other 6.5; f16 at 64
+// 0.66, -, 3.4, -; f32 at 64 1.6, 3.8, 1.7, 1.2.
 struct Costs {
-    int32_t few_key, tile_key;
+    int32_t few_key, tile_key, few_own, tile_own;
 };
-constexpr int32_t kFewOverhead = 1600, kTileOverhead = 2400;
 constexpr int32_t kMinPart = 1024;  // the cost below which work is not cut further
 VKML_HD Costs costs(uint32_t head_dim, bool f16) {
     const int32_t few = static_cast<int32_t>(head_dim / (f16 ? 16 : 8));
-    return {few, few + few * 3 / 4};
+    return {few, few + few * 3 / 4, f16 ? 2000 : 600, f16 ? 2400 : 600};
 }
 
 VKML_HD int32_t tile_tokens(int32_t group) { return kTileRows / group > 1 ? kTileRows / group : 1; }
@@ -106,7 +106,7 @@ struct Segment {
     int32_t base = 0;      // positions from lo() on before the first token's; shared keys: all
     int32_t tiles = 0, step = 1;
     bool few = false, shared = false;
-    int32_t key_cost = 0;
+    int32_t key_cost = 0, own_cost = 0;
 
     // The first position read, a multiple of 16.
     VKML_HD int32_t lo() const { return from & ~15; }
@@ -120,13 +120,12 @@ struct Segment {
         }
         return lead_span() + own;
     }
-    VKML_HD int32_t overhead() const { return few ? kFewOverhead : kTileOverhead; }
-    VKML_HD int32_t tile_cost(int32_t i) const { return overhead() + key_cost * keys(i); }  // (2^26 keys' fits)
+    VKML_HD int32_t tile_cost(int32_t i) const { return own_cost + key_cost * keys(i); }  // (2^26 keys' fits)
     // The cost of the tiles before tile i.
     VKML_HD int64_t before(int32_t i) const {
         if (i == 0) return 0;
         const bool equal = shared || base < 0;
-        const int64_t k = i, each = overhead() + static_cast<int64_t>(key_cost) * (equal ? keys(0) : lead_span() + base);
+        const int64_t k = i, each = own_cost + static_cast<int64_t>(key_cost) * (equal ? keys(0) : lead_span() + base);
         return equal ? k * each : k * each + key_cost * (step * (k * (k + 1) / 2));
     }
     VKML_HD int64_t cost() const { return tiles ? before(tiles - 1) + tile_cost(tiles - 1) : 0; }
@@ -190,6 +189,7 @@ VKML_HD Segment segment(const Batch& b, int32_t group, Costs costs, int32_t i) {
     s.step = s.few ? (s.n > 0 ? s.n : 1) : tile_tokens(group);
     s.tiles = s.few ? (s.n > 0 ? 1 : 0) : (s.n + s.step - 1) / s.step;
     s.key_cost = s.few ? costs.few_key : costs.tile_key;
+    s.own_cost = s.few ? costs.few_own : costs.tile_own;
     return s;
 }
 
@@ -211,16 +211,28 @@ VKML_HD int32_t part_of(int64_t cost, int32_t n_log2, int64_t u) {
     while (part_start(cost, n_log2, w + 1) <= u) ++w;
     return w;
 }
-// Where on its keys' axis a tile is cut at unit x of it: at whole blocks (or
-// the end), so that every part cuts at the same places. f32's quotient is a
-// block off at most, for all parts alike.
+// Where the tile of s with `cost` is cut at unit x of it: at its start (0), its
+// end (cost) or between (x).
+VKML_HD int32_t snap(int64_t x, const Segment& s, int32_t cost) {
+    if (x <= s.own_cost) return 0;
+    return x >= cost - s.own_cost / 8 ? cost : static_cast<int32_t>(x);
+}
+// Where on its keys' axis a tile is cut at unit x: at whole blocks (or the
+// end), so that every part cuts at the same places. f32's quotient is a block
+// off at most, for all parts alike.
 VKML_HD int32_t cut(int32_t x, const Segment& s, int32_t keys, int32_t block) {
-    if (x <= s.overhead()) return 0;
-    const float at = static_cast<float>(x - s.overhead()) / static_cast<float>(s.key_cost * block);
+    if (x <= s.own_cost) return 0;
+    const float at = static_cast<float>(x - s.own_cost) / static_cast<float>(s.key_cost * block);
     const int32_t blocks = (keys + block - 1) / block;
     if (at >= static_cast<float>(blocks)) return keys;
     const int32_t up = (static_cast<int32_t>(at) + 1) * block;
     return up < keys ? up : keys;
+}
+// Pieces of a tile of s whose unit 0 is the whole's `start`, the first of them
+// in part `first`.
+VKML_HD int32_t pieces_of(int64_t cost, int32_t n_log2, const Segment& s, int64_t start, int32_t tile_cost, int32_t first) {
+    const int32_t last = tile_cost - s.own_cost / 8 - 1;  // the last unit a cut can be made at
+    return last <= s.own_cost ? 1 : part_of(cost, n_log2, start + last) - first + 1;
 }
 
 // What a call keeps of unfinished rows: slots of kFewRows or kTileRows rows,
