@@ -11,5 +11,6 @@
 #include "vkml/generation.hpp"
 #include "vkml/llama.hpp"
 #include "vkml/ops.hpp"
+#include "vkml/pages.hpp"
 #include "vkml/sampling.hpp"
 #include "vkml/tensor.hpp"

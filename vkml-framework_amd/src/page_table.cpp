@@ -1,0 +1,138 @@
+// page_table.cpp -- the pages of a paged KV cache's sequences: taken, shared,
+// copied before a write into a shared one, given back, compacted. Host code
+// without a device.
+#include <algorithm>
+#include <string>
+
+#include "vkml/error.hpp"
+#include "vkml/pages.hpp"
+
+namespace vkml {
+
+PageTable::PageTable(std::int64_t pages, std::int64_t page_size) : page_size_(page_size) {
+    if (pages < 1 || pages > 0x7FFFFFFF) throw Error("PageTable: " + std::to_string(pages) + " pages");
+    if (page_size < 1) throw Error("PageTable: pages of " + std::to_string(page_size) + " keys");
+    users_.resize(static_cast<std::size_t>(pages));
+    std::vector<std::int32_t> all(static_cast<std::size_t>(pages));
+    for (std::size_t i = 0; i < all.size(); ++i) all[i] = static_cast<std::int32_t>(i);
+    free_ = decltype(free_)(std::greater<>{}, std::move(all));
+}
+
+const PageTable::Row& PageTable::at(std::int64_t id) const {
+    const auto it = rows_.find(id);
+    if (it == rows_.end()) throw Error("PageTable: no sequence " + std::to_string(id));
+    return it->second;
+}
+
+std::int32_t PageTable::take() {
+    const std::int32_t page = free_.top();
+    free_.pop();
+    users_[static_cast<std::size_t>(page)] = 1;
+    return page;
+}
+
+void PageTable::give(std::int32_t page) {
+    if (--users_[static_cast<std::size_t>(page)] == 0) free_.push(page);
+}
+
+std::int64_t PageTable::create() {
+    rows_.emplace(next_id_, Row{});
+    return next_id_++;
+}
+
+std::int64_t PageTable::fork(std::int64_t id) {
+    Row copy = at(id);
+    for (const std::int32_t page : copy.pages) ++users_[static_cast<std::size_t>(page)];
+    rows_.emplace(next_id_, std::move(copy));
+    return next_id_++;
+}
+
+void PageTable::release(std::int64_t id) {
+    for (const std::int32_t page : at(id).pages) give(page);
+    rows_.erase(id);
+}
+
+void PageTable::truncate(std::int64_t id, std::int64_t length) {
+    const Row& row = at(id);
+    if (length < 0 || length > row.length) {
+        throw Error("PageTable::truncate: length " + std::to_string(length) + " of a sequence of " + std::to_string(row.length));
+    }
+    Row& mine = rows_[id];
+    while (static_cast<std::int64_t>(mine.pages.size()) > pages_for(length)) {
+        give(mine.pages.back());
+        mine.pages.pop_back();
+    }
+    mine.length = length;
+}
+
+std::vector<PageCopy> PageTable::append(std::span<const std::int64_t> ids, std::span<const std::int64_t> tokens) {
+    if (ids.size() != tokens.size()) throw Error("PageTable::append: " + std::to_string(ids.size()) + " sequences, " + std::to_string(tokens.size()) + " counts");
+    // What it takes: new pages, and copies of the part-filled ones that are
+    // written into while another sequence still holds them.
+    std::int64_t need = 0;
+    std::map<std::int32_t, std::int32_t> writers;
+    std::map<std::int64_t, int> seen;
+    for (std::size_t i = 0; i < ids.size(); ++i) {
+        const Row& row = at(ids[i]);
+        if (tokens[i] < 0 || tokens[i] > 0x7FFFFFFF - row.length) throw Error("PageTable::append: " + std::to_string(tokens[i]) + " tokens");
+        if (seen[ids[i]]++) throw Error("PageTable::append: sequence " + std::to_string(ids[i]) + " twice");
+        need += pages_for(row.length + tokens[i]) - static_cast<std::int64_t>(row.pages.size());
+        if (tokens[i] > 0 && row.length % page_size_ != 0) ++writers[row.pages.back()];
+    }
+    for (const auto& [page, n] : writers) need += users_[static_cast<std::size_t>(page)] > n ? n : n - 1;
+    if (need > free_pages()) {
+        throw Error("PageTable::append: " + std::to_string(need) + " pages needed, " + std::to_string(free_pages()) + " of " + std::to_string(pages()) + " free");
+    }
+    std::vector<PageCopy> copies;
+    for (std::size_t i = 0; i < ids.size(); ++i) {
+        Row& row = rows_[ids[i]];
+        if (tokens[i] > 0 && row.length % page_size_ != 0 && users_[static_cast<std::size_t>(row.pages.back())] > 1) {
+            const std::int32_t page = take();
+            copies.push_back({row.pages.back(), page});
+            give(row.pages.back());
+            row.pages.back() = page;
+        }
+        row.length += tokens[i];
+        while (static_cast<std::int64_t>(row.pages.size()) < pages_for(row.length)) row.pages.push_back(take());
+    }
+    return copies;
+}
+
+std::vector<PageCopy> PageTable::compact() {
+    const std::int64_t used = pages() - free_pages();
+    std::vector<std::int32_t> to(users_.size(), -1), holes;
+    for (std::int64_t p = 0; p < used; ++p)
+        if (users_[static_cast<std::size_t>(p)] == 0) holes.push_back(static_cast<std::int32_t>(p));
+    std::vector<PageCopy> copies;
+    for (std::int64_t p = used; p < pages(); ++p) {
+        if (users_[static_cast<std::size_t>(p)] == 0) continue;
+        const std::int32_t hole = holes[copies.size()];
+        copies.push_back({static_cast<std::int32_t>(p), hole});
+        to[static_cast<std::size_t>(p)] = hole;
+    }
+    for (const PageCopy& c : copies) std::swap(users_[static_cast<std::size_t>(c.from)], users_[static_cast<std::size_t>(c.to)]);
+    for (auto& [id, row] : rows_)
+        for (std::int32_t& page : row.pages)
+            if (to[static_cast<std::size_t>(page)] >= 0) page = to[static_cast<std::size_t>(page)];
+    std::vector<std::int32_t> left;
+    for (std::int64_t p = used; p < pages(); ++p) left.push_back(static_cast<std::int32_t>(p));
+    free_ = decltype(free_)(std::greater<>{}, std::move(left));
+    return copies;
+}
+
+std::int64_t PageTable::shared(std::span<const std::int64_t> ids, std::span<const std::int64_t> before) const {
+    if (ids.size() != before.size()) throw Error("PageTable::shared: " + std::to_string(ids.size()) + " sequences, " + std::to_string(before.size()) + " counts");
+    if (ids.empty()) return 0;
+    const std::vector<std::int32_t>& first = row(ids[0]);
+    std::size_t same = first.size();
+    std::int64_t keys = INT64_MAX;
+    for (std::size_t i = 0; i < ids.size(); ++i) {
+        const Row& r = at(ids[i]);
+        const auto end = std::mismatch(first.begin(), first.begin() + static_cast<std::ptrdiff_t>(std::min(same, r.pages.size())), r.pages.begin());
+        same = static_cast<std::size_t>(end.first - first.begin());
+        keys = std::min(keys, r.length - before[i]);
+    }
+    return std::max<std::int64_t>(0, std::min(keys, static_cast<std::int64_t>(same) * page_size_));
+}
+
+}  // namespace vkml
