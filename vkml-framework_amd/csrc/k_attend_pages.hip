@@ -314,13 +314,22 @@ struct Limits {
     int32_t limit[RT];
 };
 
-// Zeros for the infinities and NaN among a masked block's V values; whether
-// any of the thread's were those of keys that count.
-template <typename T, uint32_t ROW>
-__device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t bytes, uint32_t thread, uint32_t threads, const Keys& keys, uint32_t dead) {
+// Zeros for the infinities and NaN among a masked block's V values, N 16-byte
+// pieces a thread; whether any of the thread's were those of keys that count.
+template <typename T, uint32_t ROW, int N>
+__device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t thread, uint32_t threads, const Keys& keys, uint32_t dead) {
+    // One more in the exponent carries into the sign's bit from those alone.
+    constexpr uint32_t kOne = sizeof(T) == 2 ? 0x04000400u : 0x00800000u, kSign = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(v + 16 * (thread + i * threads));
+        any |= ((x.x & ~kSign) + kOne) | ((x.y & ~kSign) + kOne) | ((x.z & ~kSign) + kOne) | ((x.w & ~kSign) + kOne);
+    }
     bool found = false;
+    if (!__any(any & kSign)) return found;
 #pragma unroll 1
-    for (uint32_t i = 16 * thread; i < bytes; i += 16 * threads) {
+    for (uint32_t i = 16 * thread; i < 16 * N * threads; i += 16 * threads) {
         const uint4 x = *reinterpret_cast<const uint4*>(v + i);
         uint32_t y[4] = {x.x, x.y, x.z, x.w};
         bool here = false;
@@ -622,7 +631,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
         if (x + kStep < p.x1) issue(nxt, k_next, there);
         const Pages after = pages_after(a, p.tile, nxt, x + 2 * kStep, kSpan);
         const bool masked = is_masked(p, cur.keys, kSpan, dead);
-        if (masked) unbounded |= clear_unbounded<T, B::kRow>(here, 8192, l, kWave, cur.keys, dead);
+        if (masked) unbounded |= clear_unbounded<T, B::kRow, 8>(here, l, kWave, cur.keys, dead);
         attend_block<T, HD, 1, TT, true, CAP>(q, lim, cur.keys, masked, dead, a.softcap, k, nullptr, here, run);
         cur = nxt;
         nxt = after;
@@ -723,7 +732,7 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
         const Pages after = pages_after(a, p.tile, nxt, x + 2 * kSpan, kSpan);
         const bool masked = is_masked(p, cur.keys, kSpan, dead);
         if (masked) {
-            unbounded |= clear_unbounded<T, B::kRow>(here + sizeof buf[0].k, sizeof buf[0].v, thread, kThreads, cur.keys, dead);
+            unbounded |= clear_unbounded<T, B::kRow, 4>(here + sizeof buf[0].k, thread, kThreads, cur.keys, dead);
             lds_barrier();
         }
         if (!idle && (cur.keys.lead || cur.keys.key0 < wave_end))
@@ -950,85 +959,153 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     }
 }
 
-// Joins the pieces of the rows that are in several. W waves take up to R query
-// heads of a (token, KV head): the pieces' (m, l) a lane each, then each wave its
-// share of their o, HD / 64 dims a lane, kFlight pieces in flight.
-template <int HD, int W, int R>
+// What the merge joins for a (token, KV head): its pieces' rows in the
+// workspace, those of the shared keys first.
+struct Joins {
+    int64_t row0, row1;
+    uint32_t n0, n, step0, step1;
+    __device__ __forceinline__ int64_t row(uint32_t p) const {
+        return p < n0 ? row0 + static_cast<int64_t>(p) * step0 : row1 + static_cast<int64_t>(p - n0) * step1;
+    }
+};
+// (none where there is nothing to join, or for rows of no sequence)
+__device__ __forceinline__ Joins joins_of(const PagesArgs& a, uint32_t at, int64_t ws_rows) {  // at: [kv_heads, tokens]
+    const uint4 both = ldg(reinterpret_cast<const uint4*>(a.parts + static_cast<uint64_t>(at) * 2));
+    const int32_t t = static_cast<int32_t>(at % a.batch.tokens);
+    const uint32_t n0 = both.y / 2, n = n0 + both.w / 2;
+    Joins j{both.x, both.z, n0, n, static_cast<uint32_t>(both.y & 1 ? kTileRows : kFewRows), static_cast<uint32_t>(both.w & 1 ? kTileRows : kFewRows)};
+    const int64_t last = ws_rows - a.group;
+    if (n == 0 || t < a.batch.start(0) || t >= a.batch.start(a.batch.seqs) || j.row(n - 1) > last || (n0 && j.row(n0 - 1) > last)) j.n = 0;
+    return j;
+}
+
+// Dims N l .. N l + N - 1 of a row.
+template <int N>
+__device__ __forceinline__ void load_dims(float (&x)[N], const float* row, uint32_t l) {
+    if constexpr (N == 2) {
+        const float2 y = ldg(reinterpret_cast<const float2*>(row) + l);
+        x[0] = y.x, x[1] = y.y;
+    } else {
+        x[0] = ldg(row + l);
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_dims(float* row, const float (&x)[N], uint32_t l) {
+    if constexpr (N == 2) stg(reinterpret_cast<float2*>(row) + l, make_float2(x[0], x[1]));
+    else stg(row + l, x[0]);
+}
+
+// Joins the pieces of the rows that are in several, few of them: a workgroup a
+// row, the pieces' (m, l) a lane each, then each wave its share of their o,
+// HD / 64 dims a lane, kFlight pieces in flight.
+template <int HD>
 __global__ void __launch_bounds__(kThreads) k_attend_pages_merge(PagesArgs a, int64_t ws_rows) {
     constexpr int N = HD / 64, kFlight = 8;
     __shared__ float s_o[kWaves][HD];
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
-    const uint32_t splits = (a.group + R - 1) / R;  // of a KV head's query heads
-    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * (kWaves / W) + w / W;
-    const uint32_t split = static_cast<uint32_t>(item % splits), at = static_cast<uint32_t>(item / splits);  // at: [kv_heads, tokens]
+    const uint32_t at = blockIdx.x / a.group, head = blockIdx.x % a.group;
+    const Joins j = joins_of(a, at, ws_rows);
+    if (j.n == 0) return;
+    float m = kLowest, lsum = 0.0f, o[N] = {};
+    for (uint32_t p0 = 0; p0 < j.n; p0 += kWave) {
+        const uint32_t many = min(j.n - p0, static_cast<uint32_t>(kWave));
+        const float2 ml = l < many ? ldg(a.stats + j.row(p0 + l) + head) : make_float2(kLowest, 0.0f);
+        // the first pieces' o before their weights are known
+        float x[kFlight][N];
+        const auto fetch = [&](uint32_t k0) {
+#pragma unroll
+            for (uint32_t k = 0; k < kFlight; ++k)  // past the last: its o again, not used
+                load_dims<N>(x[k], a.o + (j.row(p0 + min(k0 + kWaves * k, many - 1)) + head) * HD, l);
+        };
+        fetch(w);
+        const float mn = fmaxf(m, wave_max(ml.x)), factor = __builtin_amdgcn_exp2f(m - mn), weight = __builtin_amdgcn_exp2f(ml.x - mn);
+        lsum = lsum * factor + wave_sum(l < many ? weight * ml.y : 0.0f);
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] *= factor;
+        for (uint32_t k0 = w; k0 < many; k0 += kWaves * kFlight) {
+            if (k0 >= kWaves) fetch(k0);
+#pragma unroll
+            for (uint32_t k = 0; k < kFlight; ++k) {
+                if (k0 + kWaves * k >= many) break;
+                const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), k0 + kWaves * k));
+#pragma unroll
+                for (int i = 0; i < N; ++i) o[i] += f * x[k][i];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) s_o[w][N * l + i] = o[i];
+    __syncthreads();
+    if (threadIdx.x < HD) {
+        float y = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kWaves; ++i) y += s_o[i][threadIdx.x];
+        const uint32_t t = at % a.batch.tokens, kvh = at / a.batch.tokens;
+        stg(a.out + (static_cast<uint64_t>(t) * a.heads + kvh * a.group + head) * HD + threadIdx.x, y * (lsum == 0.0f ? 0.0f : 1.0f / lsum));
+    }
+}
+
+// The same for many rows, most of them in one piece or two: a wave up to four
+// query heads of a (token, KV head), (m, l) of 16 pieces of each in the lanes,
+// two pieces of each head in flight.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) k_attend_pages_merge_many(PagesArgs a, int64_t ws_rows) {
+    constexpr int N = HD / 64, kHeads = 4, kLanes = kWave / kHeads, kFlight = 2;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
+    const uint32_t splits = (a.group + kHeads - 1) / kHeads;
+    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * kWaves + w;
+    const uint32_t at = static_cast<uint32_t>(item / splits), head = static_cast<uint32_t>(item % splits) * kHeads;
     if (at >= a.kv_heads * static_cast<uint32_t>(a.batch.tokens)) return;
-    const uint4 both = ldg(reinterpret_cast<const uint4*>(a.parts + static_cast<uint64_t>(at) * 2));
-    const int32_t t = static_cast<int32_t>(at % a.batch.tokens);
-    const uint32_t kvh = at / a.batch.tokens;
-    if (t < a.batch.start(0) || t >= a.batch.start(a.batch.seqs)) return;
-    const uint32_t n0 = both.y / 2, n1 = both.w / 2, n = n0 + n1;
-    if (n == 0) return;
-    const uint32_t step0 = both.y & 1 ? kTileRows : kFewRows, step1 = both.w & 1 ? kTileRows : kFewRows;
-    const auto row_of = [&](uint32_t p) {
-        return p < n0 ? static_cast<int64_t>(both.x) + static_cast<int64_t>(p) * step0
-                      : static_cast<int64_t>(both.z) + static_cast<int64_t>(p - n0) * step1;
-    };
-    const int64_t last = ws_rows - a.group;
-    if (row_of(n - 1) > last || (n0 && row_of(n0 - 1) > last)) return;
-    for (uint32_t head = split * R; head < min(split * R + R, a.group); ++head) {
-        float m = kLowest, lsum = 0.0f, o[N];
+    const Joins j = joins_of(a, at, ws_rows);
+    if (j.n == 0) return;
+    const uint32_t last = min(head + kHeads, a.group) - 1;  // heads past it: its work again, not stored
+    const uint32_t mine = min(head + l / kLanes, last);
+    float m = kLowest, lsum = 0.0f, o[kHeads][N] = {};  // m and l of the lane's head
+    for (uint32_t p0 = 0; p0 < j.n; p0 += kLanes) {
+        const uint32_t many = min(j.n - p0, static_cast<uint32_t>(kLanes));
+        const float2 ml = l % kLanes < many ? ldg(a.stats + j.row(p0 + l % kLanes) + mine) : make_float2(kLowest, 0.0f);
+        float x[kFlight][kHeads][N];
+        const auto fetch = [&](uint32_t k0) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) o[i] = 0.0f;
-        for (uint32_t p0 = 0; p0 < n; p0 += kWave) {
-            const uint32_t many = min(n - p0, static_cast<uint32_t>(kWave));
-            const float2 ml = l < many ? ldg(a.stats + row_of(p0 + l) + head) : make_float2(kLowest, 0.0f);
-            // the first pieces' o before their weights are known
-            float x[kFlight][N];
-            const auto fetch = [&](uint32_t k0) {
+            for (uint32_t k = 0; k < kFlight; ++k) {
+                const int64_t row = j.row(p0 + min(k0 + k, many - 1));
 #pragma unroll
-                for (uint32_t k = 0; k < kFlight; ++k) {  // past the last: its o again, not used
-                    const float* from = a.o + (row_of(p0 + min(k0 + W * k, many - 1)) + head) * HD + N * l;
-                    if constexpr (N == 2) {
-                        const float2 y = ldg(reinterpret_cast<const float2*>(from));
-                        x[k][0] = y.x, x[k][1] = y.y;
-                    } else {
-                        x[k][0] = ldg(from);
-                    }
-                }
-            };
-            fetch(w % W);
-            const float mn = fmaxf(m, wave_max(ml.x)), factor = __builtin_amdgcn_exp2f(m - mn), weight = __builtin_amdgcn_exp2f(ml.x - mn);
-            lsum = lsum * factor + wave_sum(l < many ? weight * ml.y : 0.0f);
-            m = mn;
+                for (uint32_t h = 0; h < kHeads; ++h) load_dims<N>(x[k][h], a.o + (row + min(head + h, last)) * HD, l);
+            }
+        };
+        fetch(0);
+        const float mn = fmaxf(m, group_max<kLanes>(ml.x)), factor = __builtin_amdgcn_exp2f(m - mn), weight = __builtin_amdgcn_exp2f(ml.x - mn);
+        lsum = lsum * factor + group_sum<kLanes>(weight * ml.y);
+        m = mn;
 #pragma unroll
-            for (int i = 0; i < N; ++i) o[i] *= factor;
-            for (uint32_t k0 = w % W; k0 < many; k0 += W * kFlight) {
-                if (k0 >= W) fetch(k0);
+        for (uint32_t h = 0; h < kHeads; ++h) {
+            const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(factor), kLanes * h));
 #pragma unroll
-                for (uint32_t k = 0; k < kFlight; ++k) {
-                    if (k0 + W * k >= many) break;
-                    const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), k0 + W * k));
+            for (int i = 0; i < N; ++i) o[h][i] *= f;
+        }
+        for (uint32_t k0 = 0; k0 < many; k0 += kFlight) {
+            if (k0) fetch(k0);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) o[i] += f * x[k][i];
+            for (uint32_t k = 0; k < kFlight; ++k) {
+                if (k0 + k >= many) break;
+#pragma unroll
+                for (uint32_t h = 0; h < kHeads; ++h) {
+                    const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), kLanes * h + k0 + k));
+#pragma unroll
+                    for (int i = 0; i < N; ++i) o[h][i] += f * x[k][h][i];
                 }
             }
         }
-        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-        float* out = a.out + (static_cast<uint64_t>(t) * a.heads + kvh * a.group + head) * HD;
-        if constexpr (W > 1) {  // (R is 1: one round)
+    }
+    const uint32_t t = at % a.batch.tokens, kvh = at / a.batch.tokens;
 #pragma unroll
-            for (int i = 0; i < N; ++i) s_o[w][N * l + i] = o[i];
-            __syncthreads();
-            if (threadIdx.x < HD) {
-                float y = 0.0f;
+    for (uint32_t h = 0; h < kHeads; ++h) {
+        if (head + h > last) break;
+        const float sum = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lsum), kLanes * h)), inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-                for (int i = 0; i < W; ++i) y += s_o[i][threadIdx.x];
-                stg(out + threadIdx.x, y * inv);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) stg(out + N * l + i, o[i] * inv);
-        }
+        for (int i = 0; i < N; ++i) o[h][i] *= inv;
+        store_dims<N>(a.out + (static_cast<uint64_t>(t) * a.heads + kvh * a.group + head + h) * HD, o[h], l);
     }
 }
 
@@ -1118,8 +1195,8 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     const auto merge = [&](auto kernel, uint32_t workgroups) {
         hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kThreads), 0, vkml::abi::stream(), a, s.rows());
     };
-    if (rows <= 4096) wide ? merge(k_attend_pages_merge<128, kWaves, 1>, rows) : merge(k_attend_pages_merge<64, kWaves, 1>, rows);
-    else wide ? merge(k_attend_pages_merge<128, 1, 4>, (fours + kWaves - 1) / kWaves) : merge(k_attend_pages_merge<64, 1, 4>, (fours + kWaves - 1) / kWaves);
+    if (rows <= 4096) wide ? merge(k_attend_pages_merge<128>, rows) : merge(k_attend_pages_merge<64>, rows);
+    else wide ? merge(k_attend_pages_merge_many<128>, (fours + kWaves - 1) / kWaves) : merge(k_attend_pages_merge_many<64>, (fours + kWaves - 1) / kWaves);
     return vkml::abi::check_launch("attend_pages: merge");
 }
 
