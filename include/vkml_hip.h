@@ -698,7 +698,9 @@ int vkml_attend_step_noalloc(const vkml_attend_step_params* p, const float* d_qk
  * its own position (f32 attention within f32 rounding, as vkml_attend_fast;
  * with f32 caches on the f32 matrix instructions). d_q and d_out
  * [tokens, heads, head_dim] f32. softcap: 0 for none. A token without keys
- * gets zeros. head_dim 64 or 128; at most 128 query heads a KV head.
+ * gets zeros. What is not finite in a row of q, or among a token's keys and
+ * values, reaches that token's outputs only. head_dim 64 or 128; at most 128
+ * query heads a KV head; scale finite.
  *
  * groups > 0: sequences d_group_starts[g] .. d_group_starts[g + 1] (groups +
  * 1 entries that do not decrease; sequences outside every group share
@@ -709,7 +711,8 @@ int vkml_attend_step_noalloc(const vkml_attend_step_params* p, const float* d_qk
  * fill whole pages.
  *
  * d_workspace: vkml_attend_pages_workspace_bytes(p) bytes, 16-byte aligned,
- * of any content; calls that overlap need one each. */
+ * of any content (0 where the call would refuse p); calls that overlap need
+ * one each. */
 typedef struct vkml_attend_pages_params {
     uint32_t heads;
     uint32_t kv_heads;
@@ -764,7 +767,7 @@ int vkml_rope_kv_pages(const vkml_rope_kv_pages_params* p, const float* d_qkv, c
  * may be a destination twice, or a source and a destination. page_stride and
  * layer_stride (0: no gap) are bytes, multiples of 16 as page_bytes is. */
 typedef struct vkml_copy_pages_params {
-    uint32_t pages;
+    uint32_t pages;        /* at most 2^24 */
     uint32_t layers;
     uint32_t count;
     uint64_t page_bytes;   /* kv_heads * page_size * head_dim elements */

@@ -774,3 +774,100 @@ def test_prompts_forks_decoding_and_compaction(kv, style):
             while len(t) * page < m:
                 t.append(free.pop())
         step(tables, lengths, n, prompt, history)
+
+
+# ---------------------------------------------------------------- further calls
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+@pytest.mark.parametrize("softcap", [0.0, 4.0])
+def test_scales_of_either_sign_and_zero(kv, softcap):
+    rng = np.random.default_rng(40)
+    batch = Batch(rng, [5, 200, 77], [1, 30, 2], 16)
+    cache = Cache(rng, batch.pages, 2, 16, 64, kv).upload()
+    batch.upload()
+    q = rng.standard_normal((batch.tokens, 8, 64)).astype(np.float32)
+    close(Call(q, cache, batch, -0.125, softcap).run().result(), *attention_f64(-q, cache, batch, 0.125, softcap), what="negative")
+    close(Call(q, cache, batch, 0.0, softcap).run().result(), *attention_f64(q * 0, cache, batch, 0.125, softcap), what="zero")
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_row_of_q_that_is_not_finite_leaves_the_others_alone(kv, bad):
+    rng = np.random.default_rng(41)
+    batch = Batch(rng, [60, 200, 300, 301], [1, 70, 1, 1], 16, [(2, 4, 256)])
+    cache = Cache(rng, batch.pages, 2, 16, 128, kv)
+    batch.share(cache)
+    cache.upload()
+    batch.upload()
+    q = rng.standard_normal((batch.tokens, 8, 128)).astype(np.float32)
+    want, bound = attention_f64(q, cache, batch, 0.1)
+    rows = [(0, 3), (5, 0), (70, 7), (71, 2)]
+    for t, h in rows:
+        q[t, h, 17] = bad
+    got = Call(q, cache, batch, 0.1).run().result()
+    for t, h in rows:
+        assert not np.isfinite(got[t, h]).any()
+        got[t, h] = want[t, h]
+    close(got, want, bound)
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+def test_more_sequences_than_a_workgroup_has_threads(kv):
+    rng = np.random.default_rng(42)
+    lengths = rng.integers(1, 60, 700)
+    new = np.minimum(lengths, rng.choice([0, 1, 1, 1, 2, 9], 700))
+    lengths[100:400] += 40
+    batch = Batch(rng, lengths.tolist(), new.tolist(), 16, [(100, 400, 37), (400, 502, 0)])
+    cache = Cache(rng, batch.pages, 2, 16, 64, kv)
+    batch.share(cache)
+    cache.upload()
+    batch.upload()
+    q = rng.standard_normal((batch.tokens, 4, 64)).astype(np.float32)
+    close(Call(q, cache, batch, 0.125).run().result(), *attention_f64(q, cache, batch, 0.125))
+
+
+def test_two_graphs_share_a_workspace():
+    rng = np.random.default_rng(43)
+    calls = []
+    for lengths, new, groups in (([900 + i for i in range(12)], [1] * 12, [(0, 12, 800)]), ([400, 3000], [60, 1], [])):
+        batch = Batch(rng, lengths, new, 16, groups)
+        cache = Cache(rng, batch.pages, 2, 16, 128, H.F16)
+        batch.share(cache)
+        cache.upload()
+        batch.upload()
+        calls.append((rng.standard_normal((batch.tokens, 8, 128)).astype(np.float32), cache, batch))
+    workspace = H.empty(max(H.lib().vkml_attend_pages_workspace_bytes(C.byref(params(c, b, 8, 0.1))) for _, c, b in calls))
+    runs, graphs = [], []
+    try:
+        for q, c, b in calls:
+            runs.append(Call(q, c, b, 0.1, workspace=workspace))
+            graph = C.c_uint64()
+            H.call("vkml_graph_begin")
+            runs[-1].run()
+            H.call("vkml_graph_end", C.byref(graph))
+            graphs.append(graph)
+        for _ in range(3):
+            for graph in graphs:
+                H.call("vkml_graph_launch", graph)
+            for run, (q, c, b) in zip(runs, calls):
+                close(run.result(), *attention_f64(q, c, b, 0.1))
+                run.out.upload(np.full(run.shape, 7.5, np.float32))
+    finally:
+        for graph in graphs:
+            H.call("vkml_graph_destroy", graph)
+
+
+def test_copies_past_a_launch_of_pairs():
+    """More pairs than one launch takes, one source for several destinations."""
+    rng = np.random.default_rng(44)
+    pages, vectors = 1500, 3
+    pool = rng.integers(0, 2 ** 32, (2, pages, vectors * 4), dtype=np.uint32)
+    dst = rng.permutation(pages)[:1000]
+    src = rng.choice(np.setdiff1d(np.arange(pages), dst), 1000)
+    k, v = dev(pool[0]), dev(pool[1])
+    p = H.CopyPagesParams(pages=pages, layers=1, count=1000, page_bytes=16 * vectors)
+    s, d = np.ascontiguousarray(src, np.int32), np.ascontiguousarray(dst, np.int32)
+    H.call("vkml_copy_pages", C.byref(p), s.ctypes.data_as(C.c_void_p), d.ctypes.data_as(C.c_void_p), k.p, v.p)
+    pool[:, dst] = pool[:, src]
+    assert np.array_equal(k.download(np.uint32, pool[0].shape), pool[0]) and np.array_equal(v.download(np.uint32, pool[1].shape), pool[1])

@@ -276,3 +276,12 @@ def test_the_work_of_a_batch_that_breaks_the_rules_is_finite(pages):
             assert 0 <= lead <= 640 and 0 <= lead_row < n and (tiles == 0 or 0 <= row < n)
         for w, h, i, t, k0, k1, slot, few, whole, count in pieces(pages, b, 2, 4).tolist():
             assert 0 <= k0 <= k1 <= 660 + 768 and slot >= 0
+
+
+@pytest.mark.parametrize("change,why", [(dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("-inf")), "scale"),
+                                        (dict(softcap=float("inf")), "softcap")])
+def test_attend_refuses_what_is_not_finite(pages, change, why):
+    got = pages.check_attend_c(C.byref(H.AttendPagesParams(**{**ATTEND, **change})))
+    assert got is not None and why in got.decode(), got
+    for fine in (dict(scale=0.0), dict(scale=-0.1), dict(scale=3.0e38)):
+        assert pages.check_attend_c(C.byref(H.AttendPagesParams(**{**ATTEND, **fine}))) is None

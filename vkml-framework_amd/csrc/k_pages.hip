@@ -245,9 +245,11 @@ int vkml_copy_pages(const vkml_copy_pages_params* p, const int32_t* src, const i
     a.layer_stride = p->layer_stride ? p->layer_stride : p->pages * a.page_stride;
     a.vectors = static_cast<uint32_t>(p->page_bytes / 16);
     a.pieces = (a.vectors + kVectors * kThreads - 1) / (kVectors * kThreads);
+    // (a launch has less than 2^32 threads)
+    const uint32_t most = (1u << 31) / kThreads / a.pieces < kPairs ? (1u << 31) / kThreads / a.pieces : kPairs;
     vkml::abi::ProfileScope prof("copy_pages");
-    for (uint32_t i = 0; i < p->count; i += kPairs) {
-        const uint32_t n = p->count - i < kPairs ? p->count - i : kPairs;
+    for (uint32_t i = 0, n; i < p->count; i += n) {
+        n = p->count - i < most ? p->count - i : most;
         for (uint32_t j = 0; j < kPairs; ++j) {
             a.src[j] = j < n ? static_cast<uint32_t>(src[i + j]) : 0;
             a.dst[j] = j < n ? static_cast<uint32_t>(dst[i + j]) : 0;

@@ -19,6 +19,7 @@ namespace vkml::pages {
 constexpr uint32_t kMaxGroup = 128;       // query heads a KV head
 constexpr uint32_t kMaxSeqs = 1u << 16;   // sequences a batch
 constexpr uint32_t kMaxTokens = 1u << 22;  // new tokens a batch
+constexpr float kFinite = 3.402823466e+38f;
 
 VKML_HD int32_t clamp_to(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
@@ -277,7 +278,8 @@ inline const char* check(const vkml_attend_pages_params& p) {
     if (const char* why = check_cache(p.kv_heads, p.head_dim, p.kv_type, p.page_size, p.pages, p.page_stride)) return why;
     if (const char* why = check_batch(p.seqs, p.tokens, p.table_stride, p.page_size)) return why;
     if (p.groups > p.seqs) return "more groups than sequences";
-    if (!(p.softcap >= 0.0f)) return "softcap must not be negative";
+    if (!(p.softcap >= 0.0f && p.softcap <= kFinite)) return "softcap must be finite and not negative";
+    if (!(p.scale >= -kFinite && p.scale <= kFinite)) return "scale must be finite";
     return nullptr;
 }
 

@@ -77,8 +77,8 @@ struct PagedBatch {
     std::int64_t seqs = 0, tokens = 0, groups = 0;
 };
 
-// The keys and values of several sequences, in pages of `page_size` (a power
-// of two, 16 to 1024), f32 or f16, for every layer of a model.
+// The keys and values of several sequences, in up to 2^24 pages of `page_size`
+// (a power of two, 16 to 1024), f32 or f16, for every layer of a model.
 class PagedCache {
 public:
     PagedCache(Context& context, std::int64_t layers, std::int64_t kv_heads, std::int64_t head_dim, std::int64_t pages, std::int64_t page_size,

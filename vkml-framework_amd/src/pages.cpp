@@ -40,6 +40,7 @@ PagedCache::PagedCache(Context& context, std::int64_t layers, std::int64_t kv_he
     if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0) {
         throw Error("PagedCache: page_size must be a power of two from 16 to 1024, got " + std::to_string(page_size));
     }
+    if (pages > std::int64_t{1} << 24) throw Error("PagedCache: more than 2^24 pages");
     const Shape shape = {layers, pages, kv_heads, page_size, head_dim};
     k_ = Tensor::empty(context, shape, dtype);
     v_ = Tensor::empty(context, shape, dtype);
