@@ -47,7 +47,6 @@
 
 using namespace vkml::dev;
 using namespace vkml::pages;
-using vkml::attend::load_to_lds16;
 using vkml::attend_fast::f32x4;
 using vkml::attend_fast::half8;
 using vkml::attend_fast::kLog2e;
@@ -183,6 +182,15 @@ __device__ __forceinline__ const uint8_t* at_offset(const uint8_t* pool, uint64_
     return reinterpret_cast<const uint8_t*>(p);
 }
 
+// 16 bytes a lane, of the BYTES from `from` on, to `to` (the wave's first lane's)
+// in the LDS. (As a buffer load: the compiler takes global_load_lds for one that
+// the waits for the LDS count too, and every read of the LDS after it for late.)
+template <uint32_t BYTES>
+__device__ __forceinline__ void part_to_lds(const uint8_t* from, uint32_t lane_offset, uint8_t* to) {
+    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, BYTES, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)to, 16, static_cast<int>(lane_offset), 0, 0, 0);
+}
+
 // ---------------------------------------------------------------- q
 
 // Eight f32 values as two f16 terms each, two at a time, the remainder by an
@@ -249,17 +257,18 @@ struct Queries<_Float16, HD, RT> {
         }
         c[rt] = fmaxf(__builtin_amdgcn_ldexpf(fabsf(scale), e2), __FLT_MIN__);
     }
-    // The products of step s with the keys' tiles, in turn, so that an
+    // The products of step s with N of the keys' tiles, in turn, so that an
     // instruction does not wait for the one before it.
-    template <int TT>
-    __device__ __forceinline__ void score(int s, const uint4 (&k)[TT], f32x4 (&acc)[RT][TT]) const {
+    template <int N, int TT>
+    __device__ __forceinline__ void score(int s, const uint4 (&k)[N], int t0, f32x4 (&acc)[RT][TT]) const {
 #pragma unroll
         for (int term = 0; term < 2; ++term)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, k[tt]), term ? lo[rt][s] : hi[rt][s], acc[rt][tt], 0, 0, 0);
+                for (int i = 0; i < N; ++i)
+                    acc[rt][t0 + i] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, k[i]), term ? lo[rt][s] : hi[rt][s], acc[rt][t0 + i], 0, 0, 0);
     }
 };
 
@@ -273,17 +282,17 @@ struct Queries<float, HD, RT> {
         for (int i = 0; i < raw.N; ++i) x[rt][i] = make_float4(raw.x[i].x * sign, raw.x[i].y * sign, raw.x[i].z * sign, raw.x[i].w * sign);
         c[rt] = fmaxf(fabsf(scale), __FLT_MIN__);
     }
-    template <int TT>
-    __device__ __forceinline__ void score(int s, const uint4 (&k)[TT], f32x4 (&acc)[RT][TT]) const {
+    template <int N, int TT>
+    __device__ __forceinline__ void score(int s, const uint4 (&k)[N], int t0, f32x4 (&acc)[RT][TT]) const {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt) {
-                    const f32x4 y = __builtin_bit_cast(f32x4, k[tt]);
+                for (int i = 0; i < N; ++i) {
+                    const f32x4 y = __builtin_bit_cast(f32x4, k[i]);
                     const float4 z = x[rt][s];
-                    acc[rt][tt] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[e], e == 0 ? z.x : e == 1 ? z.y : e == 2 ? z.z : z.w, acc[rt][tt], 0, 0, 0);
+                    acc[rt][t0 + i] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[e], e == 0 ? z.x : e == 1 ? z.y : e == 2 ? z.z : z.w, acc[rt][t0 + i], 0, 0, 0);
                 }
     }
 };
@@ -348,6 +357,10 @@ __device__ __forceinline__ bool clear_unbounded(uint8_t* v, uint32_t thread, uin
     return found;
 }
 
+// What may move across the order that a loop of reads and products fixes: the
+// other VALU, SALU and transcendental instructions.
+constexpr int kOnlyAlu = 0x406;
+
 // One block of TT tiles of 16 keys, K in the lane's registers (REGS) or as
 // swizzled rows in the LDS, V's rows in the LDS. masked: some rows don't see
 // all of its keys. dead: a bit for each tile that is in no page.
@@ -368,17 +381,32 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) s[rt][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (REGS) {
 #pragma unroll
-    for (int st = 0; st < static_cast<int>(B::kSteps); ++st) {
-        uint4 kk[TT];
+        for (int st = 0; st < static_cast<int>(B::kSteps); ++st) {
+            uint4 kk[TT];
 #pragma unroll
-        for (int tt = 0; tt < TT; ++tt) {
-            if constexpr (REGS) kk[tt] = k_regs[tt][st];
-            else kk[tt] = *reinterpret_cast<const uint4*>(k + (k_at ^ (64 * st)) + 16 * tt * B::kRow);
+            for (int tt = 0; tt < TT; ++tt) kk[tt] = k_regs[tt][st];
+            q.score(st, kk, 0, s);
         }
-        q.score(st, kk, s);
+    } else {
+        // N tiles of a step at a time, the next ones' read before the products.
+        constexpr int N = RT == 1 && TT >= 4 ? 4 : 2, kGroups = static_cast<int>(B::kSteps) * TT / N;
+        uint4 kk[2][N];
+        const auto fetch = [&](int i, uint4 (&to)[N]) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) to[n] = *reinterpret_cast<const uint4*>(k + (k_at ^ (64 * (i / (TT / N)))) + 16 * (i % (TT / N) * N + n) * B::kRow);
+        };
+        fetch(0, kk[0]);
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+            if (i + 1 < kGroups) fetch(i + 1, kk[(i + 1) % 2]);
+            __builtin_amdgcn_sched_barrier(kOnlyAlu);
+            q.score(i / (TT / N), kk[i % 2], i % (TT / N) * N, s);
+            __builtin_amdgcn_sched_barrier(kOnlyAlu);
+        }
+        __builtin_amdgcn_s_setprio(0);
     }
-    if constexpr (!REGS) __builtin_amdgcn_s_setprio(0);
     constexpr float kShift = B::kF16 ? 14.0f : 0.0f;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -436,32 +464,44 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         // group: it points at row 4 g + j / 4, dims 4 (j % 4) on, and gets dim
         // j of the four rows.
         const uint32_t row = 4 * g + j / 4, at = row * B::kRow + 16 * ((j % 4 / 2) ^ B::swizzle_v(row)) + 8 * (j % 2);
-        constexpr int D = RT == 1 && HD == 128 ? 8 : 4;  // tiles of dims read at a time
-        if constexpr (!REGS) __builtin_amdgcn_s_setprio(1);
+        // D tiles of dims at a time; the next ones' read before the products where
+        // K comes from the LDS too.
+        constexpr int D = REGS ? (HD == 128 ? 8 : 4) : RT == 1 ? 4 : 2, kAt = HD / 16 / D, kGroups = TT / 2 * kAt;
+        const auto fetch = [&](int i, half8 (&to)[D]) {
 #pragma unroll
-        for (int u = 0; u < TT / 2; ++u) {
-            half8 ph[RT], pl[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) split(s[rt][2 * u], s[rt][2 * u + 1], ph[rt], pl[rt]);
-#pragma unroll
-            for (int d0 = 0; d0 < HD / 16; d0 += D) {
-                half8 vv[D];
-#pragma unroll
-                for (int i = 0; i < D; ++i) {
-                    const uint8_t* to = v + (at ^ (32 * (d0 + i))) + 32 * u * B::kRow;
-                    const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(to));
-                    const auto y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(to + 16 * B::kRow));
-                    const uint2 xx = __builtin_bit_cast(uint2, x), yy = __builtin_bit_cast(uint2, y);
-                    vv[i] = __builtin_bit_cast(half8, make_uint4(xx.x, xx.y, yy.x, yy.y));
-                }
-#pragma unroll
-                for (int term = 0; term < 2; ++term)
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int i = 0; i < D; ++i)
-                            run.o[rt][d0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv[i], term ? pl[rt] : ph[rt], run.o[rt][d0 + i], 0, 0, 0);
+            for (int d = 0; d < D; ++d) {
+                const uint8_t* from = v + (at ^ (32 * (i % kAt * D + d))) + 32 * (i / kAt) * B::kRow;
+                const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(from));
+                const auto y = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds4)(from + 16 * B::kRow));
+                const uint2 xx = __builtin_bit_cast(uint2, x), yy = __builtin_bit_cast(uint2, y);
+                to[d] = __builtin_bit_cast(half8, make_uint4(xx.x, xx.y, yy.x, yy.y));
             }
+        };
+        half8 ph[RT], pl[RT], vv[REGS ? 1 : 2][D];
+        if constexpr (!REGS) {
+            __builtin_amdgcn_s_setprio(1);
+            fetch(0, vv[0]);
+        }
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) {
+            if (i % kAt == 0) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) split(s[rt][2 * (i / kAt)], s[rt][2 * (i / kAt) + 1], ph[rt], pl[rt]);
+            }
+            half8(&now)[D] = vv[REGS ? 0 : i % 2];
+            if constexpr (REGS) fetch(i, now);
+            else if (i + 1 < kGroups) fetch(i + 1, vv[(i + 1) % 2]);
+            if constexpr (!REGS) __builtin_amdgcn_sched_barrier(kOnlyAlu);
+#pragma unroll
+            for (int term = 0; term < 2; ++term)
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int d = 0; d < D; ++d) {
+                        f32x4& o = run.o[rt][i % kAt * D + d];
+                        o = __builtin_amdgcn_mfma_f32_16x16x32_f16(now[d], term ? pl[rt] : ph[rt], o, 0, 0, 0);
+                    }
+            if constexpr (!REGS) __builtin_amdgcn_sched_barrier(kOnlyAlu);
         }
         if constexpr (!REGS) __builtin_amdgcn_s_setprio(0);
     } else {
@@ -607,7 +647,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) {
             const uint32_t u = 64 * i + l, row = u / B::kPieces;
-            load_to_lds16(v_part[64 * i / B::kPieces / 16] + (row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row))), to + 1024 * i);
+            part_to_lds<16 * B::kRow>(v_part[64 * i / B::kPieces / 16], row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row)), to + 1024 * i);
         }
     };
     uint4 k[TT][B::kSteps];
@@ -704,8 +744,8 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
             const int32_t key = at.keys.key0 + static_cast<int32_t>((i * kThreads + w * kWave) / B::kPieces / 16 * 16);
             const uint64_t part = offset_of<B::kRow>(a, p.tile.kvh, page_of(a, at, key), key);
             uint8_t* k_to = to + 16 * (i * kThreads + w * kWave);
-            load_to_lds16(at_offset(a.k, part) + (row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row))), k_to);
-            load_to_lds16(at_offset(a.v, part) + (row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row))), k_to + sizeof buf[0].k);
+            part_to_lds<16 * B::kRow>(at_offset(a.k, part), row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row)), k_to);
+            part_to_lds<16 * B::kRow>(at_offset(a.v, part), row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row)), k_to + sizeof buf[0].k);
         }
     };
     int32_t x = p.x0;
@@ -971,11 +1011,11 @@ struct Joins {
 // (none where there is nothing to join, or for rows of no sequence)
 __device__ __forceinline__ Joins joins_of(const PagesArgs& a, uint32_t at, int64_t ws_rows) {  // at: [kv_heads, tokens]
     const uint4 both = ldg(reinterpret_cast<const uint4*>(a.parts + static_cast<uint64_t>(at) * 2));
-    const int32_t t = static_cast<int32_t>(at % a.batch.tokens);
+    const int32_t t = static_cast<int32_t>(at % a.batch.tokens), first = a.batch.start(0), end = a.batch.start(a.batch.seqs);
     const uint32_t n0 = both.y / 2, n = n0 + both.w / 2;
     Joins j{both.x, both.z, n0, n, static_cast<uint32_t>(both.y & 1 ? kTileRows : kFewRows), static_cast<uint32_t>(both.w & 1 ? kTileRows : kFewRows)};
     const int64_t last = ws_rows - a.group;
-    if (n == 0 || t < a.batch.start(0) || t >= a.batch.start(a.batch.seqs) || j.row(n - 1) > last || (n0 && j.row(n0 - 1) > last)) j.n = 0;
+    if (n == 0 || t < first || t >= end || j.row(n - 1) > last || (n0 && j.row(n0 - 1) > last)) j.n = 0;
     return j;
 }
 

@@ -79,17 +79,18 @@ constexpr int32_t kTileRows = 128;
 constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
 
 // A tile's cost: a key's times its keys, and one of its own for its queries,
-// its first loads, its joining and storing. Measured (us, two workgroups a
-// compute unit): f16, head_dim 128, 64 keys of a tile of few rows, which memory
-// bounds, 1.6 and of another 2.7, by itself the one 4.1, the other 6.5; f16 at 64
-// 0.66, -, 3.4, -; f32 at 64 1.6, 3.8, 1.7, 1.2.
+// its first loads, its joining and storing. Measured (us, 64 keys, two
+// workgroups a compute unit): f16, head_dim 128, a tile of few rows, which
+// memory bounds, 1.1 beside one of many, and that one 3.4 beside it, 4.0 beside
+// its like; by themselves the tiles take 8 and 10, some of it while the other
+// workgroup works. f32, head_dim 64: 1.6 and 3.8; 1.7 and 1.2.
 struct Costs {
     int32_t few_key, tile_key, few_own, tile_own;
 };
 constexpr int32_t kMinPart = 1024;  // the cost below which work is not cut further
 VKML_HD Costs costs(uint32_t head_dim, bool f16) {
     const int32_t few = static_cast<int32_t>(head_dim / (f16 ? 16 : 8));
-    return {few, few + few * 3 / 4, f16 ? 2000 : 600, f16 ? 2400 : 600};
+    return {few, f16 ? 3 * few : few + few * 3 / 4, f16 ? 2600 : 600, f16 ? 3600 : 600};
 }
 
 VKML_HD int32_t tile_tokens(int32_t group) { return kTileRows / group > 1 ? kTileRows / group : 1; }
