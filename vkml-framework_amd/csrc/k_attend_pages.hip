@@ -750,11 +750,9 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
     };
     int32_t x = p.x0;
     Pages cur = pages_at(a, p.tile, x), nxt = cur;
-    // The wave's rows that are none of the tile's take no part; nor do blocks
-    // past all that the wave's rows see.
-    const int32_t last_row = static_cast<int32_t>(min(first + 16 * RT, rows)) - 1;
-    const int32_t wave_end = p.causal ? p.limit0 + static_cast<int32_t>(token_of(a, last_row)) : p.limit0;
-    const bool idle = first >= rows;
+    // (Waves without rows, and blocks past all that a wave's rows see, are not left
+    // out: the sums would be copied where the ways join, 64 registers twice a
+    // block, and the workgroup's other waves are waited for in any case.)
     bool unbounded = false;  // as in few_rows
     const auto block = [&](uint8_t* __restrict__ here, uint8_t* __restrict__ there) {
         if (x == p.x0) {
@@ -775,8 +773,7 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
             unbounded |= clear_unbounded<T, B::kRow, 4>(here + sizeof buf[0].k, thread, kThreads, cur.keys, dead);
             lds_barrier();
         }
-        if (!idle && (cur.keys.lead || cur.keys.key0 < wave_end))
-            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, masked, dead, a.softcap, nullptr, here, here + sizeof buf[0].k, run);
+        attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, masked, dead, a.softcap, nullptr, here, here + sizeof buf[0].k, run);
         cur = nxt;
         nxt = after;
         x += kSpan;
