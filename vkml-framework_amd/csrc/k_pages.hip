@@ -65,32 +65,24 @@ __device__ __forceinline__ void write(T* p, const Part<W>& r) {
     }
 }
 
-// Workgroup (x, y): U kThreads units of token x. A unit is 2 W values of one
-// head that one thread takes: W pairs of a turned part, or 2 W consecutive dims
-// of an unturned one (v, and q's and k's dims from rotary_dim on). A thread's
-// values are loaded first; where its token stands is found meanwhile.
-template <int W, typename T, int U>
+// Workgroup (x, y): kThreads units of token x. A unit is 2 W values of one head
+// that one thread takes: W pairs of a turned part, or 2 W consecutive dims of an
+// unturned one (v, and q's and k's dims from rotary_dim on). A thread's values
+// are loaded first; where its token stands is found meanwhile. Bound by memory:
+// 7900 tokens of 32 + 2 * 8 heads of 128 (355 MB read and written) in 68 us, 5.2
+// TB/s, where a large copy reaches 5.0; 32 such tokens 3.6 us, a launch. Two or
+// three units a thread, their loads in flight together, took as long.
+template <int W, typename T>
 __global__ void __launch_bounds__(kThreads) k_rope_kv_pages(RopeArgs a) {
     const int32_t t = static_cast<int32_t>(blockIdx.x);
     const uint32_t hd = a.head_dim, r = a.rotary_dim, per_head = hd / (2 * W), turned = r / (2 * W), units = (a.heads + 2 * a.kv_heads) * per_head;
     const float* row = a.qkv + static_cast<uint64_t>(t) * a.row_stride;
-    uint32_t head[U], e[U], ia[U], ib[U];
-    Part<W> x[U], y[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-        const uint32_t u = min((blockIdx.y * U + i) * kThreads + threadIdx.x, units - 1);  // the last again past it, not stored
-        head[i] = u / per_head;
-        e[i] = u % per_head;
-        if (head[i] >= a.heads + a.kv_heads) e[i] += turned;  // v: no part of it is turned
-        ia[i] = 2 * W * (e[i] - (head[i] >= a.heads + a.kv_heads ? turned : 0));
-        ib[i] = ia[i] + W;
-        if (e[i] < turned && a.style == 1) {
-            ia[i] = W * e[i];
-            ib[i] = r / 2 + W * e[i];
-        }
-        x[i] = read<W>(row + head[i] * hd + ia[i]);
-        y[i] = read<W>(row + head[i] * hd + ib[i]);
-    }
+    const uint32_t unit = blockIdx.y * kThreads + threadIdx.x, u = min(unit, units - 1);  // past the last: that again, not stored
+    const uint32_t head = u / per_head;
+    const bool is_v = head >= a.heads + a.kv_heads;
+    const bool turns = !is_v && u % per_head < turned;
+    const uint32_t e = u % per_head, ia = turns && a.style == 1 ? W * e : 2 * W * e, ib = turns && a.style == 1 ? r / 2 + W * e : ia + W;
+    Part<W> x = read<W>(row + head * hd + ia), y = read<W>(row + head * hd + ib);
     int32_t s = t;
     if (a.batch.starts) {  // the sequences that end at or before the token
         s = 0;
@@ -99,60 +91,55 @@ __global__ void __launch_bounds__(kThreads) k_rope_kv_pages(RopeArgs a) {
             s += __syncthreads_count(j < a.batch.seqs && a.batch.start(j + 1) <= t);
         }
     }
-    if (s >= a.batch.seqs || t < a.batch.start(s)) return;
+    if (s >= a.batch.seqs || t < a.batch.start(s) || unit >= units) return;
     const int32_t pos = a.batch.length(s) - a.batch.count(s) + t - a.batch.start(s);
-    const int32_t turn = a.at ? a.at[t] : pos;
-    const bool held = static_cast<uint32_t>(turn) < a.positions;
-    const int32_t page = pos >= 0 && pos < a.batch.table_keys ? a.table[static_cast<uint64_t>(s) * a.table_stride + pos / a.page_size] : -1;
-    const bool kept = static_cast<uint32_t>(page) < a.pages;
-    const float* angles = a.angles + static_cast<uint64_t>(held ? turn : 0) * r;
+    const int32_t page =
+        head >= a.heads && pos >= 0 && pos < a.batch.table_keys ? ldg(a.table + static_cast<uint64_t>(s) * a.table_stride + pos / a.page_size) : -1;
+    if (turns) {
+        const int32_t turn = a.at ? a.at[t] : pos;
+        float c[W], d[W];  // cos and sin of the unit's pairs
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-        if ((blockIdx.y * U + i) * kThreads + threadIdx.x >= units) break;
-        if (e[i] < turned) {
-            float c[W], d[W];  // cos and sin of the unit's pairs
-#pragma unroll
-            for (int j = 0; j < W; ++j) c[j] = d[j] = __builtin_nanf("");
-            if (held) {
-                if constexpr (W == 4) {
-                    const Part<4> lo = read<4>(angles + 8 * e[i]), hi = read<4>(angles + 8 * e[i] + 4);
-                    c[0] = lo.x[0], d[0] = lo.x[1], c[1] = lo.x[2], d[1] = lo.x[3];
-                    c[2] = hi.x[0], d[2] = hi.x[1], c[3] = hi.x[2], d[3] = hi.x[3];
-                } else {
-                    c[0] = ldg(angles + 2 * e[i]);
-                    d[0] = ldg(angles + 2 * e[i] + 1);
-                }
-            }
-            const Part<W> f = x[i], g = y[i];
-            if (W == 1 || a.style == 1) {  // the pairs are (f[j], g[j])
-#pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    x[i].x[j] = f.x[j] * c[j] - g.x[j] * d[j];
-                    y[i].x[j] = f.x[j] * d[j] + g.x[j] * c[j];
-                }
-            } else {  // neighbours in the 2 W values
-#pragma unroll
-                for (int j = 0; j < W / 2; ++j) {
-                    x[i].x[2 * j] = f.x[2 * j] * c[j] - f.x[2 * j + 1] * d[j];
-                    x[i].x[2 * j + 1] = f.x[2 * j] * d[j] + f.x[2 * j + 1] * c[j];
-                    y[i].x[2 * j] = g.x[2 * j] * c[W / 2 + j] - g.x[2 * j + 1] * d[W / 2 + j];
-                    y[i].x[2 * j + 1] = g.x[2 * j] * d[W / 2 + j] + g.x[2 * j + 1] * c[W / 2 + j];
-                }
+        for (int j = 0; j < W; ++j) c[j] = d[j] = __builtin_nanf("");
+        if (static_cast<uint32_t>(turn) < a.positions) {
+            const float* angles = a.angles + static_cast<uint64_t>(turn) * r;
+            if constexpr (W == 4) {
+                const Part<4> lo = read<4>(angles + 8 * e), hi = read<4>(angles + 8 * e + 4);
+                c[0] = lo.x[0], d[0] = lo.x[1], c[1] = lo.x[2], d[1] = lo.x[3];
+                c[2] = hi.x[0], d[2] = hi.x[1], c[3] = hi.x[2], d[3] = hi.x[3];
+            } else {
+                c[0] = ldg(angles + 2 * e);
+                d[0] = ldg(angles + 2 * e + 1);
             }
         }
-        if (head[i] < a.heads) {
-            float* to = a.q + (static_cast<uint64_t>(t) * a.heads + head[i]) * hd;
-            write<W>(to + ia[i], x[i]);
-            write<W>(to + ib[i], y[i]);
-        } else if (kept) {
-            const bool is_v = head[i] >= a.heads + a.kv_heads;
-            const uint32_t kvh = head[i] - a.heads - (is_v ? a.kv_heads : 0);
-            T* to = static_cast<T*>(is_v ? a.v : a.k) + static_cast<uint64_t>(page) * a.page_stride +
-                    (static_cast<uint64_t>(kvh) * a.page_size + pos % a.page_size) * hd;
-            write<W>(to + ia[i], x[i]);
-            write<W>(to + ib[i], y[i]);
+        const Part<W> f = x, g = y;
+        if (W == 1 || a.style == 1) {  // the pairs are (f[j], g[j])
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                x.x[j] = f.x[j] * c[j] - g.x[j] * d[j];
+                y.x[j] = f.x[j] * d[j] + g.x[j] * c[j];
+            }
+        } else {  // neighbours in the 2 W values
+#pragma unroll
+            for (int j = 0; j < W / 2; ++j) {
+                x.x[2 * j] = f.x[2 * j] * c[j] - f.x[2 * j + 1] * d[j];
+                x.x[2 * j + 1] = f.x[2 * j] * d[j] + f.x[2 * j + 1] * c[j];
+                y.x[2 * j] = g.x[2 * j] * c[W / 2 + j] - g.x[2 * j + 1] * d[W / 2 + j];
+                y.x[2 * j + 1] = g.x[2 * j] * d[W / 2 + j] + g.x[2 * j + 1] * c[W / 2 + j];
+            }
         }
     }
+    if (head < a.heads) {
+        float* to = a.q + (static_cast<uint64_t>(t) * a.heads + head) * hd;
+        write<W>(to + ia, x);
+        write<W>(to + ib, y);
+        return;
+    }
+    if (static_cast<uint32_t>(page) >= a.pages) return;
+    const uint32_t kvh = head - a.heads - (is_v ? a.kv_heads : 0);
+    T* to = static_cast<T*>(is_v ? a.v : a.k) + static_cast<uint64_t>(page) * a.page_stride +
+            (static_cast<uint64_t>(kvh) * a.page_size + pos % a.page_size) * hd;
+    write<W>(to + ia, x);
+    write<W>(to + ib, y);
 }
 
 // ---------------------------------------------------------------- page copies
@@ -170,6 +157,8 @@ struct CopyArgs {
 constexpr uint32_t kVectors = 4;  // vectors a thread has in flight
 
 // Workgroup x: piece x % pieces of pair x / pieces; y the layer, z the pool.
+// Bound by memory: 31 pages of 128 KiB in 32 layers of two pools (260 MB read and
+// as much written) in 98 us, 5.3 TB/s; a large copy reaches 5.0.
 __global__ void __launch_bounds__(kThreads) k_copy_pages(CopyArgs a) {
     const uint32_t pair = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
     uint8_t* base = a.pool[blockIdx.z] + blockIdx.y * a.layer_stride;
@@ -208,19 +197,11 @@ int vkml_rope_kv_pages(const vkml_rope_kv_pages_params* p, const float* qkv, con
     const bool wide = p->head_dim % 8 == 0 && p->rotary_dim % 8 == 0 && p->row_stride % 4 == 0 && aligned16(qkv) && aligned16(rope_table) &&
                       aligned16(q) && aligned16(k_pages) && aligned16(v_pages);
     const uint32_t units = (p->heads + 2 * p->kv_heads) * (p->head_dim / (wide ? 8 : 2));
-    // Few tokens: as many workgroups as their units give; many: a thread has
-    // several units' loads in flight.
-    const uint32_t rounds = (units + kThreads - 1) / kThreads;
-    const uint32_t each = p->tokens * rounds <= 4 * vkml::abi::compute_units() || rounds < 2 ? 1 : rounds == 2 ? 2 : 3;
-    const dim3 grid(p->tokens, (rounds + each - 1) / each);
+    const dim3 grid(p->tokens, (units + kThreads - 1) / kThreads);
     vkml::abi::ProfileScope prof("rope_kv_pages");
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, vkml::abi::stream(), a); };
-    const auto pick = [&](auto t) {
-        using T = decltype(t);
-        if (!wide) each == 1 ? go(k_rope_kv_pages<1, T, 1>) : each == 2 ? go(k_rope_kv_pages<1, T, 2>) : go(k_rope_kv_pages<1, T, 3>);
-        else each == 1 ? go(k_rope_kv_pages<4, T, 1>) : each == 2 ? go(k_rope_kv_pages<4, T, 2>) : go(k_rope_kv_pages<4, T, 3>);
-    };
-    p->kv_type == VKML_F16 ? pick(_Float16{}) : pick(0.0f);
+    if (p->kv_type == VKML_F16) wide ? go(k_rope_kv_pages<4, _Float16>) : go(k_rope_kv_pages<1, _Float16>);
+    else wide ? go(k_rope_kv_pages<4, float>) : go(k_rope_kv_pages<1, float>);
     return vkml::abi::check_launch("rope_kv_pages");
 }
 
