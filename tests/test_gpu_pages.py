@@ -871,3 +871,21 @@ def test_copies_past_a_launch_of_pairs():
     H.call("vkml_copy_pages", C.byref(p), s.ctypes.data_as(C.c_void_p), d.ctypes.data_as(C.c_void_p), k.p, v.p)
     pool[:, dst] = pool[:, src]
     assert np.array_equal(k.download(np.uint32, pool[0].shape), pool[0]) and np.array_equal(v.download(np.uint32, pool[1].shape), pool[1])
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+@pytest.mark.parametrize("scale,softcap", [(0.125, 1e-39), (3e38, 0.0), (-3e38, 2.0)])
+def test_extreme_scales_of_rows_that_are_zero(kv, scale, softcap):
+    """Every score is 0 (or a cap that is as good as 0): the values' mean."""
+    rng = np.random.default_rng(45)
+    batch = Batch(rng, [5, 200], [1, 30], 16)
+    cache = Cache(rng, batch.pages, 2, 16, 64, kv).upload()
+    batch.upload()
+    q = np.zeros((batch.tokens, 8, 64), np.float32)
+    close(Call(q, cache, batch, scale, softcap).run().result(), *attention_f64(q, cache, batch, 0.125))
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+@pytest.mark.parametrize("softcap", [0.25, 1.0, 7.0, 50.0])
+def test_softcaps_small_and_large(kv, softcap):
+    attend(46, 8, 2, 64, 16, kv, [90, 300, 400], [1, 100, 2], softcap=softcap, q_scale=3.0)
