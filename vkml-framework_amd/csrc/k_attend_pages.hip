@@ -119,6 +119,7 @@ struct Block {
 struct Buffer {
     alignas(16) uint8_t k[16384];
     alignas(16) uint8_t v[16384];
+    __device__ __forceinline__ uint8_t* all() { return reinterpret_cast<uint8_t*>(this); }
 };
 
 // Where the keys of a tile are (pages.hpp's axis: the lead, then its own).
@@ -191,13 +192,16 @@ __device__ __forceinline__ const uint8_t* at_offset(const uint8_t* pool, uint64_
     return reinterpret_cast<const uint8_t*>(p);
 }
 
-// 16 bytes a lane, of the BYTES from `from` on, to `to` (the wave's first lane's)
-// in the LDS. (As a buffer load: the compiler takes global_load_lds for one that
-// the waits for the LDS count too, and every read of the LDS after it for late.)
-template <uint32_t BYTES>
-__device__ __forceinline__ void part_to_lds(const uint8_t* from, uint32_t lane_offset, uint8_t* to) {
-    const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, BYTES, 0x00020000);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)to, 16, static_cast<int>(lane_offset), 0, 0, 0);
+// The `bytes` of a pool from `from` on, as loads take them: nothing past them is
+// read (of 0 bytes nothing at all: zeros).
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_of_pool(const uint8_t* from, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(from), 0, static_cast<int>(bytes), 0x00020000);
+}
+// 16 bytes a lane to `to` (the wave's first lane's) in the LDS. (A buffer load: the
+// compiler takes global_load_lds for one that the waits for the LDS count too, and
+// every read of the LDS after it for late.)
+__device__ __forceinline__ void part_to_lds(__amdgpu_buffer_rsrc_t part, uint32_t lane_offset, uint8_t* to) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(part, (__attribute__((address_space(3))) void*)to, 16, static_cast<int>(lane_offset), 0, 0, 0);
 }
 
 // ---------------------------------------------------------------- q
@@ -537,7 +541,7 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
                 const uint32_t row = 16 * tt + 4 * g + e;
 #pragma unroll
                 for (int dt = 0; dt < HD / 16; ++dt) {
-                    const float vv = *reinterpret_cast<const float*>(v + row * B::kRow + 16 * ((4 * dt + j / 4) ^ B::swizzle_v(row)) + 4 * (j % 4));
+                    const float vv = *reinterpret_cast<const float*>(v + (row * B::kRow + 16 * ((4 * dt + j / 4) ^ B::swizzle_v(row)) + 4 * (j % 4)));
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) run.o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv, s[rt][tt][e], run.o[rt][dt], 0, 0, 0);
                 }
@@ -562,8 +566,17 @@ struct Piece {
 // wrote there is there, and what they read is read (unlike __syncthreads(),
 // stores to memory need not have arrived).
 __device__ __forceinline__ void lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Every load of the wave has landed, those to the LDS among them. (The builtin:
+// what asm waits for, the compiler would wait for again.)
+__device__ __forceinline__ void loads_landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     asm volatile("" ::: "memory");
 }
 
@@ -642,7 +655,7 @@ __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Piece& p
 
 // At most 16 rows: each wave by itself over blocks of kWaveKeys keys in turn.
 template <typename T, int HD, bool CAP>
-__device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buffer* buf) {
+__device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buffer& buf0, Buffer& buf1) {
     using B = Block<T, HD>;
     constexpr int TT = B::kWaveTiles;
     const uint32_t thread = thread_index(), w = __builtin_amdgcn_readfirstlane(thread / kWave), l = thread % kWave, j = l % 16, g = l / 16;
@@ -650,73 +663,75 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
     Limits<1> lim{{p.limit0}};
     Running<HD, 1> run;
     run.clear();
-    uint8_t* v = reinterpret_cast<uint8_t*>(buf) + 8192 * w;  // and as far into the second buffer
     constexpr int32_t kStep = kWaves * B::kWaveKeys, kSpan = B::kWaveKeys;
-    const int32_t first = p.x0 + static_cast<int32_t>(w) * kSpan;
-    int32_t x = first;
+    int32_t x = p.x0 + static_cast<int32_t>(w) * kSpan;
     const auto issue = [&](const Pages& at, uint4 (&k)[TT][B::kSteps], uint8_t* to) {
-        const uint8_t *k_part[TT], *v_part[TT];
+        __amdgpu_buffer_rsrc_t k_part[TT], v_part[TT];
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
             const int32_t key = at.keys.key0 + 16 * i;
             const uint64_t part = offset_of<B::kRow>(a, p.tile.kvh, page_of(a, at, key), key);
-            k_part[i] = at_offset(a.k, part);
-            v_part[i] = at_offset(a.v, part);
+            k_part[i] = part_of_pool(at_offset(a.k, part), 16 * B::kRow);
+            v_part[i] = part_of_pool(at_offset(a.v, part), 16 * B::kRow);
         }
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int s = 0; s < static_cast<int>(B::kSteps); ++s)
-                k[tt][s] = ldg(reinterpret_cast<const uint4*>(k_part[tt] + (j * B::kRow + 64 * s + 16 * g)));
+                k[tt][s] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(k_part[tt], static_cast<int>(j * B::kRow + 64 * s + 16 * g), 0, 0));
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) {
             const uint32_t u = 64 * i + l, row = u / B::kPieces;
-            part_to_lds<16 * B::kRow>(v_part[64 * i / B::kPieces / 16], row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row)), to + 1024 * i);
+            part_to_lds(v_part[64 * i / B::kPieces / 16], row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row)), to + 1024 * i);
         }
     };
-    uint4 k[TT][B::kSteps];
-    Pages cur = pages_at(a, p.tile, x), nxt = cur;
     // Values of V that are not finite in blocks that some rows see less of than
     // others are left out of the product and added at the end.
     bool unbounded = false;
-    // The buffers don't overlap. Said so (__restrict__), and with both's loads
-    // issued in here, the reads of one do not wait for the loads into the other.
-    const auto block = [&](uint8_t* __restrict__ here, uint8_t* __restrict__ there) {
-        if (x == first) {
-            RawRow<T, HD> raw[1];
-            load_rows(a, p, 0, raw, lim);
-            issue(cur, k, here);
-            nxt = pages_after(a, p.tile, cur, x + kStep, kSpan);
-            q.take(0, raw[0], a.score_scale);
+    // The buffers are variables of their own, used by turns, and a load into each
+    // (for the second, of nothing) is on every way to the loop: that is what it takes
+    // for the compiler not to let reads of one wait for the loads into the other.
+    const auto blocks = [&](uint8_t* v0, uint8_t* v1) {
+        uint4 k0[TT][B::kSteps], k1[TT][B::kSteps];
+        RawRow<T, HD> raw[1];
+        Pages cur = pages_at(a, p.tile, x);
+        load_rows(a, p, 0, raw, lim);
+        part_to_lds(part_of_pool(a.v, 0), 0, v1);
+        issue(cur, k0, v0);
+        Pages nxt = pages_after(a, p.tile, cur, x + kStep, kSpan);
+        q.take(0, raw[0], a.score_scale);
+        const auto block = [&](uint4 (&k)[TT][B::kSteps], uint8_t* here, uint4 (&k_next)[TT][B::kSteps], uint8_t* there) {
+            loads_landed();  // this block's, and the next one's pages
+            const uint32_t dead = dead_tiles<TT>(a, cur);
+            if (x + kStep < p.x1) issue(nxt, k_next, there);
+            const Pages after = pages_after(a, p.tile, nxt, x + 2 * kStep, kSpan);
+            const bool masked = is_masked(p, cur.keys, kSpan, dead);
+            if (masked) unbounded |= clear_unbounded<T, B::kRow, 8>(here, l, kWave, cur.keys, dead);
+            attend_block<T, HD, 1, TT, true, CAP>(q, lim, cur.keys, masked, dead, a.softcap, k, nullptr, here, run);
+            cur = nxt;
+            nxt = after;
+            x += kStep;
+        };
+        for (;;) {
+            block(k0, v0, k1, v1);
+            if (x >= p.x1) break;
+            block(k1, v1, k0, v0);
+            if (x >= p.x1) break;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this block and the next one's pages have landed
-        uint4 k_next[TT][B::kSteps] = {};
-        const uint32_t dead = dead_tiles<TT>(a, cur);
-        if (x + kStep < p.x1) issue(nxt, k_next, there);
-        const Pages after = pages_after(a, p.tile, nxt, x + 2 * kStep, kSpan);
-        const bool masked = is_masked(p, cur.keys, kSpan, dead);
-        if (masked) unbounded |= clear_unbounded<T, B::kRow, 8>(here, l, kWave, cur.keys, dead);
-        attend_block<T, HD, 1, TT, true, CAP>(q, lim, cur.keys, masked, dead, a.softcap, k, nullptr, here, run);
-        cur = nxt;
-        nxt = after;
-        x += kStep;
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int s = 0; s < static_cast<int>(B::kSteps); ++s) k[tt][s] = k_next[tt][s];
     };
-    for (uint32_t n = 0; x < p.x1; n ^= sizeof(Buffer)) block(v + n, v + (n ^ sizeof(Buffer)));
+    if (x < p.x1) blocks(buf0.all() + 8192 * w, buf1.all() + 8192 * w);
     // The waves' parts join in the LDS, rows HD + 4 floats apart.
     const float sum = lanes_sum(run.l[0]);
     constexpr uint32_t kStride = HD + 4;
-    float* part = reinterpret_cast<float*>(buf);  // [waves][16][kStride], then [waves][16] of (m, l)
-    float2* ml = reinterpret_cast<float2*>(part + kWaves * 16 * kStride);
+    // [16][kStride] of a wave, two waves a buffer; then [waves][16] of (m, l)
+    const auto part = [&](uint32_t wave) { return reinterpret_cast<float*>(wave < 2 ? buf0.all() : buf1.all()) + wave % 2 * 16 * kStride; };
+    float2* ml = reinterpret_cast<float2*>(part(0) + 2 * 16 * kStride);
     uint32_t* found = reinterpret_cast<uint32_t*>(ml + kWaves * 16);  // [waves]
     const bool mine = __any(unbounded);
     lds_barrier();
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt)
-        *reinterpret_cast<f32x4*>(part + (16 * w + j) * kStride + 16 * dt + 4 * g) = run.o[0][dt];
+        *reinterpret_cast<f32x4*>(part(w) + j * kStride + 16 * dt + 4 * g) = run.o[0][dt];
     if (g == 0) ml[16 * w + j] = make_float2(run.m[0], sum);
     if (l == 0) found[w] = mine;
     lds_barrier();
@@ -738,7 +753,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (uint32_t i = 0; i < kWaves; ++i) {
-                const f32x4 y = *reinterpret_cast<const f32x4*>(part + (16 * i + r) * kStride + dim);
+                const f32x4 y = *reinterpret_cast<const f32x4*>(part(i) + r * kStride + dim);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] += f[i] * y[e];
             }
@@ -750,7 +765,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
 
 // Many rows: RT tiles of 16 a wave, the blocks shared.
 template <typename T, int HD, int RT, bool CAP>
-__device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Buffer* buf) {
+__device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Buffer& buf0, Buffer& buf1) {
     using B = Block<T, HD>;
     constexpr int TT = B::kTiles;
     constexpr int32_t kSpan = B::kKeys;
@@ -768,41 +783,48 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
             const int32_t key = at.keys.key0 + static_cast<int32_t>((i * kThreads + w * kWave) / B::kPieces / 16 * 16);
             const uint64_t part = offset_of<B::kRow>(a, p.tile.kvh, page_of(a, at, key), key);
             uint8_t* k_to = to + 16 * (i * kThreads + w * kWave);
-            part_to_lds<16 * B::kRow>(at_offset(a.k, part), row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row)), k_to);
-            part_to_lds<16 * B::kRow>(at_offset(a.v, part), row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row)), k_to + sizeof buf[0].k);
+            part_to_lds(part_of_pool(at_offset(a.k, part), 16 * B::kRow), row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_k(row)), k_to);
+            part_to_lds(part_of_pool(at_offset(a.v, part), 16 * B::kRow), row % 16 * B::kRow + 16 * (u % B::kPieces ^ B::swizzle_v(row)), k_to + sizeof buf0.k);
         }
     };
     int32_t x = p.x0;
-    Pages cur = pages_at(a, p.tile, x), nxt = cur;
     // (Waves without rows, and blocks past all that a wave's rows see, are not left
     // out: the sums would be copied where the ways join, 64 registers twice a
     // block, and the workgroup's other waves are waited for in any case.)
-    bool unbounded = false;  // as in few_rows
-    const auto block = [&](uint8_t* __restrict__ here, uint8_t* __restrict__ there) {
-        if (x == p.x0) {
-            RawRow<T, HD> raw[RT];
-            load_rows(a, p, first, raw, lim);
-            issue(cur, here);
-            nxt = pages_after(a, p.tile, cur, x + kSpan, kSpan);
+    bool unbounded = false;
+    const auto blocks = [&](uint8_t* b0, uint8_t* b1) {  // as in few_rows
+        RawRow<T, HD> raw[RT];
+        Pages cur = pages_at(a, p.tile, x);
+        load_rows(a, p, first, raw, lim);
+        part_to_lds(part_of_pool(a.v, 0), 0, b1 + 1024 * w);
+        issue(cur, b0);
+        Pages nxt = pages_after(a, p.tile, cur, x + kSpan, kSpan);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) q.take(rt, raw[rt], a.score_scale);
+        for (int rt = 0; rt < RT; ++rt) q.take(rt, raw[rt], a.score_scale);
+        const auto block = [&](uint8_t* here, uint8_t* there) {
+            loads_landed();
+            lds_barrier();  // every wave's loads have landed, and the other buffer is read no more
+            const uint32_t dead = dead_tiles<TT>(a, cur);
+            if (x + kSpan < p.x1) issue(nxt, there);
+            const Pages after = pages_after(a, p.tile, nxt, x + 2 * kSpan, kSpan);
+            const bool masked = is_masked(p, cur.keys, kSpan, dead);
+            if (masked) {
+                unbounded |= clear_unbounded<T, B::kRow, 4>(here + sizeof buf0.k, thread, kThreads, cur.keys, dead);
+                lds_barrier();
+            }
+            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, masked, dead, a.softcap, nullptr, here, here + sizeof buf0.k, run);
+            cur = nxt;
+            nxt = after;
+            x += kSpan;
+        };
+        for (;;) {
+            block(b0, b1);
+            if (x >= p.x1) break;
+            block(b1, b0);
+            if (x >= p.x1) break;
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        lds_barrier();  // every wave's loads have landed, and the other buffer is read no more
-        const uint32_t dead = dead_tiles<TT>(a, cur);
-        if (x + kSpan < p.x1) issue(nxt, there);
-        const Pages after = pages_after(a, p.tile, nxt, x + 2 * kSpan, kSpan);
-        const bool masked = is_masked(p, cur.keys, kSpan, dead);
-        if (masked) {
-            unbounded |= clear_unbounded<T, B::kRow, 4>(here + sizeof buf[0].k, thread, kThreads, cur.keys, dead);
-            lds_barrier();
-        }
-        attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, masked, dead, a.softcap, nullptr, here, here + sizeof buf[0].k, run);
-        cur = nxt;
-        nxt = after;
-        x += kSpan;
     };
-    for (uint32_t n = 0; x < p.x1; n ^= 1) block(buf[n].k, buf[n ^ 1].k);
+    if (x < p.x1) blocks(buf0.all(), buf1.all());
     const bool found = __syncthreads_or(unbounded);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -951,7 +973,7 @@ __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scrat
 template <typename T, int HD, bool CAP>
 __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     using B = Block<T, HD>;
-    __shared__ Buffer buf[2];
+    __shared__ Buffer buf0, buf1;  // apart: the compiler then knows that they are
     __shared__ Scratch scratch;
     Place at;
     if (!find_place(a, at, scratch)) return;
@@ -1007,9 +1029,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             }
             if (again) lds_barrier();  // the last piece's LDS
             again = true;
-            if (s.few) few_rows<T, HD, CAP>(a, p, buf);
-            else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1, CAP>(a, p, buf);
-            else many_rows<T, HD, 2, CAP>(a, p, buf);
+            if (s.few) few_rows<T, HD, CAP>(a, p, buf0, buf1);
+            else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1, CAP>(a, p, buf0, buf1);
+            else many_rows<T, HD, 2, CAP>(a, p, buf0, buf1);
             if (end <= 0) return;
         }
         (s.few ? few : tiles) += s.tiles;
