@@ -36,11 +36,11 @@
 // cleared in the LDS before the product. So are infinities and NaN of keys that
 // some rows see and others don't, which are added to those rows at the end.
 //
-// Measured (32 query and 8 KV heads of 128, f16): one token over 32768 keys 31 us
-// and 5 to join its pieces, 134 MB at 4.3 TB/s (a large copy reaches 5.0); 64
-// sequences with 32768 shared keys and 1000 of their own 124 us and 9 (407 MB and
-// 71 GFLOP, the split counted twice: memory and the matrix units half each);
-// 2600 tokens of six prompts 147 us and 16, 115 GFLOP issued at 780 TFLOP/s.
+// Measured (32 query and 8 KV heads of 128, f16): one token over 32768 keys 30 us
+// and 5 to join its pieces, 134 MB at 4.4 TB/s (a large copy reaches 5.0); 64
+// sequences with 32768 shared keys and 1000 of their own 112 us and 8 (407 MB and
+// 71 GFLOP, the split counted twice: memory and the matrix units at once); 2600
+// tokens of six prompts 148 us and 16, 115 GFLOP issued at 780 TFLOP/s.
 // Short ones are a chain of waits: 1.0 us for the batch's arrays, 0.8 to find the
 // part, 1.3 its first tile, 1.2 for pages and keys, 2 to 3 the block, 0.8 the end.
 #include <hip/hip_runtime.h>
