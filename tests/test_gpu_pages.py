@@ -889,3 +889,57 @@ def test_extreme_scales_of_rows_that_are_zero(kv, scale, softcap):
 @pytest.mark.parametrize("softcap", [0.25, 1.0, 7.0, 50.0])
 def test_softcaps_small_and_large(kv, softcap):
     attend(46, 8, 2, 64, 16, kv, [90, 300, 400], [1, 100, 2], softcap=softcap, q_scale=3.0)
+
+
+def test_a_captured_step_appends_and_copies():
+    """Rope into pages, a page copy and attention in one graph: replayed with
+    new lengths and inputs between eager work, each replay as the eager calls."""
+    rng = np.random.default_rng(47)
+    heads, kv_heads, hd, page, stride, pages = 8, 2, 64, 16, 4, 12
+    table = rng.permutation(pages - 2)[:8].astype(np.int32).reshape(2, stride)
+    cache = Cache(rng, pages, kv_heads, page, hd, H.F16)
+    angles = rng.standard_normal((64, hd // 2, 2)).astype(np.float32)
+    src, dst = np.asarray([table[0, 0], table[1, 1]], np.int32), np.asarray([pages - 2, pages - 1], np.int32)
+    order = dict(heads=heads, kv_heads=kv_heads, head_dim=hd, kv_type=H.F16, page_size=page, pages=pages, seqs=2, tokens=2, table_stride=stride)
+    r = H.RopeKvPagesParams(**order, row_stride=(heads + 2 * kv_heads) * hd, rotary_dim=hd, positions=64)
+    a = H.AttendPagesParams(**order, scale=0.125)
+    c = H.CopyPagesParams(pages=pages, layers=1, count=2, page_bytes=2 * kv_heads * page * hd)
+    workspace = H.empty(H.lib().vkml_attend_pages_workspace_bytes(C.byref(a)))
+    d_table, d_angles, src_p, dst_p = dev(table), dev(angles), src.copy(), dst.copy()
+
+    class Side:
+        def __init__(self):
+            self.k, self.v = dev(cache.k), dev(cache.v)
+            self.qkv, self.lengths = dev(np.zeros((2, (heads + 2 * kv_heads) * hd), np.float32)), dev(np.zeros(2, np.int32))
+            self.q, self.out = dev(np.zeros((2, heads, hd), np.float32)), dev(np.zeros((2, heads, hd), np.float32))
+
+        def step(self):
+            H.call("vkml_rope_kv_pages", C.byref(r), self.qkv.p, d_angles.p, d_table.p, self.lengths.p, None, None, self.q.p, self.k.p, self.v.p)
+            H.call("vkml_copy_pages", C.byref(c), src_p.ctypes.data_as(C.c_void_p), dst_p.ctypes.data_as(C.c_void_p), self.k.p, self.v.p)
+            H.call("vkml_attend_pages", C.byref(a), self.q.p, self.k.p, self.v.p, d_table.p, self.lengths.p, None, None, None, workspace.p, self.out.p)
+
+        def results(self):
+            return [b.download(t, n) for b, t, n in ((self.k, np.uint16, cache.k.shape), (self.v, np.uint16, cache.k.shape),
+                                                    (self.q, np.uint32, (2, heads, hd)), (self.out, np.uint32, (2, heads, hd)))]
+
+    replayed, eager = Side(), Side()
+    graph = C.c_uint64()
+    H.call("vkml_graph_begin")
+    replayed.step()
+    H.call("vkml_graph_end", C.byref(graph))
+    src_p[:], dst_p[:] = -1, -1  # read when the calls were made
+    try:
+        for i in range(4):
+            qkv, lengths = rng.standard_normal((2, (heads + 2 * kv_heads) * hd)).astype(np.float32), np.asarray([1 + i, 30 + 9 * i], np.int32)
+            for side in (replayed, eager):
+                side.qkv.upload(qkv)
+                side.lengths.upload(lengths)
+            H.call("vkml_graph_launch", graph)
+            got = replayed.results()
+            src_p[:], dst_p[:] = src, dst
+            eager.step()
+            src_p[:], dst_p[:] = -1, -1
+            for x, y in zip(got, eager.results()):
+                assert np.array_equal(x, y)
+    finally:
+        H.call("vkml_graph_destroy", graph)
