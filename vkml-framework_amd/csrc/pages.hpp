@@ -87,7 +87,10 @@ constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
 struct Costs {
     int32_t few_key, tile_key, few_own, tile_own;
 };
-constexpr int32_t kMinPart = 1024;  // the cost below which work is not cut further
+// The cost below which work is not cut further. Measured (us a call, with 1024, 512
+// and 256): 8 sequences, 2000 shared keys, f32, head_dim 64, 19.6, 17.8, 17.8; one
+// sequence of 2000 keys 13.3, 12.1, 13.8; three of 5 to 40 11.2, 11.0, 12.5.
+constexpr int32_t kMinPart = 512;
 VKML_HD Costs costs(uint32_t head_dim, bool f16) {
     const int32_t few = static_cast<int32_t>(head_dim / (f16 ? 16 : 8));
     return {few, f16 ? 3 * few : few + few * 3 / 4, f16 ? 2600 : 600, f16 ? 3600 : 600};
