@@ -943,3 +943,55 @@ def test_a_captured_step_appends_and_copies():
                 assert np.array_equal(x, y)
     finally:
         H.call("vkml_graph_destroy", graph)
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+@pytest.mark.parametrize("lengths,new,groups", [([0], [1], []), ([100, 0], [1, 1], []), ([40, 0], [1, 40], []), ([0] * 64, [1] * 64, []),
+                                                ([700, 33, 512] + [0] * 13, [1] * 16, []), ([520, 501, 505, 0, 0], [1] * 5, [(0, 3, 500)]), ([0, 90, 3], [33, 20, 9], [])])
+def test_empty_sequences_get_zeros(lengths, new, groups, kv):
+    """A padded batch's empty slots, last among them, over a workspace that
+    holds another call's pieces and records."""
+    rng = np.random.default_rng(48)
+    other = Batch(rng, [900 + i for i in range(70)], [1] * 70, 16, [(0, 70, 800)])
+    other_cache = Cache(rng, other.pages, 8, 16, 64, kv)
+    other.share(other_cache)
+    other_cache.upload()
+    other.upload()
+    batch = Batch(rng, lengths, new, 16, groups)
+    cache = Cache(rng, batch.pages, 8, 16, 64, kv)
+    batch.share(cache)
+    cache.upload()
+    batch.upload()
+    q = rng.standard_normal((max(70, batch.tokens), 32, 64)).astype(np.float32)
+    print("empty sequences", lengths, new, groups, kv, flush=True)
+    workspace = H.empty(max(H.lib().vkml_attend_pages_workspace_bytes(C.byref(params(c, b, 32, 0.125))) for c, b in ((other_cache, other), (cache, batch))))
+    Call(q[:70], other_cache, other, 0.125, workspace=workspace).run()
+    got = Call(q[:batch.tokens], cache, batch, 0.125, starts=max(new) > 1, workspace=workspace).run().result()
+    close(got, *attention_f64(q[:batch.tokens], cache, batch, 0.125))
+    seen = [length - n + i + 1 for length, n in zip(lengths, new) for i in range(n)]
+    for t, keys in enumerate(seen):
+        assert got[t].any() == (keys > 0), t
+
+
+def test_a_captured_call_follows_sequences_that_end():
+    rng = np.random.default_rng(49)
+    batch = Batch(rng, [300, 200, 100, 50], [1] * 4, 16, stride=20)
+    cache = Cache(rng, batch.pages, 8, 16, 64, H.F16).upload()
+    batch.upload()
+    q = rng.standard_normal((4, 32, 64)).astype(np.float32)
+    call = Call(q, cache, batch, 0.125, starts=False)
+    graph = C.c_uint64()
+    H.call("vkml_graph_begin")
+    call.run()
+    H.call("vkml_graph_end", C.byref(graph))
+    try:
+        for lengths in ([300, 200, 100, 50], [300, 200, 100, 0], [300, 0, 0, 0], [0, 0, 0, 0], [0, 0, 0, 50]):
+            batch.lengths = lengths
+            batch.d_lengths.upload(np.asarray(lengths, np.int32))
+            call.out.upload(np.full(call.shape, 7.5, np.float32))
+            H.call("vkml_graph_launch", graph)
+            got = call.result()
+            close(got, *attention_f64(q, cache, batch, 0.125))
+            assert got.any((1, 2)).tolist() == [n > 0 for n in lengths]
+    finally:
+        H.call("vkml_graph_destroy", graph)

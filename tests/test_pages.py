@@ -285,3 +285,38 @@ def test_attend_refuses_what_is_not_finite(pages, change, why):
     assert got is not None and why in got.decode(), got
     for fine in (dict(scale=0.0), dict(scale=-0.1), dict(scale=3.0e38)):
         assert pages.check_attend_c(C.byref(H.AttendPagesParams(**{**ATTEND, **fine}))) is None
+
+
+EMPTY = [([0], [1]), ([100, 0], [1, 1]), ([2, 2, 2, 0], [1, 1, 1, 1]), ([40, 0], [1, 40]), ([0] * 64, [1] * 64), ([0, 0, 0], [40, 1, 200]), ([0, 700, 0, 3, 0], [1, 300, 33, 7, 4]),
+         ([3000] * 5 + [0] * 27, [1] * 32), ([33, 20, 5], [50, 20, 40])]
+
+
+@pytest.mark.parametrize("block", [32, 64, 128])
+@pytest.mark.parametrize("workgroups_log2", [3, 9])
+@pytest.mark.parametrize("kv_heads,group", [(1, 1), (2, 4), (8, 4), (2, 3), (1, 16), (1, 128)])
+def test_the_parts_cover_tokens_without_keys(pages, kv_heads, group, workgroups_log2, block):
+    """Empty slots of a padded batch, last, alone and among others, and more
+    new tokens than keys: a tile whose cost is its own cost alone belongs to
+    the part that reaches its end."""
+    for lengths, new in EMPTY:
+        check_cut(pages, lengths, new, None, None, kv_heads, group, workgroups_log2, block)
+    # behind and before a group, and in one that shares nothing
+    check_cut(pages, [520, 501, 505, 0, 0], [1] * 5, [0, 3], [500], kv_heads, group, workgroups_log2, block)
+    check_cut(pages, [0, 520, 501, 0], [1] * 4, [1, 3], [500], kv_heads, group, workgroups_log2, block)
+    check_cut(pages, [0, 0, 0], [1] * 3, [0, 3], [0], kv_heads, group, workgroups_log2, block)
+
+
+def test_the_parts_of_a_batch_that_breaks_the_rules_cover_its_tiles(pages):
+    rng = np.random.default_rng(3)
+    edge = [-2 ** 31, -1, 0, 1, 5, 64, 65, 1000, 2 ** 31 - 1]
+    for _ in range(200):
+        n = int(rng.integers(1, 9))
+        pick = lambda k: rng.choice(edge, k)  # noqa: E731
+        g = int(rng.integers(0, n + 1))
+        b, keep = batch(pick(n), pick(n + 1), pick(g + 1), pick(g), 20, 640)
+        got, seg = pieces(pages, b, 2, 4), segments(pages, b, 4)
+        tiles = {}
+        for w, h, i, t, k0, k1, slot, few, whole, count in got.tolist():
+            tiles.setdefault((h, i, t), []).append(count)
+        assert len(tiles) == 2 * sum(x[5] for x in seg.tolist())
+        assert all(p[0] == len(p) for p in tiles.values())

@@ -217,8 +217,10 @@ VKML_HD int32_t part_of(int64_t cost, int32_t n_log2, int64_t u) {
     return w;
 }
 // Where the tile of s with `cost` is cut at unit x of it: at its start (0), its
-// end (cost) or between (x).
+// end (cost) or between (x). Its end comes first: a tile without keys has its own
+// cost alone, and the part that ends with it takes it.
 VKML_HD int32_t snap(int64_t x, const Segment& s, int32_t cost) {
+    if (x >= cost) return cost;
     if (x <= s.own_cost) return 0;
     return x >= cost - s.own_cost / 8 ? cost : static_cast<int32_t>(x);
 }
