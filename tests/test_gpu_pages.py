@@ -995,3 +995,71 @@ def test_a_captured_call_follows_sequences_that_end():
             assert got.any((1, 2)).tolist() == [n > 0 for n in lengths]
     finally:
         H.call("vkml_graph_destroy", graph)
+
+
+LARGE = [(2.0 ** 25, 0.0), (2.0 ** 27, 0.0), (2.0 ** 30, 0.0), (2.0 ** 33, 0.0), (2.0 ** 60, 0.0), (2.0 ** 100, 0.0), (2.0 ** 25, 2.0 ** 28), (2.0 ** 30, 1e30)]
+
+
+def large_scores(seed, kv, heads, kv_heads, lengths, new, groups, make_k):
+    rng = np.random.default_rng(seed)
+    batch = Batch(rng, lengths, new, 16, groups)
+    cache = Cache(rng, batch.pages, kv_heads, 16, 128, kv)
+    cache.k[:] = make_k(rng, cache.k.shape)
+    batch.share(cache)
+    cache.upload()
+    batch.upload()
+    return rng, batch, cache
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+@pytest.mark.parametrize("size,softcap", LARGE)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_large_scores_that_are_equal(sign, size, softcap, kv):
+    """Every key of a head is the same, so that a row's scores, of about
+    `size`, are equal to the last bit: each is the same products in the same
+    order. All weights are 1 and the output is the values' mean, whatever the
+    score's own rounding: the sums' share of the bound above, without delta
+    and x."""
+    lengths, new, groups = [40, 700, 900, 20, 333], [1, 1, 1, 1, 60], [(1, 3, 300)]
+    rng, batch, cache = large_scores(51, kv, 8, 2, lengths, new, groups,
+                                     lambda r, shape: np.broadcast_to(np.abs(r.standard_normal((1, shape[1], 1, shape[3]))) + 0.5, shape))
+    q = np.abs(rng.standard_normal((batch.tokens, 8, 128))).astype(np.float32)
+    scale = sign * size / 100  # q k is 80 to 160
+    got = Call(q, cache, batch, scale, softcap).run().result()
+    want, _ = attention_f64(q * 0, cache, batch, 0.1)
+    plain, _ = attention_f64(q * 0, cache, batch, 0.1, v=np.abs(cache.v))
+    keys = np.concatenate([np.arange(length - n, length) + 1 for length, n in zip(lengths, new)])
+    close(got, want, plain * ((keys / 16 + 64) * 2.0 ** -24 + 2.0 ** -20)[:, None, None], f"{size} {softcap}")
+
+
+@pytest.mark.parametrize("kv", [H.F16, H.F32])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 25, 2.0 ** 27, 2.0 ** 30, 2.0 ** 33, 2.0 ** 60, 2.0 ** 100])
+def test_large_scores_pick_the_largest(size, kv):
+    """Scores of random signs of about `size`: a row whose largest stands out
+    by more than the scores' errors (delta and 2^-22 max|x| of the bound
+    above, on either side) and 64 more has the weight 1 for that key and less
+    than e^-64 for each other one, so that its output is that key's value,
+    within the weight's and the sums' rounding. Rows without such a key stay
+    finite and among the values."""
+    lengths, new, groups = [40, 700, 900, 20, 333], [1, 1, 1, 1, 60], [(1, 3, 300)]
+    rng, batch, cache = large_scores(52, kv, 8, 2, lengths, new, groups, lambda r, shape: r.standard_normal(shape))
+    q = rng.standard_normal((batch.tokens, 8, 128)).astype(np.float32)
+    scale = size / 11.3
+    got = Call(q, cache, batch, scale).run().result().astype(np.float64)
+    picked = 0
+    for s, (length, n) in enumerate(zip(lengths, new)):
+        kk, _ = rows_of(cache, cache.k, batch.table[s], length)
+        vv, _ = rows_of(cache, cache.v, batch.table[s], length)
+        for i in range(n):
+            t, seen = batch.starts[s] + i, length - n + i + 1
+            for h in range(8):
+                K, V, Q = kk[:seen, h // 4].astype(np.float64), vv[:seen, h // 4].astype(np.float64), q[t, h].astype(np.float64)
+                x = K @ Q * scale
+                off = scale * (2.0 ** -22 * np.abs(Q).max() * np.abs(K).sum(1) + 136 * 2.0 ** -24 * (np.abs(K) @ np.abs(Q))).max() + 2.0 ** -22 * np.abs(x).max()
+                most = np.abs(V).max(0)
+                assert np.all(np.abs(got[t, h]) <= most * (1 + 2.0 ** -10)), (t, h, got[t, h])
+                order = np.argsort(x)
+                if seen == 1 or x[order[-1]] - x[order[-2]] > 2 * off + 64:
+                    picked += 1
+                    assert np.all(np.abs(got[t, h] - V[order[-1]]) <= np.abs(V[order[-1]]) * ((seen / 16 + 64) * 2.0 ** -24 + 2.0 ** -20) + seen * math.exp(-64) * most), (t, h)
+    assert picked > 8 * batch.tokens * 0.9

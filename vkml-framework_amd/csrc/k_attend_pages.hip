@@ -313,7 +313,8 @@ struct Queries<float, HD, RT> {
 // ---------------------------------------------------------------- a block
 
 // What a wave has of RT tiles of 16 rows: lane (j, g) has row j's dims 16 dt +
-// 4 g + e, its maximum, and the sum over the keys of its own lane.
+// 4 g + e, its maximum (of the scores as attend_block has them), and the sum over
+// the keys of its own lane.
 template <int HD, int RT>
 struct Running {
     f32x4 o[RT][HD / 16];
@@ -389,13 +390,27 @@ __device__ __forceinline__ float tanh_of(float y) {
     return z < 0.4f ? __builtin_fmaf(y * z, p, y) : __builtin_copysignf(far, y);
 }
 
+// What turns a row's maximum as attend_block keeps it into log2 units: f16 caches
+// keep the product with the row of q as it is, a soft cap natural units. Within
+// f32's range, so that the maxima of two parts can be subtracted.
+template <typename T, bool CAP>
+__device__ __forceinline__ float in_log2(float m, float c) {
+    return __builtin_amdgcn_fmed3f(CAP ? m * kLog2e : sizeof(T) == 2 ? m * c : m, kLowest, __FLT_MAX__);
+}
+
 // One block of TT tiles of 16 keys, K in the lane's registers (REGS) or as
 // swizzled rows in the LDS, V's rows in the LDS. masked: some rows don't see
 // all of its keys. dead: a bit for each tile that is in no page.
+//
+// A weight is 2^(c (x - m)), the difference taken of the values whose maximum m is:
+// it is 0 at the maximum, however large x is. (2^(c x - c m) by an fma is one
+// instruction less, but its two products round apart: at scores of 2^25 the
+// maximum's weight was up to four times too large, past f16's range.)
 template <typename T, int HD, int RT, int TT, bool REGS, bool CAP>
 __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const Limits<RT>& lim, const Keys& keys, bool masked, uint32_t dead, float softcap,
                                              const uint4 (*k_regs)[Block<T, HD>::kSteps], const uint8_t* k, const uint8_t* v,
                                              Running<HD, RT>& run) {
+#pragma clang fp contract(off)
     using B = Block<T, HD>;
     // (from a fresh thread index, so that the addresses are not kept in
     // registers from one block to the next)
@@ -445,6 +460,11 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[rt][tt][e] = softcap * tanh_of(s[rt][tt][e] * c);
             c = kLog2e;
+        } else if constexpr (!B::kF16) {  // q k^T itself may be near the end of f32's range
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[rt][tt][e] *= c;
         }
         if (masked) {
             const int32_t limit = keys.lead ? keys.end : lim.limit[rt];
@@ -465,17 +485,18 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         bm = fmaxf(__uint_as_float(a16.x), __uint_as_float(a16.y));
         const uint2 a32 = swap_rows<32>(__float_as_uint(bm));
         bm = fmaxf(__uint_as_float(a32.x), __uint_as_float(a32.y));
-        const float mn = fmaxf(run.m[rt], bm * c), factor = __builtin_amdgcn_exp2f(run.m[rt] - mn), mm = mn - kShift;
+        constexpr bool kLog2 = !B::kF16 && !CAP;  // in log2 units already
+        const float mn = fmaxf(run.m[rt], bm), down = run.m[rt] - mn, factor = __builtin_amdgcn_exp2f(kLog2 ? down : down * c);
         float bs = 0.0f;
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][tt][e], c, -mm));
+                const float x = s[rt][tt][e] - mn, p = __builtin_amdgcn_exp2f(kLog2 ? x : __builtin_fmaf(x, c, kShift));
                 s[rt][tt][e] = p;
                 bs += p;
             }
-        run.l[rt] = run.l[rt] * factor + bs;
+        run.l[rt] = __builtin_fmaf(run.l[rt], factor, bs);
         run.m[rt] = mn;
         // Once the maxima have settled, most blocks leave the output's scale.
         if (__any(factor != 1.0f)) {
@@ -660,6 +681,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
     constexpr int TT = B::kWaveTiles;
     const uint32_t thread = thread_index(), w = __builtin_amdgcn_readfirstlane(thread / kWave), l = thread % kWave, j = l % 16, g = l / 16;
     Queries<T, HD, 1> q;
+    q.c[0] = 1.0f;  // where there are no keys
     Limits<1> lim{{p.limit0}};
     Running<HD, 1> run;
     run.clear();
@@ -732,7 +754,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
 #pragma unroll
     for (int dt = 0; dt < HD / 16; ++dt)
         *reinterpret_cast<f32x4*>(part(w) + j * kStride + 16 * dt + 4 * g) = run.o[0][dt];
-    if (g == 0) ml[16 * w + j] = make_float2(run.m[0], sum);
+    if (g == 0) ml[16 * w + j] = make_float2(in_log2<T, CAP>(run.m[0], q.c[0]), sum);
     if (l == 0) found[w] = mine;
     lds_barrier();
     const uint32_t r = thread / 16;
@@ -772,6 +794,8 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
     const uint32_t thread = thread_index(), w = __builtin_amdgcn_readfirstlane(thread / kWave), l = thread % kWave, j = l % 16, g = l / 16;
     const uint32_t rows = p.tokens * a.group, first = 16 * RT * w;
     Queries<T, HD, RT> q;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) q.c[rt] = 1.0f;  // where there are no keys
     Limits<RT> lim;
     Running<HD, RT> run;
     run.clear();
@@ -832,7 +856,7 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
         const uint32_t r = first + 16 * rt + j;
         if (r < rows) {
             float times;
-            float* to = row_to<HD>(a, p, r, g == 0, run.m[rt], sum, times);
+            float* to = row_to<HD>(a, p, r, g == 0, in_log2<T, CAP>(run.m[rt], q.c[rt]), sum, times);
             if (to) {
 #pragma unroll
                 for (int dt = 0; dt < HD / 16; ++dt) {
