@@ -184,3 +184,78 @@ def test_refusals(exe):
         assert got.startswith("error: PageTable") and why in got, (words, got)
         assert t.state() == before
     t.close()
+
+
+@pytest.fixture(scope="module")
+def host_check(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("bin") / "paged_cache_host_check")
+    pkg = os.path.join(ROOT, "vkml-framework_amd")
+    subprocess.run(["g++", "-std=c++20", "-O1", "-g", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover", "-I" + os.path.join(pkg, "include"),
+                    "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(pkg, "src"), os.path.join(ROOT, "tests", "cpp", "paged_cache_host_check.cpp"),
+                    *(os.path.join(pkg, "src", f) for f in ("pages.cpp", "page_table.cpp", "runtime.cpp")), "-o", out], check=True)
+    return out
+
+
+def test_a_cache_that_fails_changes_nothing(host_check):
+    """vkml::PagedCache over a C ABI in host memory whose n-th call fails:
+    every batch and compaction that throws leaves the lengths, the pages and
+    the keys as they were."""
+    r = subprocess.run([host_check], capture_output=True, text=True, timeout=100)
+    print(r.stdout)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert sum(line.startswith("ok ") for line in r.stdout.split("\n")) == 4
+
+
+@pytest.fixture(scope="module")
+def exe_undo(tmp_path_factory):
+    """The check program with two verbs more: "undo", and "append-undo", an
+    append that is taken back where it succeeded."""
+    d = tmp_path_factory.mktemp("bin")
+    with open(os.path.join(ROOT, "tests", "cpp", "page_table_check.cpp")) as f:
+        source = f.read()
+    verb = 'if (verb == "compact")'
+    assert source.count(verb) == 1
+    more = ['if (verb == "append-undo") table.undo(ids, counts, table.append(ids, counts));', 'if (verb == "undo") table.undo(ids, counts, copies);', verb]
+    (d / "undo.cpp").write_text(source.replace(verb, "\n                ".join(more)))
+    out = str(d / "undo")
+    subprocess.run(["g++", "-std=c++20", "-O1", "-Wall", "-Werror", "-I" + os.path.join(ROOT, "vkml-framework_amd", "include"), str(d / "undo.cpp"),
+                    os.path.join(ROOT, "vkml-framework_amd", "src", "page_table.cpp"), "-o", out], check=True)
+    return out
+
+
+@pytest.mark.parametrize("seed", [0, 1, 2])
+def test_an_append_taken_back_leaves_no_trace(exe_undo, seed):
+    rng = np.random.default_rng(seed)
+    t = Table(exe_undo, 30, 4)
+    for _ in range(300):
+        ids = list(t.want)
+        what = rng.choice(["create", "fork", "append", "undo", "undo", "truncate", "release", "compact"])
+        if what == "create" and len(ids) < 6:
+            t.want[t.numbers("create")[0]] = []
+        elif what == "fork" and ids and len(ids) < 9:
+            i = int(rng.choice(ids))
+            t.want[t.numbers("fork", i)[0]] = list(t.want[i])
+        elif what in ("append", "undo") and ids:
+            some = [int(i) for i in rng.permutation(ids)[:rng.integers(1, len(ids) + 1)]]
+            counts = [int(rng.choice([0, 1, 1, 2, 4, 7])) for _ in some]
+            if what == "append":
+                t.append(some, counts)
+            else:
+                before = t.state()
+                t.ask("append-undo", *[w for pair in zip(some, counts) for w in pair])
+                assert t.state() == before
+        elif what == "truncate" and ids:
+            i = int(rng.choice(ids))
+            n = int(rng.integers(0, len(t.want[i]) + 1))
+            assert t.ask("truncate", i, n) == ""
+            del t.want[i][n:]
+        elif what == "release" and len(ids) > 3:
+            i = int(rng.choice(ids))
+            assert t.ask("release", i) == ""
+            del t.want[i]
+        elif what == "compact":
+            t.copies(t.numbers("compact"))
+        t.check()
+    assert t.ask("undo", 99, 1).startswith("error: PageTable") and t.ask("undo", next(iter(t.want)), 10 ** 6).startswith("error: PageTable")
+    t.check()
+    t.close()

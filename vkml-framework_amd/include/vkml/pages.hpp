@@ -38,6 +38,9 @@ public:
     // copies are to be made before those keys are written.
     std::vector<PageCopy> append(std::span<const std::int64_t> ids, std::span<const std::int64_t> tokens);
     std::vector<PageCopy> append(std::int64_t id, std::int64_t tokens) { return append(std::span(&id, 1), std::span(&tokens, 1)); }
+    // Takes back the append that returned `copies`, where they or the keys could
+    // not be written; no other call may have changed the table since.
+    void undo(std::span<const std::int64_t> ids, std::span<const std::int64_t> tokens, std::span<const PageCopy> copies);
 
     // The pages in use become the lowest ones: the rows change, and the copies
     // are to be made before anything is read or written through them.
@@ -78,7 +81,9 @@ struct PagedBatch {
 };
 
 // The keys and values of several sequences, in up to 2^24 pages of `page_size`
-// (a power of two, 16 to 1024), f32 or f16, for every layer of a model.
+// (a power of two, 16 to 1024), f32 or f16, for every layer of a model. What
+// throws changes nothing: a batch that is refused, or for which there is no
+// memory, leaves every sequence with the keys that it had.
 class PagedCache {
 public:
     PagedCache(Context& context, std::int64_t layers, std::int64_t kv_heads, std::int64_t head_dim, std::int64_t pages, std::int64_t page_size,
@@ -94,7 +99,9 @@ public:
     // A step in which sequence ids[i] gets tokens[i] new keys: makes room for
     // them and uploads what the step's calls read. group_sizes: so many
     // neighbours in ids read the keys that they share once, from the first on
-    // (sequences past the last group each read their own).
+    // (sequences past the last group each read their own). At most 65536
+    // sequences, 2^22 new tokens and 2^26 keys a sequence. The new keys count
+    // from here on: where a step is given up before its appends, truncate.
     PagedBatch batch(std::span<const std::int64_t> ids, std::span<const std::int64_t> tokens, std::span<const std::int64_t> group_sizes = {});
 
     // The new tokens' q | k | v, f32 [tokens, (heads + 2 kv_heads) * head_dim],

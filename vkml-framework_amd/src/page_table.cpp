@@ -98,6 +98,28 @@ std::vector<PageCopy> PageTable::append(std::span<const std::int64_t> ids, std::
     return copies;
 }
 
+void PageTable::undo(std::span<const std::int64_t> ids, std::span<const std::int64_t> tokens, std::span<const PageCopy> copies) {
+    if (ids.size() != tokens.size()) throw Error("PageTable::undo: " + std::to_string(ids.size()) + " sequences, " + std::to_string(tokens.size()) + " counts");
+    for (std::size_t i = 0; i < ids.size(); ++i) {
+        if (tokens[i] < 0 || tokens[i] > at(ids[i]).length) throw Error("PageTable::undo: " + std::to_string(tokens[i]) + " tokens");
+    }
+    auto copy = copies.begin();  // in the order of the sequences
+    for (std::size_t i = 0; i < ids.size(); ++i) {
+        Row& row = rows_.find(ids[i])->second;
+        row.length -= tokens[i];
+        while (static_cast<std::int64_t>(row.pages.size()) > pages_for(row.length)) {
+            give(row.pages.back());
+            row.pages.pop_back();
+        }
+        if (tokens[i] > 0 && copy != copies.end() && !row.pages.empty() && row.pages.back() == copy->to) {
+            give(copy->to);
+            row.pages.back() = copy->from;
+            ++users_[static_cast<std::size_t>(copy->from)];
+            ++copy;
+        }
+    }
+}
+
 std::vector<PageCopy> PageTable::compact() {
     const std::int64_t used = pages() - free_pages();
     std::vector<std::int32_t> to(users_.size(), -1), holes;

@@ -23,10 +23,13 @@ std::int64_t positive(std::int64_t v, const char* what) {
     return v;
 }
 
-Tensor upload(detail::Runtime& runtime, const std::vector<std::int32_t>& values, Shape shape) {
-    Tensor t = TensorAccess::empty(runtime, std::move(shape), DType::I32);
+// What a batch of the kernels holds at most (csrc/pages.hpp).
+constexpr std::int64_t kMaxSeqs = 1 << 16, kMaxTokens = 1 << 22, kMaxKeys = 1 << 26;
+
+Tensor array(detail::Runtime& runtime, Shape shape) { return TensorAccess::empty(runtime, std::move(shape), DType::I32); }
+
+void upload(const Tensor& t, const std::vector<std::int32_t>& values) {
     if (!values.empty()) check(vkml_memcpy_h2d(t.data(), values.data(), values.size() * sizeof(std::int32_t)), "PagedCache::batch");
-    return t;
 }
 
 const std::int32_t* ints(const Tensor& t) { return static_cast<const std::int32_t*>(t.data()); }
@@ -66,42 +69,70 @@ void PagedCache::copy(const std::vector<PageCopy>& copies) {
     check(vkml_copy_pages(&p, from.data(), to.data(), k_.data(), v_.data()), "PagedCache");
 }
 
-void PagedCache::compact() { copy(table_.compact()); }
+void PagedCache::compact() {
+    PageTable compacted = table_;
+    copy(compacted.compact());
+    table_ = std::move(compacted);
+}
 
 PagedBatch PagedCache::batch(std::span<const std::int64_t> ids, std::span<const std::int64_t> tokens, std::span<const std::int64_t> group_sizes) {
+    if (ids.size() != tokens.size()) throw Error("PagedCache::batch: " + std::to_string(ids.size()) + " sequences, " + std::to_string(tokens.size()) + " counts");
     std::int64_t grouped = 0;
     for (const std::int64_t n : group_sizes) {
         if (n < 1 || n > static_cast<std::int64_t>(ids.size()) - grouped) throw Error("PagedCache::batch: a group of " + std::to_string(n) + " sequences");
         grouped += n;
     }
-    copy(table_.append(ids, tokens));
+    // Whatever can be refused or fail comes before the table changes, but for
+    // the uploads and copies of what it changes to.
     PagedBatch b;
     b.seqs = static_cast<std::int64_t>(ids.size());
     b.groups = static_cast<std::int64_t>(group_sizes.size());
-    std::size_t stride = 1;
-    for (const std::int64_t id : ids) stride = std::max(stride, table_.row(id).size());
-    std::vector<std::int32_t> table(ids.size() * stride, -1), lengths, starts = {0}, group_starts = {0}, group_keys;
+    if (b.seqs > kMaxSeqs) throw Error("PagedCache::batch: more than 65536 sequences");
+    std::int64_t most = 1;
     for (std::size_t i = 0; i < ids.size(); ++i) {
-        const auto& row = table_.row(ids[i]);
-        std::copy(row.begin(), row.end(), table.begin() + static_cast<std::ptrdiff_t>(i * stride));
-        lengths.push_back(static_cast<std::int32_t>(table_.length(ids[i])));
+        const std::int64_t length = table_.length(ids[i]);
+        if (tokens[i] < 0) throw Error("PagedCache::batch: " + std::to_string(tokens[i]) + " tokens");
+        if (tokens[i] > kMaxKeys - length) throw Error("PagedCache::batch: a sequence of more than 2^26 keys");
         b.tokens += tokens[i];
-        starts.push_back(static_cast<std::int32_t>(u32(b.tokens)));
+        if (b.tokens > kMaxTokens) throw Error("PagedCache::batch: more than 2^22 new tokens");
+        most = std::max(most, length + tokens[i]);
     }
-    std::size_t at = 0;
-    for (const std::int64_t n : group_sizes) {
-        const auto count = static_cast<std::size_t>(n);
-        group_keys.push_back(static_cast<std::int32_t>(table_.shared(ids.subspan(at, count), tokens.subspan(at, count))));
-        at += count;
-        group_starts.push_back(static_cast<std::int32_t>(at));
-    }
+    const std::int64_t stride = (most + table_.page_size() - 1) / table_.page_size();
     detail::Runtime& runtime = TensorAccess::runtime(k_);
-    b.table = upload(runtime, table, {b.seqs, static_cast<std::int64_t>(stride)});
-    b.lengths = upload(runtime, lengths, {b.seqs});
-    b.starts = upload(runtime, starts, {b.seqs + 1});
+    b.table = array(runtime, {b.seqs, stride});
+    b.lengths = array(runtime, {b.seqs});
+    b.starts = array(runtime, {b.seqs + 1});
     if (b.groups > 0) {
-        b.group_starts = upload(runtime, group_starts, {b.groups + 1});
-        b.group_keys = upload(runtime, group_keys, {b.groups});
+        b.group_starts = array(runtime, {b.groups + 1});
+        b.group_keys = array(runtime, {b.groups});
+    }
+    const std::vector<PageCopy> copies = table_.append(ids, tokens);
+    try {
+        std::vector<std::int32_t> table(ids.size() * static_cast<std::size_t>(stride), -1), lengths, starts = {0}, group_starts = {0}, group_keys;
+        for (std::size_t i = 0; i < ids.size(); ++i) {
+            const auto& row = table_.row(ids[i]);
+            std::copy(row.begin(), row.end(), table.begin() + static_cast<std::ptrdiff_t>(i * static_cast<std::size_t>(stride)));
+            lengths.push_back(static_cast<std::int32_t>(table_.length(ids[i])));
+            starts.push_back(static_cast<std::int32_t>(starts.back() + tokens[i]));
+        }
+        std::size_t at = 0;
+        for (const std::int64_t n : group_sizes) {
+            const auto count = static_cast<std::size_t>(n);
+            group_keys.push_back(static_cast<std::int32_t>(table_.shared(ids.subspan(at, count), tokens.subspan(at, count))));
+            at += count;
+            group_starts.push_back(static_cast<std::int32_t>(at));
+        }
+        upload(b.table, table);
+        upload(b.lengths, lengths);
+        upload(b.starts, starts);
+        if (b.groups > 0) {
+            upload(b.group_starts, group_starts);
+            upload(b.group_keys, group_keys);
+        }
+        copy(copies);  // (into pages that were free, should it fail)
+    } catch (...) {
+        table_.undo(ids, tokens, copies);
+        throw;
     }
     return b;
 }
