@@ -81,3 +81,8 @@ extern "C" void segment_c(const Batch* b, int32_t group, int32_t i, int32_t* out
     for (int k = 0; k < 12; ++k) out[k] = v[k];
 }
 extern "C" int32_t limit_c(const Batch* b, int32_t group, int32_t i, int32_t token) { return segment(*b, group, costs(128, true), i).limit(token); }
+
+extern "C" void grid_c(uint32_t workgroups, uint32_t* out) {
+    const Grid g = grid_of(workgroups);
+    out[0] = g.x, out[1] = g.y;
+}

@@ -1063,3 +1063,33 @@ def test_large_scores_pick_the_largest(size, kv):
                     picked += 1
                     assert np.all(np.abs(got[t, h] - V[order[-1]]) <= np.abs(V[order[-1]]) * ((seen / 16 + 64) * 2.0 ** -24 + 2.0 ** -20) + seen * math.exp(-64) * most), (t, h)
     assert picked > 8 * batch.tokens * 0.9
+
+
+def test_more_rows_than_a_launch_has_threads_for():
+    """2129920 new tokens of 32 heads with KV heads of their own: the join's
+    waves are 2^32 threads and more. All sequences read the same pages, and q
+    is zero: each token's output is the mean of the values up to its own."""
+    rng = np.random.default_rng(53)
+    heads, hd, page, seqs, n = 32, 64, 16, 4096, 520
+    tokens = seqs * n
+    assert tokens * heads * 64 >= 2 ** 32
+    cache = Cache(rng, 33, heads, page, hd, H.F16).upload()
+    p = H.AttendPagesParams(heads=heads, kv_heads=heads, head_dim=hd, kv_type=H.F16, page_size=page, pages=33, seqs=seqs, tokens=tokens, table_stride=33, scale=0.125)
+    table = np.broadcast_to(rng.permutation(33).astype(np.int32), (seqs, 33))
+    bufs = [dev(table), dev(np.full(seqs, n, np.int32)), dev(np.arange(0, tokens + 1, n, dtype=np.int32))]
+    row = heads * hd * 4
+    q, out, workspace = H.empty(tokens * row), H.empty(tokens * row), H.empty(H.lib().vkml_attend_pages_workspace_bytes(C.byref(p)))
+    print("large", tokens, workspace.nbytes, flush=True)
+    H.call("vkml_fill_u32", q.p, 0, tokens * row // 4)
+    H.call("vkml_fill_u32", out.p, 0x7FC00000, tokens * row // 4)
+    H.call("vkml_attend_pages", C.byref(p), q.p, cache.dk.p, cache.dv.p, *(b.p for b in bufs), None, None, workspace.p, out.p)
+    at = np.arange(n)
+    v = cache.v[table[0, at // page], :, at % page].astype(np.float64)
+    keys = at[:, None, None] + 1
+    mean, size = np.cumsum(v, 0) / keys, np.cumsum(np.abs(v), 0) / keys
+    bound = size * ((keys / 16 + 64) * 2.0 ** -24 + 2.0 ** -20)
+    # the parts of a KV head's work end at every 256th sequence or so
+    for s in sorted({min(max(256 * i + d, 0), seqs - 1) for i in range(17) for d in (-2, -1, 0, 1)}):
+        got = np.empty((n, heads, hd), np.float32)
+        H.call("vkml_memcpy_d2h", got.ctypes.data_as(C.c_void_p), C.c_void_p(out.p.value + s * n * row), got.nbytes)
+        close(got, mean, bound, f"sequence {s}")

@@ -320,3 +320,13 @@ def test_the_parts_of_a_batch_that_breaks_the_rules_cover_its_tiles(pages):
             tiles.setdefault((h, i, t), []).append(count)
         assert len(tiles) == 2 * sum(x[5] for x in seg.tolist())
         assert all(p[0] == len(p) for p in tiles.values())
+
+
+def test_a_grid_holds_every_workgroup_below_2_32_threads(pages):
+    for n in (1, 2, 4096, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 1, 2 ** 24, 3 * 2 ** 23 + 5, 2 ** 29 - 1, 2 ** 29):
+        out = np.zeros(2, np.uint32)
+        pages.grid_c(C.c_uint32(n), out.ctypes.data_as(C.c_void_p))
+        x, y = out.tolist()
+        assert n <= x * y < n + x and x * 256 < 2 ** 32 and 0 < y < 65536
+        # the waves' numbers, four a workgroup, fit 32 bits
+        assert x * y * 4 < 2 ** 32

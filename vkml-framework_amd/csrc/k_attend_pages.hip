@@ -1161,8 +1161,8 @@ __global__ void __launch_bounds__(kThreads) k_attend_pages_merge_many(PagesArgs 
     constexpr int N = HD / 64, kHeads = 4, kLanes = kWave / kHeads, kFlight = 2;
     const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), l = threadIdx.x % kWave;
     const uint32_t splits = (a.group + kHeads - 1) / kHeads;
-    const uint64_t item = static_cast<uint64_t>(blockIdx.x) * kWaves + w;
-    const uint32_t at = static_cast<uint32_t>(item / splits), head = static_cast<uint32_t>(item % splits) * kHeads;
+    const uint32_t item = (blockIdx.y * gridDim.x + blockIdx.x) * kWaves + w;  // less than 2^31 + 2^25
+    const uint32_t at = item / splits, head = item % splits * kHeads;
     if (at >= a.kv_heads * static_cast<uint32_t>(a.batch.tokens)) return;
     const Joins j = joins_of(a, at, ws_rows);
     if (j.n == 0) return;
@@ -1300,7 +1300,8 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     // and 66.9; 2600 tokens 228 and 158.
     const uint32_t rows = p->tokens * p->heads, fours = p->tokens * p->kv_heads * ((a.group + 3) / 4);
     const auto merge = [&](auto kernel, uint32_t workgroups) {
-        hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kThreads), 0, vkml::abi::stream(), a, s.rows());
+        const Grid grid = grid_of(workgroups);
+        hipLaunchKernelGGL(kernel, dim3(grid.x, grid.y), dim3(kThreads), 0, vkml::abi::stream(), a, s.rows());
     };
     if (rows <= 4096) wide ? merge(k_attend_pages_merge<128>, rows) : merge(k_attend_pages_merge<64>, rows);
     else wide ? merge(k_attend_pages_merge_many<128>, (fours + kWaves - 1) / kWaves) : merge(k_attend_pages_merge_many<64>, (fours + kWaves - 1) / kWaves);

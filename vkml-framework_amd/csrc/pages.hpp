@@ -257,6 +257,16 @@ VKML_HD Slots slots(int64_t kv_heads, int64_t group, int64_t seqs, int64_t group
     return {workgroups + kv_heads * (seqs + groups), workgroups + kv_heads * tiles};
 }
 
+// The grid of `workgroups`, numbered y * x + x's own: a launch has less than 2^32
+// threads in x.
+struct Grid {
+    uint32_t x, y;
+};
+VKML_HD Grid grid_of(uint32_t workgroups) {
+    constexpr uint32_t kMost = 1u << 23;  // of 256 threads
+    return workgroups <= kMost ? Grid{workgroups, 1} : Grid{kMost, (workgroups + kMost - 1) / kMost};
+}
+
 // ---------------------------------------------------------------- checks
 
 inline const char* check_cache(uint32_t kv_heads, uint32_t head_dim, uint32_t kv_type, uint32_t page_size, uint32_t pages, uint64_t page_stride) {
