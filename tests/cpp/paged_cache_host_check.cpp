@@ -203,9 +203,32 @@ void limits() {
     std::printf("%s limits\n", wrong ? "WRONG" : "ok");
 }
 
+void construction() {
+    vkml::Context ctx;
+    const auto refused = [&](const char* why, std::int64_t layers, std::int64_t kv_heads, std::int64_t head_dim, std::int64_t pages, std::int64_t page) {
+        try {
+            vkml::PagedCache c(ctx, layers, kv_heads, head_dim, pages, page, vkml::DType::F32);
+            expect(false, std::string("not refused: ") + why);
+        } catch (const vkml::Error& e) {
+            expect(std::string(e.what()).find(why) != std::string::npos, e.what());
+        }
+    };
+    refused("65535 layers", 65536, 1, 2, 4, 16);
+    refused("2^24 pages", 1, 1, 2, (1 << 24) + 1, 16);
+    refused("KV heads", 1, 4097, 2, 4, 16);
+    refused("KV heads", 1, 1, 1026, 4, 16);
+    refused("KV heads", 1, 1, 3, 4, 16);
+    refused("2^30 bytes", 1, 4096, 1024, 4, 128);
+    refused("2^62 bytes", 1 << 14, 512, 512, 1 << 24, 1024);  // 2^68 in all: 0 in 64 bits
+    refused("0 pages", 1, 1, 2, 0, 16);
+    vkml::PagedCache(ctx, 65535, 1, 2, 1, 16, vkml::DType::F16);
+    std::printf("%s construction\n", wrong ? "WRONG" : "ok");
+}
+
 }  // namespace
 
 int main() {
+    construction();
     batches();
     limits();
     return wrong ? 1 : 0;

@@ -81,7 +81,8 @@ struct PagedBatch {
 };
 
 // The keys and values of several sequences, in up to 2^24 pages of `page_size`
-// (a power of two, 16 to 1024), f32 or f16, for every layer of a model. What
+// (a power of two, 16 to 1024) and 2^30 bytes, f32 or f16, for every layer of a
+// model (up to 65535), of up to 4096 KV heads of up to 1024 dims. What
 // throws changes nothing: a batch that is refused, or for which there is no
 // memory, leaves every sequence with the keys that it had.
 class PagedCache {

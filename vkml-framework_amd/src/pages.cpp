@@ -1,5 +1,6 @@
 // pages.cpp -- vkml::PagedCache over the C ABI (vkml_rope_kv_pages,
 // vkml_attend_pages, vkml_copy_pages).
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -26,6 +27,24 @@ std::int64_t positive(std::int64_t v, const char* what) {
 // What a batch of the kernels holds at most (csrc/pages.hpp).
 constexpr std::int64_t kMaxSeqs = 1 << 16, kMaxTokens = 1 << 22, kMaxKeys = 1 << 26;
 
+// The table of a cache whose every call the kernels take (csrc/pages.hpp), and
+// whose pools' bytes can be counted.
+PageTable table_of(std::int64_t layers, std::int64_t kv_heads, std::int64_t head_dim, std::int64_t pages, std::int64_t page_size, DType dtype) {
+    if (dtype != DType::F32 && dtype != DType::F16) throw Error("PagedCache: no kernel for " + std::string(to_string(dtype)) + " yet");
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0) {
+        throw Error("PagedCache: page_size must be a power of two from 16 to 1024, got " + std::to_string(page_size));
+    }
+    if (pages > std::int64_t{1} << 24) throw Error("PagedCache: more than 2^24 pages");
+    if (layers > 65535) throw Error("PagedCache: more than 65535 layers");
+    if (kv_heads > 4096 || head_dim > 1024 || head_dim % 2 != 0) {
+        throw Error("PagedCache: at most 4096 KV heads of an even number of dims up to 1024, got " + std::to_string(kv_heads) + " of " + std::to_string(head_dim));
+    }
+    const std::int64_t page_bytes = kv_heads * page_size * head_dim * static_cast<std::int64_t>(element_size(dtype));
+    if (page_bytes > std::int64_t{1} << 30) throw Error("PagedCache: a page of more than 2^30 bytes");
+    if (page_bytes > (std::int64_t{1} << 62) / layers / std::max<std::int64_t>(pages, 1)) throw Error("PagedCache: pools of more than 2^62 bytes");
+    return PageTable(pages, page_size);
+}
+
 Tensor array(detail::Runtime& runtime, Shape shape) { return TensorAccess::empty(runtime, std::move(shape), DType::I32); }
 
 void upload(const Tensor& t, const std::vector<std::int32_t>& values) {
@@ -38,12 +57,8 @@ const std::int32_t* ints(const Tensor& t) { return static_cast<const std::int32_
 
 PagedCache::PagedCache(Context& context, std::int64_t layers, std::int64_t kv_heads, std::int64_t head_dim, std::int64_t pages, std::int64_t page_size,
                        DType dtype)
-    : layers_(positive(layers, "layers")), kv_heads_(positive(kv_heads, "KV heads")), head_dim_(positive(head_dim, "dims a head")), table_(pages, page_size) {
-    if (dtype != DType::F32 && dtype != DType::F16) throw Error("PagedCache: no kernel for " + std::string(to_string(dtype)) + " yet");
-    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0) {
-        throw Error("PagedCache: page_size must be a power of two from 16 to 1024, got " + std::to_string(page_size));
-    }
-    if (pages > std::int64_t{1} << 24) throw Error("PagedCache: more than 2^24 pages");
+    : layers_(positive(layers, "layers")), kv_heads_(positive(kv_heads, "KV heads")), head_dim_(positive(head_dim, "dims a head")),
+      table_(table_of(layers, kv_heads, head_dim, pages, page_size, dtype)) {
     const Shape shape = {layers, pages, kv_heads, page_size, head_dim};
     k_ = Tensor::empty(context, shape, dtype);
     v_ = Tensor::empty(context, shape, dtype);
