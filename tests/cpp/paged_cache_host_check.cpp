@@ -225,9 +225,31 @@ void construction() {
     std::printf("%s construction\n", wrong ? "WRONG" : "ok");
 }
 
+void tables() {
+    vkml::Context ctx;
+    vkml::PagedCache c(ctx, 1, 1, 2, kPages, kPage, vkml::DType::F32);
+    const std::int64_t a = c.create(), b = c.create();
+    const vkml::PagedBatch first = c.batch(Ids{a, b}, Ids{40, 7}), idle = c.batch(Ids{a, b}, Ids{0, 1});
+    const auto takes = [&](const vkml::PagedBatch& batch, const vkml::Tensor& table) {
+        try {
+            c.append(0, batch, vkml::Tensor::empty(ctx, {batch.tokens, 6}, vkml::DType::F32), table, vkml::RopeStyle::Interleaved);
+        } catch (const vkml::Error& e) {
+            expect(std::string(e.what()).find("positions") != std::string::npos, e.what());
+            return false;
+        }
+        return true;
+    };
+    const auto rows = [&](std::int64_t n) { return vkml::Tensor::empty(ctx, {n, 1, 2}, vkml::DType::F32); };
+    expect(takes(first, rows(40)) && takes(first, vkml::Tensor()), "a table that holds every position is refused");
+    expect(!takes(first, rows(39)) && !takes(first, rows(0)), "a table that is too short is taken");
+    expect(takes(idle, rows(8)) && !takes(idle, rows(7)), "positions of a sequence without new tokens count");
+    std::printf("%s tables\n", wrong ? "WRONG" : "ok");
+}
+
 }  // namespace
 
 int main() {
+    tables();
     construction();
     batches();
     limits();

@@ -203,7 +203,7 @@ def test_a_cache_that_fails_changes_nothing(host_check):
     r = subprocess.run([host_check], capture_output=True, text=True, timeout=100)
     print(r.stdout)
     assert r.returncode == 0, r.stdout + r.stderr
-    assert sum(line.startswith("ok ") for line in r.stdout.split("\n")) == 5
+    assert sum(line.startswith("ok ") for line in r.stdout.split("\n")) == 6
 
 
 @pytest.fixture(scope="module")

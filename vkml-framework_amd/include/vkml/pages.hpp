@@ -78,6 +78,7 @@ struct PagedBatch {
     Tensor table, lengths, starts;     // i32 [seqs, stride], [seqs], [seqs + 1]
     Tensor group_starts, group_keys;   // i32 [groups + 1], [groups]; null without groups
     std::int64_t seqs = 0, tokens = 0, groups = 0;
+    std::int64_t positions = 0;        // past the last position of a new token
 };
 
 // The keys and values of several sequences, in up to 2^24 pages of `page_size`
@@ -108,7 +109,8 @@ public:
     // The new tokens' q | k | v, f32 [tokens, (heads + 2 kv_heads) * head_dim],
     // sequence after sequence: q and k rotated at their positions by a table
     // from rope_table (for a part of the head: of that many dims; null: not
-    // rotated), k and v into a layer's pages. Returns q [tokens, heads, head_dim].
+    // rotated) that holds them all, k and v into a layer's pages. Returns q
+    // [tokens, heads, head_dim].
     Tensor append(std::int64_t layer, const PagedBatch& batch, const Tensor& qkv, const Tensor& rope_table, RopeStyle style);
 
     // softmax(q k^T / sqrt(head_dim)) v of each new token over its sequence's

@@ -111,6 +111,7 @@ PagedBatch PagedCache::batch(std::span<const std::int64_t> ids, std::span<const 
         b.tokens += tokens[i];
         if (b.tokens > kMaxTokens) throw Error("PagedCache::batch: more than 2^22 new tokens");
         most = std::max(most, length + tokens[i]);
+        if (tokens[i] > 0) b.positions = std::max(b.positions, length + tokens[i]);
     }
     const std::int64_t stride = (most + table_.page_size() - 1) / table_.page_size();
     detail::Runtime& runtime = TensorAccess::runtime(k_);
@@ -160,9 +161,12 @@ Tensor PagedCache::append(std::int64_t layer, const PagedBatch& batch, const Ten
                     std::to_string(head_dim_) + "], got " + std::string(to_string(qkv.dtype())) + " " + to_string(s));
     }
     const Shape& t = rope_table.shape();
-    const bool rotated = rope_table.numel() > 0;
+    const bool rotated = t != Tensor().shape();
     if (rotated && (rope_table.dtype() != DType::F32 || t.size() != 3 || t[1] * 2 > head_dim_ || t[2] != 2)) {
         throw Error("PagedCache::append: heads of " + std::to_string(head_dim_) + " do not match the table " + to_string(t) + " from rope_table");
+    }
+    if (rotated && batch.positions > t[0]) {
+        throw Error("PagedCache::append: positions up to " + std::to_string(batch.positions - 1) + " are outside the table's " + std::to_string(t[0]) + " positions");
     }
     Tensor q = TensorAccess::empty(TensorAccess::runtime(qkv), {batch.tokens, heads, head_dim_}, DType::F32);
     if (batch.tokens == 0) return q;
