@@ -259,3 +259,16 @@ def test_an_append_taken_back_leaves_no_trace(exe_undo, seed):
     assert t.ask("undo", 99, 1).startswith("error: PageTable") and t.ask("undo", next(iter(t.want)), 10 ** 6).startswith("error: PageTable")
     t.check()
     t.close()
+
+
+def test_shared_refuses_negative_counts(exe):
+    """Keys past the end of a sequence's pages' used part are nobody's."""
+    t = Table(exe, 8, 4)
+    a = t.numbers("create")[0]
+    t.want[a] = []
+    t.append([a], [5])
+    b = t.numbers("fork", a)[0]
+    assert t.numbers("shared", a, 0, b, 0) == [5] and t.numbers("shared", a, 9, b, 0) == [0]
+    for words in ((a, -1, b, -1), (a, 0, b, -3), (a, -2 ** 63, b, 0)):
+        assert "error: PageTable::shared" in t.ask("shared", *words)
+    t.close()

@@ -150,6 +150,7 @@ std::int64_t PageTable::shared(std::span<const std::int64_t> ids, std::span<cons
     std::int64_t keys = INT64_MAX;
     for (std::size_t i = 0; i < ids.size(); ++i) {
         const Row& r = at(ids[i]);
+        if (before[i] < 0) throw Error("PageTable::shared: " + std::to_string(before[i]) + " keys");
         const auto end = std::mismatch(first.begin(), first.begin() + static_cast<std::ptrdiff_t>(std::min(same, r.pages.size())), r.pages.begin());
         same = static_cast<std::size_t>(end.first - first.begin());
         keys = std::min(keys, r.length - before[i]);
