@@ -272,3 +272,13 @@ def test_shared_refuses_negative_counts(exe):
     for words in ((a, -1, b, -1), (a, 0, b, -3), (a, -2 ** 63, b, 0)):
         assert "error: PageTable::shared" in t.ask("shared", *words)
     t.close()
+
+
+def test_a_table_without_memory_changes_nothing(tmp_path):
+    exe = str(tmp_path / "page_table_memory_check")
+    subprocess.run(["g++", "-std=c++20", "-O1", "-Wall", "-I" + os.path.join(ROOT, "vkml-framework_amd", "include"),
+                    os.path.join(ROOT, "tests", "cpp", "page_table_memory_check.cpp"), os.path.join(ROOT, "vkml-framework_amd", "src", "page_table.cpp"), "-o", exe],
+                   check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert r.stdout.startswith("ok: ")

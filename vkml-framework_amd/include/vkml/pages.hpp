@@ -2,7 +2,6 @@
 
 #include <cstdint>
 #include <map>
-#include <queue>
 #include <span>
 #include <vector>
 
@@ -24,7 +23,7 @@ struct PageCopy {
 // Which pages of a pool hold which sequence's keys (host only): key p of a
 // sequence is row p % page_size of its page p / page_size. Sequences that were
 // forked share pages; one that writes into a shared page gets a copy first.
-// Errors throw vkml::Error and change nothing.
+// What throws (vkml::Error, or std::bad_alloc) changes nothing.
 class PageTable {
 public:
     PageTable(std::int64_t pages, std::int64_t page_size);
@@ -69,7 +68,7 @@ private:
     std::int64_t page_size_;
     std::int64_t next_id_ = 0;
     std::vector<std::int32_t> users_;  // sequences that hold each page
-    std::priority_queue<std::int32_t, std::vector<std::int32_t>, std::greater<>> free_;
+    std::vector<std::int32_t> free_;   // a heap, the lowest first
     std::map<std::int64_t, Row> rows_;
 };
 

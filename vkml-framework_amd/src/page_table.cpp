@@ -2,6 +2,7 @@
 // copied before a write into a shared one, given back, compacted. Host code
 // without a device.
 #include <algorithm>
+#include <functional>
 #include <string>
 
 #include "vkml/error.hpp"
@@ -13,9 +14,8 @@ PageTable::PageTable(std::int64_t pages, std::int64_t page_size) : page_size_(pa
     if (pages < 1 || pages > 0x7FFFFFFF) throw Error("PageTable: " + std::to_string(pages) + " pages");
     if (page_size < 1) throw Error("PageTable: pages of " + std::to_string(page_size) + " keys");
     users_.resize(static_cast<std::size_t>(pages));
-    std::vector<std::int32_t> all(static_cast<std::size_t>(pages));
-    for (std::size_t i = 0; i < all.size(); ++i) all[i] = static_cast<std::int32_t>(i);
-    free_ = decltype(free_)(std::greater<>{}, std::move(all));
+    free_.resize(users_.size());
+    for (std::size_t i = 0; i < free_.size(); ++i) free_[i] = static_cast<std::int32_t>(i);  // in order: a heap
 }
 
 const PageTable::Row& PageTable::at(std::int64_t id) const {
@@ -25,14 +25,17 @@ const PageTable::Row& PageTable::at(std::int64_t id) const {
 }
 
 std::int32_t PageTable::take() {
-    const std::int32_t page = free_.top();
-    free_.pop();
+    std::pop_heap(free_.begin(), free_.end(), std::greater<>());
+    const std::int32_t page = free_.back();
+    free_.pop_back();
     users_[static_cast<std::size_t>(page)] = 1;
     return page;
 }
 
 void PageTable::give(std::int32_t page) {
-    if (--users_[static_cast<std::size_t>(page)] == 0) free_.push(page);
+    if (--users_[static_cast<std::size_t>(page)] != 0) return;
+    free_.push_back(page);
+    std::push_heap(free_.begin(), free_.end(), std::greater<>());
 }
 
 std::int64_t PageTable::create() {
@@ -41,13 +44,13 @@ std::int64_t PageTable::create() {
 }
 
 std::int64_t PageTable::fork(std::int64_t id) {
-    Row copy = at(id);
-    for (const std::int32_t page : copy.pages) ++users_[static_cast<std::size_t>(page)];
-    rows_.emplace(next_id_, std::move(copy));
-    return next_id_++;
+    const auto& [to, row] = *rows_.emplace(next_id_, at(id)).first;
+    for (const std::int32_t page : row.pages) ++users_[static_cast<std::size_t>(page)];
+    return next_id_++, to;
 }
 
 void PageTable::release(std::int64_t id) {
+    free_.reserve(users_.size());  // (a copied table's has room for its free pages alone)
     for (const std::int32_t page : at(id).pages) give(page);
     rows_.erase(id);
 }
@@ -57,7 +60,8 @@ void PageTable::truncate(std::int64_t id, std::int64_t length) {
     if (length < 0 || length > row.length) {
         throw Error("PageTable::truncate: length " + std::to_string(length) + " of a sequence of " + std::to_string(row.length));
     }
-    Row& mine = rows_[id];
+    free_.reserve(users_.size());
+    Row& mine = rows_.find(id)->second;
     while (static_cast<std::int64_t>(mine.pages.size()) > pages_for(length)) {
         give(mine.pages.back());
         mine.pages.pop_back();
@@ -79,13 +83,22 @@ std::vector<PageCopy> PageTable::append(std::span<const std::int64_t> ids, std::
         need += pages_for(row.length + tokens[i]) - static_cast<std::int64_t>(row.pages.size());
         if (tokens[i] > 0 && row.length % page_size_ != 0) ++writers[row.pages.back()];
     }
+    std::size_t most = 0;  // copies
+    for (const auto& [page, n] : writers) most += static_cast<std::size_t>(n);
     for (const auto& [page, n] : writers) need += users_[static_cast<std::size_t>(page)] > n ? n : n - 1;
     if (need > free_pages()) {
         throw Error("PageTable::append: " + std::to_string(need) + " pages needed, " + std::to_string(free_pages()) + " of " + std::to_string(pages()) + " free");
     }
+    // The memory that it takes, before anything changes.
     std::vector<PageCopy> copies;
+    copies.reserve(most);
     for (std::size_t i = 0; i < ids.size(); ++i) {
-        Row& row = rows_[ids[i]];
+        Row& row = rows_.find(ids[i])->second;
+        const auto pages = static_cast<std::size_t>(pages_for(row.length + tokens[i]));
+        if (row.pages.capacity() < pages) row.pages.reserve(std::max(pages, 2 * row.pages.size()));
+    }
+    for (std::size_t i = 0; i < ids.size(); ++i) {
+        Row& row = rows_.find(ids[i])->second;
         if (tokens[i] > 0 && row.length % page_size_ != 0 && users_[static_cast<std::size_t>(row.pages.back())] > 1) {
             const std::int32_t page = take();
             copies.push_back({row.pages.back(), page});
@@ -132,13 +145,14 @@ std::vector<PageCopy> PageTable::compact() {
         copies.push_back({static_cast<std::int32_t>(p), hole});
         to[static_cast<std::size_t>(p)] = hole;
     }
+    std::vector<std::int32_t> left;
+    left.reserve(users_.size());
+    for (std::int64_t p = used; p < pages(); ++p) left.push_back(static_cast<std::int32_t>(p));
     for (const PageCopy& c : copies) std::swap(users_[static_cast<std::size_t>(c.from)], users_[static_cast<std::size_t>(c.to)]);
     for (auto& [id, row] : rows_)
         for (std::int32_t& page : row.pages)
             if (to[static_cast<std::size_t>(page)] >= 0) page = to[static_cast<std::size_t>(page)];
-    std::vector<std::int32_t> left;
-    for (std::int64_t p = used; p < pages(); ++p) left.push_back(static_cast<std::int32_t>(p));
-    free_ = decltype(free_)(std::greater<>{}, std::move(left));
+    free_ = std::move(left);
     return copies;
 }
 
