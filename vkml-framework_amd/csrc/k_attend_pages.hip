@@ -600,6 +600,13 @@ __device__ __forceinline__ void loads_landed() {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     asm volatile("" ::: "memory");
 }
+// And what the wave has read from the LDS is read, so that loads into it may be
+// issued: where no barrier says so.
+__device__ __forceinline__ void loads_and_reads_landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
 
 __device__ __forceinline__ float lanes_sum(float v) {  // over a row's four lanes
     const uint2 l16 = swap_rows<16>(__float_as_uint(v));
@@ -723,7 +730,7 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
         Pages nxt = pages_after(a, p.tile, cur, x + kStep, kSpan);
         q.take(0, raw[0], a.score_scale);
         const auto block = [&](uint4 (&k)[TT][B::kSteps], uint8_t* here, uint4 (&k_next)[TT][B::kSteps], uint8_t* there) {
-            loads_landed();  // this block's, and the next one's pages
+            loads_and_reads_landed();  // this block's, the next one's pages; the last block's reads
             const uint32_t dead = dead_tiles<TT>(a, cur);
             if (x + kStep < p.x1) issue(nxt, k_next, there);
             const Pages after = pages_after(a, p.tile, nxt, x + 2 * kStep, kSpan);
