@@ -699,8 +699,9 @@ int vkml_attend_step_noalloc(const vkml_attend_step_params* p, const float* d_qk
  * with f32 caches on the f32 matrix instructions). d_q and d_out
  * [tokens, heads, head_dim] f32. softcap: 0 for none. A token without keys
  * gets zeros. What is not finite in a row of q, or among a token's keys and
- * values, reaches that token's outputs only. head_dim 64 or 128; at most 128
- * query heads a KV head; scale finite.
+ * values, reaches that token's outputs only; a score of -infinity weighs
+ * nothing, and a token all of whose scores are gets zeros too. head_dim 64 or
+ * 128; at most 128 query heads a KV head; scale finite.
  *
  * groups > 0: sequences d_group_starts[g] .. d_group_starts[g + 1] (groups +
  * 1 entries that do not decrease; sequences outside every group share

@@ -1093,3 +1093,37 @@ def test_more_rows_than_a_launch_has_threads_for():
         got = np.empty((n, heads, hd), np.float32)
         H.call("vkml_memcpy_d2h", got.ctypes.data_as(C.c_void_p), C.c_void_p(out.p.value + s * n * row), got.nbytes)
         close(got, mean, bound, f"sequence {s}")
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (40, 2)])
+def test_scores_of_minus_infinity_weigh_nothing(heads, kv_heads):
+    """f32 caches, queries of positive values: a key of -infinity in a dim is
+    left out, and a token that sees no other gets zeros."""
+    rng = np.random.default_rng(54)
+    batch = Batch(rng, [30, 200, 3], [30, 1, 3], 16)
+    cache = Cache(rng, batch.pages, kv_heads, 16, 64, H.F32)
+    q = (np.abs(rng.standard_normal((batch.tokens, heads, 64))) + 0.1).astype(np.float32)
+    out = {0: [0, 1, 2, 17], 1: [5, 190], 2: [0, 1, 2]}
+    for s, keys in out.items():
+        for pos in keys:
+            cache.k[batch.table[s, pos // 16], :, pos % 16, 7] = -np.inf
+    cache.upload()
+    batch.upload()
+    got = Call(q, cache, batch, 0.1).run().result()
+    for s, keys in out.items():
+        n, length = batch.new[s], batch.lengths[s]
+        for i in range(n):
+            t = batch.starts[s] + i
+            on = [p for p in range(length - n + i + 1) if p not in keys]
+            if not on:
+                assert not got[t].any(), (s, i)
+                continue
+            for h in range(heads):
+                K, V = (np.stack([x[batch.table[s, p // 16], h // (heads // kv_heads), p % 16] for p in on]).astype(np.float64) for x in (cache.k, cache.v))
+                Q = q[t, h].astype(np.float64)
+                x = K @ Q * 0.1
+                w = np.exp(x - x.max())
+                w /= w.sum()
+                delta = 0.1 * 72 * 2.0 ** -24 * (np.abs(K) @ np.abs(Q)).max()
+                bound = (w @ np.abs(V)) * (2 * delta + 2.0 ** -22 * np.abs(x).max() + (len(on) / 16 + 64) * 2.0 ** -24 + 2.0 ** -20)
+                assert np.all(np.abs(got[t, h] - w @ V) <= bound), (s, i, h)
