@@ -86,3 +86,15 @@ extern "C" void grid_c(uint32_t workgroups, uint32_t* out) {
     const Grid g = grid_of(workgroups);
     out[0] = g.x, out[1] = g.y;
 }
+
+// Segment i's cost, and for each tile: its cost, what comes before it, and the
+// tile that its first and its last unit are found in.
+extern "C" int64_t costs_c(const Batch* b, int32_t group, int32_t head_dim, int32_t f16, int32_t i, int64_t* out, int64_t most) {
+    const Segment s = segment(*b, group, costs(head_dim, f16 != 0), i);
+    for (int32_t t = 0; t < s.tiles && t < most; ++t) {
+        int64_t* o = out + 4 * t;
+        o[0] = s.tile_cost(t), o[1] = s.before(t);
+        o[2] = s.tile_at(o[1]), o[3] = s.tile_at(o[1] + o[0] - 1);
+    }
+    return s.cost();
+}

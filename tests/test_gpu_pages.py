@@ -1127,3 +1127,26 @@ def test_scores_of_minus_infinity_weigh_nothing(heads, kv_heads):
                 delta = 0.1 * 72 * 2.0 ** -24 * (np.abs(K) @ np.abs(Q)).max()
                 bound = (w @ np.abs(V)) * (2 * delta + 2.0 ** -22 * np.abs(x).max() + (len(on) / 16 + 64) * 2.0 ** -24 + 2.0 ** -20)
                 assert np.all(np.abs(got[t, h] - w @ V) <= bound), (s, i, h)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(seed):
+    """Batches of every make: ragged, padded, grouped or not, decoding and
+    prompts, more new tokens than keys, over a workspace of NaN bits."""
+    rng = np.random.default_rng(1000 + seed)
+    heads, kv_heads = HEADS[int(rng.integers(len(HEADS)))]
+    hd, page, kv = int(rng.choice([64, 128])), int(rng.choice([16, 32, 128])), [H.F16, H.F32][int(rng.integers(2))]
+    n = int(rng.choice([1, 2, 7, 20, 70]))
+    new = rng.integers(0, 40, n) if rng.random() < 0.5 and n < 20 else np.ones(n, int)
+    own = np.where(rng.random(n) < 0.2, 0, rng.integers(0, 400, n))
+    groups, lengths = [], own.copy()
+    if n > 1 and rng.random() < 0.7:
+        a, b = sorted(rng.choice(n + 1, 2, replace=False).tolist())
+        shared = int(rng.integers(1, 600))
+        lengths[a:b] = shared + new[a:b] + own[a:b]  # at most the keys before a sequence's new tokens
+        groups = [(a, b, shared)]
+    if new.sum() == 0:
+        new[0] = 1
+        lengths[0] = max(lengths[0], 1)
+    attend(seed, heads, kv_heads, hd, page, kv, lengths.tolist(), new.tolist(), groups, softcap=float(rng.choice([0.0, 0.0, 20.0])),
+           starts=not bool(np.all(new == 1) and rng.random() < 0.5))

@@ -330,3 +330,54 @@ def test_a_grid_holds_every_workgroup_below_2_32_threads(pages):
         assert n <= x * y < n + x and x * 256 < 2 ** 32 and 0 < y < 65536
         # the waves' numbers, four a workgroup, fit 32 bits
         assert x * y * 4 < 2 ** 32
+
+
+def tile_costs(pages, b, group, hd, f16, i, most):
+    out = np.zeros((most, 4), np.int64)
+    pages.costs_c.restype = C.c_int64
+    total = pages.costs_c(C.byref(b), group, hd, f16, i, out.ctypes.data_as(C.c_void_p), C.c_int64(most))
+    return total, out
+
+
+@pytest.mark.parametrize("hd,f16", [(64, 0), (64, 1), (128, 0), (128, 1)])
+@pytest.mark.parametrize("length,new,group", [(2 ** 26, 2 ** 22, 128), (2 ** 26, 2 ** 22, 1), (2 ** 22, 2 ** 22, 128), (2 ** 26, 1, 1), (5, 2 ** 20, 4), (0, 100, 8)])
+def test_costs_of_long_batches_fit_64_bits(pages, length, new, group, hd, f16):
+    """Tile costs against whole numbers of any size: their sums, the order and
+    what is found from a unit."""
+    b, keep = batch([length], [0, new], None, None, new, 2 ** 26)
+    step = max(1, 128 // group)
+    few = new * group <= 16
+    tiles = 1 if few else -(-new // step)
+    total, got = tile_costs(pages, b, group, hd, f16, 0, tiles)
+    key = {(64, 1): (4, 12), (128, 1): (8, 24), (64, 0): (8, 14), (128, 0): (16, 28)}[hd, f16][0 if few else 1]
+    own = (2600 if few else 3600) if f16 else 600
+    # the keys that a tile's last token sees; where the first tokens see none, all that any sees
+    last = np.full(tiles, new) if few or length < new else np.minimum((np.arange(tiles) + 1) * step, new)
+    want = own + key * np.maximum(0, length - new + last).astype(np.int64)
+    assert want.max() < 2 ** 31 and int(want.max()) * tiles < 2 ** 63
+    assert np.array_equal(got[:, 0], want)
+    assert np.array_equal(got[:, 1], np.cumsum(want) - want)
+    assert np.array_equal(got[:, 2], np.arange(tiles)) and np.array_equal(got[:, 3], np.arange(tiles))
+    assert total == want.sum()
+
+
+@pytest.mark.parametrize("kv_heads,group,lengths,new", [(8, 4, [4096, 33], [4096, 1]), (8, 4, [30, 4000, 900, 2500], [1] * 4), (32, 1, [32768], [1]), (8, 4, [2000] * 64, [1] * 64)])
+def test_parts_cost_the_same_but_for_their_ends(pages, kv_heads, group, lengths, new):
+    """What a workgroup takes, in the rule's own costs: a part's share, and at
+    most a tile's own cost and a block of keys more at each end."""
+    got = check_cut(pages, lengths, new, None, None, kv_heads, group, 9, 64)
+    b, keep = batch(lengths, np.concatenate([[0], np.cumsum(new)]), None, None, sum(new), 1 << 20)
+    seg = segments(pages, b, group)
+    few = [bool(n * group <= 16) for n in new]
+    key, own = {True: 8, False: 24}, {True: 2600, False: 3600}
+    load, parts, total = np.zeros(512), set(), 0
+    for i in range(len(lengths)):
+        total += kv_heads * tile_costs(pages, b, group, 128, 1, i, int(seg[i][5]))[0]
+    for w, h, i, t, k0, k1, *_ in got.tolist():
+        load[w] += (own[few[i]] if k0 == 0 else 0) + key[few[i]] * (k1 - k0)
+    n = 512
+    while n > 8 and total // n < 512:
+        n //= 2
+    ends = max(own[f] + 64 * key[f] for f in few)
+    assert load.max() <= total / n + 2 * ends
+    assert abs(load.sum() - total) <= sum(own[f] / 8 + 1 for f in few) * kv_heads * len(got)
