@@ -685,35 +685,41 @@ int vkml_attend_step_noalloc(const vkml_attend_step_params* p, const float* d_qk
 /* A call's new tokens are the rows of q (or qkv), a sequence's one after  */
 /* another: d_starts[s] .. d_starts[s + 1] are sequence s's (seqs + 1      */
 /* entries from 0 .. tokens that do not decrease; NULL: token s is         */
-/* sequence s's only one, and tokens = seqs). d_lengths[s] are its keys,   */
-/* the new tokens' last among them: of n new tokens, token i stands at     */
-/* position d_lengths[s] - n + i. Rows of no sequence are left as they     */
-/* were. These arrays are device memory, read when the launch runs, so a   */
-/* captured graph follows them. Values that break these rules give         */
-/* unspecified results, but nothing outside the arrays named here is       */
-/* touched.                                                                */
+/* sequence s's only one, and tokens = seqs). d_lengths[s] are its keys, 0 */
+/* to table_stride * page_size, the new tokens' last among them: of n new  */
+/* tokens, token i stands at position d_lengths[s] - n + i. Rows of no     */
+/* sequence are left as they were. These arrays are device memory, read    */
+/* when the launch runs, so a captured graph follows them. Values that     */
+/* break these rules give unspecified results, but nothing outside the     */
+/* arrays named here is touched.                                           */
 /* ---------------------------------------------------------------------- */
 
 /* softmax(q k^T scale) v of each new token over its sequence's keys up to
  * its own position (f32 attention within f32 rounding, as vkml_attend_fast;
- * with f32 caches on the f32 matrix instructions). d_q and d_out
+ * with f32 caches on the f32 matrix instructions; with f16 caches q and the
+ * weights are two f16 terms each, so that an element of q is off by up to
+ * 2^-23 of itself or 2^-24 of its row's largest, whichever is more, and a
+ * weight by 2^-23 of itself or 2^-39 of the row's largest). d_q and d_out
  * [tokens, heads, head_dim] f32. softcap: 0 for none. A token without keys
  * gets zeros. What is not finite in a row of q, or among a token's keys and
- * values, reaches that token's outputs only; a score of -infinity weighs
- * nothing, and a token all of whose scores are gets zeros too. head_dim 64 or
- * 128; at most 128 query heads a KV head; scale finite.
+ * values, reaches that token's outputs only. With f32 caches a score of
+ * -infinity weighs nothing, and a token all of whose scores are gets zeros
+ * too; an f16 key that is not finite gives NaN. head_dim 64 or 128; at most
+ * 128 query heads a KV head; scale finite.
  *
  * groups > 0: sequences d_group_starts[g] .. d_group_starts[g + 1] (groups +
  * 1 entries that do not decrease; sequences outside every group share
  * nothing) have their first d_group_keys[g] keys in common: these are read
- * once for all of the group's tokens, through its first sequence's row of
- * the table, and only the rest through each one's own. d_group_keys[g] is at
- * most the keys that each of them has before its new tokens; it need not
- * fill whole pages.
+ * through its first sequence's row of the table, and only the rest through
+ * each one's own. A KV head's shared keys are read once for each 128 rows
+ * (token, query head) of the group, whichever sequences those are of; where
+ * its sequences bring 64 rows or more each on average, for each one's tokens
+ * apart. d_group_keys[g] is at most the keys that each of them has before
+ * its new tokens; it need not fill whole pages.
  *
  * d_workspace: vkml_attend_pages_workspace_bytes(p) bytes, 16-byte aligned,
- * of any content (0 where the call would refuse p); calls that overlap need
- * one each. */
+ * of any content (0 where the call would refuse p; 2600 tokens of 32 heads
+ * and 8 KV heads of 128: 129 MB); calls that overlap need one each. */
 typedef struct vkml_attend_pages_params {
     uint32_t heads;
     uint32_t kv_heads;

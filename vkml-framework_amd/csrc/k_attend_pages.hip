@@ -1,7 +1,7 @@
 // k_attend_pages.hip -- attention of a batch's new tokens over a paged KV
 // cache (vkml_attend_pages): softmax(q k^T scale) v over each token's keys,
-// the ones that a group shares through its first sequence's table and once for
-// all of its tokens, the rest through the sequence's own.
+// the ones that a group shares through its first sequence's table, for 128 of its
+// rows at a time, the rest through the sequence's own.
 //
 // Softmax in one pass: a row (token, query head) keeps the running maximum m
 // of its scores in log2 units, the sum l of 2^(x - m) and the sum o of
@@ -36,11 +36,15 @@
 // cleared in the LDS before the product. So are infinities and NaN of keys that
 // some rows see and others don't, which are added to those rows at the end.
 //
-// Measured (32 query and 8 KV heads of 128, f16): one token over 32768 keys 30 us
-// and 5 to join its pieces, 134 MB at 4.4 TB/s (a large copy reaches 5.0); 64
-// sequences with 32768 shared keys and 1000 of their own 112 us and 8 (407 MB and
-// 71 GFLOP, the split counted twice: memory and the matrix units at once); 2600
-// tokens of six prompts 148 us and 16, 115 GFLOP issued at 780 TFLOP/s.
+// Measured (a whole call, 32 query and 8 KV heads of 128, f16): one token over
+// 32768 keys 35 us, 5 of them to join its pieces, 134 MB at 4.4 TB/s before that (a
+// large copy reaches 5.0); 64 sequences with 32768 shared keys and 1000 of their own
+// 121 us, 8 to join (71 GFLOP, the split counted twice, and 547 MB read where 407
+// are needed: the group's 256 rows are two tiles, one after the other, and each
+// reads the shared keys from memory); 2600 tokens of six prompts 149 us, 16 to join
+// (115 GFLOP).
+// What the three ways through a tile need at once is more than the scalar registers
+// hold: 160 to 209 are spilled to lanes of vector registers; of those none is.
 // Short ones are a chain of waits: 1.0 us for the batch's arrays, 0.8 to find the
 // part, 1.3 its first tile, 1.2 for pages and keys, 2 to 3 the block, 0.8 the end.
 #include <hip/hip_runtime.h>
@@ -377,9 +381,9 @@ constexpr int kOnlyAlu = 0x406;
 
 // tanh y: below sqrt(0.4) y + y^3 p(y^2), p of degree 4 fitted to (tanh y / y -
 // 1) / y^2 for the least relative error of the whole (5e-9, and f32's rounding);
-// above, 1 - 2 / (e^2|y| + 1), whose subtraction loses less than a bit there.
-// 256 rows over 32768 keys with a soft cap 114 us, 139 with the library's tanhf
-// and a division, 90 without the cap.
+// above, 1 - 2 / (e^2|y| + 1), whose subtraction loses less than a bit there. No
+// division, but the compiler makes the choice a branch, one a score: 256 rows over
+// 32768 keys 107 us with a soft cap and 98 without at head_dim 128, 87 and 59 at 64.
 __device__ __forceinline__ float tanh_of(float y) {
     const float z = y * y;
     float p = __builtin_fmaf(z, -0.00566077698f, 0.0206019953f);
@@ -1303,8 +1307,8 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     if (const int r = vkml::abi::check_launch("attend_pages")) return r;
     // Few rows, in many pieces: a workgroup a row. Many, in a piece or two: a wave
     // for four. Measured (us a call): one token of 32 heads over 32768 keys, 64
-    // pieces a row, 37.5, the waves' 59; 64 tokens of 32 heads in two pieces 68.1
-    // and 66.9; 2600 tokens 228 and 158.
+    // pieces a row, 35.4, the waves' 57.2; 64 tokens of 32 heads in two pieces 64.4
+    // and 63.1; 2600 tokens 222.6 and 149.4.
     const uint32_t rows = p->tokens * p->heads, fours = p->tokens * p->kv_heads * ((a.group + 3) / 4);
     const auto merge = [&](auto kernel, uint32_t workgroups) {
         const Grid grid = grid_of(workgroups);

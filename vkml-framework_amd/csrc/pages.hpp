@@ -73,7 +73,9 @@ struct Batch {
 // A tile has a cost, and the whole of all KV heads' tiles, laid end to end, is
 // cut into equal parts of it, one a workgroup: what a workgroup takes of a tile
 // is a piece. A cut within a tile's own cost is made at its start instead, and one
-// near its end there: the rest would cost more by itself than it evens out.
+// near its end there: the rest would cost more by itself than it evens out. (The
+// parts follow the tiles one by one: a group of more than 128 rows reads its shared
+// keys once for each tile, far apart in time.)
 constexpr int32_t kFewRows = 16;
 constexpr int32_t kTileRows = 128;
 constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
@@ -83,7 +85,8 @@ constexpr int32_t kLeadStep = 128;  // a multiple of every block of keys
 // workgroups a compute unit): f16, head_dim 128, a tile of few rows, which
 // memory bounds, 1.1 beside one of many, and that one 3.4 beside it, 4.0 beside
 // its like; by themselves the tiles take 8 and 10, some of it while the other
-// workgroup works. f32, head_dim 64: 1.6 and 3.8; 1.7 and 1.2.
+// workgroup works. f32, head_dim 64: 1.6 and 3.8; 1.7 and 1.2. f16 at 64 and f32
+// at 128 are not measured: a key's cost goes by its bytes, a tile's own stays.
 struct Costs {
     int32_t few_key, tile_key, few_own, tile_own;
 };
