@@ -9,6 +9,7 @@
 #include <functional>
 #include <map>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "vkml/pages.hpp"
@@ -70,6 +71,9 @@ int vkml_attend_pages(const vkml_attend_pages_params*, const float*, const void*
 }
 
 namespace {
+
+static_assert(!std::is_copy_constructible_v<vkml::PagedCache> && !std::is_copy_assignable_v<vkml::PagedCache>);  // one table for its pools
+static_assert(std::is_move_constructible_v<vkml::PagedCache> && std::is_move_assignable_v<vkml::PagedCache>);
 
 using Ids = std::vector<std::int64_t>;
 constexpr std::int64_t kPages = 40, kPage = 16;

@@ -407,7 +407,7 @@ __device__ __forceinline__ float in_log2(float m, float c) {
 // all of its keys. dead: a bit for each tile that is in no page.
 //
 // A weight is 2^(c (x - m)), the difference taken of the values whose maximum m is:
-// it is 0 at the maximum, however large x is. (2^(c x - c m) by an fma is one
+// its exponent is 0 at the maximum, however large x is. (2^(c x - c m) by an fma is one
 // instruction less, but its two products round apart: at scores of 2^25 the
 // maximum's weight was up to four times too large, past f16's range.)
 template <typename T, int HD, int RT, int TT, bool REGS, bool CAP>

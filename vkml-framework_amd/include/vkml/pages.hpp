@@ -89,6 +89,11 @@ class PagedCache {
 public:
     PagedCache(Context& context, std::int64_t layers, std::int64_t kv_heads, std::int64_t head_dim, std::int64_t pages, std::int64_t page_size,
                DType dtype);
+    // (a copy would have the same pools under a table of its own)
+    PagedCache(const PagedCache&) = delete;
+    PagedCache& operator=(const PagedCache&) = delete;
+    PagedCache(PagedCache&&) = default;
+    PagedCache& operator=(PagedCache&&) = default;
 
     std::int64_t create() { return table_.create(); }
     std::int64_t fork(std::int64_t id) { return table_.fork(id); }
