@@ -1150,3 +1150,71 @@ def test_random_batches(seed):
         lengths[0] = max(lengths[0], 1)
     attend(seed, heads, kv_heads, hd, page, kv, lengths.tolist(), new.tolist(), groups, softcap=float(rng.choice([0.0, 0.0, 20.0])),
            starts=not bool(np.all(new == 1) and rng.random() < 0.5))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_the_longest_sequence(new):
+    """2^26 keys, the same 64 pages over and over: key p's score and value are
+    those of key p % 1024, so that the softmax is over those with 2^16 times
+    their weight (short of the last keys that a token does not see)."""
+    rng = np.random.default_rng(55)
+    heads, hd, page, keys = 4, 64, 16, 2 ** 26
+    cache = Cache(rng, 64, 1, page, hd, H.F16).upload()
+    order = rng.permutation(64).astype(np.int32)
+    p = H.AttendPagesParams(heads=heads, kv_heads=1, head_dim=hd, kv_type=H.F16, page_size=page, pages=64, seqs=1, tokens=new, table_stride=keys // page, scale=0.125)
+    q = rng.standard_normal((new, heads, hd)).astype(np.float32)
+    bufs = [dev(np.tile(order, keys // 1024)), dev(np.array([keys], np.int32)), dev(np.array([0, new], np.int32))]
+    d_q, out, workspace = dev(q), dev(np.full(q.shape, 7.5, np.float32)), H.empty(H.lib().vkml_attend_pages_workspace_bytes(C.byref(p)))
+    print("longest", new, flush=True)
+    H.call("vkml_attend_pages", C.byref(p), d_q.p, cache.dk.p, cache.dv.p, *(b.p for b in bufs), None, None, workspace.p, out.p)
+    got = out.download(np.float32, q.shape)
+    at = np.arange(1024)
+    K, V = (x[order[at // page], 0, at % page].astype(np.float64) for x in (cache.k, cache.v))
+    want = np.empty(q.shape)
+    for t in range(new):
+        x = q[t].astype(np.float64) @ K.T * 0.125
+        w = np.exp(x - x.max(1, keepdims=True)) * (2 ** 16 - (at >= 1024 - (new - 1 - t)))
+        want[t] = (w / w.sum(1, keepdims=True)) @ V
+    # Scores off by up to 2e-6, as in the bound above (scale (2^-22 4 * 52 + 72 2^-24 52)), twice;
+    # the sums go through blocks of 64 or 128 keys, a wave's or workgroup's run of them and the
+    # parts: at most 2^26 / 512 / 64 + 1024 additions in a row, 2^-24 each, of Sum p |v| < 4
+    bound = 4 * (4e-5 + (2 ** 26 / 512 / 64 + 1024) * 2.0 ** -24 + 2.0 ** -20)
+    assert np.abs(got - want).max() <= bound, np.abs(got - want).max()
+    assert np.linalg.norm(got - want) <= 1e-4 * np.linalg.norm(want)
+
+
+def test_as_many_sequences_as_a_batch_takes():
+    """65536 sequences of 0 to 2 keys in a decode step: rope into their pages
+    (16 rows a page, a sequence each), then attention."""
+    rng = np.random.default_rng(56)
+    heads, kv_heads, hd, seqs = 2, 1, 64, 65536
+    lengths = rng.integers(0, 3, seqs).astype(np.int32)
+    lengths[-5:] = [2, 1, 0, 0, 0]
+    table = rng.permutation(seqs).astype(np.int32)
+    cache = Cache(rng, seqs, kv_heads, 16, hd, H.F32).upload()
+    qkv = rng.standard_normal((seqs, (heads + 2 * kv_heads) * hd)).astype(np.float32)
+    common = dict(heads=heads, kv_heads=kv_heads, head_dim=hd, kv_type=H.F32, page_size=16, pages=seqs, seqs=seqs, tokens=seqs, table_stride=1)
+    rp, ap = H.RopeKvPagesParams(row_stride=qkv.shape[1], **common), H.AttendPagesParams(scale=0.125, **common)
+    d = [dev(qkv), dev(table), dev(lengths), dev(np.arange(seqs + 1, dtype=np.int32))]
+    d_q, out, workspace = H.empty(seqs * heads * hd * 4), dev(np.full((seqs, heads, hd), 7.5, np.float32)), H.empty(H.lib().vkml_attend_pages_workspace_bytes(C.byref(ap)))
+    print("sequences", seqs, workspace.nbytes, flush=True)
+    H.call("vkml_rope_kv_pages", C.byref(rp), d[0].p, None, d[1].p, d[2].p, d[3].p, None, d_q.p, cache.dk.p, cache.dv.p)
+    H.call("vkml_attend_pages", C.byref(ap), d_q.p, cache.dk.p, cache.dv.p, d[1].p, d[2].p, d[3].p, None, None, workspace.p, out.p)
+    x = qkv.reshape(seqs, heads + 2 * kv_heads, hd)
+    assert np.array_equal(d_q.download(np.float32, (seqs, heads, hd)), x[:, :heads])
+    some = lengths > 0
+    for pool, got, lane in zip((cache.k, cache.v), cache.download(), (heads, heads + 1)):
+        pool[table[some], 0, lengths[some] - 1] = x[some, lane]
+        assert np.array_equal(got, pool)
+    got = out.download(np.float32, (seqs, heads, hd))
+    K, V = (p[table, 0, :2].astype(np.float64) for p in (cache.k, cache.v))
+    s = np.matmul(x[:, :heads].astype(np.float64), np.ascontiguousarray(K.transpose(0, 2, 1))) * 0.125
+    s[lengths < 2, :, 1] = -np.inf
+    w = np.exp(s - s.max(2, keepdims=True))
+    w /= w.sum(2, keepdims=True)
+    w[~some] = 0
+    size = np.matmul(w, np.abs(V))
+    # delta = 0.125 * 72 2^-24 sum|q k|, at most that of both keys
+    delta = 0.125 * 72 * 2.0 ** -24 * np.matmul(np.abs(x[:, :heads].astype(np.float64)), np.abs(K).sum(1)[:, :, None])
+    top = np.where(np.isfinite(s), np.abs(s), 0).max(2, keepdims=True)
+    close(got, np.matmul(w, V), size * (2 * delta + 2.0 ** -22 * top + 65 * 2.0 ** -24 + 2.0 ** -20))
