@@ -98,3 +98,5 @@ extern "C" int64_t costs_c(const Batch* b, int32_t group, int32_t head_dim, int3
     }
     return s.cost();
 }
+
+extern "C" int64_t most_tiles_c(int64_t group, int64_t seqs, int64_t groups, int64_t tokens) { return most_tiles(group, seqs, groups, tokens); }

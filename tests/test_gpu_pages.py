@@ -1218,3 +1218,23 @@ def test_as_many_sequences_as_a_batch_takes():
     delta = 0.125 * 72 * 2.0 ** -24 * np.matmul(np.abs(x[:, :heads].astype(np.float64)), np.abs(K).sum(1)[:, :, None])
     top = np.where(np.isfinite(s), np.abs(s), 0).max(2, keepdims=True)
     close(got, np.matmul(w, V), size * (2 * delta + 2.0 ** -22 * top + 65 * 2.0 ** -24 + 2.0 ** -20))
+
+
+@pytest.mark.parametrize("seqs,each", [(40, 300), (300, 300)])
+def test_sequences_that_overlap_are_not_worked_on(seqs, each):
+    """Starts that go up and down, which the rules exclude: the call returns
+    and touches the named arrays alone; the next one is as ever."""
+    rng = np.random.default_rng(57)
+    batch = Batch(rng, [each] * seqs, [each] + [0] * (seqs - 1), 16)
+    cache = Cache(rng, batch.pages, 2, 16, 64, H.F16).upload()
+    batch.upload()
+    q = rng.standard_normal((each, 8, 64)).astype(np.float32)
+    call = Call(q, cache, batch, 0.125)
+    want = call.run().result()
+    close(want, *attention_f64(q, cache, batch, 0.125))
+    batch.d_starts.upload(np.asarray([0, each] * (seqs // 2) + [0], np.int32))
+    call.run().result()
+    k, v = cache.download()
+    assert np.array_equal(k, cache.k) and np.array_equal(v, cache.v) and np.array_equal(call.q.download(np.float32, q.shape), q)
+    batch.d_starts.upload(batch.starts)
+    assert np.array_equal(call.run().result().view(np.uint32), want.view(np.uint32))

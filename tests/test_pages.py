@@ -381,3 +381,23 @@ def test_parts_cost_the_same_but_for_their_ends(pages, kv_heads, group, lengths,
     ends = max(own[f] + 64 * key[f] for f in few)
     assert load.max() <= total / n + 2 * ends
     assert abs(load.sum() - total) <= sum(own[f] / 8 + 1 for f in few) * kv_heads * len(got)
+
+
+def test_most_tiles(pages):
+    """No batch within the rules has more tiles of more than 16 rows a KV head;
+    one whose sequences or groups overlap does. 256 threads' sums of one more
+    than that each fit the 32 bits in which they are counted."""
+    pages.most_tiles_c.restype = C.c_int64
+    most = lambda *n: pages.most_tiles_c(*[C.c_int64(int(x)) for x in n])  # noqa: E731
+    assert max(most(g, 65536, 65536, 2 ** 22) for g in (1, 2, 3, 4, 64, 65, 128)) * 257 < 2 ** 32
+    rng = np.random.default_rng(4)
+    for k in range(300):
+        n, group = int(rng.integers(1, 30)), int(rng.choice([1, 3, 4, 16, 65, 128]))
+        new = rng.integers(0, [2, 9, 300][k % 3], n)
+        cuts = sorted(int(x) for x in rng.integers(0, n + 1, 4))
+        starts = np.concatenate([[0], np.cumsum(new)])
+        b, keep = batch(new + 700, starts, cuts, [int(x) for x in rng.integers(0, 700, 3)], int(starts[-1]), 4096)
+        seg = segments(pages, b, group)
+        assert sum(x[5] for x in seg.tolist() if x[1] * group > 16) <= most(group, n, 3, starts[-1])
+    b, keep = batch([500] * 40, [0, 300] * 20 + [0], None, None, 300, 4096)
+    assert sum(x[5] for x in segments(pages, b, 4).tolist()) == 200 > most(4, 40, 0, 300)

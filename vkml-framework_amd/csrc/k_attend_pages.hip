@@ -89,6 +89,7 @@ struct PagesArgs {
     int64_t few_slots, tile_slots;
     uint32_t heads, kv_heads, group, page_shift, pages, table_stride;
     int32_t workgroups_log2;
+    uint32_t most_tiles;
     float score_scale;  // what turns q k^T into a score in log2 units; with a soft cap, into tanh's argument
     float softcap, group_inverse;
     Costs costs;
@@ -952,6 +953,7 @@ __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scrat
         if (each == 1) lds.segments[t] = kept(s);
         cost += s.cost();
         counts += s.few ? static_cast<int64_t>(s.tiles) : static_cast<int64_t>(s.tiles) << 32;
+        if (counts >> 32 > a.most_tiles) break;  // and more in all: nothing is done below
     }
     lds.cost[t] = inclusive_sum(cost);
     lds.counts[t] = inclusive_sum(counts);
@@ -968,7 +970,7 @@ __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scrat
     out.parts_log2 = parts_log2(out.cost, a.workgroups_log2);
     // dealt to the XCDs round-robin: the parts of one are neighbours
     const int32_t b = static_cast<int32_t>(blockIdx.x);
-    if (out.cost == 0 || b >> out.parts_log2) return false;
+    if (out.cost == 0 || b >> out.parts_log2 || static_cast<uint64_t>(counts_head) >> 32 > a.most_tiles) return false;
     out.part = (b % 8 << (out.parts_log2 - 3)) + b / 8;
     out.kvh = static_cast<int32_t>(static_cast<int64_t>(a.kv_heads) * out.part >> out.parts_log2);
     const int64_t unit = part_start(out.cost, out.parts_log2, out.part) - out.kvh * per_head;
@@ -1290,6 +1292,7 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     a.pages = p->pages;
     a.table_stride = p->table_stride;
     a.workgroups_log2 = workgroups_log2();
+    a.most_tiles = static_cast<uint32_t>(most_tiles(a.group, p->seqs, p->groups, p->tokens));  // at most 2^23 + 2^17
     a.score_scale = p->softcap > 0.0f ? p->scale / p->softcap : p->scale * kLog2e;
     a.softcap = p->softcap;
     a.costs = costs(p->head_dim, p->kv_type == VKML_F16);

@@ -253,11 +253,16 @@ struct Slots {
     int64_t few, tile;  // of each kind
     VKML_HD int64_t rows() const { return few * kFewRows + tile * kTileRows; }
 };
-VKML_HD Slots slots(int64_t kv_heads, int64_t group, int64_t seqs, int64_t groups, int64_t tokens, int64_t workgroups) {
+// A KV head's tiles of more than kFewRows rows, at most. A batch whose sequences
+// or groups overlap (which the rules exclude) may have any number, as many as would
+// keep the GPU busy for hours: nothing is done for one that has more.
+VKML_HD int64_t most_tiles(int64_t group, int64_t seqs, int64_t groups, int64_t tokens) {
     const int64_t many = tokens * group / (kFewRows + 1);  // segments of each kind with more than kFewRows rows, at most
     const int64_t step = tile_tokens(static_cast<int32_t>(group));
-    const int64_t tiles = 2 * (tokens / step) + (seqs < many ? seqs : many) + (groups < many ? groups : many);
-    return {workgroups + kv_heads * (seqs + groups), workgroups + kv_heads * tiles};
+    return 2 * (tokens / step) + (seqs < many ? seqs : many) + (groups < many ? groups : many);
+}
+VKML_HD Slots slots(int64_t kv_heads, int64_t group, int64_t seqs, int64_t groups, int64_t tokens, int64_t workgroups) {
+    return {workgroups + kv_heads * (seqs + groups), workgroups + kv_heads * most_tiles(group, seqs, groups, tokens)};
 }
 
 // The grid of `workgroups`, numbered y * x + x's own: a launch has less than 2^32
