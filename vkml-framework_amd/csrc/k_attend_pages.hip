@@ -44,7 +44,7 @@
 // reads the shared keys from memory); 2600 tokens of six prompts 149 us, 16 to join
 // (115 GFLOP).
 // What the three ways through a tile need at once is more than the scalar registers
-// hold: 160 to 209 are spilled to lanes of vector registers; of those none is.
+// hold: 155 to 198 are spilled to lanes of vector registers; of those none is.
 // Short ones are a chain of waits: 1.0 us for the batch's arrays, 0.8 to find the
 // part, 1.3 its first tile, 1.2 for pages and keys, 2 to 3 the block, 0.8 the end.
 #include <hip/hip_runtime.h>
