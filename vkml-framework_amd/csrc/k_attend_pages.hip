@@ -39,9 +39,9 @@
 // Measured (a whole call, 32 query and 8 KV heads of 128, f16): one token over
 // 32768 keys 35 us, 5 of them to join its pieces, 134 MB at 4.4 TB/s before that (a
 // large copy reaches 5.0); 64 sequences with 32768 shared keys and 1000 of their own
-// 121 us, 8 to join (71 GFLOP, the split counted twice, and 547 MB read where 407
+// 122 us, 8 to join (71 GFLOP, the split counted twice, and 547 MB read where 407
 // are needed: the group's 256 rows are two tiles, one after the other, and each
-// reads the shared keys from memory); 2600 tokens of six prompts 149 us, 16 to join
+// reads the shared keys from memory); 2600 tokens of six prompts 147 us, 16 to join
 // (115 GFLOP).
 // What the three ways through a tile need at once is more than the scalar registers
 // hold: 155 to 198 are spilled to lanes of vector registers; of those none is.
