@@ -740,6 +740,89 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* d_q, const
                       const int32_t* d_table, const int32_t* d_lengths, const int32_t* d_starts,
                       const int32_t* d_group_starts, const int32_t* d_group_keys, void* d_workspace, float* d_out);
 
+/* vkml_attend_pages for a tree of tokens, as in speculative decoding: a token
+ * sees its sequence's keys before the new tokens, and of these only what its row
+ * of d_seen says: bit i % 32 of word i / 32 of d_seen [tokens, seen_words] is set
+ * where the token sees its sequence's new token i. Bits of later tokens than
+ * itself count as 0 (so do new tokens past the row's bits); its own does not: a
+ * token that sees itself, as a tree's node does, has its own bit set. The rest, the
+ * groups and the workspace are vkml_attend_pages's. seen_words 1 to 128. */
+int vkml_attend_pages_tree(const vkml_attend_pages_params* p, uint32_t seen_words, const float* d_q, const void* d_k_pages,
+                           const void* d_v_pages, const int32_t* d_table, const int32_t* d_lengths,
+                           const int32_t* d_starts, const int32_t* d_group_starts, const int32_t* d_group_keys,
+                           const uint32_t* d_seen, void* d_workspace, float* d_out);
+
+/* vkml_attend_pages with a window: a token at position p sees the keys past p -
+ * window up to its own, and its sequence's first `sinks` (0: none). Pages of which
+ * no token sees a key are not read: their table entries may be -1. window at
+ * least 1; no groups (p->groups 0). */
+int vkml_attend_pages_window(const vkml_attend_pages_params* p, uint32_t window, uint32_t sinks, const float* d_q,
+                             const void* d_k_pages, const void* d_v_pages, const int32_t* d_table,
+                             const int32_t* d_lengths, const int32_t* d_starts, void* d_workspace, float* d_out);
+
+/* The end of a step of speculative decoding. A sequence's new tokens are a tree:
+ * node 0 the token that the last step picked, node i > 0 drafted after its parent
+ * d_parents[i] (an index among the sequence's new tokens, less than i; what is not
+ * makes the node no one's child), its token d_drafted[i]; d_picked[i] is what the
+ * model picked after node i (vkml_sample, or an argmax of its logits). From node 0
+ * on, the path goes to the first child whose drafted token is the pick, until there
+ * is none. d_path holds the path's nodes where the sequence's new tokens are, then
+ * -1; d_counts[s] their number (0 for a sequence without new tokens) and d_next[s]
+ * the pick after the last (-1). In every layer the keys and values of the path's
+ * nodes move to the positions after one another that follow the sequence's earlier
+ * keys, so that it goes on with d_lengths[s] - n + d_counts[s] keys (the caller's
+ * to set); the rows behind them are unspecified, all others stay as they were. At
+ * most 4096 nodes a sequence: those past them are left out. layer_stride in
+ * elements as page_stride (0: no gap). d_drafted, d_picked and the outputs [tokens]
+ * and [seqs]; all but the pools may be any 32-bit values. */
+typedef struct vkml_keep_drafts_params {
+    uint32_t kv_heads;
+    uint32_t head_dim;
+    uint32_t kv_type;
+    uint32_t page_size;
+    uint32_t pages;
+    uint32_t layers;
+    uint32_t seqs;
+    uint32_t tokens;
+    uint32_t table_stride;
+    uint64_t page_stride;
+    uint64_t layer_stride; /* from one layer's pool to the next's */
+} vkml_keep_drafts_params;
+int vkml_keep_drafts(const vkml_keep_drafts_params* p, const int32_t* d_parents, const int32_t* d_drafted,
+                     const int32_t* d_picked, const int32_t* d_table, const int32_t* d_lengths, const int32_t* d_starts,
+                     int32_t* d_path, int32_t* d_counts, int32_t* d_next, void* d_k_pages, void* d_v_pages);
+
+/* A token for each row of logits, as vkml::Sampler picks one (sampling.hpp; no
+ * penalties: they change the logits before). A row's candidates are ranked by
+ * logit, equal ones by id. temperature 0 (or less, or NaN) or top_k 1: the first.
+ * Otherwise a candidate weighs exp((l - largest) / temperature); top_k > 0 keeps the
+ * first top_k, then top_p < 1 the fewest whose weights reach top_p of those kept (at
+ * least one), then min_p > 0 those that weigh at least min_p times the first; the
+ * pick is the first candidate whose weight and those before it pass d_random[row]
+ * (in [0, 1); values outside count as its ends) times the kept weight. d_options
+ * [rows], 16-byte aligned, device memory that the launch reads. Logits that are NaN
+ * or -infinity are never picked, beside +infinity nothing else is; a row without a
+ * candidate gives -1. Weights are rounded to 2^-min(51, 62 - ceil(log2(vocab))) of
+ * the largest and summed exactly, so that the same row gives the same token in every
+ * call. A row starts every row_stride floats; vocab at most 2^22. d_workspace:
+ * vkml_sample_workspace_bytes(p) bytes of any content, 16-byte aligned (0, and NULL
+ * taken, up to 32765 logits; 40 rows of 128256: 3.9 MB); calls that overlap need
+ * one each. */
+typedef struct vkml_sampling {
+    float temperature;
+    int32_t top_k;
+    float top_p;
+    float min_p;
+} vkml_sampling;
+typedef struct vkml_sample_params {
+    uint32_t rows;
+    uint32_t vocab;
+    uint64_t row_stride;
+} vkml_sample_params;
+uint64_t vkml_sample_workspace_bytes(const vkml_sample_params* p);
+int vkml_sample(const vkml_sample_params* p, const float* d_logits, const vkml_sampling* d_options,
+                const double* d_random, void* d_workspace, int32_t* d_tokens);
+
 /* The new tokens' q | k | v (rows of d_qkv, row_stride floats apart): q and
  * k rotated at the token's position (or d_positions[token], if non-NULL) by
  * d_rope_table [positions, rotary_dim / 2, 2] (cos, sin; vkml::rope_table,

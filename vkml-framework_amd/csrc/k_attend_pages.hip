@@ -93,7 +93,20 @@ struct PagesArgs {
     float score_scale;  // what turns q k^T into a score in log2 units; with a soft cap, into tanh's argument
     float softcap, group_inverse;
     Costs costs;
+    Window window;         // kWindow
+    const uint32_t* seen;  // kTree: [tokens, seen_words]
+    uint32_t seen_words;
 };
+
+// What a row sees of its sequence's keys up to its own position: all, those before
+// the new tokens and its bits' among these, or a window and the sinks.
+enum Mask { kCausal, kTree, kWindow };
+
+template <int MASK>
+__device__ __forceinline__ Window window_of(const PagesArgs& a) {
+    if constexpr (MASK == kWindow) return a.window;
+    else return {};
+}
 
 // A value that a wave's lanes share, in a scalar register.
 __device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -342,6 +355,22 @@ struct Limits {
     int32_t limit[RT];
 };
 
+// kTree: the position of a piece's sequence's first new token, and what makes a
+// row's limit its token.
+struct Sees {
+    int32_t base, to_token;
+};
+
+// The 64 bits from new token b on (b < 0: before the first; keys there are seen) of a
+// token's words.
+__device__ __forceinline__ uint64_t seen_bits(const PagesArgs& a, int32_t token, int32_t b) {
+    const int32_t w = b >> 5, words = static_cast<int32_t>(a.seen_words);
+    const uint32_t* row = a.seen + static_cast<uint64_t>(static_cast<uint32_t>(token)) * a.seen_words;
+    const auto word = [&](int32_t i) { return i < 0 ? ~0u : i < words ? ldg(row + i) : 0u; };
+    const uint64_t two = static_cast<uint64_t>(word(w + 1)) << 32 | word(w);
+    return b & 31 ? two >> (b & 31) | static_cast<uint64_t>(word(w + 2)) << (64 - (b & 31)) : two;
+}
+
 // Zeros for the infinities and NaN among a masked block's V values, N 16-byte
 // pieces a thread; whether any of the thread's were those of keys that count.
 template <typename T, uint32_t ROW, int N>
@@ -411,8 +440,8 @@ __device__ __forceinline__ float in_log2(float m, float c) {
 // its exponent is 0 at the maximum, however large x is. (2^(c x - c m) by an fma is one
 // instruction less, but its two products round apart: at scores of 2^25 the
 // maximum's weight was up to four times too large, past f16's range.)
-template <typename T, int HD, int RT, int TT, bool REGS, bool CAP>
-__device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const Limits<RT>& lim, const Keys& keys, bool masked, uint32_t dead, float softcap,
+template <typename T, int HD, int RT, int TT, bool REGS, bool CAP, int MASK>
+__device__ __forceinline__ void attend_block(const PagesArgs& a, const Sees& sees, const Queries<T, HD, RT>& q, const Limits<RT>& lim, const Keys& keys, bool masked, uint32_t dead, float softcap,
                                              const uint4 (*k_regs)[Block<T, HD>::kSteps], const uint8_t* k, const uint8_t* v,
                                              Running<HD, RT>& run) {
 #pragma clang fp contract(off)
@@ -473,13 +502,24 @@ __device__ __forceinline__ void attend_block(const Queries<T, HD, RT>& q, const 
         }
         if (masked) {
             const int32_t limit = keys.lead ? keys.end : lim.limit[rt];
+            uint64_t bits[(TT + 3) / 4];  // of the lane's first key in each four tiles on
+            if constexpr (MASK == kTree) {
 #pragma unroll
-            for (int tt = 0; tt < TT; ++tt)
+                for (int i = 0; i < (TT + 3) / 4; ++i)
+                    bits[i] = keys.lead ? ~0ull : seen_bits(a, lim.limit[rt] + sees.to_token, keys.key0 + 64 * i + 4 * static_cast<int32_t>(g) - sees.base);
+            }
+#pragma unroll
+            for (int tt = 0; tt < TT; ++tt) {
+                const int32_t key0 = keys.key0 + 16 * tt + 4 * static_cast<int32_t>(g);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int32_t key = keys.key0 + 16 * tt + 4 * static_cast<int32_t>(g) + e;
-                    if (key < keys.from || key >= limit || (dead >> tt & 1)) s[rt][tt][e] = -__builtin_inff();
+                    const int32_t key = key0 + e;
+                    bool hidden = key < keys.from || key >= limit || (dead >> tt & 1);
+                    if constexpr (MASK == kTree) hidden |= !(bits[tt / 4] >> (tt % 4 * 16 + e) & 1);
+                    if constexpr (MASK == kWindow) hidden |= !keys.lead && key < limit - a.window.keys && key >= a.window.sinks;
+                    if (hidden) s[rt][tt][e] = -__builtin_inff();
                 }
+            }
         }
         float bm = -__builtin_inff();
 #pragma unroll
@@ -583,6 +623,7 @@ struct Piece {
     int32_t x0, x1;
     int32_t token0, tokens;
     int32_t limit0;    // the position below which the first token sees
+    Sees sees;
     bool causal;       // and each further token one more
     bool whole;        // all of its rows' work: the output itself
     int64_t slot_row;  // else the rows of the workspace, -1 for none
@@ -652,14 +693,17 @@ __device__ __forceinline__ float* row_to(const PagesArgs& a, const Piece& p, uin
 }
 
 // Whether some of a tile's rows don't see all of a block of `span` keys.
-__device__ __forceinline__ bool is_masked(const Piece& p, const Keys& keys, int32_t span, uint32_t dead) {
-    return keys.key0 < keys.from || keys.key0 + span > (keys.lead ? keys.end : p.limit0) || dead;
+template <int MASK>
+__device__ __forceinline__ bool is_masked(const PagesArgs& a, const Piece& p, const Keys& keys, int32_t span, uint32_t dead) {
+    const bool cut = keys.key0 < keys.from || keys.key0 + span > (keys.lead ? keys.end : MASK == kTree ? p.sees.base : p.limit0) || dead;
+    if constexpr (MASK == kWindow) return cut || (!keys.lead && keys.key0 < p.limit0 + p.tokens - 1 - a.window.keys && keys.key0 + span > a.window.sinks);
+    else return cut;
 }
 
 // The infinities and NaN of V in a piece's masked blocks, which the products
 // have left out, for the rows that see them, where the workgroup has stored
 // those: a row's value there is their sum, whatever the finite ones are.
-template <typename T, int HD>
+template <typename T, int HD, int MASK>
 __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Piece& p) {
     using B = Block<T, HD>;
     if (!p.whole && p.slot_row < 0) return;
@@ -667,7 +711,7 @@ __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Piece& p
     __syncthreads();  // the rows are stored
     for (int32_t x = p.x0; x < p.x1; x += B::kKeys) {
         const Pages at = pages_at(a, p.tile, x);
-        if (!is_masked(p, at.keys, B::kKeys, dead_tiles<B::kTiles>(a, at))) continue;
+        if (!is_masked<MASK>(a, p, at.keys, B::kKeys, dead_tiles<B::kTiles>(a, at))) continue;
 #pragma unroll 1
         for (int32_t key = max(at.keys.key0, at.keys.from); key < min(at.keys.key0 + static_cast<int32_t>(B::kKeys), at.keys.end); ++key) {
             const int32_t id = ld_scalar_i32(at.keys.table + (key >> a.page_shift));
@@ -677,7 +721,14 @@ __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Piece& p
 #pragma unroll 1
             for (uint32_t r = thread / HD; r < rows; r += kThreads / HD) {
                 const uint32_t t = token_of(a, r);
-                if (!at.keys.lead && p.causal && key >= p.limit0 + static_cast<int32_t>(t)) continue;
+                const int32_t limit = p.limit0 + static_cast<int32_t>(t);
+                if (!at.keys.lead && p.causal && key >= limit) continue;
+                if constexpr (MASK == kTree) {
+                    if (!at.keys.lead && !(seen_bits(a, p.token0 + static_cast<int32_t>(t), key - p.sees.base) & 1)) continue;
+                }
+                if constexpr (MASK == kWindow) {
+                    if (!at.keys.lead && key < limit - a.window.keys && key >= a.window.sinks) continue;
+                }
                 float* to = p.whole ? a.out + (static_cast<uint64_t>(p.token0 + t) * a.heads + p.tile.kvh * a.group + r - t * a.group) * HD + dim
                                     : a.o + (p.slot_row + r) * HD + dim;
                 stg(to, ldg(to) + v);
@@ -687,7 +738,7 @@ __device__ __forceinline__ void add_unbounded(const PagesArgs& a, const Piece& p
 }
 
 // At most 16 rows: each wave by itself over blocks of kWaveKeys keys in turn.
-template <typename T, int HD, bool CAP>
+template <typename T, int HD, bool CAP, int MASK>
 __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buffer& buf0, Buffer& buf1) {
     using B = Block<T, HD>;
     constexpr int TT = B::kWaveTiles;
@@ -739,9 +790,9 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             const uint32_t dead = dead_tiles<TT>(a, cur);
             if (x + kStep < p.x1) issue(nxt, k_next, there);
             const Pages after = pages_after(a, p.tile, nxt, x + 2 * kStep, kSpan);
-            const bool masked = is_masked(p, cur.keys, kSpan, dead);
+            const bool masked = is_masked<MASK>(a, p, cur.keys, kSpan, dead);
             if (masked) unbounded |= clear_unbounded<T, B::kRow, 8>(here, l, kWave, cur.keys, dead);
-            attend_block<T, HD, 1, TT, true, CAP>(q, lim, cur.keys, masked, dead, a.softcap, k, nullptr, here, run);
+            attend_block<T, HD, 1, TT, true, CAP, MASK>(a, p.sees, q, lim, cur.keys, masked, dead, a.softcap, k, nullptr, here, run);
             cur = nxt;
             nxt = after;
             x += kStep;
@@ -794,11 +845,11 @@ __device__ __forceinline__ void few_rows(const PagesArgs& a, const Piece& p, Buf
             if (to) stg(reinterpret_cast<float4*>(to + dim), make_float4(o[0] * times, o[1] * times, o[2] * times, o[3] * times));
         }
     }
-    if (uniform(static_cast<int32_t>(found[0] | found[1] | found[2] | found[3]))) add_unbounded<T, HD>(a, p);
+    if (uniform(static_cast<int32_t>(found[0] | found[1] | found[2] | found[3]))) add_unbounded<T, HD, MASK>(a, p);
 }
 
 // Many rows: RT tiles of 16 a wave, the blocks shared.
-template <typename T, int HD, int RT, bool CAP>
+template <typename T, int HD, int RT, bool CAP, int MASK>
 __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Buffer& buf0, Buffer& buf1) {
     using B = Block<T, HD>;
     constexpr int TT = B::kTiles;
@@ -843,12 +894,12 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
             const uint32_t dead = dead_tiles<TT>(a, cur);
             if (x + kSpan < p.x1) issue(nxt, there);
             const Pages after = pages_after(a, p.tile, nxt, x + 2 * kSpan, kSpan);
-            const bool masked = is_masked(p, cur.keys, kSpan, dead);
+            const bool masked = is_masked<MASK>(a, p, cur.keys, kSpan, dead);
             if (masked) {
                 unbounded |= clear_unbounded<T, B::kRow, 4>(here + sizeof buf0.k, thread, kThreads, cur.keys, dead);
                 lds_barrier();
             }
-            attend_block<T, HD, RT, TT, false, CAP>(q, lim, cur.keys, masked, dead, a.softcap, nullptr, here, here + sizeof buf0.k, run);
+            attend_block<T, HD, RT, TT, false, CAP, MASK>(a, p.sees, q, lim, cur.keys, masked, dead, a.softcap, nullptr, here, here + sizeof buf0.k, run);
             cur = nxt;
             nxt = after;
             x += kSpan;
@@ -878,7 +929,7 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
             }
         }
     }
-    if (found) add_unbounded<T, HD>(a, p);
+    if (found) add_unbounded<T, HD, MASK>(a, p);
 }
 
 // ---------------------------------------------------------------- the launch
@@ -908,7 +959,7 @@ struct Kept {
 __device__ __forceinline__ Kept kept(const Segment& s) {
     return {{s.row, s.lead_row, s.lead, s.token0, s.n, s.from, s.base, s.tiles, s.step, (s.few ? 1 : 0) + (s.shared ? 2 : 0)}};
 }
-__device__ __forceinline__ Segment taken(const Kept& k, Costs costs) {
+__device__ __forceinline__ Segment taken(const Kept& k, Costs costs, Window window) {
     Segment s;
     s.row = uniform(k.v[0]);
     s.lead_row = uniform(k.v[1]);
@@ -924,6 +975,7 @@ __device__ __forceinline__ Segment taken(const Kept& k, Costs costs) {
     s.shared = flags & 2;
     s.key_cost = s.few ? costs.few_key : costs.tile_key;
     s.own_cost = s.few ? costs.few_own : costs.tile_own;
+    s.set(window);
     return s;
 }
 
@@ -944,12 +996,13 @@ struct Place {
 
 // Every thread sums its run of segments (one, up to kThreads of them), and the
 // waves' sums place the part's first unit among them.
+template <int MASK>
 __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scratch& lds) {
     const int32_t n = a.batch.groups + a.batch.seqs, each = n <= static_cast<int32_t>(kThreads) ? 1 : (n + kThreads - 1) / kThreads;
     const int32_t t = static_cast<int32_t>(threadIdx.x), i0 = t * each, i1 = min(i0 + each, n);
     int64_t cost = 0, counts = 0;
     for (int32_t i = i0; i < i1; ++i) {
-        const Segment s = segment(a.batch, a.group, a.costs, i);
+        const Segment s = segment(a.batch, a.group, a.costs, i, window_of<MASK>(a));
         if (each == 1) lds.segments[t] = kept(s);
         cost += s.cost();
         counts += s.few ? static_cast<int64_t>(s.tiles) : static_cast<int64_t>(s.tiles) << 32;
@@ -995,7 +1048,7 @@ __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scrat
     }
     int32_t i = static_cast<int32_t>(kWave * w + lane) * each;
     for (; each > 1; ++i) {
-        const Segment s = segment(a.batch, a.group, a.costs, i);
+        const Segment s = segment(a.batch, a.group, a.costs, i, window_of<MASK>(a));
         if (unit < off + s.cost()) break;
         off += s.cost();
         before += s.few ? static_cast<int64_t>(s.tiles) : static_cast<int64_t>(s.tiles) << 32;
@@ -1007,13 +1060,13 @@ __device__ __forceinline__ bool find_place(const PagesArgs& a, Place& out, Scrat
     return true;
 }
 
-template <typename T, int HD, bool CAP>
+template <typename T, int HD, bool CAP, int MASK>
 __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     using B = Block<T, HD>;
     __shared__ Buffer buf0, buf1;  // apart: the compiler then knows that they are
     __shared__ Scratch scratch;
     Place at;
-    if (!find_place(a, at, scratch)) return;
+    if (!find_place<MASK>(a, at, scratch)) return;
     const int64_t part_end = part_start(at.cost, at.parts_log2, at.part + 1);
     const int32_t segments = a.batch.groups + a.batch.seqs;
     int32_t kvh = at.kvh, i = at.segment, few = at.few, tiles = at.tiles, tile = 0;
@@ -1021,7 +1074,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
     int64_t begin = at.unit, end = begin + part_end - part_start(at.cost, at.parts_log2, at.part);
     bool again = false;
     for (;;) {
-        const Segment s = segments <= static_cast<int32_t>(kThreads) ? taken(scratch.segments[i], a.costs) : segment(a.batch, a.group, a.costs, i);
+        const Segment s = segments <= static_cast<int32_t>(kThreads) ? taken(scratch.segments[i], a.costs, window_of<MASK>(a)) : segment(a.batch, a.group, a.costs, i, window_of<MASK>(a));
         tile = 0;
         if (begin > 0 && s.tiles > 1) {
             tile = s.tile_at(begin);
@@ -1041,11 +1094,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             Piece p;
             p.x0 = cut(from, s, keys, B::kKeys);
             p.x1 = ends ? keys : cut(to, s, keys, B::kKeys);
+            const Segment::Where in = s.where(tile);
             p.tile = {a.table + static_cast<uint64_t>(s.lead_row) * a.table_stride, a.table + static_cast<uint64_t>(s.row) * a.table_stride,
-                      s.lead_span(), s.lead, s.lo(), s.from, s.lo() + keys - s.lead_span(), static_cast<uint32_t>(kvh)};
+                      in.span, in.lead, in.lo, in.from, in.end, static_cast<uint32_t>(kvh)};
             p.token0 = s.token0 + tile * s.step;
             p.tokens = s.tile_n(tile);
             p.limit0 = s.limit(tile * s.step);
+            p.sees = {s.shared ? p.limit0 : s.lo() + s.base, p.token0 - p.limit0};
             p.causal = !s.shared;
             // the rows' own keys are all there is, but for a shared segment's
             const bool all = !s.shared && s.from == s.lead;
@@ -1066,9 +1121,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_attend_pages(PagesArgs a) {
             }
             if (again) lds_barrier();  // the last piece's LDS
             again = true;
-            if (s.few) few_rows<T, HD, CAP>(a, p, buf0, buf1);
-            else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1, CAP>(a, p, buf0, buf1);
-            else many_rows<T, HD, 2, CAP>(a, p, buf0, buf1);
+            if (s.few) few_rows<T, HD, CAP, MASK>(a, p, buf0, buf1);
+            else if (p.tokens * a.group <= kTileRows / 2) many_rows<T, HD, 1, CAP, MASK>(a, p, buf0, buf1);
+            else many_rows<T, HD, 2, CAP, MASK>(a, p, buf0, buf1);
             if (end <= 0) return;
         }
         (s.few ? few : tiles) += s.tiles;
@@ -1244,39 +1299,44 @@ Slots slots_of(const vkml_attend_pages_params& p) {
 
 uint64_t up16(uint64_t bytes) { return (bytes + 15) / 16 * 16; }
 
-}  // namespace
+struct Call {
+    const char* name;
+    const float* q;
+    const void* k;
+    const void* v;
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* starts;
+    const int32_t* group_starts;
+    const int32_t* group_keys;
+    void* workspace;
+    float* out;
+};
 
-extern "C" {
-
-uint64_t vkml_attend_pages_workspace_bytes(const vkml_attend_pages_params* p) {
-    if (!p || !vkml::abi::initialized() || check(*p)) return 0;
-    const uint64_t rows = slots_of(*p).rows();
-    return up16(static_cast<uint64_t>(p->kv_heads) * p->tokens * 2 * sizeof(Parts)) + up16(rows * sizeof(float2)) + rows * p->head_dim * sizeof(float);
-}
-
-int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const void* k_pages, const void* v_pages, const int32_t* table,
-                      const int32_t* lengths, const int32_t* starts, const int32_t* group_starts, const int32_t* group_keys, void* workspace,
-                      float* out) {
+// One of the calls, whose own arguments `set` takes and checks.
+template <int MASK, typename Set>
+int attend(const vkml_attend_pages_params* p, const Call& c, const Set& set) {
     VKML_REQUIRE_INIT();
-    VKML_CHECK_ARG(p, "attend_pages: null params");
-    if (const char* why = check(*p)) return vkml::abi::fail(VKML_ERROR_INVALID_ARGUMENT, std::string("attend_pages: ") + why);
+    const auto refuse = [&](const char* why) { return vkml::abi::fail(VKML_ERROR_INVALID_ARGUMENT, std::string(c.name) + ": " + why); };
+    if (!p) return refuse("null params");
+    if (const char* why = check(*p)) return refuse(why);
+    PagesArgs a{};
+    if (const char* why = set(a)) return refuse(why);
     if (p->seqs == 0 || p->tokens == 0) return VKML_OK;
-    VKML_CHECK_ARG(starts || p->tokens == p->seqs, "attend_pages: without starts every sequence has one token");
-    VKML_CHECK_ARG(q && k_pages && v_pages && table && lengths && workspace && out && (p->groups == 0 || (group_starts && group_keys)),
-                   "attend_pages: null buffer");
-    VKML_CHECK_ARG(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(workspace) && aligned16(out),
-                   "attend_pages: q, the pools, the workspace and out must be 16-byte aligned");
-    const Batch batch{lengths, starts, group_starts, group_keys, static_cast<int32_t>(p->seqs), static_cast<int32_t>(p->tokens),
+    if (!c.starts && p->tokens != p->seqs) return refuse("without starts every sequence has one token");
+    if (!(c.q && c.k && c.v && c.table && c.lengths && c.workspace && c.out && (p->groups == 0 || (c.group_starts && c.group_keys)))) return refuse("null buffer");
+    if (!(aligned16(c.q) && aligned16(c.k) && aligned16(c.v) && aligned16(c.workspace) && aligned16(c.out)))
+        return refuse("q, the pools, the workspace and out must be 16-byte aligned");
+    const Batch batch{c.lengths, c.starts, c.group_starts, c.group_keys, static_cast<int32_t>(p->seqs), static_cast<int32_t>(p->tokens),
                       static_cast<int32_t>(p->groups), static_cast<int32_t>(p->table_stride * p->page_size)};
     const uint64_t stride = p->page_stride ? p->page_stride : static_cast<uint64_t>(p->kv_heads) * p->page_size * p->head_dim;
     const Slots s = slots_of(*p);
-    auto* at = static_cast<uint8_t*>(workspace);
-    PagesArgs a{};
-    a.q = q;
-    a.k = static_cast<const uint8_t*>(k_pages);
-    a.v = static_cast<const uint8_t*>(v_pages);
-    a.table = table;
-    a.out = out;
+    auto* at = static_cast<uint8_t*>(c.workspace);
+    a.q = c.q;
+    a.k = static_cast<const uint8_t*>(c.k);
+    a.v = static_cast<const uint8_t*>(c.v);
+    a.table = c.table;
+    a.out = c.out;
     a.parts = reinterpret_cast<Parts*>(at);
     at += up16(static_cast<uint64_t>(p->kv_heads) * p->tokens * 2 * sizeof(Parts));
     a.stats = reinterpret_cast<float2*>(at);
@@ -1297,17 +1357,17 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     a.softcap = p->softcap;
     a.costs = costs(p->head_dim, p->kv_type == VKML_F16);
     a.group_inverse = 1.0f / static_cast<float>(a.group);
-    vkml::abi::ProfileScope prof("attend_pages");
+    vkml::abi::ProfileScope prof(c.name);
     const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(1u << a.workgroups_log2), dim3(kThreads), 0, vkml::abi::stream(), a); };
     const bool wide = p->head_dim == 128;
     if (p->kv_type == VKML_F16) {
-        if (p->softcap > 0.0f) wide ? go(k_attend_pages<_Float16, 128, true>) : go(k_attend_pages<_Float16, 64, true>);
-        else wide ? go(k_attend_pages<_Float16, 128, false>) : go(k_attend_pages<_Float16, 64, false>);
+        if (p->softcap > 0.0f) wide ? go(k_attend_pages<_Float16, 128, true, MASK>) : go(k_attend_pages<_Float16, 64, true, MASK>);
+        else wide ? go(k_attend_pages<_Float16, 128, false, MASK>) : go(k_attend_pages<_Float16, 64, false, MASK>);
     } else {
-        if (p->softcap > 0.0f) wide ? go(k_attend_pages<float, 128, true>) : go(k_attend_pages<float, 64, true>);
-        else wide ? go(k_attend_pages<float, 128, false>) : go(k_attend_pages<float, 64, false>);
+        if (p->softcap > 0.0f) wide ? go(k_attend_pages<float, 128, true, MASK>) : go(k_attend_pages<float, 64, true, MASK>);
+        else wide ? go(k_attend_pages<float, 128, false, MASK>) : go(k_attend_pages<float, 64, false, MASK>);
     }
-    if (const int r = vkml::abi::check_launch("attend_pages")) return r;
+    if (const int r = vkml::abi::check_launch(c.name)) return r;
     // Few rows, in many pieces: a workgroup a row. Many, in a piece or two: a wave
     // for four. Measured (us a call): one token of 32 heads over 32768 keys, 64
     // pieces a row, 35.4, the waves' 57.2; 64 tokens of 32 heads in two pieces 64.4
@@ -1319,7 +1379,46 @@ int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const v
     };
     if (rows <= 4096) wide ? merge(k_attend_pages_merge<128>, rows) : merge(k_attend_pages_merge<64>, rows);
     else wide ? merge(k_attend_pages_merge_many<128>, (fours + kWaves - 1) / kWaves) : merge(k_attend_pages_merge_many<64>, (fours + kWaves - 1) / kWaves);
-    return vkml::abi::check_launch("attend_pages: merge");
+    return vkml::abi::check_launch(c.name);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t vkml_attend_pages_workspace_bytes(const vkml_attend_pages_params* p) {
+    if (!p || !vkml::abi::initialized() || check(*p)) return 0;
+    const uint64_t rows = slots_of(*p).rows();
+    return up16(static_cast<uint64_t>(p->kv_heads) * p->tokens * 2 * sizeof(Parts)) + up16(rows * sizeof(float2)) + rows * p->head_dim * sizeof(float);
+}
+
+int vkml_attend_pages(const vkml_attend_pages_params* p, const float* q, const void* k_pages, const void* v_pages, const int32_t* table,
+                      const int32_t* lengths, const int32_t* starts, const int32_t* group_starts, const int32_t* group_keys, void* workspace,
+                      float* out) {
+    const Call c{"attend_pages", q, k_pages, v_pages, table, lengths, starts, group_starts, group_keys, workspace, out};
+    return attend<kCausal>(p, c, [](PagesArgs&) -> const char* { return nullptr; });
+}
+
+int vkml_attend_pages_tree(const vkml_attend_pages_params* p, uint32_t seen_words, const float* q, const void* k_pages, const void* v_pages,
+                           const int32_t* table, const int32_t* lengths, const int32_t* starts, const int32_t* group_starts,
+                           const int32_t* group_keys, const uint32_t* seen, void* workspace, float* out) {
+    const Call c{"attend_pages_tree", q, k_pages, v_pages, table, lengths, starts, group_starts, group_keys, workspace, out};
+    return attend<kTree>(p, c, [=](PagesArgs& a) -> const char* {
+        a.seen = seen;
+        a.seen_words = seen_words;
+        const char* why = check_tree(seen_words);
+        return why ? why : seen || p->seqs == 0 || p->tokens == 0 ? nullptr : "null buffer";
+    });
+}
+
+int vkml_attend_pages_window(const vkml_attend_pages_params* p, uint32_t window, uint32_t sinks, const float* q, const void* k_pages,
+                             const void* v_pages, const int32_t* table, const int32_t* lengths, const int32_t* starts, void* workspace, float* out) {
+    const Call c{"attend_pages_window", q, k_pages, v_pages, table, lengths, starts, nullptr, nullptr, workspace, out};
+    return attend<kWindow>(p, c, [=](PagesArgs& a) -> const char* {
+        // (whole blocks of many rows, Block::kKeys)
+        a.window = vkml::pages::window_of(*p, window, sinks, 16384 / (p->head_dim * (p->kv_type == VKML_F16 ? 2 : 4)));
+        return check_window(*p, window);
+    });
 }
 
 }  // extern "C"

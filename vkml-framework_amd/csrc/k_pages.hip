@@ -1,7 +1,7 @@
-// k_pages.hip -- rotary positions into a paged KV cache, and copies of its
-// pages (vkml_rope_kv_pages, vkml_copy_pages). Both move bytes and compute
-// next to nothing: what bounds them is memory, and a launch's latency where
-// there are few.
+// k_pages.hip -- rotary positions into a paged KV cache, copies of its pages,
+// and the drafted tokens that stay in it (vkml_rope_kv_pages, vkml_copy_pages,
+// vkml_keep_drafts). All move bytes and compute next to nothing: what bounds them
+// is memory, and a launch's latency where there are few.
 #include <hip/hip_runtime.h>
 
 #include <new>
@@ -174,6 +174,106 @@ __global__ void __launch_bounds__(kThreads) k_copy_pages(CopyArgs a) {
         if (first + i * kThreads < a.vectors) stg(dst + first + i * kThreads, v[i]);
 }
 
+// ---------------------------------------------------------------- drafts that stay
+
+struct KeepArgs {
+    const int32_t* parents;  // [tokens]
+    const int32_t* drafted;
+    const int32_t* picked;
+    const int32_t* table;
+    int32_t* path;    // [tokens]
+    int32_t* counts;  // [seqs]
+    int32_t* next;
+    uint8_t* pool[2];
+    Batch batch;
+    uint64_t page_bytes, layer_bytes;  // from one to the next
+    uint32_t row_bytes;                // a key's of one head
+    uint32_t kv_heads, page_shift, pages, table_stride;
+};
+constexpr uint32_t kKeepVectors = 4;  // a thread has in flight
+
+// Workgroup (sequence, layer, pool). Wave 0 walks the tree: the first node after the
+// one it is at, of that parent, whose drafted token is the parent's pick, 64 nodes
+// looked at at once. (Every workgroup for itself: a walk of 6 of 13 nodes is some
+// 0.3 us, a launch of its own were 2.) Then the rows of the path move to the places
+// after one another that it takes. They are read and written by turns, 16 KB at
+// most, since a row may go to where another one comes from: never to where one of
+// a later turn does, as a path's k-th node is the k-th of the tree or a later one.
+template <typename V>
+__global__ void __launch_bounds__(kThreads) k_keep_drafts(KeepArgs a) {
+    __shared__ int32_t s_parent[vkml::pages::kMaxNodes], s_path[vkml::pages::kMaxNodes];
+    __shared__ int32_t s_count;
+    const int32_t s = static_cast<int32_t>(blockIdx.x), token0 = a.batch.start(s), n = min(a.batch.count(s), static_cast<int32_t>(vkml::pages::kMaxNodes));
+    const int32_t base = a.batch.length(s) - a.batch.count(s);
+    // The parent of each node that its parent's pick is the token of; of the others none.
+    for (int32_t i = static_cast<int32_t>(threadIdx.x); i < n; i += kThreads) {
+        const int32_t parent = ldg(a.parents + token0 + i);
+        s_parent[i] = parent >= 0 && parent < i && ldg(a.picked + token0 + parent) == ldg(a.drafted + token0 + i) ? parent : -1;
+    }
+    __syncthreads();
+    if (threadIdx.x < kWave) {
+        const int32_t l = static_cast<int32_t>(threadIdx.x);
+        int32_t at = 0, count = n > 0 ? 1 : 0;
+        if (l == 0 && n > 0) s_path[0] = 0;
+        for (int32_t i = 0; i < n;) {
+            const uint64_t found = __ballot(i + l > at && i + l < n && s_parent[min(i + l, n - 1)] == at);
+            if (found == 0) {
+                i += kWave;
+                continue;
+            }
+            at = i + static_cast<int32_t>(__builtin_ctzll(found));
+            i = at / kWave * kWave;
+            if (l == 0) s_path[count] = at;
+            ++count;
+        }
+        if (l == 0) s_count = count;
+    }
+    __syncthreads();
+    const int32_t count = s_count;
+    if (blockIdx.y == 0 && blockIdx.z == 0) {
+        const int32_t all = a.batch.count(s);
+        for (int32_t i = static_cast<int32_t>(threadIdx.x); i < all; i += kThreads) stg(a.path + token0 + i, i < count ? s_path[i] : -1);
+        if (threadIdx.x == 0) {
+            stg(a.counts + s, count);
+            stg(a.next + s, count > 0 ? ldg(a.picked + token0 + s_path[count - 1]) : -1);
+        }
+    }
+    uint8_t* pool = a.pool[blockIdx.z] + blockIdx.y * a.layer_bytes;
+    const int32_t* table = a.table + static_cast<uint64_t>(s) * a.table_stride;
+    const uint32_t pieces = a.row_bytes / sizeof(V), per_node = a.kv_heads * pieces;
+    const uint32_t head_bytes = a.row_bytes << a.page_shift;
+    const uint64_t units = static_cast<uint64_t>(count) * per_node;
+    const auto place = [&](int32_t pos, uint32_t unit) -> uint8_t* {  // null: in no page
+        if (pos < 0 || pos >= a.batch.table_keys) return nullptr;
+        const uint32_t page = static_cast<uint32_t>(ldg(table + (pos >> a.page_shift)));
+        if (page >= a.pages) return nullptr;
+        const uint32_t head = unit / pieces, row = static_cast<uint32_t>(pos) & ((1u << a.page_shift) - 1);
+        return pool + page * a.page_bytes + static_cast<uint64_t>(head) * head_bytes + row * a.row_bytes + unit % pieces * sizeof(V);
+    };
+    for (uint64_t first = per_node; first < units; first += kKeepVectors * kThreads) {  // (node 0 stays)
+        V v[kKeepVectors];
+        uint8_t* to[kKeepVectors];
+#pragma unroll
+        for (uint32_t i = 0; i < kKeepVectors; ++i) {
+            const uint64_t u = first + i * kThreads + threadIdx.x;
+            to[i] = nullptr;
+            if (u >= units) continue;
+            const int32_t j = static_cast<int32_t>(u / per_node), node = s_path[j];
+            const uint32_t unit = static_cast<uint32_t>(u % per_node);
+            const uint8_t* from = node == j ? nullptr : place(base + node, unit);
+            if (!from) continue;
+            to[i] = place(base + j, unit);
+            v[i] = ldg(reinterpret_cast<const V*>(from));
+        }
+        // Every load of the turn has landed before the first store.
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kKeepVectors; ++i)
+            if (to[i]) stg(reinterpret_cast<V*>(to[i]), v[i]);
+    }
+}
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
@@ -203,6 +303,43 @@ int vkml_rope_kv_pages(const vkml_rope_kv_pages_params* p, const float* qkv, con
     if (p->kv_type == VKML_F16) wide ? go(k_rope_kv_pages<4, _Float16>) : go(k_rope_kv_pages<1, _Float16>);
     else wide ? go(k_rope_kv_pages<4, float>) : go(k_rope_kv_pages<1, float>);
     return vkml::abi::check_launch("rope_kv_pages");
+}
+
+int vkml_keep_drafts(const vkml_keep_drafts_params* p, const int32_t* parents, const int32_t* drafted, const int32_t* picked, const int32_t* table,
+                     const int32_t* lengths, const int32_t* starts, int32_t* path, int32_t* counts, int32_t* next, void* k_pages, void* v_pages) {
+    VKML_REQUIRE_INIT();
+    VKML_CHECK_ARG(p, "keep_drafts: null params");
+    if (const char* why = vkml::pages::check(*p)) return vkml::abi::fail(VKML_ERROR_INVALID_ARGUMENT, std::string("keep_drafts: ") + why);
+    if (p->seqs == 0) return VKML_OK;
+    VKML_CHECK_ARG(starts || p->tokens == p->seqs, "keep_drafts: without starts every sequence has one token");
+    VKML_CHECK_ARG(table && lengths && counts && next && k_pages && v_pages && (p->tokens == 0 || (parents && drafted && picked && path)), "keep_drafts: null buffer");
+    const uint32_t size = p->kv_type == VKML_F16 ? 2 : 4;
+    const uint64_t page = p->page_stride ? p->page_stride : static_cast<uint64_t>(p->kv_heads) * p->page_size * p->head_dim;
+    KeepArgs a{};
+    a.parents = parents;
+    a.drafted = drafted;
+    a.picked = picked;
+    a.table = table;
+    a.path = path;
+    a.counts = counts;
+    a.next = next;
+    a.pool[0] = static_cast<uint8_t*>(k_pages);
+    a.pool[1] = static_cast<uint8_t*>(v_pages);
+    a.batch = Batch{lengths, starts, nullptr, nullptr, static_cast<int32_t>(p->seqs), static_cast<int32_t>(p->tokens), 0,
+                    static_cast<int32_t>(p->table_stride * p->page_size)};
+    a.page_bytes = page * size;
+    a.layer_bytes = (p->layer_stride ? p->layer_stride : p->pages * page) * size;
+    a.row_bytes = p->head_dim * size;
+    a.kv_heads = p->kv_heads;
+    a.page_shift = static_cast<uint32_t>(__builtin_ctz(p->page_size));
+    a.pages = p->pages;
+    a.table_stride = p->table_stride;
+    // (strides are multiples of 8 elements, so that rows start on 16 bytes as the pools and a row's bytes do)
+    const bool wide = a.row_bytes % 16 == 0 && a.page_bytes % 16 == 0 && a.layer_bytes % 16 == 0 && aligned16(k_pages) && aligned16(v_pages);
+    vkml::abi::ProfileScope prof("keep_drafts");
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(p->seqs, p->layers, 2), dim3(kThreads), 0, vkml::abi::stream(), a); };
+    wide ? go(k_keep_drafts<uint4>) : go(k_keep_drafts<uint32_t>);
+    return vkml::abi::check_launch("keep_drafts");
 }
 
 int vkml_copy_pages(const vkml_copy_pages_params* p, const int32_t* src, const int32_t* dst, void* k_pages, void* v_pages) {

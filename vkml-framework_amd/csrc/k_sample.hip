@@ -1,0 +1,605 @@
+// k_sample.hip -- a token for each row of logits (vkml_sample): vkml::Sampler's
+// definition (src/sampling.cpp) for the device, from given random numbers.
+//
+// Candidates are ranked by logit, then id. With peak the row's largest logit a
+// candidate weighs e^((l - peak) / T); top_k, top_p and min_p each keep a first part
+// of the ranking, so that only the kept mass M has to be known, and the pick is the
+// first candidate whose weight and those before it pass random * M. Nothing is
+// sorted: a candidate is found by its count or mass before it, in a histogram of the
+// logits, then among its bin's candidates.
+//
+// Weights are whole numbers, units of 2^-shift of the largest (45 bits for 2^17
+// logits, so that all of a row's fit 62 bits): sums of them are exact in any order,
+// so that the same row gives the same token whatever the atomics' order. e^x is
+// found in 64 bits, 2^(-n / 64) from a table times a polynomial of degree 5, good to
+// 2^-50: the picks are those of sums in f64 unless a border is nearer than that.
+#include <hip/hip_runtime.h>
+
+#include <string>
+
+#include "device.hpp"
+#include "internal.hpp"
+#include "sample.hpp"
+
+using namespace vkml::dev;
+using namespace vkml::sample;
+
+namespace {
+
+constexpr uint32_t kWaves = kThreads / kWave;
+constexpr uint32_t kList = 2048;  // candidates in the LDS
+constexpr uint32_t kSubs = 1024;  // parts of a range of candidates
+constexpr uint32_t kFew = 128;    // candidates that are counted one by one
+constexpr uint64_t kNone = ~0ull;
+
+struct Args {
+    const float* logits;
+    const vkml_sampling* options;
+    const double* random;
+    int32_t* tokens;
+    uint64_t* peaks;   // [rows, slices]: the places of the slices' largest
+    SliceSums* sums;   // [rows, slices]
+    uint64_t row_stride;
+    uint32_t vocab, slices;
+    int32_t shift;
+};
+
+// A candidate's place in the ranking: its logit's bits as a number that falls as the
+// logit rises (zeros alike), then its id.
+__device__ __forceinline__ uint32_t falling(float l) {
+    const uint32_t u = __float_as_uint(l + 0.0f);
+    return u & 0x80000000u ? u : ~u & 0x7FFFFFFFu;
+}
+__device__ __forceinline__ uint64_t place_of(float l, uint32_t id) { return static_cast<uint64_t>(falling(l)) << 32 | id; }
+__device__ __forceinline__ float logit_at(uint64_t place) {
+    const uint32_t u = static_cast<uint32_t>(place >> 32);
+    return __uint_as_float(u & 0x80000000u ? u : ~u & 0x7FFFFFFFu);
+}
+
+struct Row {
+    float peak;
+    double turns;      // 64 log2(e) / T
+    float bins_per;    // bins a unit of l
+    double least;      // weights below it are not within min_p
+    int32_t shift;
+};
+
+struct Scratch {
+    uint64_t mass[kBins];  // of a bin, then of it and those before
+    uint32_t count[kBins];
+    uint64_t place[kList], weight[kList];
+    uint64_t sub_mass[kSubs];
+    uint32_t sub_count[kSubs];
+    uint64_t wave_mass[kWaves], wave_place[kWaves];
+    uint32_t wave_count[kWaves];
+    uint64_t few_place[kFew], few_weight[kFew];
+    double table[64];
+    uint64_t lo, hi, likely;  // a range of places; the mass within min_p
+    uint64_t found_mass, found_before;
+    uint32_t found, found_count, listed;
+};
+
+// ---------------------------------------------------------------- weights
+
+__device__ __forceinline__ void fill_table(Scratch& lds) {
+    if (threadIdx.x < 64) lds.table[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 64.0);
+}
+
+__device__ __forceinline__ Row row_of(float peak, const vkml_sampling& o, int32_t shift) {
+    Row r;
+    r.peak = peak;
+    r.turns = 64.0 * 1.4426950408889634 / static_cast<double>(o.temperature);
+    // beyond T ln2 (shift + 1) a weight rounds to 0
+    const float span = o.temperature * 0.6931472f * static_cast<float>(shift + 2);
+    r.bins_per = fminf(static_cast<float>(kBins) / span, 1e30f);
+    r.least = (o.min_p > 0.0f ? static_cast<double>(o.min_p) : 0.0) * __builtin_ldexp(1.0, shift);
+    r.shift = shift;
+    return r;
+}
+
+// NaN and -infinity weigh nothing; beside +infinity, nothing else does.
+__device__ __forceinline__ uint64_t weight_of(const Row& r, float l, const double* table) {
+    const double d = l == r.peak ? 0.0 : static_cast<double>(r.peak) - static_cast<double>(l);
+    const double z = d * r.turns;
+    const bool some = l > -__builtin_inff() && z < 64.0 * (r.shift + 2);
+    const double zz = some ? z : 0.0, n = __builtin_rint(zz);
+    const double f = (zz - n) * (-0.6931471805599453 / 64.0);
+    double p = __builtin_fma(f, 1.0 / 120.0, 1.0 / 24.0);
+    p = __builtin_fma(p, f, 1.0 / 6.0);
+    p = __builtin_fma(p, f, 0.5);
+    p = __builtin_fma(p, f, 1.0);
+    p = __builtin_fma(p, f, 1.0);
+    const int32_t i = static_cast<int32_t>(n);
+    const double w = __builtin_amdgcn_ldexp(table[i & 63] * p, r.shift - (i >> 6));
+    // rounded to a whole number in the sum's low bits
+    const uint64_t whole = __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    return some ? whole : 0;
+}
+
+__device__ __forceinline__ uint32_t bin_of(const Row& r, float l) {
+    const float d = l == r.peak ? 0.0f : r.peak - l;
+    return static_cast<uint32_t>(fminf(d * r.bins_per, static_cast<float>(kBins - 1)));
+}
+
+// ---------------------------------------------------------------- a row's values
+
+// The row's vectors of four values, the first of which holds its first one (or, off
+// values before, nothing); what is not the row's reads as NaN.
+struct Source {
+    const float* row;
+    uint32_t vocab, off;
+    __device__ __forceinline__ uint32_t vectors() const { return (vocab + off + 3) / 4; }
+    __device__ __forceinline__ float4 load(uint32_t v) const {
+        const int32_t at = static_cast<int32_t>(4 * v) - static_cast<int32_t>(off);
+        if (at >= 0 && at + 4 <= static_cast<int32_t>(vocab)) return ldg(reinterpret_cast<const float4*>(row + at));
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = at + e >= 0 && at + e < static_cast<int32_t>(vocab) ? ldg(row + (at + e)) : __builtin_nanf("");
+        return make_float4(x[0], x[1], x[2], x[3]);
+    }
+};
+__device__ __forceinline__ Source source_of(const Args& a, uint32_t row) {
+    const float* p = a.logits + row * a.row_stride;
+    return {p, a.vocab, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) / 4 % 4)};
+}
+
+// A slice of them in the workgroup's registers.
+struct Held {
+    float4 x[kVectors];
+    uint32_t id0;  // of the thread's first value (it may wrap below 0, where that is none of the row's)
+    __device__ __forceinline__ void load(const Source& s, uint32_t slice) {
+        const uint32_t v0 = slice * kVectors * kThreads + threadIdx.x;
+        id0 = 4 * v0 - s.off;
+#pragma unroll
+        for (uint32_t i = 0; i < kVectors; ++i) x[i] = s.load(v0 + i * kThreads);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(const F& f) const {
+#pragma unroll
+        for (uint32_t i = 0; i < kVectors; ++i) {
+            const uint32_t id = id0 + 4 * i * kThreads;
+            f(x[i].x, id);
+            f(x[i].y, id + 1);
+            f(x[i].z, id + 2);
+            f(x[i].w, id + 3);
+        }
+    }
+};
+
+// All of them, read again each time.
+struct Streamed {
+    Source s;
+    template <typename F>
+    __device__ __forceinline__ void each(const F& f) const {
+        constexpr uint32_t kFlight = 2;
+        const uint32_t n = s.vectors();
+        for (uint32_t v = threadIdx.x; v < n; v += kFlight * kThreads) {
+            float4 x[kFlight];
+#pragma unroll
+            for (uint32_t i = 0; i < kFlight; ++i) x[i] = s.load(v + i * kThreads);
+#pragma unroll
+            for (uint32_t i = 0; i < kFlight; ++i) {
+                const uint32_t id = 4 * (v + i * kThreads) - s.off;
+                f(x[i].x, id);
+                f(x[i].y, id + 1);
+                f(x[i].z, id + 2);
+                f(x[i].w, id + 3);
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------- the workgroup together
+
+__device__ __forceinline__ uint64_t exchanged(uint64_t v, int o) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__shfl_xor(static_cast<int>(v >> 32), o))) << 32 | static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o));
+}
+__device__ __forceinline__ uint64_t wave_min(uint64_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint64_t w = exchanged(v, o);
+        v = w < v ? w : v;
+    }
+    return v;
+}
+
+// The place of the largest of the values, kNone where there is none.
+template <typename V>
+__device__ __forceinline__ uint64_t first_of(const V& values, Scratch& lds) {
+    float best = -__builtin_inff();
+    uint32_t id = 0;
+    values.each([&](float l, uint32_t i) {
+        if (l > best) best = l, id = i;  // (ids rise: the first of equal ones)
+    });
+    const uint64_t mine = wave_min(best > -__builtin_inff() ? place_of(best, id) : kNone);
+    if (threadIdx.x % kWave == 0) lds.wave_place[threadIdx.x / kWave] = mine;
+    __syncthreads();
+    uint64_t all = kNone;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaves; ++i) all = lds.wave_place[i] < all ? lds.wave_place[i] : all;
+    return all;
+}
+
+__device__ __forceinline__ void add(uint64_t* to, uint64_t v) { __hip_atomic_fetch_add(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+__device__ __forceinline__ void add(uint32_t* to, uint32_t v) { __hip_atomic_fetch_add(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+
+// Clears the bins; with a barrier after it.
+__device__ __forceinline__ void clear_bins(Scratch& lds) {
+    for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) lds.mass[i] = 0, lds.count[i] = 0;
+    if (threadIdx.x == 0) lds.likely = 0;
+    __syncthreads();
+}
+// The values' weights to the bins. A barrier has to follow.
+template <typename V>
+__device__ __forceinline__ void fill_bins(const V& values, const Row& r, Scratch& lds) {
+    uint64_t likely = 0;
+    values.each([&](float l, uint32_t) {
+        const uint64_t w = weight_of(r, l, lds.table);
+        if (w == 0) return;
+        const uint32_t b = bin_of(r, l);
+        add(&lds.mass[b], w);
+        add(&lds.count[b], 1u);
+        if (static_cast<double>(w) >= r.least) likely += w;
+    });
+    if (r.least > 0.0 && likely) add(&lds.likely, likely);
+}
+
+// mass and count of n parts (two a thread, or one) become those of the part and all
+// before it.
+template <uint32_t N>
+__device__ __forceinline__ void sum_up(uint64_t* mass, uint32_t* count, Scratch& lds) {
+    constexpr uint32_t kEach = N / kThreads;
+    const uint32_t t = threadIdx.x, l = t % kWave, w = t / kWave;
+    uint64_t m[kEach], ms = 0;
+    uint32_t c[kEach], cs = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) {
+        ms = m[i] = ms + mass[kEach * t + i];
+        cs = c[i] = cs + count[kEach * t + i];
+    }
+    uint64_t mi = ms;
+    uint32_t ci = cs;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const uint64_t mo = static_cast<uint64_t>(static_cast<uint32_t>(__shfl_up(static_cast<int>(mi >> 32), o))) << 32 | static_cast<uint32_t>(__shfl_up(static_cast<int>(mi), o));
+        const uint32_t co = static_cast<uint32_t>(__shfl_up(static_cast<int>(ci), o));
+        if (l >= static_cast<uint32_t>(o)) mi += mo, ci += co;
+    }
+    if (l == kWave - 1) lds.wave_mass[w] = mi, lds.wave_count[w] = ci;
+    __syncthreads();
+    uint64_t m0 = mi - ms;
+    uint32_t c0 = ci - cs;
+#pragma unroll
+    for (uint32_t i = 0; i < kWaves; ++i)
+        if (i < w) m0 += lds.wave_mass[i], c0 += lds.wave_count[i];
+#pragma unroll
+    for (uint32_t i = 0; i < kEach; ++i) mass[kEach * t + i] = m0 + m[i], count[kEach * t + i] = c0 + c[i];
+    __syncthreads();
+}
+
+// What is searched for: the candidate that `before` others come before, or that
+// holds unit `before` of the mass.
+struct Wanted {
+    bool by_count;
+    uint64_t before;
+};
+
+// The part of n (summed up) that holds it: its number, and what comes before it.
+struct Part {
+    uint32_t i, count;       // count: in the part
+    uint64_t mass_before;
+    uint32_t count_before;
+};
+template <uint32_t N>
+__device__ __forceinline__ Part part_with(const uint64_t* mass, const uint32_t* count, Wanted x, Scratch& lds) {
+#pragma unroll
+    for (uint32_t i = threadIdx.x; i < N; i += kThreads) {
+        const uint64_t m0 = i ? mass[i - 1] : 0;
+        const uint32_t c0 = i ? count[i - 1] : 0;
+        const bool here = x.by_count ? c0 <= x.before && x.before < count[i] : m0 <= x.before && x.before < mass[i];
+        if (here) lds.found = i, lds.found_count = count[i] - c0, lds.found_mass = m0, lds.found_before = c0;
+    }
+    __syncthreads();
+    const Part p{lds.found, lds.found_count, lds.found_mass, static_cast<uint32_t>(lds.found_before)};
+    __syncthreads();
+    return p;
+}
+
+// What was found: its mass and all before it, and its id.
+struct Found {
+    uint64_t mass;
+    uint32_t id;
+};
+
+// Which bins' candidates the list in the LDS holds all of.
+struct Listed {
+    uint32_t first = 1, last = 0, n = 0;
+};
+
+// The candidate with x before it, of those in bin b whose places are in lds.lo ..
+// lds.hi, n of them in all (visit(f): f(place, weight) for each that may be).
+template <typename Visit>
+__device__ __forceinline__ Found among(const Visit& visit, Wanted x, uint64_t lo, uint64_t hi, uint32_t n, uint64_t mass, Scratch& lds) {
+    // Ranges of a thousandth of the last, until few are in one. (Places are all
+    // different: the seventh at the latest is a place.)
+    for (int level = 0; n > kFew && level < 7; ++level) {
+        const int bits = 64 - __builtin_clzll(hi - lo | 1);
+        const int step = bits > 10 ? bits - 10 : 0;
+        lds.sub_mass[threadIdx.x] = 0;
+        lds.sub_count[threadIdx.x] = 0;
+        __syncthreads();
+        visit([&](uint64_t at, uint64_t w) {
+            if (at < lo || at > hi) return;
+            const uint32_t i = static_cast<uint32_t>((at - lo) >> step);
+            add(&lds.sub_mass[i], w);
+            add(&lds.sub_count[i], 1u);
+        });
+        __syncthreads();
+        sum_up<kSubs>(lds.sub_mass, lds.sub_count, lds);
+        const Part p = part_with<kSubs>(lds.sub_mass, lds.sub_count, x, lds);
+        mass += p.mass_before;
+        x.before -= x.by_count ? p.count_before : p.mass_before;
+        n = p.count;
+        lo += static_cast<uint64_t>(p.i) << step;
+        const uint64_t end = lo + ((1ull << step) - 1);
+        hi = end < hi ? end : hi;
+    }
+    if (threadIdx.x == 0) lds.listed = 0;
+    __syncthreads();
+    visit([&](uint64_t at, uint64_t w) {
+        if (at < lo || at > hi) return;
+        const uint32_t i = __hip_atomic_fetch_add(&lds.listed, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (i < kFew) lds.few_place[i] = at, lds.few_weight[i] = w;
+    });
+    __syncthreads();
+    // Eight threads a candidate count those before it.
+    const uint32_t j = threadIdx.x / 8;
+    n = min(n, kFew);
+    if (j < n) {
+        const uint64_t at = lds.few_place[j];
+        uint64_t m = 0, c = 0;
+        for (uint32_t i = threadIdx.x % 8; i < n; i += 8)
+            if (lds.few_place[i] < at) m += lds.few_weight[i], ++c;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) m += exchanged(m, o), c += exchanged(c, o);
+        const uint64_t w = lds.few_weight[j];
+        const bool here = x.by_count ? c == x.before : m <= x.before && x.before < m + w;
+        if (here && threadIdx.x % 8 == 0) lds.found_mass = mass + m + w, lds.found = static_cast<uint32_t>(at);
+    }
+    __syncthreads();
+    const Found f{lds.found_mass, lds.found};
+    __syncthreads();
+    return f;
+}
+
+// The candidate with x before it, in the bins' sums and the row's values.
+__device__ __forceinline__ Found find(const Streamed& values, const Row& r, Wanted x, Listed& listed, Scratch& lds) {
+    const Part p = part_with<kBins>(lds.mass, lds.count, x, lds);
+    x.before -= x.by_count ? p.count_before : p.mass_before;
+    const uint32_t b = p.i;
+    if (p.count <= kList && !(listed.first <= b && b <= listed.last)) {
+        // The bin's candidates to the list, and all before them if they fit too.
+        const bool all = p.count_before + p.count <= kList;
+        listed = {all ? 0 : b, b, all ? p.count_before + p.count : p.count};
+        if (threadIdx.x == 0) lds.listed = 0;
+        __syncthreads();
+        values.each([&](float l, uint32_t id) {
+            if (!(l > -__builtin_inff())) return;
+            const uint32_t i = bin_of(r, l);
+            if (i < listed.first || i > listed.last) return;
+            const uint64_t w = weight_of(r, l, lds.table);
+            if (w == 0) return;
+            const uint32_t to = __hip_atomic_fetch_add(&lds.listed, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (to < kList) lds.place[to] = place_of(l, id), lds.weight[to] = w;
+        });
+        __syncthreads();
+    }
+    const bool from_list = listed.first <= b && b <= listed.last;
+    const auto visit = [&](const auto& f) {
+        if (from_list) {
+            for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads)
+                if (bin_of(r, logit_at(lds.place[i])) == b) f(lds.place[i], lds.weight[i]);
+        } else {
+            values.each([&](float l, uint32_t id) {
+                if (!(l > -__builtin_inff()) || bin_of(r, l) != b) return;
+                const uint64_t w = weight_of(r, l, lds.table);
+                if (w) f(place_of(l, id), w);
+            });
+        }
+    };
+    if (threadIdx.x == 0) lds.lo = kNone, lds.hi = 0;
+    __syncthreads();
+    uint64_t lo = kNone, hi = 0;
+    if (p.count > kFew) {  // how far apart the bin's are
+        visit([&](uint64_t at, uint64_t) {
+            lo = at < lo ? at : lo;
+            hi = at > hi ? at : hi;
+        });
+        lo = wave_min(lo);
+        hi = ~wave_min(~hi);
+        if (threadIdx.x % kWave == 0) {
+            __hip_atomic_fetch_min(&lds.lo, lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            __hip_atomic_fetch_max(&lds.hi, hi, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+        __syncthreads();
+        lo = lds.lo;
+        hi = lds.hi;
+    } else {
+        lo = 0;
+        hi = kNone;
+    }
+    return among(visit, x, lo, hi, p.count, p.mass_before, lds);
+}
+
+// The pick of a row whose bins are summed up.
+__device__ __forceinline__ uint32_t pick(const Streamed& values, const Row& r, const vkml_sampling& o, double random, Scratch& lds) {
+    Listed listed;
+    uint64_t mass = lds.mass[kBins - 1];
+    const uint32_t count = lds.count[kBins - 1];
+    // top_k, top_p, the draw: each looks for a candidate by what the one before leaves
+#pragma unroll 1
+    for (int step = 0;; ++step) {
+        Wanted x{false, 0};
+        if (step == 0) {
+            if (o.top_k <= 0 || static_cast<uint32_t>(o.top_k) >= count) continue;
+            x = {true, static_cast<uint64_t>(o.top_k - 1)};
+        } else if (step == 1) {
+            if (!(o.top_p < 1.0f)) continue;
+            // the fewest whose mass reaches top_p of it: up to the one that holds the last unit of that
+            const double share = __builtin_ceil(static_cast<double>(fmaxf(o.top_p, 0.0f)) * static_cast<double>(mass));
+            const uint64_t least = static_cast<uint64_t>(share);
+            x.before = (least < 1 ? 1 : least < mass ? least : mass) - 1;
+        } else {
+            if (r.least > 0.0) {
+                const uint64_t likely = lds.likely < (1ull << r.shift) ? 1ull << r.shift : lds.likely;  // the first at least
+                mass = likely < mass ? likely : mass;
+            }
+            const double at = random * static_cast<double>(mass);
+            const uint64_t unit = at > 0.0 ? (at < 9.2e18 ? static_cast<uint64_t>(at) : mass) : 0;
+            x.before = unit < mass ? unit : mass - 1;
+        }
+        const Found f = find(values, r, x, listed, lds);
+        if (step == 2) return f.id;
+        mass = f.mass;
+    }
+}
+
+__device__ __forceinline__ bool greedy(const vkml_sampling& o) { return !(o.temperature > 0.0f) || o.top_k == 1; }
+__device__ __forceinline__ vkml_sampling options_of(const Args& a, uint32_t row) {
+    const uint4 x = ldg(reinterpret_cast<const uint4*>(a.options + row));
+    return {__uint_as_float(x.x), static_cast<int32_t>(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
+}
+
+// ---------------------------------------------------------------- the launches
+
+// Rows of one slice: a workgroup a row, its values in registers until they are in
+// their bins. (The candidates that are looked for are few, and read again.)
+__global__ void __launch_bounds__(kThreads) k_sample(Args a) {
+    __shared__ Scratch lds;
+    const uint32_t row = blockIdx.x;
+    const vkml_sampling o = options_of(a, row);
+    Held values;
+    values.load(source_of(a, row), 0);
+    fill_table(lds);
+    clear_bins(lds);
+    const uint64_t first = first_of(values, lds);
+    if (first == kNone || greedy(o)) {
+        if (threadIdx.x == 0) stg(a.tokens + row, first == kNone ? -1 : static_cast<int32_t>(first));
+        return;
+    }
+    const Row r = row_of(logit_at(first), o, a.shift);
+    fill_bins(values, r, lds);
+    __syncthreads();
+    sum_up<kBins>(lds.mass, lds.count, lds);
+    const uint32_t id = pick({source_of(a, row)}, r, o, a.random[row], lds);
+    if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
+}
+
+// Longer rows: their slices' largest, then their slices' bins, then the picks.
+__global__ void __launch_bounds__(kThreads) k_sample_peaks(Args a) {
+    __shared__ Scratch lds;
+    Held values;
+    values.load(source_of(a, blockIdx.x / a.slices), blockIdx.x % a.slices);
+    const uint64_t first = first_of(values, lds);
+    if (threadIdx.x == 0) stg(a.peaks + blockIdx.x, first);
+}
+
+__device__ __forceinline__ uint64_t peak_of(const Args& a, uint32_t row) {
+    uint64_t first = kNone;
+    for (uint32_t i = 0; i < a.slices; ++i) {
+        const uint64_t p = ldg(a.peaks + static_cast<uint64_t>(row) * a.slices + i);
+        first = p < first ? p : first;
+    }
+    return first;
+}
+
+__global__ void __launch_bounds__(kThreads) k_sample_sums(Args a) {
+    __shared__ Scratch lds;
+    const uint32_t row = blockIdx.x / a.slices;
+    const vkml_sampling o = options_of(a, row);
+    const uint64_t first = peak_of(a, row);
+    if (first == kNone || greedy(o)) return;
+    Held values;
+    values.load(source_of(a, row), blockIdx.x % a.slices);
+    fill_table(lds);
+    clear_bins(lds);
+    fill_bins(values, row_of(logit_at(first), o, a.shift), lds);
+    __syncthreads();
+    SliceSums* to = a.sums + blockIdx.x;
+    for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
+    if (threadIdx.x == 0) stg(&to->likely, lds.likely);
+}
+
+__global__ void __launch_bounds__(kThreads) k_sample_pick(Args a) {
+    __shared__ Scratch lds;
+    const uint32_t row = blockIdx.x;
+    const vkml_sampling o = options_of(a, row);
+    const uint64_t first = peak_of(a, row);
+    if (first == kNone || greedy(o)) {
+        if (threadIdx.x == 0) stg(a.tokens + row, first == kNone ? -1 : static_cast<int32_t>(first));
+        return;
+    }
+    fill_table(lds);
+    const SliceSums* from = a.sums + static_cast<uint64_t>(row) * a.slices;
+    for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
+        uint64_t m = 0;
+        uint32_t c = 0;
+        for (uint32_t s = 0; s < a.slices; ++s) m += ldg(from[s].mass + i), c += ldg(from[s].count + i);
+        lds.mass[i] = m, lds.count[i] = c;
+    }
+    if (threadIdx.x == 0) {
+        uint64_t likely = 0;
+        for (uint32_t s = 0; s < a.slices; ++s) likely += ldg(&from[s].likely);
+        lds.likely = likely;
+    }
+    __syncthreads();
+    sum_up<kBins>(lds.mass, lds.count, lds);
+    const Row r = row_of(logit_at(first), o, a.shift);
+    const uint32_t id = pick({source_of(a, row)}, r, o, a.random[row], lds);
+    if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
+}
+
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+}  // namespace
+
+extern "C" {
+
+uint64_t vkml_sample_workspace_bytes(const vkml_sample_params* p) { return !p || check(*p) ? 0 : workspace_bytes(*p); }
+
+int vkml_sample(const vkml_sample_params* p, const float* logits, const vkml_sampling* options, const double* random, void* workspace, int32_t* tokens) {
+    VKML_REQUIRE_INIT();
+    VKML_CHECK_ARG(p, "sample: null params");
+    if (const char* why = check(*p)) return vkml::abi::fail(VKML_ERROR_INVALID_ARGUMENT, std::string("sample: ") + why);
+    if (p->rows == 0) return VKML_OK;
+    VKML_CHECK_ARG(logits && options && random && tokens && (workspace || workspace_bytes(*p) == 0), "sample: null buffer");
+    VKML_CHECK_ARG(aligned(logits, 4) && aligned(options, 16) && aligned(random, 8) && aligned(tokens, 4) && aligned(workspace, 16),
+                   "sample: options and the workspace must be 16-byte aligned, the other buffers as their types are");
+    Args a{};
+    a.logits = logits;
+    a.options = options;
+    a.random = random;
+    a.tokens = tokens;
+    a.row_stride = p->row_stride;
+    a.vocab = p->vocab;
+    a.slices = slices(p->vocab);
+    if (a.slices > 1) {
+        a.peaks = static_cast<uint64_t*>(workspace);
+        a.sums = reinterpret_cast<SliceSums*>(static_cast<uint8_t*>(workspace) + peaks_bytes(*p));
+    }
+    // a row's weights fit 62 bits, one of them 51
+    int32_t bits = 0;
+    while ((1u << bits) < p->vocab) ++bits;
+    a.shift = 62 - bits < 51 ? 62 - bits : 51;
+    vkml::abi::ProfileScope prof("sample");
+    const auto go = [&](auto kernel, uint32_t workgroups) {
+        hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kThreads), 0, vkml::abi::stream(), a);
+        return vkml::abi::check_launch("sample");
+    };
+    if (a.slices == 1) return go(k_sample, p->rows);
+    if (const int r = go(k_sample_peaks, p->rows * a.slices)) return r;
+    if (const int r = go(k_sample_sums, p->rows * a.slices)) return r;
+    return go(k_sample_pick, p->rows);
+}
+
+}  // extern "C"

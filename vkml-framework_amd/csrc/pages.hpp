@@ -19,6 +19,8 @@ namespace vkml::pages {
 constexpr uint32_t kMaxGroup = 128;       // query heads a KV head
 constexpr uint32_t kMaxSeqs = 1u << 16;   // sequences a batch
 constexpr uint32_t kMaxTokens = 1u << 22;  // new tokens a batch
+constexpr uint32_t kMaxSeenWords = 128;    // words of a tree's row
+constexpr uint32_t kMaxNodes = 32 * kMaxSeenWords;  // nodes of a tree
 constexpr float kFinite = 3.402823466e+38f;
 
 VKML_HD int32_t clamp_to(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
@@ -99,11 +101,24 @@ VKML_HD Costs costs(uint32_t head_dim, bool f16) {
     return {few, f16 ? 3 * few : few + few * 3 / 4, f16 ? 2600 : 600, f16 ? 3600 : 600};
 }
 
+// A window over the keys: a token at position p sees those past p - keys, and the
+// first `sinks` of its sequence. keys 0: none.
+struct Window {
+    int32_t keys = 0, sinks = 0;
+    int32_t span = 0;  // the sinks filled up to whole blocks of keys
+};
+
 VKML_HD int32_t tile_tokens(int32_t group) { return kTileRows / group > 1 ? kTileRows / group : 1; }
 
 // The keys of a segment lie on one axis: first the `lead` keys that its tokens
 // read through the table row of their group's first sequence, filled up to a
 // multiple of kLeadStep, then those from position lo on, of its own row.
+//
+// With a window a tile's first token may be so far on that the keys that none of
+// its tokens see are worth leaving out: such a tile slides, and its lead are the
+// sinks, through the sequence's own row. Its axis is as long as any sliding tile's,
+// up to 15 keys and, in the last one, the tokens it lacks past its last key, so
+// that the costs before a tile stay a formula.
 struct Segment {
     int32_t row = 0;       // the sequence whose table holds the keys from lo on
     int32_t lead_row = 0;  // and the `lead` keys
@@ -115,12 +130,25 @@ struct Segment {
     int32_t tiles = 0, step = 1;
     bool few = false, shared = false;
     int32_t key_cost = 0, own_cost = 0;
+    Window window;
+    int32_t straight = 0;  // with a window: the tiles before the first that slides
+
+    // Called once the other members stand.
+    VKML_HD void set(Window w) {
+        window = w;
+        if (w.keys == 0) return;
+        const int32_t last = w.span + w.keys - 1 - base;  // a tile slides if its first token is further than this from the first one's
+        straight = base < 0 ? tiles : last < 0 ? 0 : last / step + 1 < tiles ? last / step + 1 : tiles;
+    }
+    VKML_HD bool slides(int32_t i) const { return window.keys > 0 && i >= straight; }
+    VKML_HD int32_t sliding_keys() const { return window.span + window.keys + step + 14; }
 
     // The first position read, a multiple of 16.
     VKML_HD int32_t lo() const { return from & ~15; }
     VKML_HD int32_t lead_span() const { return (lead + kLeadStep - 1) / kLeadStep * kLeadStep; }
     // The axis' length for tile i's tokens.
     VKML_HD int32_t keys(int32_t i) const {
+        if (slides(i)) return sliding_keys();
         int32_t own = base;
         if (!shared) {
             own += base < 0 || (i + 1) * step > n ? n : (i + 1) * step;
@@ -133,8 +161,13 @@ struct Segment {
     VKML_HD int64_t before(int32_t i) const {
         if (i == 0) return 0;
         const bool equal = shared || base < 0;
+        int64_t sliding = 0;
+        if (window.keys > 0 && i > straight) {
+            sliding = (i - straight) * (own_cost + static_cast<int64_t>(key_cost) * sliding_keys());
+            i = straight;
+        }
         const int64_t k = i, each = own_cost + static_cast<int64_t>(key_cost) * (equal ? keys(0) : lead_span() + base);
-        return equal ? k * each : k * each + key_cost * (step * (k * (k + 1) / 2));
+        return sliding + (equal ? k * each : k * each + key_cost * (step * (k * (k + 1) / 2)));
     }
     VKML_HD int64_t cost() const { return tiles ? before(tiles - 1) + tile_cost(tiles - 1) : 0; }
     // The tile that holds unit u of the segment, 0 <= u < cost().
@@ -150,6 +183,18 @@ struct Segment {
     // The position past the last that token i of the segment sees.
     VKML_HD int32_t limit(int32_t i) const { return shared ? base : lo() + base + i + 1; }
     VKML_HD int32_t tile_n(int32_t i) const { return n - i * step < step ? n - i * step : step; }
+    // Where tile i's keys are: the lead's part of the axis and its keys; of the
+    // others the first read, the first and past the last that count.
+    struct Where {
+        int32_t span, lead, lo, from, end;
+    };
+    VKML_HD Where where(int32_t i) const {
+        if (slides(i)) {
+            const int32_t first = base + i * step, seen = first - window.keys + 1;
+            return {window.span, window.sinks, seen & ~15, seen, first + tile_n(i)};
+        }
+        return {lead_span(), lead, lo(), from, lo() + keys(i) - lead_span()};
+    }
 };
 
 // Segment i of a batch: groups 0 .. groups - 1, then the sequences. (Loads that
@@ -159,7 +204,9 @@ struct Segment {
 // half a tile of tokens or more on average: then their own tiles read few
 // blocks more than the group's would, and no rows are in two parts. A group of
 // one sequence shares nothing.
-VKML_HD Segment segment(const Batch& b, int32_t group, Costs costs, int32_t i) {
+//
+// (A window comes without groups.)
+VKML_HD Segment segment(const Batch& b, int32_t group, Costs costs, int32_t i, Window window = {}) {
     const bool of_group = i < b.groups;
     const int32_t q = of_group ? 0 : i - b.groups;
     const int32_t own0 = b.start(q), own1 = b.start(q + 1), length = b.length(q);
@@ -198,6 +245,8 @@ VKML_HD Segment segment(const Batch& b, int32_t group, Costs costs, int32_t i) {
     s.tiles = s.few ? (s.n > 0 ? 1 : 0) : (s.n + s.step - 1) / s.step;
     s.key_cost = s.few ? costs.few_key : costs.tile_key;
     s.own_cost = s.few ? costs.few_own : costs.tile_own;
+    if (window.keys > 0) s.lead_row = s.row;
+    s.set(window);
     return s;
 }
 
@@ -307,6 +356,22 @@ inline const char* check(const vkml_attend_pages_params& p) {
     return nullptr;
 }
 
+inline const char* check_tree(uint32_t seen_words) {
+    return seen_words == 0 || seen_words > kMaxSeenWords ? "seen_words must be 1 to 128" : nullptr;
+}
+
+inline const char* check_window(const vkml_attend_pages_params& p, uint32_t window) {
+    if (window == 0) return "the window must hold 1 key or more";
+    if (p.groups) return "a window takes no groups";
+    return nullptr;
+}
+// The window as the kernel has it, of a table row's keys at most (one of all of them
+// hides none), its sinks filled up to whole blocks.
+inline Window window_of(const vkml_attend_pages_params& p, uint32_t window, uint32_t sinks, uint32_t block) {
+    const uint32_t most = p.table_stride * p.page_size, held = sinks < most ? sinks : most;
+    return {static_cast<int32_t>(window < most ? window : most), static_cast<int32_t>(held), static_cast<int32_t>((held + block - 1) / block * block)};
+}
+
 inline const char* check(const vkml_rope_kv_pages_params& p) {
     if (p.kv_heads == 0 || p.heads == 0 || p.head_dim == 0 || p.head_dim % 2 || p.head_dim > 1024 || p.heads > 4096 || p.kv_heads > 4096) return "bad head layout";
     if (const char* why = check_cache(p.kv_heads, p.head_dim, p.kv_type, p.page_size, p.pages, p.page_stride)) return why;
@@ -326,6 +391,18 @@ inline const char* check(const vkml_copy_pages_params& p) {
     if (stride > (1ull << 40)) return "page_stride is too large";
     if (p.layer_stride && p.layer_stride < (p.pages - 1) * stride + p.page_bytes) return "layers overlap";
     if (p.layers == 0 || p.layers > 65535) return "1 to 65535 layers";
+    return nullptr;
+}
+
+inline const char* check(const vkml_keep_drafts_params& p) {
+    if (p.kv_heads == 0 || p.head_dim == 0 || p.head_dim % 2 || p.head_dim > 1024 || p.kv_heads > 4096) return "bad head layout";
+    if (const char* why = check_cache(p.kv_heads, p.head_dim, p.kv_type, p.page_size, p.pages, p.page_stride)) return why;
+    if (const char* why = check_batch(p.seqs, p.tokens, p.table_stride, p.page_size)) return why;
+    if (p.layers == 0 || p.layers > 65535) return "1 to 65535 layers";
+    const uint64_t page = static_cast<uint64_t>(p.kv_heads) * p.page_size * p.head_dim, stride = p.page_stride ? p.page_stride : page;
+    if (p.layer_stride && p.layer_stride < (p.pages - 1) * stride + page) return "layers overlap";
+    if (p.layer_stride % 8) return "layer_stride must be a multiple of 8";
+    if (p.layer_stride > (1ull << 46)) return "layer_stride is too large";
     return nullptr;
 }
 

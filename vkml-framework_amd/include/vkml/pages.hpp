@@ -1,6 +1,7 @@
 #pragma once
 
 #include <cstdint>
+#include <functional>
 #include <map>
 #include <span>
 #include <vector>
@@ -8,6 +9,8 @@
 #include "vkml/context.hpp"
 #include "vkml/ops.hpp"
 #include "vkml/tensor.hpp"
+
+struct vkml_attend_pages_params;  // vkml_hip.h's
 
 // Several sequences over one paged KV cache. The reference keeps one sequence
 // in contiguous caches (include/vkml/llama.hpp:199-209 there) and has no
@@ -78,6 +81,23 @@ struct PagedBatch {
     Tensor group_starts, group_keys;   // i32 [groups + 1], [groups]; null without groups
     std::int64_t seqs = 0, tokens = 0, groups = 0;
     std::int64_t positions = 0;        // past the last position of a new token
+    std::vector<std::int64_t> ids, before, added;  // the sequences, their earlier keys and their new tokens
+};
+
+// A batch's new tokens as trees, for speculative decoding: a sequence's first new
+// token is the one that its last step picked, the others are drafted after one of
+// those before them.
+struct PagedTrees {
+    Tensor parents, seen, positions;  // i32 [tokens], [tokens, words], [tokens]
+    std::int64_t deepest = 0;         // past the last position
+};
+
+// What a step of speculative decoding keeps of each of a batch's sequences: the
+// confirmed nodes of its tree in order, and the pick after the last of them, which
+// is the sequence's next token (nothing and -1 for a sequence without new tokens).
+struct KeptDrafts {
+    std::vector<std::vector<std::int32_t>> paths;
+    std::vector<std::int32_t> next;
 };
 
 // The keys and values of several sequences, in up to 2^24 pages of `page_size`
@@ -114,13 +134,36 @@ public:
     // sequence after sequence: q and k rotated at their positions by a table
     // from rope_table (for a part of the head: of that many dims; null: not
     // rotated) that holds them all, k and v into a layer's pages. Returns q
-    // [tokens, heads, head_dim].
-    Tensor append(std::int64_t layer, const PagedBatch& batch, const Tensor& qkv, const Tensor& rope_table, RopeStyle style);
+    // [tokens, heads, head_dim]. With trees (of this batch) a token is rotated at its
+    // depth's position, not at its place in the sequence.
+    Tensor append(std::int64_t layer, const PagedBatch& batch, const Tensor& qkv, const Tensor& rope_table, RopeStyle style,
+                  const PagedTrees* trees = nullptr);
 
     // softmax(q k^T / sqrt(head_dim)) v of each new token over its sequence's
     // keys up to its own; q and the result [tokens, heads, head_dim].
     // head_dim 64 or 128.
     Tensor attention(std::int64_t layer, const PagedBatch& batch, const Tensor& q, float softcap = 0.0f) const;
+    // The same over a window: a token sees the last `window` keys up to its own, and
+    // its sequence's first `sinks`. A batch without groups.
+    Tensor attention_window(std::int64_t layer, const PagedBatch& batch, const Tensor& q, std::int64_t window, std::int64_t sinks = 0, float softcap = 0.0f) const;
+
+    // A step of speculative decoding: trees of a batch's new tokens; for each layer
+    // append (with the trees) and attention_tree; the model's pick after
+    // every token (vkml::sample or argmax of its logits); then keep.
+    // parents [tokens], sequence after sequence: the index, among its sequence's new
+    // tokens, of the one that a token was drafted after; -1 for a sequence's first (and
+    // for a token that sees no other new one, which is never kept). At most 4096 new
+    // tokens a sequence.
+    PagedTrees trees(const PagedBatch& batch, std::span<const std::int32_t> parents) const;
+    // attention, a token seeing its sequence's earlier keys, itself and those of
+    // the new tokens that it was drafted after.
+    Tensor attention_tree(std::int64_t layer, const PagedBatch& batch, const PagedTrees& trees, const Tensor& q, float softcap = 0.0f) const;
+    // drafted and picked, i32 [tokens]: each token, and the model's pick after it.
+    // Along each tree's path of tokens that are the pick after the one before, the keys
+    // and values of every layer move to follow the sequence's earlier keys, and the
+    // sequence ends there. Waits for the step. The sequences must be as the batch left
+    // them.
+    KeptDrafts keep(const PagedBatch& batch, const PagedTrees& trees, const Tensor& drafted, const Tensor& picked);
 
     const Tensor& k_pages() const noexcept { return k_; }  // [layers, pages, kv_heads, page_size, head_dim]
     const Tensor& v_pages() const noexcept { return v_; }
@@ -128,6 +171,9 @@ public:
 private:
     void copy(const std::vector<PageCopy>& copies);
     void* pool(const Tensor& pools, std::int64_t layer) const;
+    // One of the attention calls: its parameters, workspace and output.
+    using Attend = std::function<int(const vkml_attend_pages_params&, void*, float*)>;
+    Tensor attend(const char* name, const PagedBatch& batch, const Tensor& q, float softcap, const Attend& call) const;
 
     std::int64_t layers_, kv_heads_, head_dim_;
     PageTable table_;

@@ -7,6 +7,8 @@
 #include <utility>
 #include <vector>
 
+#include "vkml/tensor.hpp"
+
 namespace vkml {
 
 // How the next token is picked from a model's logits (reference:
@@ -57,6 +59,13 @@ private:
     std::mt19937_64 rng_;
     std::unordered_map<std::int32_t, int> picked_;  // times each token was picked, for the penalties
 };
+
+// A token for each row of logits, f32 [.., vocab], picked on the device as a Sampler
+// of that row's options would with its draw at random[row] (in [0, 1)) of the kept
+// weight; i32 [..]. options: one for every row, or one for all. Their penalties
+// must be off (they change the logits before), their seeds are not used. A row
+// without a token to pick (all NaN or -infinity) gives -1.
+Tensor sample(const Tensor& logits, std::span<const SamplingOptions> options, std::span<const double> random);
 
 // A token's log probability under logits (their log-softmax, computed in
 // double and rounded to float), and the `top` most likely tokens with

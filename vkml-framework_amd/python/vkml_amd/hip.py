@@ -82,6 +82,10 @@ RopeKvPagesParams = _struct("RopeKvPagesParams", [("heads", u32), ("kv_heads", u
                                                   ("page_size", u32), ("pages", u32), ("seqs", u32), ("tokens", u32),
                                                   ("table_stride", u32), ("row_stride", u32), ("page_stride", u64),
                                                   ("rotary_dim", u32), ("style", u32), ("positions", u32)])
+KeepDraftsParams = _struct("KeepDraftsParams", [("kv_heads", u32), ("head_dim", u32), ("kv_type", u32), ("page_size", u32),
+                                                ("pages", u32), ("layers", u32), ("seqs", u32), ("tokens", u32),
+                                                ("table_stride", u32), ("page_stride", u64), ("layer_stride", u64)])
+SampleParams = _struct("SampleParams", [("rows", u32), ("vocab", u32), ("row_stride", u64)])
 CopyPagesParams = _struct("CopyPagesParams", [("pages", u32), ("layers", u32), ("count", u32), ("page_bytes", u64),
                                               ("page_stride", u64), ("layer_stride", u64)])
 
@@ -160,6 +164,11 @@ SIGNATURES = {
     "vkml_attend_step_noalloc": [P(AttendStepParams), vp, vp, vp, vp, vp, vp, vp, vp],
     "vkml_attend_pages_workspace_bytes": [P(AttendPagesParams)],
     "vkml_attend_pages": [P(AttendPagesParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp],
+    "vkml_attend_pages_tree": [P(AttendPagesParams), u32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp],
+    "vkml_attend_pages_window": [P(AttendPagesParams), u32, u32, vp, vp, vp, vp, vp, vp, vp, vp],
+    "vkml_keep_drafts": [P(KeepDraftsParams), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp],
+    "vkml_sample_workspace_bytes": [P(SampleParams)],
+    "vkml_sample": [P(SampleParams), vp, vp, vp, vp, vp],
     "vkml_rope_kv_pages": [P(RopeKvPagesParams), vp, vp, vp, vp, vp, vp, vp, vp, vp],
     "vkml_copy_pages": [P(CopyPagesParams), vp, vp, vp, vp],
     "vkml_attend_o_sync_bytes": [],
@@ -191,6 +200,7 @@ def lib() -> C.CDLL:
         _lib.vkml_attend_o_sync_bytes.restype = C.c_uint64
         _lib.vkml_attend_fused_sync_bytes.restype = C.c_uint64
         _lib.vkml_attend_pages_workspace_bytes.restype = C.c_uint64
+        _lib.vkml_sample_workspace_bytes.restype = C.c_uint64
     return _lib
 
 

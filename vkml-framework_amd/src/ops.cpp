@@ -9,6 +9,7 @@
 
 #include "runtime.hpp"
 #include "vkml/ops.hpp"
+#include "vkml/sampling.hpp"
 
 namespace vkml {
 
@@ -137,6 +138,34 @@ Tensor argmax(const Tensor& x) {
     Tensor out = like(x, Shape(x.shape().begin(), x.shape().end() - 1), DType::I32);
     if (out.numel() == 0) return out;
     check(vkml_argmax(r.rows, r.cols, static_cast<const float*>(x.data()), static_cast<std::int32_t*>(out.data())), "argmax");
+    return out;
+}
+
+Tensor sample(const Tensor& logits, std::span<const SamplingOptions> options, std::span<const double> random) {
+    const Rows r = row_shape("sample", logits);
+    if (r.cols == 0) throw Error("sample: the last dimension is empty");
+    if ((options.size() != 1 && options.size() != r.rows) || random.size() != r.rows) {
+        throw Error("sample: " + std::to_string(options.size()) + " options and " + std::to_string(random.size()) + " random numbers for " + std::to_string(r.rows) + " rows");
+    }
+    std::vector<vkml_sampling> each(r.rows);
+    for (std::size_t i = 0; i < options.size(); ++i) {
+        const SamplingOptions& o = options[i];
+        Sampler checked(o);  // (throws what its options may not be)
+        if (o.repetition_penalty != 1.0f || o.frequency_penalty != 0.0f || o.presence_penalty != 0.0f) throw Error("sample: penalties change the logits before");
+        if (i < each.size()) each[i] = {o.temperature, o.top_k, o.top_p, o.min_p};
+    }
+    for (std::size_t i = options.size(); i < each.size(); ++i) each[i] = each[0];
+    Tensor out = like(logits, Shape(logits.shape().begin(), logits.shape().end() - 1), DType::I32);
+    if (out.numel() == 0) return out;
+    const vkml_sample_params p{r.rows, r.cols, r.cols};
+    const std::int64_t rows = r.rows, bytes = static_cast<std::int64_t>(vkml_sample_workspace_bytes(&p));
+    // Released when this returns: later work on the stream runs after the call's.
+    const Tensor settings = like(logits, {rows, 4}, DType::I32), draws = like(logits, {rows, 2}, DType::I32), workspace = like(logits, {bytes / 4}, DType::I32);
+    check(vkml_memcpy_h2d(settings.data(), each.data(), each.size() * sizeof(vkml_sampling)), "sample");
+    check(vkml_memcpy_h2d(draws.data(), random.data(), random.size() * sizeof(double)), "sample");
+    check(vkml_sample(&p, static_cast<const float*>(logits.data()), static_cast<const vkml_sampling*>(settings.data()), static_cast<const double*>(draws.data()),
+                      workspace.data(), static_cast<std::int32_t*>(out.data())),
+          "sample");
     return out;
 }
 

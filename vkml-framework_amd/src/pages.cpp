@@ -1,31 +1,23 @@
 // pages.cpp -- vkml::PagedCache over the C ABI (vkml_rope_kv_pages,
-// vkml_attend_pages, vkml_copy_pages).
+// vkml_attend_pages, vkml_copy_pages). Its windows and trees are in drafts.cpp.
 #include <algorithm>
 #include <cmath>
 #include <string>
 
-#include "runtime.hpp"
-#include "vkml/pages.hpp"
+#include "paged.hpp"
 
 namespace vkml {
 
 using detail::check;
 using detail::TensorAccess;
+using namespace detail::paged;
 
 namespace {
-
-std::uint32_t u32(std::int64_t v) {
-    if (v < 0 || v > 0xFFFFFFFFll) throw Error("PagedCache: size " + std::to_string(v) + " does not fit 32 bits");
-    return static_cast<std::uint32_t>(v);
-}
 
 std::int64_t positive(std::int64_t v, const char* what) {
     if (v < 1) throw Error("PagedCache: " + std::to_string(v) + " " + what);
     return v;
 }
-
-// What a batch of the kernels holds at most (csrc/pages.hpp).
-constexpr std::int64_t kMaxSeqs = 1 << 16, kMaxTokens = 1 << 22, kMaxKeys = 1 << 26;
 
 // The table of a cache whose every call the kernels take (csrc/pages.hpp), and
 // whose pools' bytes can be counted.
@@ -44,14 +36,6 @@ PageTable table_of(std::int64_t layers, std::int64_t kv_heads, std::int64_t head
     if (page_bytes > (std::int64_t{1} << 62) / layers / std::max<std::int64_t>(pages, 1)) throw Error("PagedCache: pools of more than 2^62 bytes");
     return PageTable(pages, page_size);
 }
-
-Tensor array(detail::Runtime& runtime, Shape shape) { return TensorAccess::empty(runtime, std::move(shape), DType::I32); }
-
-void upload(const Tensor& t, const std::vector<std::int32_t>& values) {
-    if (!values.empty()) check(vkml_memcpy_h2d(t.data(), values.data(), values.size() * sizeof(std::int32_t)), "PagedCache::batch");
-}
-
-const std::int32_t* ints(const Tensor& t) { return static_cast<const std::int32_t*>(t.data()); }
 
 }  // namespace
 
@@ -112,7 +96,10 @@ PagedBatch PagedCache::batch(std::span<const std::int64_t> ids, std::span<const 
         if (b.tokens > kMaxTokens) throw Error("PagedCache::batch: more than 2^22 new tokens");
         most = std::max(most, length + tokens[i]);
         if (tokens[i] > 0) b.positions = std::max(b.positions, length + tokens[i]);
+        b.before.push_back(length);
     }
+    b.ids.assign(ids.begin(), ids.end());
+    b.added.assign(tokens.begin(), tokens.end());
     const std::int64_t stride = (most + table_.page_size() - 1) / table_.page_size();
     detail::Runtime& runtime = TensorAccess::runtime(k_);
     b.table = array(runtime, {b.seqs, stride});
@@ -153,7 +140,7 @@ PagedBatch PagedCache::batch(std::span<const std::int64_t> ids, std::span<const 
     return b;
 }
 
-Tensor PagedCache::append(std::int64_t layer, const PagedBatch& batch, const Tensor& qkv, const Tensor& rope_table, RopeStyle style) {
+Tensor PagedCache::append(std::int64_t layer, const PagedBatch& batch, const Tensor& qkv, const Tensor& rope_table, RopeStyle style, const PagedTrees* trees) {
     const Shape& s = qkv.shape();
     const std::int64_t heads = s.size() == 2 && s[1] % head_dim_ == 0 ? s[1] / head_dim_ - 2 * kv_heads_ : 0;
     if (qkv.dtype() != DType::F32 || heads < 1 || s[0] != batch.tokens) {
@@ -165,8 +152,10 @@ Tensor PagedCache::append(std::int64_t layer, const PagedBatch& batch, const Ten
     if (rotated && (rope_table.dtype() != DType::F32 || t.size() != 3 || t[1] * 2 > head_dim_ || t[2] != 2)) {
         throw Error("PagedCache::append: heads of " + std::to_string(head_dim_) + " do not match the table " + to_string(t) + " from rope_table");
     }
-    if (rotated && batch.positions > t[0]) {
-        throw Error("PagedCache::append: positions up to " + std::to_string(batch.positions - 1) + " are outside the table's " + std::to_string(t[0]) + " positions");
+    if (trees && trees->positions.shape() != Shape{batch.tokens}) throw Error("PagedCache::append: the trees are of another batch");
+    const std::int64_t positions = trees ? trees->deepest : batch.positions;
+    if (rotated && positions > t[0]) {
+        throw Error("PagedCache::append: positions up to " + std::to_string(positions - 1) + " are outside the table's " + std::to_string(t[0]) + " positions");
     }
     Tensor q = TensorAccess::empty(TensorAccess::runtime(qkv), {batch.tokens, heads, head_dim_}, DType::F32);
     if (batch.tokens == 0) return q;
@@ -185,15 +174,16 @@ Tensor PagedCache::append(std::int64_t layer, const PagedBatch& batch, const Ten
     p.style = style == RopeStyle::Interleaved ? 0 : 1;
     p.positions = rotated ? u32(t[0]) : 0;
     check(vkml_rope_kv_pages(&p, static_cast<const float*>(qkv.data()), rotated ? static_cast<const float*>(rope_table.data()) : nullptr, ints(batch.table),
-                             ints(batch.lengths), ints(batch.starts), nullptr, static_cast<float*>(q.data()), pool(k_, layer), pool(v_, layer)),
+                             ints(batch.lengths), ints(batch.starts), trees ? ints(trees->positions) : nullptr, static_cast<float*>(q.data()), pool(k_, layer),
+                             pool(v_, layer)),
           "PagedCache::append");
     return q;
 }
 
-Tensor PagedCache::attention(std::int64_t layer, const PagedBatch& batch, const Tensor& q, float softcap) const {
+Tensor PagedCache::attend(const char* name, const PagedBatch& batch, const Tensor& q, float softcap, const Attend& call) const {
     const Shape& s = q.shape();
     if (q.dtype() != DType::F32 || s.size() != 3 || s[0] != batch.tokens || s[1] < 1 || s[1] % kv_heads_ != 0 || s[2] != head_dim_) {
-        throw Error("PagedCache::attention: q must be f32 [" + std::to_string(batch.tokens) + ", heads, " + std::to_string(head_dim_) + "] with heads a multiple of " +
+        throw Error(std::string(name) + ": q must be f32 [" + std::to_string(batch.tokens) + ", heads, " + std::to_string(head_dim_) + "] with heads a multiple of " +
                     std::to_string(kv_heads_) + ", got " + std::string(to_string(q.dtype())) + " " + to_string(s));
     }
     detail::Runtime& runtime = TensorAccess::runtime(q);
@@ -215,11 +205,15 @@ Tensor PagedCache::attention(std::int64_t layer, const PagedBatch& batch, const 
     const std::uint64_t bytes = vkml_attend_pages_workspace_bytes(&p);
     // Released when this returns: later work on the stream runs after the call's.
     const Tensor workspace = TensorAccess::empty(runtime, {static_cast<std::int64_t>(std::max<std::uint64_t>(bytes, 16) / 4)}, DType::F32);
-    check(vkml_attend_pages(&p, static_cast<const float*>(q.data()), pool(k_, layer), pool(v_, layer), ints(batch.table), ints(batch.lengths), ints(batch.starts),
-                            batch.groups > 0 ? ints(batch.group_starts) : nullptr, batch.groups > 0 ? ints(batch.group_keys) : nullptr, workspace.data(),
-                            static_cast<float*>(out.data())),
-          "PagedCache::attention");
+    check(call(p, workspace.data(), static_cast<float*>(out.data())), name);
     return out;
+}
+
+Tensor PagedCache::attention(std::int64_t layer, const PagedBatch& batch, const Tensor& q, float softcap) const {
+    return attend("PagedCache::attention", batch, q, softcap, [&](const vkml_attend_pages_params& p, void* workspace, float* out) {
+        return vkml_attend_pages(&p, static_cast<const float*>(q.data()), pool(k_, layer), pool(v_, layer), ints(batch.table), ints(batch.lengths), ints(batch.starts),
+                                 batch.groups > 0 ? ints(batch.group_starts) : nullptr, batch.groups > 0 ? ints(batch.group_keys) : nullptr, workspace, out);
+    });
 }
 
 }  // namespace vkml
