@@ -73,8 +73,8 @@ def test_sample_refuses(host, change, why):
 
 def test_the_workspace_of_a_sample(host):
     need = lambda rows, vocab: host.sample_workspace_c(C.byref(H.SampleParams(rows=rows, vocab=vocab, row_stride=vocab)))  # noqa: E731
-    assert need(7, 1) == need(7, 32765) == 0
-    assert need(1, 32766) > 0 and need(3, 128256) % 8 == 0 and need(1, 2 ** 22) > 0
+    assert need(7, 1) == need(7, 32768) == 0
+    assert need(1, 32769) > 0 and need(3, 128256) % 8 == 0 and need(1, 2 ** 22) > 0
     assert need(40, 128256) < 4 << 20
 
 

@@ -189,6 +189,26 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
+// v of lane i - n (DPP's row shifts and broadcasts), 0 where there is none:
+// the steps of an inclusive sum over the wave.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int32_t shifted(int32_t v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t shifted(int64_t v) {
+    const int lo = shifted<CTRL, ROWS>(static_cast<int32_t>(v)), hi = shifted<CTRL, ROWS>(static_cast<int32_t>(v >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
+}
+template <typename T>
+__device__ __forceinline__ T inclusive_sum(T v) {
+    v += shifted<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8: within 16 lanes
+    v += shifted<0x112, 0xF>(v);
+    v += shifted<0x114, 0xF>(v);
+    v += shifted<0x118, 0xF>(v);
+    v += shifted<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    v += shifted<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
 // Block-wide sum for blockDim.x a multiple of 64, at most 1024; every
 // thread gets the result. scratch: 16 floats of LDS.
 __device__ __forceinline__ float block_sum(float v, float* scratch) {

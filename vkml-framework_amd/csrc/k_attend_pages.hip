@@ -934,24 +934,6 @@ __device__ __forceinline__ void many_rows(const PagesArgs& a, const Piece& p, Bu
 
 // ---------------------------------------------------------------- the launch
 
-// v of lane i - n (DPP's row shifts and broadcasts), 0 where there is none:
-// the steps of an inclusive sum over the wave.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int64_t shifted(int64_t v) {
-    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, true);
-    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xF, true);
-    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
-}
-__device__ __forceinline__ int64_t inclusive_sum(int64_t v) {
-    v += shifted<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8: within 16 lanes
-    v += shifted<0x112, 0xF>(v);
-    v += shifted<0x114, 0xF>(v);
-    v += shifted<0x118, 0xF>(v);
-    v += shifted<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-    v += shifted<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-    return v;
-}
-
 // Segments as the workgroup keeps them, the first kThreads of a batch.
 struct Kept {
     int32_t v[10];

@@ -11,7 +11,7 @@
 // Weights are whole numbers, units of 2^-shift of the largest (45 bits for 2^17
 // logits, so that all of a row's fit 62 bits): sums of them are exact in any order,
 // so that the same row gives the same token whatever the atomics' order. e^x is
-// found in 64 bits, 2^(-n / 64) from a table times a polynomial of degree 5, good to
+// found in 64 bits, 2^(-n / 512) from a table times a polynomial of degree 4, good to
 // 2^-50: the picks are those of sums in f64 unless a border is nearer than that.
 #include <hip/hip_runtime.h>
 
@@ -31,6 +31,9 @@ constexpr uint32_t kList = 2048;  // candidates in the LDS
 constexpr uint32_t kSubs = 1024;  // parts of a range of candidates
 constexpr uint32_t kFew = 128;    // candidates that are counted one by one
 constexpr uint64_t kNone = ~0ull;
+constexpr int32_t kTurns = 512;   // to a factor of two between weights
+constexpr int32_t kBinTurns = 16;
+static_assert(kTurns / kBinTurns * 53 <= kBins);
 
 struct Args {
     const float* logits;
@@ -57,10 +60,10 @@ __device__ __forceinline__ float logit_at(uint64_t place) {
 }
 
 struct Row {
-    float peak;
-    double turns;      // 64 log2(e) / T
-    float bins_per;    // bins a unit of l
-    double least;      // weights below it are not within min_p
+    double peak;
+    double turns;  // 512 log2(e) / T
+    double limit;  // a candidate is less turns below the largest
+    double least;  // weights below it are not within min_p
     int32_t shift;
 };
 
@@ -68,12 +71,17 @@ struct Scratch {
     uint64_t mass[kBins];  // of a bin, then of it and those before
     uint32_t count[kBins];
     uint64_t place[kList], weight[kList];
-    uint64_t sub_mass[kSubs];
-    uint32_t sub_count[kSubs];
+    union {
+        uint32_t id[kList];  // of what is listed, until its places are
+        struct {
+            uint64_t sub_mass[kSubs];
+            uint32_t sub_count[kSubs];
+        };
+    };
     uint64_t wave_mass[kWaves], wave_place[kWaves];
     uint32_t wave_count[kWaves];
     uint64_t few_place[kFew], few_weight[kFew];
-    double table[64];
+    double table[kTurns];
     uint64_t lo, hi, likely;  // a range of places; the mass within min_p
     uint64_t found_mass, found_before;
     uint32_t found, found_count, listed;
@@ -82,110 +90,162 @@ struct Scratch {
 // ---------------------------------------------------------------- weights
 
 __device__ __forceinline__ void fill_table(Scratch& lds) {
-    if (threadIdx.x < 64) lds.table[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 64.0);
+    if (threadIdx.x < kTurns) lds.table[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / kTurns);
 }
 
 __device__ __forceinline__ Row row_of(float peak, const vkml_sampling& o, int32_t shift) {
     Row r;
-    r.peak = peak;
-    r.turns = 64.0 * 1.4426950408889634 / static_cast<double>(o.temperature);
-    // beyond T ln2 (shift + 1) a weight rounds to 0
-    const float span = o.temperature * 0.6931472f * static_cast<float>(shift + 2);
-    r.bins_per = fminf(static_cast<float>(kBins) / span, 1e30f);
+    r.peak = static_cast<double>(peak);
+    r.turns = fmax(kTurns * 1.4426950408889634 / static_cast<double>(o.temperature), 1e-300);  // (not 0, of which -infinity makes NaN)
+    r.limit = kTurns * (shift + 1);  // less than half a unit from there on
     r.least = (o.min_p > 0.0f ? static_cast<double>(o.min_p) : 0.0) * __builtin_ldexp(1.0, shift);
     r.shift = shift;
+    // Where top_p does not ask for the mass of all, those that min_p leaves out need no
+    // weight (but for a turn, so that the weights decide).
+    if (o.min_p > 0.0f && !(o.top_p < 1.0f)) r.limit = fmin(r.limit, fmax(1.0 - kTurns * static_cast<double>(log2f(o.min_p)), 1.0));
     return r;
 }
 
-// NaN and -infinity weigh nothing; beside +infinity, nothing else does.
-__device__ __forceinline__ uint64_t weight_of(const Row& r, float l, const double* table) {
-    const double d = l == r.peak ? 0.0 : static_cast<double>(r.peak) - static_cast<double>(l);
-    const double z = d * r.turns;
-    const bool some = l > -__builtin_inff() && z < 64.0 * (r.shift + 2);
-    const double zz = some ? z : 0.0, n = __builtin_rint(zz);
-    const double f = (zz - n) * (-0.6931471805599453 / 64.0);
-    double p = __builtin_fma(f, 1.0 / 120.0, 1.0 / 24.0);
-    p = __builtin_fma(p, f, 1.0 / 6.0);
+// How far a logit's weight is below the largest: whether it is a candidate at all, and
+// the turns, z, also to the next whole number. (+infinity beside itself is none below;
+// beside it, as -infinity always, the rest is no candidate. NaN comes as -infinity.)
+struct Turns {
+    double z, whole;
+    int32_t n;
+    bool candidate;
+};
+__device__ __forceinline__ Turns turns_of(const Row& r, float l) {
+    constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: a sum with it is whole, in the low bits
+    const double z = fmax((r.peak - static_cast<double>(l)) * r.turns, 0.0), sum = z + kMagic;
+    return {z, sum - kMagic, static_cast<int32_t>(__builtin_bit_cast(uint64_t, sum)), z < r.limit};
+}
+__device__ __forceinline__ uint32_t bin_of(const Turns& t) { return static_cast<uint32_t>(t.n) / kBinTurns; }
+// 2^(shift - z / kTurns), the nearest whole number: 2^-(n / kTurns) from the table, the
+// rest, at most half a turn, by e^f's first terms (f^5 / 120 < 2^-59).
+__device__ __forceinline__ uint64_t weight_of(const Row& r, const Turns& t, const double* table) {
+    const double f = (t.whole - t.z) * (0.6931471805599453 / kTurns);
+    double p = __builtin_fma(f, 1.0 / 24.0, 1.0 / 6.0);
     p = __builtin_fma(p, f, 0.5);
     p = __builtin_fma(p, f, 1.0);
     p = __builtin_fma(p, f, 1.0);
-    const int32_t i = static_cast<int32_t>(n);
-    const double w = __builtin_amdgcn_ldexp(table[i & 63] * p, r.shift - (i >> 6));
-    // rounded to a whole number in the sum's low bits
-    const uint64_t whole = __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
-    return some ? whole : 0;
-}
-
-__device__ __forceinline__ uint32_t bin_of(const Row& r, float l) {
-    const float d = l == r.peak ? 0.0f : r.peak - l;
-    return static_cast<uint32_t>(fminf(d * r.bins_per, static_cast<float>(kBins - 1)));
+    const double w = __builtin_amdgcn_ldexp(table[t.n & (kTurns - 1)] * p, r.shift - (t.n >> 9));
+    static_assert(kTurns == 1 << 9);
+    return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
 }
 
 // ---------------------------------------------------------------- a row's values
 
-// The row's vectors of four values, the first of which holds its first one (or, off
-// values before, nothing); what is not the row's reads as NaN.
+// A row: its vectors of four values from the first multiple of 16 bytes on, and up
+// to three values before them and behind.
 struct Source {
     const float* row;
-    uint32_t vocab, off;
-    __device__ __forceinline__ uint32_t vectors() const { return (vocab + off + 3) / 4; }
+    uint32_t vocab, head, vectors;
     __device__ __forceinline__ float4 load(uint32_t v) const {
-        const int32_t at = static_cast<int32_t>(4 * v) - static_cast<int32_t>(off);
-        if (at >= 0 && at + 4 <= static_cast<int32_t>(vocab)) return ldg(reinterpret_cast<const float4*>(row + at));
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = at + e >= 0 && at + e < static_cast<int32_t>(vocab) ? ldg(row + (at + e)) : __builtin_nanf("");
-        return make_float4(x[0], x[1], x[2], x[3]);
+        const float4 x = ldg(reinterpret_cast<const float4*>(row + head) + v);
+        return make_float4(number(x.x), number(x.y), number(x.z), number(x.w));
     }
+    __device__ __forceinline__ float value(uint32_t id) const { return number(ldg(row + id)); }
+    __device__ __forceinline__ static float number(float l) { return fmaxf(l, -__builtin_inff()); }  // NaN: -infinity
+    __device__ __forceinline__ uint32_t id(uint32_t v) const { return head + 4 * v; }
+    // The values outside the vectors, six at most: their ids.
+    __device__ __forceinline__ uint32_t edges() const { return vocab - 4 * vectors; }
+    __device__ __forceinline__ uint32_t edge(uint32_t i) const { return i < head ? i : i + 4 * vectors; }
 };
 __device__ __forceinline__ Source source_of(const Args& a, uint32_t row) {
     const float* p = a.logits + row * a.row_stride;
-    return {p, a.vocab, static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) / 4 % 4)};
+    const uint32_t head = min(static_cast<uint32_t>(-(reinterpret_cast<uintptr_t>(p) / 4) % 4), a.vocab);
+    return {p, a.vocab, head, (a.vocab - head) / 4};
 }
 
-// A slice of them in the workgroup's registers.
+// A slice of it in the workgroup's registers, the first one's with the values outside
+// the vectors. (What is none of the row's is -infinity.)
 struct Held {
     float4 x[kVectors];
-    uint32_t id0;  // of the thread's first value (it may wrap below 0, where that is none of the row's)
+    float edge;
+    uint32_t id0, edge_id;
     __device__ __forceinline__ void load(const Source& s, uint32_t slice) {
         const uint32_t v0 = slice * kVectors * kThreads + threadIdx.x;
-        id0 = 4 * v0 - s.off;
-#pragma unroll
-        for (uint32_t i = 0; i < kVectors; ++i) x[i] = s.load(v0 + i * kThreads);
-    }
-    template <typename F>
-    __device__ __forceinline__ void each(const F& f) const {
+        const float none = -__builtin_inff();
+        id0 = s.id(v0);
 #pragma unroll
         for (uint32_t i = 0; i < kVectors; ++i) {
+            x[i] = make_float4(none, none, none, none);
+            if (v0 + i * kThreads < s.vectors) x[i] = s.load(v0 + i * kThreads);
+        }
+        edge = none;
+        edge_id = s.edge(threadIdx.x);
+        if (slice == 0 && threadIdx.x < s.edges()) edge = s.value(edge_id);
+    }
+    // f(value, id). (Through an empty asm, so that what one pass finds of the values
+    // and ids is not kept in registers for the next.)
+    template <typename F>
+    __device__ __forceinline__ void each(const F& f) {
+#pragma unroll
+        for (uint32_t i = 0; i < kVectors; ++i) {
+            asm volatile("" : "+v"(x[i].x), "+v"(x[i].y), "+v"(x[i].z), "+v"(x[i].w), "+v"(id0));
             const uint32_t id = id0 + 4 * i * kThreads;
             f(x[i].x, id);
             f(x[i].y, id + 1);
             f(x[i].z, id + 2);
             f(x[i].w, id + 3);
         }
+        f(edge, edge_id);
+    }
+    // The ids of the candidates in bins first .. last to the list, lds.listed of them:
+    // which they are as bits first, then one addition a wave for their places there.
+    __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
+        static_assert(4 * kVectors == 32);
+        uint32_t bits = 0, k = 0, at_edge = 0;
+        each([&](float l, uint32_t) {
+            const Turns t = turns_of(r, l);
+            const uint32_t b = bin_of(t), hit = t.candidate && b >= first && b <= last;
+            if (k < 32) bits |= hit << k++;
+            else at_edge = hit;
+        });
+        const uint32_t n = static_cast<uint32_t>(__builtin_popcount(bits)) + at_edge;
+        const uint32_t upto = static_cast<uint32_t>(inclusive_sum(static_cast<int32_t>(n))), all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), kWave - 1));
+        if (all == 0) return;
+        uint32_t base = 0;
+        if (threadIdx.x % kWave == 0) base = __hip_atomic_fetch_add(&lds.listed, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(base))) + upto - n;
+        if (at_edge && to < kList) lds.id[to++] = edge_id;
+        for (; bits; bits &= bits - 1, ++to) {
+            const uint32_t i = static_cast<uint32_t>(__builtin_ctz(bits));
+            if (to < kList) lds.id[to] = id0 + 4 * (i / 4) * kThreads + i % 4;
+        }
     }
 };
 
-// All of them, read again each time.
+// All of it, read again each time.
 struct Streamed {
     Source s;
     template <typename F>
-    __device__ __forceinline__ void each(const F& f) const {
+    __device__ __forceinline__ void each(const F& f) {
         constexpr uint32_t kFlight = 2;
-        const uint32_t n = s.vectors();
-        for (uint32_t v = threadIdx.x; v < n; v += kFlight * kThreads) {
+        for (uint32_t v = threadIdx.x; v < s.vectors; v += kFlight * kThreads) {
             float4 x[kFlight];
 #pragma unroll
-            for (uint32_t i = 0; i < kFlight; ++i) x[i] = s.load(v + i * kThreads);
+            for (uint32_t i = 0; i < kFlight; ++i) x[i] = s.load(min(v + i * kThreads, s.vectors - 1));
 #pragma unroll
             for (uint32_t i = 0; i < kFlight; ++i) {
-                const uint32_t id = 4 * (v + i * kThreads) - s.off;
+                if (v + i * kThreads >= s.vectors) break;
+                const uint32_t id = s.id(v + i * kThreads);
                 f(x[i].x, id);
                 f(x[i].y, id + 1);
                 f(x[i].z, id + 2);
                 f(x[i].w, id + 3);
             }
         }
+        if (threadIdx.x < s.edges()) f(s.value(s.edge(threadIdx.x)), s.edge(threadIdx.x));
+    }
+    __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
+        each([&](float l, uint32_t id) {
+            const Turns t = turns_of(r, l);
+            const uint32_t b = bin_of(t);
+            if (!t.candidate || b < first || b > last) return;
+            const uint32_t to = __hip_atomic_fetch_add(&lds.listed, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (to < kList) lds.id[to] = id;
+        });
     }
 };
 
@@ -205,17 +265,17 @@ __device__ __forceinline__ uint64_t wave_min(uint64_t v) {
 
 // The place of the largest of the values, kNone where there is none.
 template <typename V>
-__device__ __forceinline__ uint64_t first_of(const V& values, Scratch& lds) {
+__device__ __forceinline__ uint64_t first_of(V& values, Scratch& lds) {
     float best = -__builtin_inff();
     uint32_t id = 0;
     values.each([&](float l, uint32_t i) {
-        if (l > best) best = l, id = i;  // (ids rise: the first of equal ones)
+        if (l > best || (l == best && i < id)) best = l, id = i;
     });
     const uint64_t mine = wave_min(best > -__builtin_inff() ? place_of(best, id) : kNone);
     if (threadIdx.x % kWave == 0) lds.wave_place[threadIdx.x / kWave] = mine;
     __syncthreads();
     uint64_t all = kNone;
-#pragma unroll
+#pragma unroll 4
     for (uint32_t i = 0; i < kWaves; ++i) all = lds.wave_place[i] < all ? lds.wave_place[i] : all;
     return all;
 }
@@ -229,51 +289,61 @@ __device__ __forceinline__ void clear_bins(Scratch& lds) {
     if (threadIdx.x == 0) lds.likely = 0;
     __syncthreads();
 }
-// The values' weights to the bins. A barrier has to follow.
-template <typename V>
-__device__ __forceinline__ void fill_bins(const V& values, const Row& r, Scratch& lds) {
+// The candidates' weights to the bins, or how many they are alone. A barrier has to
+// follow.
+template <bool MASS, bool COUNT, typename V>
+__device__ __forceinline__ void fill_bins(V& values, const Row& r, Scratch& lds) {
     uint64_t likely = 0;
     values.each([&](float l, uint32_t) {
-        const uint64_t w = weight_of(r, l, lds.table);
-        if (w == 0) return;
-        const uint32_t b = bin_of(r, l);
-        add(&lds.mass[b], w);
-        add(&lds.count[b], 1u);
-        if (static_cast<double>(w) >= r.least) likely += w;
+        const Turns t = turns_of(r, l);
+        if (!t.candidate) return;
+        const uint32_t b = bin_of(t);
+        if constexpr (COUNT) add(&lds.count[b], 1u);
+        if constexpr (MASS) {
+            const uint64_t w = weight_of(r, t, lds.table);
+            add(&lds.mass[b], w);
+            if (static_cast<double>(w) >= r.least) likely += w;
+        }
     });
-    if (r.least > 0.0 && likely) add(&lds.likely, likely);
+    if (MASS && r.least > 0.0 && likely) add(&lds.likely, likely);
 }
 
-// mass and count of n parts (two a thread, or one) become those of the part and all
-// before it.
-template <uint32_t N>
+// What of N parts becomes that of the part and all before it. A barrier has to come
+// before; one comes after.
+template <uint32_t N, bool MASS, bool COUNT>
 __device__ __forceinline__ void sum_up(uint64_t* mass, uint32_t* count, Scratch& lds) {
     constexpr uint32_t kEach = N / kThreads;
-    const uint32_t t = threadIdx.x, l = t % kWave, w = t / kWave;
-    uint64_t m[kEach], ms = 0;
-    uint32_t c[kEach], cs = 0;
+    const uint32_t t = threadIdx.x, w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(t / kWave)));
+    uint64_t m[kEach], ms = 0, mi = 0;
+    uint32_t c[kEach], cs = 0, ci = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kEach; ++i) {
-        ms = m[i] = ms + mass[kEach * t + i];
-        cs = c[i] = cs + count[kEach * t + i];
+        if constexpr (MASS) ms = m[i] = ms + mass[kEach * t + i];
+        if constexpr (COUNT) cs = c[i] = cs + count[kEach * t + i];
     }
-    uint64_t mi = ms;
-    uint32_t ci = cs;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const uint64_t mo = static_cast<uint64_t>(static_cast<uint32_t>(__shfl_up(static_cast<int>(mi >> 32), o))) << 32 | static_cast<uint32_t>(__shfl_up(static_cast<int>(mi), o));
-        const uint32_t co = static_cast<uint32_t>(__shfl_up(static_cast<int>(ci), o));
-        if (l >= static_cast<uint32_t>(o)) mi += mo, ci += co;
-    }
-    if (l == kWave - 1) lds.wave_mass[w] = mi, lds.wave_count[w] = ci;
+    if constexpr (MASS) mi = static_cast<uint64_t>(inclusive_sum(static_cast<int64_t>(ms)));
+    if constexpr (COUNT) ci = static_cast<uint32_t>(inclusive_sum(static_cast<int32_t>(cs)));
+    if (t % kWave == kWave - 1) lds.wave_mass[w] = mi, lds.wave_count[w] = ci;
     __syncthreads();
-    uint64_t m0 = mi - ms;
-    uint32_t c0 = ci - cs;
+    // the sums of the waves before: a lane each, summed up by every wave
+    const uint32_t l = t % kWave % kWaves;
+    uint64_t m0 = 0;
+    uint32_t c0 = 0;
+    if constexpr (MASS) {
+        const uint64_t all = static_cast<uint64_t>(inclusive_sum(static_cast<int64_t>(lds.wave_mass[l])));
+        if (w > 0)
+            m0 = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all >> 32), w - 1))) << 32 |
+                 static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all), w - 1));
+    }
+    if constexpr (COUNT) {
+        const int32_t all = inclusive_sum(static_cast<int32_t>(lds.wave_count[l]));
+        if (w > 0) c0 = static_cast<uint32_t>(__builtin_amdgcn_readlane(all, w - 1));
+    }
 #pragma unroll
-    for (uint32_t i = 0; i < kWaves; ++i)
-        if (i < w) m0 += lds.wave_mass[i], c0 += lds.wave_count[i];
-#pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) mass[kEach * t + i] = m0 + m[i], count[kEach * t + i] = c0 + c[i];
+    for (uint32_t i = 0; i < kEach; ++i) {
+        if constexpr (MASS) mass[kEach * t + i] = m0 + mi - ms + m[i];
+        if constexpr (COUNT) count[kEach * t + i] = c0 + ci - cs + c[i];
+    }
     __syncthreads();
 }
 
@@ -335,7 +405,7 @@ __device__ __forceinline__ Found among(const Visit& visit, Wanted x, uint64_t lo
             add(&lds.sub_count[i], 1u);
         });
         __syncthreads();
-        sum_up<kSubs>(lds.sub_mass, lds.sub_count, lds);
+        sum_up<kSubs, true, true>(lds.sub_mass, lds.sub_count, lds);
         const Part p = part_with<kSubs>(lds.sub_mass, lds.sub_count, x, lds);
         mass += p.mass_before;
         x.before -= x.by_count ? p.count_before : p.mass_before;
@@ -372,8 +442,25 @@ __device__ __forceinline__ Found among(const Visit& visit, Wanted x, uint64_t lo
     return f;
 }
 
+// The candidates of bins first .. last, n of them, to the list.
+template <typename V>
+__device__ __forceinline__ void list_bins(V& values, const Source& source, const Row& r, const Listed& listed, Scratch& lds) {
+    if (threadIdx.x == 0) lds.listed = 0;
+    __syncthreads();
+    values.list(r, listed.first, listed.last, lds);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
+        const uint32_t id = lds.id[i];
+        const float l = source.value(id);
+        lds.place[i] = place_of(l, id);
+        lds.weight[i] = weight_of(r, turns_of(r, l), lds.table);
+    }
+    __syncthreads();
+}
+
 // The candidate with x before it, in the bins' sums and the row's values.
-__device__ __forceinline__ Found find(const Streamed& values, const Row& r, Wanted x, Listed& listed, Scratch& lds) {
+template <typename V>
+__device__ __forceinline__ Found find(V& values, Streamed again, const Row& r, Wanted x, Listed& listed, Scratch& lds) {
     const Part p = part_with<kBins>(lds.mass, lds.count, x, lds);
     x.before -= x.by_count ? p.count_before : p.mass_before;
     const uint32_t b = p.i;
@@ -381,36 +468,26 @@ __device__ __forceinline__ Found find(const Streamed& values, const Row& r, Want
         // The bin's candidates to the list, and all before them if they fit too.
         const bool all = p.count_before + p.count <= kList;
         listed = {all ? 0 : b, b, all ? p.count_before + p.count : p.count};
-        if (threadIdx.x == 0) lds.listed = 0;
-        __syncthreads();
-        values.each([&](float l, uint32_t id) {
-            if (!(l > -__builtin_inff())) return;
-            const uint32_t i = bin_of(r, l);
-            if (i < listed.first || i > listed.last) return;
-            const uint64_t w = weight_of(r, l, lds.table);
-            if (w == 0) return;
-            const uint32_t to = __hip_atomic_fetch_add(&lds.listed, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            if (to < kList) lds.place[to] = place_of(l, id), lds.weight[to] = w;
-        });
-        __syncthreads();
+        list_bins(values, again.s, r, listed, lds);
     }
     const bool from_list = listed.first <= b && b <= listed.last;
-    const auto visit = [&](const auto& f) {
+    const auto visit = [&](const auto& f) {  // (more than the list holds: they are read again)
         if (from_list) {
-            for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads)
-                if (bin_of(r, logit_at(lds.place[i])) == b) f(lds.place[i], lds.weight[i]);
+            for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
+                const Turns t = turns_of(r, logit_at(lds.place[i]));
+                if (bin_of(t) == b) f(lds.place[i], lds.weight[i]);
+            }
         } else {
-            values.each([&](float l, uint32_t id) {
-                if (!(l > -__builtin_inff()) || bin_of(r, l) != b) return;
-                const uint64_t w = weight_of(r, l, lds.table);
-                if (w) f(place_of(l, id), w);
+            again.each([&](float l, uint32_t id) {
+                const Turns t = turns_of(r, l);
+                if (t.candidate && bin_of(t) == b) f(place_of(l, id), weight_of(r, t, lds.table));
             });
         }
     };
-    if (threadIdx.x == 0) lds.lo = kNone, lds.hi = 0;
-    __syncthreads();
     uint64_t lo = kNone, hi = 0;
     if (p.count > kFew) {  // how far apart the bin's are
+        if (threadIdx.x == 0) lds.lo = kNone, lds.hi = 0;
+        __syncthreads();
         visit([&](uint64_t at, uint64_t) {
             lo = at < lo ? at : lo;
             hi = at > hi ? at : hi;
@@ -431,9 +508,37 @@ __device__ __forceinline__ Found find(const Streamed& values, const Row& r, Want
     return among(visit, x, lo, hi, p.count, p.mass_before, lds);
 }
 
+// Whether a row's candidates are only counted at first: those that top_k keeps are
+// then few enough to be listed, and the others need no weight.
+__device__ __forceinline__ bool counts_first(const vkml_sampling& o) { return o.top_k > 0 && static_cast<uint32_t>(o.top_k) <= kList / 2; }
+
+// After the counts alone: weights of those that top_k keeps, and what else is in
+// their bins; or of all, where these are more than the list holds. The bins are then
+// as if all had theirs, up to the last that top_k asks for.
+template <typename V>
+__device__ __forceinline__ void weigh_counted(V& values, const Source& source, const Row& r, const vkml_sampling& o, Listed& listed, Scratch& lds) {
+    const uint32_t count = lds.count[kBins - 1], k = min(static_cast<uint32_t>(o.top_k), count);
+    const Part p = part_with<kBins>(lds.mass, lds.count, {true, k - 1}, lds);
+    if (p.count_before + p.count <= kList) {
+        listed = {0, p.i, p.count_before + p.count};
+        list_bins(values, source, r, listed, lds);
+        uint64_t likely = 0;
+        for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
+            const uint64_t w = lds.weight[i];
+            add(&lds.mass[bin_of(turns_of(r, logit_at(lds.place[i])))], w);
+            if (static_cast<double>(w) >= r.least) likely += w;
+        }
+        if (r.least > 0.0 && likely) add(&lds.likely, likely);
+    } else {
+        fill_bins<true, false>(values, r, lds);
+    }
+    __syncthreads();
+    sum_up<kBins, true, false>(lds.mass, lds.count, lds);
+}
+
 // The pick of a row whose bins are summed up.
-__device__ __forceinline__ uint32_t pick(const Streamed& values, const Row& r, const vkml_sampling& o, double random, Scratch& lds) {
-    Listed listed;
+template <typename V>
+__device__ __forceinline__ uint32_t pick(V& values, const Streamed& again, const Row& r, const vkml_sampling& o, double random, Listed listed, Scratch& lds) {
     uint64_t mass = lds.mass[kBins - 1];
     const uint32_t count = lds.count[kBins - 1];
     // top_k, top_p, the draw: each looks for a candidate by what the one before leaves
@@ -458,7 +563,7 @@ __device__ __forceinline__ uint32_t pick(const Streamed& values, const Row& r, c
             const uint64_t unit = at > 0.0 ? (at < 9.2e18 ? static_cast<uint64_t>(at) : mass) : 0;
             x.before = unit < mass ? unit : mass - 1;
         }
-        const Found f = find(values, r, x, listed, lds);
+        const Found f = find(values, again, r, x, listed, lds);
         if (step == 2) return f.id;
         mass = f.mass;
     }
@@ -472,8 +577,7 @@ __device__ __forceinline__ vkml_sampling options_of(const Args& a, uint32_t row)
 
 // ---------------------------------------------------------------- the launches
 
-// Rows of one slice: a workgroup a row, its values in registers until they are in
-// their bins. (The candidates that are looked for are few, and read again.)
+// Rows of one slice: a workgroup a row, its values in registers.
 __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
     __shared__ Scratch lds;
     const uint32_t row = blockIdx.x;
@@ -488,10 +592,19 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
         return;
     }
     const Row r = row_of(logit_at(first), o, a.shift);
-    fill_bins(values, r, lds);
-    __syncthreads();
-    sum_up<kBins>(lds.mass, lds.count, lds);
-    const uint32_t id = pick({source_of(a, row)}, r, o, a.random[row], lds);
+    const Streamed again{source_of(a, row)};
+    Listed listed;
+    if (counts_first(o)) {
+        fill_bins<false, true>(values, r, lds);
+        __syncthreads();
+        sum_up<kBins, false, true>(lds.mass, lds.count, lds);
+        weigh_counted(values, again.s, r, o, listed, lds);
+    } else {
+        fill_bins<true, true>(values, r, lds);
+        __syncthreads();
+        sum_up<kBins, true, true>(lds.mass, lds.count, lds);
+    }
+    const uint32_t id = pick(values, again, r, o, a.random[row], listed, lds);
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
 
@@ -523,7 +636,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_sums(Args a) {
     values.load(source_of(a, row), blockIdx.x % a.slices);
     fill_table(lds);
     clear_bins(lds);
-    fill_bins(values, row_of(logit_at(first), o, a.shift), lds);
+    const Row r = row_of(logit_at(first), o, a.shift);
+    if (counts_first(o)) fill_bins<false, true>(values, r, lds);
+    else fill_bins<true, true>(values, r, lds);
     __syncthreads();
     SliceSums* to = a.sums + blockIdx.x;
     for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
@@ -553,9 +668,14 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Args a) {
         lds.likely = likely;
     }
     __syncthreads();
-    sum_up<kBins>(lds.mass, lds.count, lds);
+    sum_up<kBins, true, true>(lds.mass, lds.count, lds);
     const Row r = row_of(logit_at(first), o, a.shift);
-    const uint32_t id = pick({source_of(a, row)}, r, o, a.random[row], lds);
+    Streamed values{source_of(a, row)};
+    Listed listed;
+    if (counts_first(o)) {
+        weigh_counted(values, values.s, r, o, listed, lds);  // (no mass in the bins yet)
+    }
+    const uint32_t id = pick(values, values, r, o, a.random[row], listed, lds);
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
 

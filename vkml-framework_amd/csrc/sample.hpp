@@ -16,8 +16,7 @@ constexpr uint32_t kBins = 2048;
 constexpr uint32_t kMaxVocab = 1u << 22;
 constexpr uint32_t kMaxSlices = 1u << 21;
 
-// A row starts up to three values past a multiple of 16 bytes.
-inline uint32_t slices(uint32_t vocab) { return (vocab + 3 + kSlice - 1) / kSlice; }
+inline uint32_t slices(uint32_t vocab) { return (vocab + kSlice - 1) / kSlice; }
 
 inline const char* check(const vkml_sample_params& p) {
     if (p.vocab == 0 || p.vocab > kMaxVocab) return "rows must hold 1 to 2^22 logits";
