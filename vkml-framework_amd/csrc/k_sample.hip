@@ -6,7 +6,13 @@
 // of the ranking, so that only the kept mass M has to be known, and the pick is the
 // first candidate whose weight and those before it pass random * M. Nothing is
 // sorted: a candidate is found by its count or mass before it, in a histogram of the
-// logits, then among its bin's candidates.
+// weights' logarithms, then among its bin's candidates.
+//
+// Where top_k (of at most as many as a workgroup has threads) or min_p alone leave few,
+// these are listed first, and the rest is never weighed: the k-th largest of the
+// threads' own largest logits is a bound that at least k reach, and few more do. A list
+// of up to a quarter of the threads is ranked outright, every candidate against every
+// other; a longer one goes through a histogram of its own.
 //
 // Weights are whole numbers, units of 2^-shift of the largest (45 bits for 2^17
 // logits, so that all of a row's fit 62 bits): sums of them are exact in any order,
@@ -26,10 +32,7 @@ using namespace vkml::sample;
 
 namespace {
 
-constexpr uint32_t kWaves = kThreads / kWave;
-constexpr uint32_t kList = 2048;  // candidates in the LDS
 constexpr uint32_t kSubs = 1024;  // parts of a range of candidates
-constexpr uint32_t kFew = 128;    // candidates that are counted one by one
 constexpr uint64_t kNone = ~0ull;
 constexpr int32_t kTurns = 512;   // to a factor of two between weights
 constexpr int32_t kBinTurns = 16;
@@ -40,8 +43,8 @@ struct Args {
     const vkml_sampling* options;
     const double* random;
     int32_t* tokens;
-    uint64_t* peaks;   // [rows, slices]: the places of the slices' largest
-    SliceSums* sums;   // [rows, slices]
+    uint64_t* peaks;  // [rows, slices]: the places of the slices' largest
+    Slice* parts;     // [rows, slices]
     uint64_t row_stride;
     uint32_t vocab, slices;
     int32_t shift;
@@ -59,39 +62,16 @@ __device__ __forceinline__ float logit_at(uint64_t place) {
     return __uint_as_float(u & 0x80000000u ? u : ~u & 0x7FFFFFFFu);
 }
 
+// ---------------------------------------------------------------- weights
+
 struct Row {
     double peak;
     double turns;  // 512 log2(e) / T
     double limit;  // a candidate is less turns below the largest
     double least;  // weights below it are not within min_p
     int32_t shift;
+    bool all;      // top_p asks for the mass of all, or nothing leaves any out
 };
-
-struct Scratch {
-    uint64_t mass[kBins];  // of a bin, then of it and those before
-    uint32_t count[kBins];
-    uint64_t place[kList], weight[kList];
-    union {
-        uint32_t id[kList];  // of what is listed, until its places are
-        struct {
-            uint64_t sub_mass[kSubs];
-            uint32_t sub_count[kSubs];
-        };
-    };
-    uint64_t wave_mass[kWaves], wave_place[kWaves];
-    uint32_t wave_count[kWaves];
-    uint64_t few_place[kFew], few_weight[kFew];
-    double table[kTurns];
-    uint64_t lo, hi, likely;  // a range of places; the mass within min_p
-    uint64_t found_mass, found_before;
-    uint32_t found, found_count, listed;
-};
-
-// ---------------------------------------------------------------- weights
-
-__device__ __forceinline__ void fill_table(Scratch& lds) {
-    if (threadIdx.x < kTurns) lds.table[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / kTurns);
-}
 
 __device__ __forceinline__ Row row_of(float peak, const vkml_sampling& o, int32_t shift) {
     Row r;
@@ -100,9 +80,10 @@ __device__ __forceinline__ Row row_of(float peak, const vkml_sampling& o, int32_
     r.limit = kTurns * (shift + 1);  // less than half a unit from there on
     r.least = (o.min_p > 0.0f ? static_cast<double>(o.min_p) : 0.0) * __builtin_ldexp(1.0, shift);
     r.shift = shift;
+    r.all = o.top_p < 1.0f || !(o.min_p > 0.0f);
     // Where top_p does not ask for the mass of all, those that min_p leaves out need no
     // weight (but for a turn, so that the weights decide).
-    if (o.min_p > 0.0f && !(o.top_p < 1.0f)) r.limit = fmin(r.limit, fmax(1.0 - kTurns * static_cast<double>(log2f(o.min_p)), 1.0));
+    if (!r.all) r.limit = fmin(r.limit, fmax(1.0 - kTurns * static_cast<double>(log2f(o.min_p)), 1.0));
     return r;
 }
 
@@ -133,7 +114,30 @@ __device__ __forceinline__ uint64_t weight_of(const Row& r, const Turns& t, cons
     return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
 }
 
-// ---------------------------------------------------------------- a row's values
+// The mass that top_p, `share` of it, asks for at the least, and the unit of it that
+// the draw falls on.
+__device__ __forceinline__ uint64_t reach_of(float share, uint64_t mass) {
+    const double of = __builtin_ceil(static_cast<double>(fmaxf(share, 0.0f)) * static_cast<double>(mass));
+    const uint64_t least = static_cast<uint64_t>(of);
+    return least < 1 ? 1 : least < mass ? least : mass;
+}
+__device__ __forceinline__ uint64_t unit_of(double random, uint64_t mass) {
+    const double at = random * static_cast<double>(mass);
+    const uint64_t unit = at > 0.0 ? (at < 9.2e18 ? static_cast<uint64_t>(at) : mass) : 0;
+    return unit < mass ? unit : mass - 1;
+}
+// What min_p leaves of a mass: the first candidate at least.
+__device__ __forceinline__ uint64_t within(const Row& r, uint64_t mass, uint64_t likely) {
+    if (!(r.least > 0.0)) return mass;
+    const uint64_t first = 1ull << r.shift, some = likely < first ? first : likely;
+    return some < mass ? some : mass;
+}
+
+__device__ __forceinline__ bool greedy(const vkml_sampling& o) { return !(o.temperature > 0.0f) || o.top_k == 1; }
+__device__ __forceinline__ vkml_sampling options_of(const Args& a, uint32_t row) {
+    const uint4 x = ldg(reinterpret_cast<const uint4*>(a.options + row));
+    return {__uint_as_float(x.x), static_cast<int32_t>(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
+}
 
 // A row: its vectors of four values from the first multiple of 16 bytes on, and up
 // to three values before them and behind.
@@ -157,100 +161,6 @@ __device__ __forceinline__ Source source_of(const Args& a, uint32_t row) {
     return {p, a.vocab, head, (a.vocab - head) / 4};
 }
 
-// A slice of it in the workgroup's registers, the first one's with the values outside
-// the vectors. (What is none of the row's is -infinity.)
-struct Held {
-    float4 x[kVectors];
-    float edge;
-    uint32_t id0, edge_id;
-    __device__ __forceinline__ void load(const Source& s, uint32_t slice) {
-        const uint32_t v0 = slice * kVectors * kThreads + threadIdx.x;
-        const float none = -__builtin_inff();
-        id0 = s.id(v0);
-#pragma unroll
-        for (uint32_t i = 0; i < kVectors; ++i) {
-            x[i] = make_float4(none, none, none, none);
-            if (v0 + i * kThreads < s.vectors) x[i] = s.load(v0 + i * kThreads);
-        }
-        edge = none;
-        edge_id = s.edge(threadIdx.x);
-        if (slice == 0 && threadIdx.x < s.edges()) edge = s.value(edge_id);
-    }
-    // f(value, id). (Through an empty asm, so that what one pass finds of the values
-    // and ids is not kept in registers for the next.)
-    template <typename F>
-    __device__ __forceinline__ void each(const F& f) {
-#pragma unroll
-        for (uint32_t i = 0; i < kVectors; ++i) {
-            asm volatile("" : "+v"(x[i].x), "+v"(x[i].y), "+v"(x[i].z), "+v"(x[i].w), "+v"(id0));
-            const uint32_t id = id0 + 4 * i * kThreads;
-            f(x[i].x, id);
-            f(x[i].y, id + 1);
-            f(x[i].z, id + 2);
-            f(x[i].w, id + 3);
-        }
-        f(edge, edge_id);
-    }
-    // The ids of the candidates in bins first .. last to the list, lds.listed of them:
-    // which they are as bits first, then one addition a wave for their places there.
-    __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
-        static_assert(4 * kVectors == 32);
-        uint32_t bits = 0, k = 0, at_edge = 0;
-        each([&](float l, uint32_t) {
-            const Turns t = turns_of(r, l);
-            const uint32_t b = bin_of(t), hit = t.candidate && b >= first && b <= last;
-            if (k < 32) bits |= hit << k++;
-            else at_edge = hit;
-        });
-        const uint32_t n = static_cast<uint32_t>(__builtin_popcount(bits)) + at_edge;
-        const uint32_t upto = static_cast<uint32_t>(inclusive_sum(static_cast<int32_t>(n))), all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), kWave - 1));
-        if (all == 0) return;
-        uint32_t base = 0;
-        if (threadIdx.x % kWave == 0) base = __hip_atomic_fetch_add(&lds.listed, all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(base))) + upto - n;
-        if (at_edge && to < kList) lds.id[to++] = edge_id;
-        for (; bits; bits &= bits - 1, ++to) {
-            const uint32_t i = static_cast<uint32_t>(__builtin_ctz(bits));
-            if (to < kList) lds.id[to] = id0 + 4 * (i / 4) * kThreads + i % 4;
-        }
-    }
-};
-
-// All of it, read again each time.
-struct Streamed {
-    Source s;
-    template <typename F>
-    __device__ __forceinline__ void each(const F& f) {
-        constexpr uint32_t kFlight = 2;
-        for (uint32_t v = threadIdx.x; v < s.vectors; v += kFlight * kThreads) {
-            float4 x[kFlight];
-#pragma unroll
-            for (uint32_t i = 0; i < kFlight; ++i) x[i] = s.load(min(v + i * kThreads, s.vectors - 1));
-#pragma unroll
-            for (uint32_t i = 0; i < kFlight; ++i) {
-                if (v + i * kThreads >= s.vectors) break;
-                const uint32_t id = s.id(v + i * kThreads);
-                f(x[i].x, id);
-                f(x[i].y, id + 1);
-                f(x[i].z, id + 2);
-                f(x[i].w, id + 3);
-            }
-        }
-        if (threadIdx.x < s.edges()) f(s.value(s.edge(threadIdx.x)), s.edge(threadIdx.x));
-    }
-    __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
-        each([&](float l, uint32_t id) {
-            const Turns t = turns_of(r, l);
-            const uint32_t b = bin_of(t);
-            if (!t.candidate || b < first || b > last) return;
-            const uint32_t to = __hip_atomic_fetch_add(&lds.listed, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            if (to < kList) lds.id[to] = id;
-        });
-    }
-};
-
-// ---------------------------------------------------------------- the workgroup together
-
 __device__ __forceinline__ uint64_t exchanged(uint64_t v, int o) {
     return static_cast<uint64_t>(static_cast<uint32_t>(__shfl_xor(static_cast<int>(v >> 32), o))) << 32 | static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), o));
 }
@@ -262,362 +172,539 @@ __device__ __forceinline__ uint64_t wave_min(uint64_t v) {
     }
     return v;
 }
-
-// The place of the largest of the values, kNone where there is none.
-template <typename V>
-__device__ __forceinline__ uint64_t first_of(V& values, Scratch& lds) {
-    float best = -__builtin_inff();
-    uint32_t id = 0;
-    values.each([&](float l, uint32_t i) {
-        if (l > best || (l == best && i < id)) best = l, id = i;
-    });
-    const uint64_t mine = wave_min(best > -__builtin_inff() ? place_of(best, id) : kNone);
-    if (threadIdx.x % kWave == 0) lds.wave_place[threadIdx.x / kWave] = mine;
-    __syncthreads();
-    uint64_t all = kNone;
-#pragma unroll 4
-    for (uint32_t i = 0; i < kWaves; ++i) all = lds.wave_place[i] < all ? lds.wave_place[i] : all;
-    return all;
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, uint32_t lane) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane))) << 32 |
+           static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
-
 __device__ __forceinline__ void add(uint64_t* to, uint64_t v) { __hip_atomic_fetch_add(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 __device__ __forceinline__ void add(uint32_t* to, uint32_t v) { __hip_atomic_fetch_add(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+__device__ __forceinline__ uint32_t taken(uint32_t* from, uint32_t n) { return __hip_atomic_fetch_add(from, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
 
-// Clears the bins; with a barrier after it.
-__device__ __forceinline__ void clear_bins(Scratch& lds) {
-    for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) lds.mass[i] = 0, lds.count[i] = 0;
-    if (threadIdx.x == 0) lds.likely = 0;
-    __syncthreads();
-}
-// The candidates' weights to the bins, or how many they are alone. A barrier has to
-// follow.
-template <bool MASS, bool COUNT, typename V>
-__device__ __forceinline__ void fill_bins(V& values, const Row& r, Scratch& lds) {
-    uint64_t likely = 0;
-    values.each([&](float l, uint32_t) {
-        const Turns t = turns_of(r, l);
-        if (!t.candidate) return;
-        const uint32_t b = bin_of(t);
-        if constexpr (COUNT) add(&lds.count[b], 1u);
-        if constexpr (MASS) {
+// ---------------------------------------------------------------- a workgroup's work on a row
+
+// Of kThreads threads, which hold kVectors vectors each of a slice.
+template <uint32_t kThreads>
+struct Picker {
+    static constexpr uint32_t kWaves = kThreads / kWave;
+    static constexpr uint32_t kFew = kThreads / 4;  // candidates that are ranked one by one, by four threads each
+
+    struct Scratch {
+        uint64_t mass[kBins];  // of a bin, then of it and those before
+        uint32_t count[kBins];
+        uint64_t place[kList], weight[kList];
+        union {
+            uint32_t id[kList];  // of what is listed, until its places are
+            struct {
+                uint64_t sub_mass[kSubs];
+                uint32_t sub_count[kSubs];
+            };
+        };
+        uint64_t few_place[kFew], few_weight[kFew];
+        uint64_t ranked_mass[kFew];  // of the ranked candidates up to each
+        uint32_t ranked_id[kFew];
+        uint64_t wave_mass[kWaves];
+        uint32_t wave_count[kWaves];
+        double table[kTurns];
+        uint64_t lo, hi, likely;  // a range of places; the mass within min_p
+        uint64_t found_mass, found_before;
+        uint32_t found, found_count, listed, lowest;
+    };
+
+    static __device__ __forceinline__ void fill_table(Scratch& lds) {
+        for (uint32_t i = threadIdx.x; i < kTurns; i += kThreads) lds.table[i] = exp2(-static_cast<double>(i) / kTurns);
+    }
+
+    // A slice in the workgroup's registers, the first one's with the values outside the
+    // vectors. (What is none of the row's is -infinity.)
+    struct Held {
+        float4 x[kVectors];
+        float edge;
+        uint32_t id0, edge_id;
+        __device__ __forceinline__ void load(const Source& s, uint32_t slice) {
+            const uint32_t v0 = slice * kVectors * kThreads + threadIdx.x;
+            const float none = -__builtin_inff();
+            id0 = s.id(v0);
+#pragma unroll
+            for (uint32_t i = 0; i < kVectors; ++i) {
+                x[i] = make_float4(none, none, none, none);
+                if (v0 + i * kThreads < s.vectors) x[i] = s.load(v0 + i * kThreads);
+            }
+            edge = none;
+            edge_id = s.edge(threadIdx.x);
+            if (slice == 0 && threadIdx.x < s.edges()) edge = s.value(edge_id);
+        }
+        // f(value, id). (Through an empty asm, so that what one pass finds of the values
+        // and ids is not kept in registers for the next.)
+        template <typename F>
+        __device__ __forceinline__ void each(const F& f) {
+#pragma unroll
+            for (uint32_t i = 0; i < kVectors; ++i) {
+                asm volatile("" : "+v"(x[i].x), "+v"(x[i].y), "+v"(x[i].z), "+v"(x[i].w), "+v"(id0));
+                const uint32_t id = id0 + 4 * i * kThreads;
+                f(x[i].x, id);
+                f(x[i].y, id + 1);
+                f(x[i].z, id + 2);
+                f(x[i].w, id + 3);
+            }
+            f(edge, edge_id);
+        }
+        __device__ __forceinline__ float largest() const {
+            float m = edge;
+#pragma unroll
+            for (uint32_t i = 0; i < kVectors; ++i) m = fmaxf(fmaxf(m, fmaxf(x[i].x, x[i].y)), fmaxf(x[i].z, x[i].w));
+            return m;
+        }
+        // The ids of the candidates in bins first .. last to the list, lds.listed of them:
+        // which they are as bits first, then one addition a wave for their places there.
+        __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
+            static_assert(4 * kVectors == 32);
+            uint32_t bits = 0, k = 0, at_edge = 0;
+            each([&](float l, uint32_t) {
+                const Turns t = turns_of(r, l);
+                const uint32_t b = bin_of(t), hit = t.candidate && b >= first && b <= last;
+                if (k < 32) bits |= hit << k++;
+                else at_edge = hit;
+            });
+            const uint32_t n = static_cast<uint32_t>(__builtin_popcount(bits)) + at_edge;
+            const uint32_t upto = static_cast<uint32_t>(inclusive_sum(static_cast<int32_t>(n))), all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), kWave - 1));
+            if (all == 0) return;
+            uint32_t base = 0;
+            if (threadIdx.x % kWave == 0) base = taken(&lds.listed, all);
+            uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(base))) + upto - n;
+            if (at_edge) {
+                if (to < kList) lds.id[to] = edge_id;
+                ++to;
+            }
+            for (; bits && to < kList; bits &= bits - 1, ++to) {
+                const uint32_t i = static_cast<uint32_t>(__builtin_ctz(bits));
+                lds.id[to] = id0 + 4 * (i / 4) * kThreads + i % 4;
+            }
+        }
+    };
+
+    // A row read again each time.
+    struct Streamed {
+        Source s;
+        template <typename F>
+        __device__ __forceinline__ void each(const F& f) {
+            constexpr uint32_t kFlight = 2;
+            for (uint32_t v = threadIdx.x; v < s.vectors; v += kFlight * kThreads) {
+                float4 x[kFlight];
+#pragma unroll
+                for (uint32_t i = 0; i < kFlight; ++i) x[i] = s.load(min(v + i * kThreads, s.vectors - 1));
+#pragma unroll
+                for (uint32_t i = 0; i < kFlight; ++i) {
+                    if (v + i * kThreads >= s.vectors) break;
+                    const uint32_t id = s.id(v + i * kThreads);
+                    f(x[i].x, id);
+                    f(x[i].y, id + 1);
+                    f(x[i].z, id + 2);
+                    f(x[i].w, id + 3);
+                }
+            }
+            if (threadIdx.x < s.edges()) f(s.value(s.edge(threadIdx.x)), s.edge(threadIdx.x));
+        }
+        __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
+            for (uint32_t i = 0; i * kVectors * kThreads < s.vectors || i == 0; ++i) {
+                Held h;
+                h.load(s, i);
+                h.list(r, first, last, lds);
+            }
+        }
+    };
+
+    // The largest of the threads' values.
+    static __device__ __forceinline__ float peak_of(float largest, Scratch& lds) {
+        const float m = wave_max(largest);
+        if (threadIdx.x % kWave == 0) lds.wave_count[threadIdx.x / kWave] = __float_as_uint(m);
+        __syncthreads();
+        float all = -__builtin_inff();
+#pragma unroll
+        for (uint32_t i = 0; i < kWaves; ++i) all = fmaxf(all, __uint_as_float(lds.wave_count[i]));
+        return all;
+    }
+    // The first id of those with the value peak, ~0 where there is none.
+    template <typename V>
+    static __device__ __forceinline__ uint32_t first_with(V& values, float peak, Scratch& lds) {
+        if (threadIdx.x == 0) lds.lowest = ~0u;
+        __syncthreads();
+        uint32_t id = ~0u;
+        values.each([&](float l, uint32_t i) {
+            if (l == peak) id = i < id ? i : id;
+        });
+        if (id != ~0u) __hip_atomic_fetch_min(&lds.lowest, id, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        __syncthreads();
+        return lds.lowest;
+    }
+
+    // Clears the bins; with a barrier after it.
+    static __device__ __forceinline__ void clear_bins(Scratch& lds) {
+        for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) lds.mass[i] = 0, lds.count[i] = 0;
+        if (threadIdx.x == 0) lds.likely = 0, lds.listed = 0;
+        __syncthreads();
+    }
+    // The candidates' weights to the bins. A barrier has to follow.
+    template <typename V>
+    static __device__ __forceinline__ void fill_bins(V& values, const Row& r, Scratch& lds) {
+        uint64_t likely = 0;
+        values.each([&](float l, uint32_t) {
+            const Turns t = turns_of(r, l);
+            if (!t.candidate) return;
+            const uint32_t b = bin_of(t);
             const uint64_t w = weight_of(r, t, lds.table);
+            add(&lds.count[b], 1u);
             add(&lds.mass[b], w);
             if (static_cast<double>(w) >= r.least) likely += w;
-        }
-    });
-    if (MASS && r.least > 0.0 && likely) add(&lds.likely, likely);
-}
+        });
+        if (r.least > 0.0 && likely) add(&lds.likely, likely);
+    }
 
-// What of N parts becomes that of the part and all before it. A barrier has to come
-// before; one comes after.
-template <uint32_t N, bool MASS, bool COUNT>
-__device__ __forceinline__ void sum_up(uint64_t* mass, uint32_t* count, Scratch& lds) {
-    constexpr uint32_t kEach = N / kThreads;
-    const uint32_t t = threadIdx.x, w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(t / kWave)));
-    uint64_t m[kEach], ms = 0, mi = 0;
-    uint32_t c[kEach], cs = 0, ci = 0;
+    // What of N parts becomes that of the part and all before it. A barrier has to come
+    // before; one comes after.
+    template <uint32_t N, bool MASS>
+    static __device__ __forceinline__ void sum_up(uint64_t* mass, uint32_t* count, Scratch& lds) {
+        constexpr uint32_t kEach = N / kThreads;
+        const uint32_t t = threadIdx.x, w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(t / kWave)));
+        uint64_t m[kEach], ms = 0, mi = 0;
+        uint32_t c[kEach], cs = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        if constexpr (MASS) ms = m[i] = ms + mass[kEach * t + i];
-        if constexpr (COUNT) cs = c[i] = cs + count[kEach * t + i];
-    }
-    if constexpr (MASS) mi = static_cast<uint64_t>(inclusive_sum(static_cast<int64_t>(ms)));
-    if constexpr (COUNT) ci = static_cast<uint32_t>(inclusive_sum(static_cast<int32_t>(cs)));
-    if (t % kWave == kWave - 1) lds.wave_mass[w] = mi, lds.wave_count[w] = ci;
-    __syncthreads();
-    // the sums of the waves before: a lane each, summed up by every wave
-    const uint32_t l = t % kWave % kWaves;
-    uint64_t m0 = 0;
-    uint32_t c0 = 0;
-    if constexpr (MASS) {
-        const uint64_t all = static_cast<uint64_t>(inclusive_sum(static_cast<int64_t>(lds.wave_mass[l])));
-        if (w > 0)
-            m0 = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all >> 32), w - 1))) << 32 |
-                 static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(all), w - 1));
-    }
-    if constexpr (COUNT) {
+        for (uint32_t i = 0; i < kEach; ++i) {
+            if constexpr (MASS) ms = m[i] = ms + mass[kEach * t + i];
+            cs = c[i] = cs + count[kEach * t + i];
+        }
+        if constexpr (MASS) mi = static_cast<uint64_t>(inclusive_sum(static_cast<int64_t>(ms)));
+        const uint32_t ci = static_cast<uint32_t>(inclusive_sum(static_cast<int32_t>(cs)));
+        if (t % kWave == kWave - 1) lds.wave_mass[w] = mi, lds.wave_count[w] = ci;
+        __syncthreads();
+        // the sums of the waves before: a lane each, summed up by every wave
+        const uint32_t l = t % kWave % kWaves;
+        uint64_t m0 = 0;
+        uint32_t c0 = 0;
+        if constexpr (MASS) {
+            const uint64_t all = static_cast<uint64_t>(inclusive_sum(static_cast<int64_t>(lds.wave_mass[l])));
+            if (w > 0) m0 = lane_of(all, w - 1);
+        }
         const int32_t all = inclusive_sum(static_cast<int32_t>(lds.wave_count[l]));
         if (w > 0) c0 = static_cast<uint32_t>(__builtin_amdgcn_readlane(all, w - 1));
-    }
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        if constexpr (MASS) mass[kEach * t + i] = m0 + mi - ms + m[i];
-        if constexpr (COUNT) count[kEach * t + i] = c0 + ci - cs + c[i];
+        for (uint32_t i = 0; i < kEach; ++i) {
+            if constexpr (MASS) mass[kEach * t + i] = m0 + mi - ms + m[i];
+            count[kEach * t + i] = c0 + ci - cs + c[i];
+        }
+        __syncthreads();
     }
-    __syncthreads();
-}
 
-// What is searched for: the candidate that `before` others come before, or that
-// holds unit `before` of the mass.
-struct Wanted {
-    bool by_count;
-    uint64_t before;
-};
+    // What is searched for: the candidate that `before` others come before, or that
+    // holds unit `before` of the mass.
+    struct Wanted {
+        bool by_count;
+        uint64_t before;
+    };
 
-// The part of n (summed up) that holds it: its number, and what comes before it.
-struct Part {
-    uint32_t i, count;       // count: in the part
-    uint64_t mass_before;
-    uint32_t count_before;
-};
-template <uint32_t N>
-__device__ __forceinline__ Part part_with(const uint64_t* mass, const uint32_t* count, Wanted x, Scratch& lds) {
+    // The part of N (summed up) that holds it: its number, what is in it, and what comes
+    // before it.
+    struct Part {
+        uint32_t i, count;
+        uint64_t mass_before;
+        uint32_t count_before;
+    };
+    template <uint32_t N>
+    static __device__ __forceinline__ Part part_with(const uint64_t* mass, const uint32_t* count, Wanted x, Scratch& lds) {
 #pragma unroll
-    for (uint32_t i = threadIdx.x; i < N; i += kThreads) {
-        const uint64_t m0 = i ? mass[i - 1] : 0;
-        const uint32_t c0 = i ? count[i - 1] : 0;
-        const bool here = x.by_count ? c0 <= x.before && x.before < count[i] : m0 <= x.before && x.before < mass[i];
-        if (here) lds.found = i, lds.found_count = count[i] - c0, lds.found_mass = m0, lds.found_before = c0;
+        for (uint32_t i = threadIdx.x; i < N; i += kThreads) {
+            const uint64_t m0 = i ? mass[i - 1] : 0;
+            const uint32_t c0 = i ? count[i - 1] : 0;
+            const bool here = x.by_count ? c0 <= x.before && x.before < count[i] : m0 <= x.before && x.before < mass[i];
+            if (here) lds.found = i, lds.found_count = count[i] - c0, lds.found_mass = m0, lds.found_before = c0;
+        }
+        __syncthreads();
+        const Part p{lds.found, lds.found_count, lds.found_mass, static_cast<uint32_t>(lds.found_before)};
+        __syncthreads();
+        return p;
     }
-    __syncthreads();
-    const Part p{lds.found, lds.found_count, lds.found_mass, static_cast<uint32_t>(lds.found_before)};
-    __syncthreads();
-    return p;
-}
 
-// What was found: its mass and all before it, and its id.
-struct Found {
-    uint64_t mass;
-    uint32_t id;
-};
+    // What was found: its mass and all before it, and its id.
+    struct Found {
+        uint64_t mass;
+        uint32_t id;
+    };
 
-// Which bins' candidates the list in the LDS holds all of.
-struct Listed {
-    uint32_t first = 1, last = 0, n = 0;
-};
-
-// The candidate with x before it, of those in bin b whose places are in lds.lo ..
-// lds.hi, n of them in all (visit(f): f(place, weight) for each that may be).
-template <typename Visit>
-__device__ __forceinline__ Found among(const Visit& visit, Wanted x, uint64_t lo, uint64_t hi, uint32_t n, uint64_t mass, Scratch& lds) {
-    // Ranges of a thousandth of the last, until few are in one. (Places are all
-    // different: the seventh at the latest is a place.)
-    for (int level = 0; n > kFew && level < 7; ++level) {
-        const int bits = 64 - __builtin_clzll(hi - lo | 1);
-        const int step = bits > 10 ? bits - 10 : 0;
-        lds.sub_mass[threadIdx.x] = 0;
-        lds.sub_count[threadIdx.x] = 0;
+    // The candidate with x before it, of those that visit(f) gives, f(place, weight), with
+    // places in lo .. hi, n of them in all; mass: what comes before these.
+    template <typename Visit>
+    static __device__ __forceinline__ Found among(const Visit& visit, Wanted x, uint64_t lo, uint64_t hi, uint32_t n, uint64_t mass, Scratch& lds) {
+        // Ranges of a thousandth of the last, until few are in one. (Places are all
+        // different: the seventh at the latest is a place.)
+        for (int level = 0; n > kFew && level < 7; ++level) {
+            const int bits = 64 - __builtin_clzll(hi - lo | 1);
+            const int step = bits > 10 ? bits - 10 : 0;
+            for (uint32_t i = threadIdx.x; i < kSubs; i += kThreads) lds.sub_mass[i] = 0, lds.sub_count[i] = 0;
+            __syncthreads();
+            visit([&](uint64_t at, uint64_t w) {
+                if (at < lo || at > hi) return;
+                const uint32_t i = static_cast<uint32_t>((at - lo) >> step);
+                add(&lds.sub_mass[i], w);
+                add(&lds.sub_count[i], 1u);
+            });
+            __syncthreads();
+            sum_up<kSubs, true>(lds.sub_mass, lds.sub_count, lds);
+            const Part p = part_with<kSubs>(lds.sub_mass, lds.sub_count, x, lds);
+            mass += p.mass_before;
+            x.before -= x.by_count ? p.count_before : p.mass_before;
+            n = p.count;
+            lo += static_cast<uint64_t>(p.i) << step;
+            const uint64_t end = lo + ((1ull << step) - 1);
+            hi = end < hi ? end : hi;
+        }
+        if (threadIdx.x == 0) lds.listed = 0;
         __syncthreads();
         visit([&](uint64_t at, uint64_t w) {
             if (at < lo || at > hi) return;
-            const uint32_t i = static_cast<uint32_t>((at - lo) >> step);
-            add(&lds.sub_mass[i], w);
-            add(&lds.sub_count[i], 1u);
+            const uint32_t i = taken(&lds.listed, 1);
+            if (i < kFew) lds.few_place[i] = at, lds.few_weight[i] = w;
         });
         __syncthreads();
-        sum_up<kSubs, true, true>(lds.sub_mass, lds.sub_count, lds);
-        const Part p = part_with<kSubs>(lds.sub_mass, lds.sub_count, x, lds);
-        mass += p.mass_before;
-        x.before -= x.by_count ? p.count_before : p.mass_before;
-        n = p.count;
-        lo += static_cast<uint64_t>(p.i) << step;
-        const uint64_t end = lo + ((1ull << step) - 1);
-        hi = end < hi ? end : hi;
-    }
-    if (threadIdx.x == 0) lds.listed = 0;
-    __syncthreads();
-    visit([&](uint64_t at, uint64_t w) {
-        if (at < lo || at > hi) return;
-        const uint32_t i = __hip_atomic_fetch_add(&lds.listed, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        if (i < kFew) lds.few_place[i] = at, lds.few_weight[i] = w;
-    });
-    __syncthreads();
-    // Eight threads a candidate count those before it.
-    const uint32_t j = threadIdx.x / 8;
-    n = min(n, kFew);
-    if (j < n) {
-        const uint64_t at = lds.few_place[j];
-        uint64_t m = 0, c = 0;
-        for (uint32_t i = threadIdx.x % 8; i < n; i += 8)
-            if (lds.few_place[i] < at) m += lds.few_weight[i], ++c;
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) m += exchanged(m, o), c += exchanged(c, o);
-        const uint64_t w = lds.few_weight[j];
-        const bool here = x.by_count ? c == x.before : m <= x.before && x.before < m + w;
-        if (here && threadIdx.x % 8 == 0) lds.found_mass = mass + m + w, lds.found = static_cast<uint32_t>(at);
-    }
-    __syncthreads();
-    const Found f{lds.found_mass, lds.found};
-    __syncthreads();
-    return f;
-}
-
-// The candidates of bins first .. last, n of them, to the list.
-template <typename V>
-__device__ __forceinline__ void list_bins(V& values, const Source& source, const Row& r, const Listed& listed, Scratch& lds) {
-    if (threadIdx.x == 0) lds.listed = 0;
-    __syncthreads();
-    values.list(r, listed.first, listed.last, lds);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
-        const uint32_t id = lds.id[i];
-        const float l = source.value(id);
-        lds.place[i] = place_of(l, id);
-        lds.weight[i] = weight_of(r, turns_of(r, l), lds.table);
-    }
-    __syncthreads();
-}
-
-// The candidate with x before it, in the bins' sums and the row's values.
-template <typename V>
-__device__ __forceinline__ Found find(V& values, Streamed again, const Row& r, Wanted x, Listed& listed, Scratch& lds) {
-    const Part p = part_with<kBins>(lds.mass, lds.count, x, lds);
-    x.before -= x.by_count ? p.count_before : p.mass_before;
-    const uint32_t b = p.i;
-    if (p.count <= kList && !(listed.first <= b && b <= listed.last)) {
-        // The bin's candidates to the list, and all before them if they fit too.
-        const bool all = p.count_before + p.count <= kList;
-        listed = {all ? 0 : b, b, all ? p.count_before + p.count : p.count};
-        list_bins(values, again.s, r, listed, lds);
-    }
-    const bool from_list = listed.first <= b && b <= listed.last;
-    const auto visit = [&](const auto& f) {  // (more than the list holds: they are read again)
-        if (from_list) {
-            for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
-                const Turns t = turns_of(r, logit_at(lds.place[i]));
-                if (bin_of(t) == b) f(lds.place[i], lds.weight[i]);
-            }
-        } else {
-            again.each([&](float l, uint32_t id) {
-                const Turns t = turns_of(r, l);
-                if (t.candidate && bin_of(t) == b) f(place_of(l, id), weight_of(r, t, lds.table));
-            });
+        const uint32_t j = threadIdx.x / 4;
+        if (j < min(n, kFew)) {
+            const Ranked k = ranked(lds.few_place, lds.few_weight, j, min(n, kFew));
+            const bool here = x.by_count ? k.before == x.before : k.mass <= x.before && x.before < k.mass + lds.few_weight[j];
+            if (here && threadIdx.x % 4 == 0) lds.found_mass = mass + k.mass + lds.few_weight[j], lds.found = static_cast<uint32_t>(lds.few_place[j]);
         }
+        __syncthreads();
+        const Found f{lds.found_mass, lds.found};
+        __syncthreads();
+        return f;
+    }
+
+    // How many of n come before the j-th, and their mass, by four threads.
+    struct Ranked {
+        uint32_t before;
+        uint64_t mass;
     };
-    uint64_t lo = kNone, hi = 0;
-    if (p.count > kFew) {  // how far apart the bin's are
-        if (threadIdx.x == 0) lds.lo = kNone, lds.hi = 0;
-        __syncthreads();
-        visit([&](uint64_t at, uint64_t) {
-            lo = at < lo ? at : lo;
-            hi = at > hi ? at : hi;
-        });
-        lo = wave_min(lo);
-        hi = ~wave_min(~hi);
-        if (threadIdx.x % kWave == 0) {
-            __hip_atomic_fetch_min(&lds.lo, lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            __hip_atomic_fetch_max(&lds.hi, hi, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    static __device__ __forceinline__ Ranked ranked(const uint64_t* places, const uint64_t* weights, uint32_t j, uint32_t n) {
+        const uint64_t at = places[j];
+        uint64_t m = 0;
+        uint32_t c = 0;
+        for (uint32_t i = threadIdx.x % 4; i < n; i += 4)
+            if (places[i] < at) m += weights[i], ++c;
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) m += exchanged(m, o), c += static_cast<uint32_t>(__shfl_xor(static_cast<int>(c), o));
+        return {c, m};
+    }
+
+    // Which bins' candidates the list in the LDS holds all of.
+    struct Listed {
+        uint32_t first = 1, last = 0, n = 0;
+    };
+
+    // The places and weights of the n listed ids. With a barrier after it.
+    static __device__ __forceinline__ void weigh_listed(const Source& source, const Row& r, uint32_t n, Scratch& lds) {
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const uint32_t id = lds.id[i];
+            const float l = source.value(id);
+            lds.place[i] = place_of(l, id);
+            lds.weight[i] = weight_of(r, turns_of(r, l), lds.table);
         }
         __syncthreads();
-        lo = lds.lo;
-        hi = lds.hi;
-    } else {
-        lo = 0;
-        hi = kNone;
     }
-    return among(visit, x, lo, hi, p.count, p.mass_before, lds);
-}
 
-// Whether a row's candidates are only counted at first: those that top_k keeps are
-// then few enough to be listed, and the others need no weight.
-__device__ __forceinline__ bool counts_first(const vkml_sampling& o) { return o.top_k > 0 && static_cast<uint32_t>(o.top_k) <= kList / 2; }
+    // The candidate with x before it, in the bins' sums and the row's values.
+    static __device__ __forceinline__ Found find(Streamed values, const Row& r, Wanted x, Listed& listed, Scratch& lds) {
+        const Part p = part_with<kBins>(lds.mass, lds.count, x, lds);
+        x.before -= x.by_count ? p.count_before : p.mass_before;
+        const uint32_t b = p.i;
+        if (p.count <= kList && !(listed.first <= b && b <= listed.last)) {
+            // The bin's candidates to the list, and all before them if they fit too.
+            const bool all = p.count_before + p.count <= kList;
+            listed = {all ? 0 : b, b, all ? p.count_before + p.count : p.count};
+            if (threadIdx.x == 0) lds.listed = 0;
+            __syncthreads();
+            values.list(r, listed.first, listed.last, lds);
+            __syncthreads();
+            weigh_listed(values.s, r, listed.n, lds);
+        }
+        const bool from_list = listed.first <= b && b <= listed.last;
+        const auto visit = [&](const auto& f) {  // (more than the list holds: they are read again)
+            if (from_list) {
+                for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
+                    const Turns t = turns_of(r, logit_at(lds.place[i]));
+                    if (bin_of(t) == b) f(lds.place[i], lds.weight[i]);
+                }
+            } else {
+                values.each([&](float l, uint32_t id) {
+                    const Turns t = turns_of(r, l);
+                    if (t.candidate && bin_of(t) == b) f(place_of(l, id), weight_of(r, t, lds.table));
+                });
+            }
+        };
+        uint64_t lo = 0, hi = kNone;
+        if (p.count > kFew) {  // how far apart the bin's are
+            if (threadIdx.x == 0) lds.lo = kNone, lds.hi = 0;
+            __syncthreads();
+            lo = kNone, hi = 0;
+            visit([&](uint64_t at, uint64_t) {
+                lo = at < lo ? at : lo;
+                hi = at > hi ? at : hi;
+            });
+            lo = wave_min(lo);
+            hi = ~wave_min(~hi);
+            if (threadIdx.x % kWave == 0) {
+                __hip_atomic_fetch_min(&lds.lo, lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                __hip_atomic_fetch_max(&lds.hi, hi, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+            __syncthreads();
+            lo = lds.lo;
+            hi = lds.hi;
+        }
+        return among(visit, x, lo, hi, p.count, p.mass_before, lds);
+    }
 
-// After the counts alone: weights of those that top_k keeps, and what else is in
-// their bins; or of all, where these are more than the list holds. The bins are then
-// as if all had theirs, up to the last that top_k asks for.
-template <typename V>
-__device__ __forceinline__ void weigh_counted(V& values, const Source& source, const Row& r, const vkml_sampling& o, Listed& listed, Scratch& lds) {
-    const uint32_t count = lds.count[kBins - 1], k = min(static_cast<uint32_t>(o.top_k), count);
-    const Part p = part_with<kBins>(lds.mass, lds.count, {true, k - 1}, lds);
-    if (p.count_before + p.count <= kList) {
-        listed = {0, p.i, p.count_before + p.count};
-        list_bins(values, source, r, listed, lds);
+    // The pick of a row whose bins are filled; n: of the candidates that are listed, more
+    // than kList where none are.
+    static __device__ __forceinline__ uint32_t pick(const Streamed& values, const Row& r, const vkml_sampling& o, double random, uint32_t n, Scratch& lds) {
+        sum_up<kBins, true>(lds.mass, lds.count, lds);
+        Listed listed;
+        if (n <= kList) listed = {0, kBins - 1, n};
+        uint64_t mass = lds.mass[kBins - 1];
+        const uint32_t count = lds.count[kBins - 1];
+        // top_k, top_p, the draw: each looks for a candidate by what the one before leaves
+#pragma unroll 1
+        for (int step = 0;; ++step) {
+            Wanted x{false, 0};
+            if (step == 0) {
+                if (o.top_k <= 0 || static_cast<uint32_t>(o.top_k) >= count) continue;
+                x = {true, static_cast<uint64_t>(o.top_k - 1)};
+            } else if (step == 1) {
+                if (!(o.top_p < 1.0f)) continue;
+                x.before = reach_of(o.top_p, mass) - 1;  // the last unit that top_p asks for
+            } else {
+                mass = within(r, mass, lds.likely);
+                x.before = unit_of(random, mass);
+            }
+            const Found f = find(values, r, x, listed, lds);
+            if (step == 2) return f.id;
+            mass = f.mass;
+        }
+    }
+
+    // The same of n candidates that are listed, up to kFew: all ranked, then looked for
+    // by halves.
+    static __device__ __forceinline__ uint32_t pick_few(const Row& r, const vkml_sampling& o, double random, uint32_t n, Scratch& lds) {
+        const uint32_t j = threadIdx.x / 4;
+        if (j < n) {
+            const Ranked k = ranked(lds.place, lds.weight, j, n);
+            if (threadIdx.x % 4 == 0) lds.ranked_mass[k.before] = k.mass + lds.weight[j], lds.ranked_id[k.before] = static_cast<uint32_t>(lds.place[j]);
+        }
+        __syncthreads();
+        const auto holds = [&](uint64_t unit) {  // the first whose mass and all before it pass it
+            uint32_t lo = 0, hi = n - 1;
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) / 2;
+                if (lds.ranked_mass[mid] > unit) hi = mid;
+                else lo = mid + 1;
+            }
+            return lo;
+        };
+        const uint32_t k = o.top_k > 0 && static_cast<uint32_t>(o.top_k) < n ? static_cast<uint32_t>(o.top_k) : n;
+        uint64_t mass = lds.ranked_mass[k - 1];
+        if (o.top_p < 1.0f) mass = lds.ranked_mass[holds(reach_of(o.top_p, mass) - 1)];
+        mass = within(r, mass, lds.likely);
+        return lds.ranked_id[holds(unit_of(random, mass))];
+    }
+
+    // Whether the candidates that top_k or min_p keep are listed first.
+    static __device__ __forceinline__ bool lists_first(const Row& r, const vkml_sampling& o) {
+        return (o.top_k > 0 && static_cast<uint32_t>(o.top_k) <= kThreads) || !r.all;
+    }
+    // Lists them, and what else is in their bins: the ids, lds.listed of them (more than
+    // the list holds: some). Largest: of the thread's values. The counts are as they were,
+    // 0, and lds.listed has to be. With a barrier after it.
+    static __device__ __forceinline__ void list_kept(Held& values, float largest, const Row& r, const vkml_sampling& o, Scratch& lds) {
+        uint32_t last = kBins - 1;
+        if (o.top_k > 0 && static_cast<uint32_t>(o.top_k) <= kThreads) {
+            const Turns t = turns_of(r, largest);
+            if (t.candidate) add(&lds.count[bin_of(t)], 1u);
+            __syncthreads();
+            sum_up<kBins, false>(lds.mass, lds.count, lds);
+            const uint32_t most = lds.count[kBins - 1], k = static_cast<uint32_t>(o.top_k);
+            if (k <= most) last = part_with<kBins>(lds.mass, lds.count, {true, k - 1}, lds).i;
+            else __syncthreads();
+            for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) lds.count[i] = 0;
+        }
+        values.list(r, 0, last, lds);
+        __syncthreads();
+    }
+    // The n listed candidates, weighed: their mass within min_p, and where they are more
+    // than few, their bins. With a barrier after it.
+    static __device__ __forceinline__ void bin_listed(const Row& r, uint32_t n, Scratch& lds) {
         uint64_t likely = 0;
-        for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             const uint64_t w = lds.weight[i];
-            add(&lds.mass[bin_of(turns_of(r, logit_at(lds.place[i])))], w);
             if (static_cast<double>(w) >= r.least) likely += w;
+            if (n > kFew) {
+                const uint32_t b = bin_of(turns_of(r, logit_at(lds.place[i])));
+                add(&lds.count[b], 1u);
+                add(&lds.mass[b], w);
+            }
         }
         if (r.least > 0.0 && likely) add(&lds.likely, likely);
-    } else {
-        fill_bins<true, false>(values, r, lds);
+        __syncthreads();
     }
-    __syncthreads();
-    sum_up<kBins, true, false>(lds.mass, lds.count, lds);
-}
-
-// The pick of a row whose bins are summed up.
-template <typename V>
-__device__ __forceinline__ uint32_t pick(V& values, const Streamed& again, const Row& r, const vkml_sampling& o, double random, Listed listed, Scratch& lds) {
-    uint64_t mass = lds.mass[kBins - 1];
-    const uint32_t count = lds.count[kBins - 1];
-    // top_k, top_p, the draw: each looks for a candidate by what the one before leaves
-#pragma unroll 1
-    for (int step = 0;; ++step) {
-        Wanted x{false, 0};
-        if (step == 0) {
-            if (o.top_k <= 0 || static_cast<uint32_t>(o.top_k) >= count) continue;
-            x = {true, static_cast<uint64_t>(o.top_k - 1)};
-        } else if (step == 1) {
-            if (!(o.top_p < 1.0f)) continue;
-            // the fewest whose mass reaches top_p of it: up to the one that holds the last unit of that
-            const double share = __builtin_ceil(static_cast<double>(fmaxf(o.top_p, 0.0f)) * static_cast<double>(mass));
-            const uint64_t least = static_cast<uint64_t>(share);
-            x.before = (least < 1 ? 1 : least < mass ? least : mass) - 1;
-        } else {
-            if (r.least > 0.0) {
-                const uint64_t likely = lds.likely < (1ull << r.shift) ? 1ull << r.shift : lds.likely;  // the first at least
-                mass = likely < mass ? likely : mass;
-            }
-            const double at = random * static_cast<double>(mass);
-            const uint64_t unit = at > 0.0 ? (at < 9.2e18 ? static_cast<uint64_t>(at) : mass) : 0;
-            x.before = unit < mass ? unit : mass - 1;
-        }
-        const Found f = find(values, again, r, x, listed, lds);
-        if (step == 2) return f.id;
-        mass = f.mass;
-    }
-}
-
-__device__ __forceinline__ bool greedy(const vkml_sampling& o) { return !(o.temperature > 0.0f) || o.top_k == 1; }
-__device__ __forceinline__ vkml_sampling options_of(const Args& a, uint32_t row) {
-    const uint4 x = ldg(reinterpret_cast<const uint4*>(a.options + row));
-    return {__uint_as_float(x.x), static_cast<int32_t>(x.y), __uint_as_float(x.z), __uint_as_float(x.w)};
-}
+};
 
 // ---------------------------------------------------------------- the launches
 
 // Rows of one slice: a workgroup a row, its values in registers.
+template <uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
-    __shared__ Scratch lds;
+    using P = Picker<kThreads>;
+    __shared__ typename P::Scratch lds;
     const uint32_t row = blockIdx.x;
     const vkml_sampling o = options_of(a, row);
-    Held values;
-    values.load(source_of(a, row), 0);
-    fill_table(lds);
-    clear_bins(lds);
-    const uint64_t first = first_of(values, lds);
-    if (first == kNone || greedy(o)) {
-        if (threadIdx.x == 0) stg(a.tokens + row, first == kNone ? -1 : static_cast<int32_t>(first));
-        return;
-    }
-    const Row r = row_of(logit_at(first), o, a.shift);
-    const Streamed again{source_of(a, row)};
-    Listed listed;
-    if (counts_first(o)) {
-        fill_bins<false, true>(values, r, lds);
-        __syncthreads();
-        sum_up<kBins, false, true>(lds.mass, lds.count, lds);
-        weigh_counted(values, again.s, r, o, listed, lds);
+    const typename P::Streamed again{source_of(a, row)};
+    typename P::Held values;
+    values.load(again.s, 0);
+    P::fill_table(lds);
+    P::clear_bins(lds);
+    const float largest = values.largest(), peak = P::peak_of(largest, lds);
+    uint32_t id = ~0u;  // -1
+    if (!(peak > -__builtin_inff())) {
+    } else if (greedy(o)) {
+        id = P::first_with(values, peak, lds);
     } else {
-        fill_bins<true, true>(values, r, lds);
-        __syncthreads();
-        sum_up<kBins, true, true>(lds.mass, lds.count, lds);
+        const Row r = row_of(peak, o, a.shift);
+        const double random = a.random[row];
+        uint32_t n = kList + 1;
+        if (P::lists_first(r, o)) {
+            P::list_kept(values, largest, r, o, lds);
+            n = lds.listed;
+        }
+        if (n <= kList) {
+            P::weigh_listed(again.s, r, n, lds);
+            P::bin_listed(r, n, lds);
+        } else {
+            P::fill_bins(values, r, lds);
+            __syncthreads();
+        }
+        id = n <= P::kFew ? P::pick_few(r, o, random, n, lds) : P::pick(again, r, o, random, n, lds);
     }
-    const uint32_t id = pick(values, again, r, o, a.random[row], listed, lds);
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
 
-// Longer rows: their slices' largest, then their slices' bins, then the picks.
-__global__ void __launch_bounds__(kThreads) k_sample_peaks(Args a) {
-    __shared__ Scratch lds;
-    Held values;
+// Longer rows: their slices' largest, then what of the slices the picks need, then
+// the picks.
+using Wide = Picker<kWideThreads>;
+
+__global__ void __launch_bounds__(kWideThreads) k_sample_peaks(Args a) {
+    __shared__ Wide::Scratch lds;
+    Wide::Held values;
     values.load(source_of(a, blockIdx.x / a.slices), blockIdx.x % a.slices);
-    const uint64_t first = first_of(values, lds);
-    if (threadIdx.x == 0) stg(a.peaks + blockIdx.x, first);
+    const float peak = Wide::peak_of(values.largest(), lds);
+    const uint32_t id = greedy(options_of(a, blockIdx.x / a.slices)) ? Wide::first_with(values, peak, lds) : 0;
+    if (threadIdx.x == 0) stg(a.peaks + blockIdx.x, peak > -__builtin_inff() ? place_of(peak, id) : kNone);
 }
 
-__device__ __forceinline__ uint64_t peak_of(const Args& a, uint32_t row) {
+__device__ __forceinline__ uint64_t first_of(const Args& a, uint32_t row) {
     uint64_t first = kNone;
     for (uint32_t i = 0; i < a.slices; ++i) {
         const uint64_t p = ldg(a.peaks + static_cast<uint64_t>(row) * a.slices + i);
@@ -626,56 +713,83 @@ __device__ __forceinline__ uint64_t peak_of(const Args& a, uint32_t row) {
     return first;
 }
 
-__global__ void __launch_bounds__(kThreads) k_sample_sums(Args a) {
-    __shared__ Scratch lds;
+__global__ void __launch_bounds__(kWideThreads) k_sample_slices(Args a) {
+    __shared__ Wide::Scratch lds;
     const uint32_t row = blockIdx.x / a.slices;
     const vkml_sampling o = options_of(a, row);
-    const uint64_t first = peak_of(a, row);
+    const uint64_t first = first_of(a, row);
     if (first == kNone || greedy(o)) return;
-    Held values;
-    values.load(source_of(a, row), blockIdx.x % a.slices);
-    fill_table(lds);
-    clear_bins(lds);
+    const Source source = source_of(a, row);
+    Wide::Held values;
+    values.load(source, blockIdx.x % a.slices);
     const Row r = row_of(logit_at(first), o, a.shift);
-    if (counts_first(o)) fill_bins<false, true>(values, r, lds);
-    else fill_bins<true, true>(values, r, lds);
+    Wide::clear_bins(lds);
+    Slice* to = a.parts + blockIdx.x;
+    if (Wide::lists_first(r, o)) {
+        Wide::list_kept(values, values.largest(), r, o, lds);
+        const uint32_t n = lds.listed;
+        if (threadIdx.x == 0) stg(&to->listed, n);
+        if (n > kList) return;
+        for (uint32_t i = threadIdx.x; i < n; i += kWideThreads) stg(to->id + i, lds.id[i]);
+        return;
+    }
+    Wide::fill_table(lds);
     __syncthreads();
-    SliceSums* to = a.sums + blockIdx.x;
-    for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
+    Wide::fill_bins(values, r, lds);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
     if (threadIdx.x == 0) stg(&to->likely, lds.likely);
 }
 
-__global__ void __launch_bounds__(kThreads) k_sample_pick(Args a) {
-    __shared__ Scratch lds;
+__global__ void __launch_bounds__(kWideThreads) k_sample_pick(Args a) {
+    __shared__ Wide::Scratch lds;
     const uint32_t row = blockIdx.x;
     const vkml_sampling o = options_of(a, row);
-    const uint64_t first = peak_of(a, row);
-    if (first == kNone || greedy(o)) {
-        if (threadIdx.x == 0) stg(a.tokens + row, first == kNone ? -1 : static_cast<int32_t>(first));
-        return;
+    const uint64_t first = first_of(a, row);
+    uint32_t id = ~0u;  // -1
+    if (first == kNone) {
+    } else if (greedy(o)) {
+        id = static_cast<uint32_t>(first);
+    } else {
+        const Row r = row_of(logit_at(first), o, a.shift);
+        const double random = a.random[row];
+        Wide::Streamed values{source_of(a, row)};
+        const Slice* from = a.parts + static_cast<uint64_t>(row) * a.slices;
+        Wide::fill_table(lds);
+        Wide::clear_bins(lds);
+        uint32_t n = kList + 1;
+        const bool lists = Wide::lists_first(r, o);
+        if (lists) {
+            n = 0;
+            for (uint32_t s = 0; s < a.slices; ++s) {
+                const uint32_t of = ldg(&from[s].listed);
+                for (uint32_t i = threadIdx.x; i < of && n + i < kList; i += kWideThreads) lds.id[n + i] = ldg(from[s].id + i);
+                n = min(n + of, kList + 1);
+            }
+            __syncthreads();
+        }
+        if (n <= kList) {
+            Wide::weigh_listed(values.s, r, n, lds);
+            Wide::bin_listed(r, n, lds);
+        } else if (lists) {
+            Wide::fill_bins(values, r, lds);
+            __syncthreads();
+        } else {
+            for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) {
+                uint64_t m = 0;
+                uint32_t c = 0;
+                for (uint32_t s = 0; s < a.slices; ++s) m += ldg(from[s].mass + i), c += ldg(from[s].count + i);
+                lds.mass[i] = m, lds.count[i] = c;
+            }
+            if (threadIdx.x == 0) {
+                uint64_t likely = 0;
+                for (uint32_t s = 0; s < a.slices; ++s) likely += ldg(&from[s].likely);
+                lds.likely = likely;
+            }
+            __syncthreads();
+        }
+        id = n <= Wide::kFew ? Wide::pick_few(r, o, random, n, lds) : Wide::pick(values, r, o, random, n, lds);
     }
-    fill_table(lds);
-    const SliceSums* from = a.sums + static_cast<uint64_t>(row) * a.slices;
-    for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) {
-        uint64_t m = 0;
-        uint32_t c = 0;
-        for (uint32_t s = 0; s < a.slices; ++s) m += ldg(from[s].mass + i), c += ldg(from[s].count + i);
-        lds.mass[i] = m, lds.count[i] = c;
-    }
-    if (threadIdx.x == 0) {
-        uint64_t likely = 0;
-        for (uint32_t s = 0; s < a.slices; ++s) likely += ldg(&from[s].likely);
-        lds.likely = likely;
-    }
-    __syncthreads();
-    sum_up<kBins, true, true>(lds.mass, lds.count, lds);
-    const Row r = row_of(logit_at(first), o, a.shift);
-    Streamed values{source_of(a, row)};
-    Listed listed;
-    if (counts_first(o)) {
-        weigh_counted(values, values.s, r, o, listed, lds);  // (no mass in the bins yet)
-    }
-    const uint32_t id = pick(values, values, r, o, a.random[row], listed, lds);
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
 
@@ -705,21 +819,22 @@ int vkml_sample(const vkml_sample_params* p, const float* logits, const vkml_sam
     a.slices = slices(p->vocab);
     if (a.slices > 1) {
         a.peaks = static_cast<uint64_t*>(workspace);
-        a.sums = reinterpret_cast<SliceSums*>(static_cast<uint8_t*>(workspace) + peaks_bytes(*p));
+        a.parts = reinterpret_cast<Slice*>(static_cast<uint8_t*>(workspace) + peaks_bytes(*p));
     }
     // a row's weights fit 62 bits, one of them 51
     int32_t bits = 0;
     while ((1u << bits) < p->vocab) ++bits;
     a.shift = 62 - bits < 51 ? 62 - bits : 51;
     vkml::abi::ProfileScope prof("sample");
-    const auto go = [&](auto kernel, uint32_t workgroups) {
-        hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kThreads), 0, vkml::abi::stream(), a);
+    const auto go = [&](auto kernel, uint32_t workgroups, uint32_t threads) {
+        hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(threads), 0, vkml::abi::stream(), a);
         return vkml::abi::check_launch("sample");
     };
-    if (a.slices == 1) return go(k_sample, p->rows);
-    if (const int r = go(k_sample_peaks, p->rows * a.slices)) return r;
-    if (const int r = go(k_sample_sums, p->rows * a.slices)) return r;
-    return go(k_sample_pick, p->rows);
+    if (p->vocab <= kNarrowRow) return go(k_sample<kNarrowThreads>, p->rows, kNarrowThreads);
+    if (a.slices == 1) return go(k_sample<kWideThreads>, p->rows, kWideThreads);
+    if (const int r = go(k_sample_peaks, p->rows * a.slices, kWideThreads)) return r;
+    if (const int r = go(k_sample_slices, p->rows * a.slices, kWideThreads)) return r;
+    return go(k_sample_pick, p->rows, kWideThreads);
 }
 
 }  // extern "C"

@@ -9,10 +9,14 @@
 
 namespace vkml::sample {
 
-constexpr uint32_t kThreads = 1024;
-constexpr uint32_t kVectors = 8;                         // of four values, a thread's of a slice
-constexpr uint32_t kSlice = 4 * kVectors * kThreads;     // values a workgroup holds in registers
-constexpr uint32_t kBins = 2048;
+// A workgroup holds a slice of a row, or the whole, in registers: so many threads,
+// vectors of four values each.
+constexpr uint32_t kWideThreads = 1024, kNarrowThreads = 256;
+constexpr uint32_t kVectors = 8;
+constexpr uint32_t kSlice = 4 * kVectors * kWideThreads;
+constexpr uint32_t kNarrowRow = 4 * kVectors * kNarrowThreads;  // rows up to that many take the narrow one
+constexpr uint32_t kBins = 2048;  // of weights
+constexpr uint32_t kList = 2048;  // candidates in the LDS
 constexpr uint32_t kMaxVocab = 1u << 22;
 constexpr uint32_t kMaxSlices = 1u << 21;
 
@@ -27,17 +31,24 @@ inline const char* check(const vkml_sample_params& p) {
     return nullptr;
 }
 
-// What a row of several slices keeps: a slice's largest, its sums and counts by
-// bin, and its mass past min_p.
-struct SliceSums {
-    uint64_t mass[kBins];
-    uint32_t count[kBins];
+// What a row of several slices keeps of one: its weights and counts by bin and its
+// mass within min_p; or the ids of the candidates that top_k or min_p leave of it,
+// more than kList where these are not all.
+struct Slice {
+    union {
+        uint64_t mass[kBins];
+        uint32_t id[kList];
+    };
+    union {
+        uint32_t count[kBins];
+        uint32_t listed;
+    };
     uint64_t likely;
 };
 inline uint64_t peaks_bytes(const vkml_sample_params& p) { return (static_cast<uint64_t>(p.rows) * slices(p.vocab) * 8 + 15) / 16 * 16; }
 inline uint64_t workspace_bytes(const vkml_sample_params& p) {
     const uint64_t n = slices(p.vocab);
-    return n == 1 ? 0 : peaks_bytes(p) + static_cast<uint64_t>(p.rows) * n * sizeof(SliceSums);
+    return n == 1 ? 0 : peaks_bytes(p) + static_cast<uint64_t>(p.rows) * n * sizeof(Slice);
 }
 
 }  // namespace vkml::sample
