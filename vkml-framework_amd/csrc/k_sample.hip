@@ -17,7 +17,7 @@
 // Weights are whole numbers, units of 2^-shift of the largest (45 bits for 2^17
 // logits, so that all of a row's fit 62 bits): sums of them are exact in any order,
 // so that the same row gives the same token whatever the atomics' order. e^x is
-// found in 64 bits, 2^(-n / 512) from a table times a polynomial of degree 4, good to
+// found in 64 bits, 2^(-n / 1024) from a table times a polynomial of degree 3, good to
 // 2^-50: the picks are those of sums in f64 unless a border is nearer than that.
 #include <hip/hip_runtime.h>
 
@@ -34,9 +34,10 @@ namespace {
 
 constexpr uint32_t kSubs = 1024;  // parts of a range of candidates
 constexpr uint64_t kNone = ~0ull;
-constexpr int32_t kTurns = 512;   // to a factor of two between weights
-constexpr int32_t kBinTurns = 16;
+constexpr int32_t kTurnsLog2 = 10, kTurns = 1 << kTurnsLog2;  // to a factor of two between weights
+constexpr int32_t kBinTurns = 32;
 static_assert(kTurns / kBinTurns * 53 <= kBins);
+constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: a sum with it is whole, in the low bits
 
 struct Args {
     const float* logits;
@@ -64,55 +65,92 @@ __device__ __forceinline__ float logit_at(uint64_t place) {
 
 // ---------------------------------------------------------------- weights
 
+// More turns below the largest than any that is within min_p.
+__device__ __forceinline__ double likely_turns(const vkml_sampling& o) { return fmax(2.0 - kTurns * static_cast<double>(log2f(o.min_p)), 2.0); }
+
 struct Row {
     double peak;
-    double turns;  // 512 log2(e) / T
-    double limit;  // a candidate is less turns below the largest
-    double least;  // weights below it are not within min_p
+    double turns;    // kTurns log2(e) / T
+    double nats;     // 1 / T
+    double limit;    // a candidate is less turns below the largest (and kMagic)
+    uint64_t least;  // weights below it are not within min_p; 0 without
     int32_t shift;
-    bool all;      // top_p asks for the mass of all, or nothing leaves any out
+    bool all;        // top_p asks for the mass of all, or nothing leaves any out
 };
 
 __device__ __forceinline__ Row row_of(float peak, const vkml_sampling& o, int32_t shift) {
     Row r;
     r.peak = static_cast<double>(peak);
-    r.turns = fmax(kTurns * 1.4426950408889634 / static_cast<double>(o.temperature), 1e-300);  // (not 0, of which -infinity makes NaN)
+    r.nats = fmax(1.0 / static_cast<double>(o.temperature), 1e-300);  // (not 0, of which -infinity makes NaN)
+    r.turns = kTurns * 1.4426950408889634 * r.nats;
     r.limit = kTurns * (shift + 1);  // less than half a unit from there on
-    r.least = (o.min_p > 0.0f ? static_cast<double>(o.min_p) : 0.0) * __builtin_ldexp(1.0, shift);
+    r.least = 0;
+    if (o.min_p > 0.0f) r.least = o.min_p <= 1.0f ? static_cast<uint64_t>(__builtin_ceil(static_cast<double>(o.min_p) * __builtin_ldexp(1.0, shift))) : ~0ull;
     r.shift = shift;
-    r.all = o.top_p < 1.0f || !(o.min_p > 0.0f);
+    r.all = o.top_p < 1.0f || r.least == 0;
     // Where top_p does not ask for the mass of all, those that min_p leaves out need no
-    // weight (but for a turn, so that the weights decide).
-    if (!r.all) r.limit = fmin(r.limit, fmax(1.0 - kTurns * static_cast<double>(log2f(o.min_p)), 1.0));
+    // weight.
+    if (!r.all) r.limit = fmin(r.limit, likely_turns(o));
+    r.limit += kMagic;
     return r;
 }
 
-// How far a logit's weight is below the largest: whether it is a candidate at all, and
-// the turns, z, also to the next whole number. (+infinity beside itself is none below;
-// beside it, as -infinity always, the rest is no candidate. NaN comes as -infinity.)
+// How far a logit's weight is below the largest, in turns: with kMagic, to the next whole
+// number n of them. (+infinity beside itself is none below; beside it, as -infinity
+// always, the rest is no candidate. NaN comes as -infinity.)
 struct Turns {
-    double z, whole;
-    int32_t n;
-    bool candidate;
+    double below, sum;  // below: the logits' difference
+    __device__ __forceinline__ uint32_t n() const { return static_cast<uint32_t>(__builtin_bit_cast(uint64_t, sum)); }
+    __device__ __forceinline__ uint32_t bin() const { return n() / kBinTurns; }
+    __device__ __forceinline__ bool candidate(const Row& r) const { return sum < r.limit; }
 };
 __device__ __forceinline__ Turns turns_of(const Row& r, float l) {
-    constexpr double kMagic = 6755399441055744.0;  // 1.5 2^52: a sum with it is whole, in the low bits
-    const double z = fmax((r.peak - static_cast<double>(l)) * r.turns, 0.0), sum = z + kMagic;
-    return {z, sum - kMagic, static_cast<int32_t>(__builtin_bit_cast(uint64_t, sum)), z < r.limit};
+    const double d = fmax(r.peak - static_cast<double>(l), 0.0);
+    return {d, __builtin_fma(d, r.turns, kMagic)};
 }
-__device__ __forceinline__ uint32_t bin_of(const Turns& t) { return static_cast<uint32_t>(t.n) / kBinTurns; }
-// 2^(shift - z / kTurns), the nearest whole number: 2^-(n / kTurns) from the table, the
-// rest, at most half a turn, by e^f's first terms (f^5 / 120 < 2^-59).
+// e^(-below / T) 2^shift, the nearest whole number: 2^(shift - n / kTurns) from the table
+// and n's upper bits, the rest, at most half a turn, by e^f's first terms (f^4 / 24 <
+// 2^-50).
 __device__ __forceinline__ uint64_t weight_of(const Row& r, const Turns& t, const double* table) {
-    const double f = (t.whole - t.z) * (0.6931471805599453 / kTurns);
-    double p = __builtin_fma(f, 1.0 / 24.0, 1.0 / 6.0);
-    p = __builtin_fma(p, f, 0.5);
+    const uint32_t n = t.n();
+    const double f = __builtin_fma(t.sum - kMagic, 0.6931471805599453 / kTurns, -t.below * r.nats);
+    double p = __builtin_fma(f, 1.0 / 6.0, 0.5);
     p = __builtin_fma(p, f, 1.0);
     p = __builtin_fma(p, f, 1.0);
-    const double w = __builtin_amdgcn_ldexp(table[t.n & (kTurns - 1)] * p, r.shift - (t.n >> 9));
-    static_assert(kTurns == 1 << 9);
-    return __builtin_bit_cast(uint64_t, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    const uint64_t power = __builtin_bit_cast(uint64_t, table[n & (kTurns - 1)]);
+    const uint32_t high = static_cast<uint32_t>(power >> 32) - ((n & ~(kTurns - 1u)) << (20 - kTurnsLog2));
+    const double w = __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | static_cast<uint32_t>(power));
+    return __builtin_bit_cast(uint64_t, __builtin_fma(w, p, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
 }
+
+// The least logit whose turns are below `sum` (there is one: the largest's are least),
+// found among all floats in their order, a 64th of what is left at a time.
+__device__ __forceinline__ float edge_of(const Row& r, double sum) {
+    uint32_t lo = 0x007FFFFFu, hi = 0xFF800000u;  // -infinity and +infinity, in numbers that rise
+    const auto value = [](uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u); };
+    while (lo < hi) {
+        const uint32_t step = (hi - lo) / kWave + 1, at = lo + min(threadIdx.x % kWave * step, hi - lo);
+        const uint64_t below = __ballot(turns_of(r, value(at)).sum < sum);
+        if (below == 0) {
+            lo += (kWave - 1) * step + 1;
+            continue;
+        }
+        const uint32_t first = static_cast<uint32_t>(__builtin_ctzll(below));
+        hi = lo + min(first * step, hi - lo);
+        if (first > 0) lo += min((first - 1) * step, hi - lo) + 1;
+        lo = min(lo, hi);
+    }
+    return value(hi);
+}
+
+// The logits of the candidates of bins first .. last.
+struct Bounds {
+    float from, to;  // to: NaN for none
+    __device__ __forceinline__ Bounds(const Row& r, uint32_t first, uint32_t last)
+        : from(edge_of(r, fmin(r.limit, kMagic + static_cast<double>(last + 1) * kBinTurns))),
+          to(first ? edge_of(r, kMagic + static_cast<double>(first) * kBinTurns) : __builtin_nanf("")) {}
+    __device__ __forceinline__ bool hold(float l) const { return l >= from && !(l >= to); }
+};
 
 // The mass that top_p, `share` of it, asks for at the least, and the unit of it that
 // the draw falls on.
@@ -128,7 +166,7 @@ __device__ __forceinline__ uint64_t unit_of(double random, uint64_t mass) {
 }
 // What min_p leaves of a mass: the first candidate at least.
 __device__ __forceinline__ uint64_t within(const Row& r, uint64_t mass, uint64_t likely) {
-    if (!(r.least > 0.0)) return mass;
+    if (r.least == 0) return mass;
     const uint64_t first = 1ull << r.shift, some = likely < first ? first : likely;
     return some < mass ? some : mass;
 }
@@ -198,10 +236,12 @@ struct Picker {
                 uint64_t sub_mass[kSubs];
                 uint32_t sub_count[kSubs];
             };
+            struct {
+                uint64_t few_place[kFew], few_weight[kFew];
+                uint64_t ranked_mass[kFew];  // of the ranked candidates up to each
+                uint32_t ranked_id[kFew];
+            };
         };
-        uint64_t few_place[kFew], few_weight[kFew];
-        uint64_t ranked_mass[kFew];  // of the ranked candidates up to each
-        uint32_t ranked_id[kFew];
         uint64_t wave_mass[kWaves];
         uint32_t wave_count[kWaves];
         double table[kTurns];
@@ -210,8 +250,8 @@ struct Picker {
         uint32_t found, found_count, listed, lowest;
     };
 
-    static __device__ __forceinline__ void fill_table(Scratch& lds) {
-        for (uint32_t i = threadIdx.x; i < kTurns; i += kThreads) lds.table[i] = exp2(-static_cast<double>(i) / kTurns);
+    static __device__ __forceinline__ void fill_table(int32_t shift, Scratch& lds) {
+        for (uint32_t i = threadIdx.x; i < kTurns; i += kThreads) lds.table[i] = exp2(shift - static_cast<double>(i) / kTurns);
     }
 
     // A slice in the workgroup's registers, the first one's with the values outside the
@@ -254,14 +294,13 @@ struct Picker {
             for (uint32_t i = 0; i < kVectors; ++i) m = fmaxf(fmaxf(m, fmaxf(x[i].x, x[i].y)), fmaxf(x[i].z, x[i].w));
             return m;
         }
-        // The ids of the candidates in bins first .. last to the list, lds.listed of them:
+        // The ids of the candidates in some bins to the list, lds.listed of them:
         // which they are as bits first, then one addition a wave for their places there.
-        __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
+        __device__ __forceinline__ void list(const Bounds& of, Scratch& lds) {
             static_assert(4 * kVectors == 32);
             uint32_t bits = 0, k = 0, at_edge = 0;
             each([&](float l, uint32_t) {
-                const Turns t = turns_of(r, l);
-                const uint32_t b = bin_of(t), hit = t.candidate && b >= first && b <= last;
+                const uint32_t hit = of.hold(l);
                 if (k < 32) bits |= hit << k++;
                 else at_edge = hit;
             });
@@ -304,11 +343,11 @@ struct Picker {
             }
             if (threadIdx.x < s.edges()) f(s.value(s.edge(threadIdx.x)), s.edge(threadIdx.x));
         }
-        __device__ __forceinline__ void list(const Row& r, uint32_t first, uint32_t last, Scratch& lds) {
+        __device__ __forceinline__ void list(const Bounds& of, Scratch& lds) {
             for (uint32_t i = 0; i * kVectors * kThreads < s.vectors || i == 0; ++i) {
                 Held h;
                 h.load(s, i);
-                h.list(r, first, last, lds);
+                h.list(of, lds);
             }
         }
     };
@@ -343,20 +382,26 @@ struct Picker {
         if (threadIdx.x == 0) lds.likely = 0, lds.listed = 0;
         __syncthreads();
     }
-    // The candidates' weights to the bins. A barrier has to follow.
+    // The candidates' weights to the bins, and the mass within min_p. A barrier has to
+    // follow.
     template <typename V>
-    static __device__ __forceinline__ void fill_bins(V& values, const Row& r, Scratch& lds) {
-        uint64_t likely = 0;
+    static __device__ __forceinline__ void fill_bins(V& values, const Row& r, const vkml_sampling& o, Scratch& lds) {
         values.each([&](float l, uint32_t) {
             const Turns t = turns_of(r, l);
-            if (!t.candidate) return;
-            const uint32_t b = bin_of(t);
-            const uint64_t w = weight_of(r, t, lds.table);
-            add(&lds.count[b], 1u);
-            add(&lds.mass[b], w);
-            if (static_cast<double>(w) >= r.least) likely += w;
+            if (!t.candidate(r)) return;
+            add(&lds.count[t.bin()], 1u);
+            add(&lds.mass[t.bin()], weight_of(r, t, lds.table));
         });
-        if (r.least > 0.0 && likely) add(&lds.likely, likely);
+        if (r.least == 0) return;
+        uint64_t likely = 0;
+        const double to = kMagic + likely_turns(o);
+        values.each([&](float l, uint32_t) {
+            const Turns t = turns_of(r, l);
+            if (t.sum >= to || !t.candidate(r)) return;
+            const uint64_t w = weight_of(r, t, lds.table);
+            if (w >= r.least) likely += w;
+        });
+        if (likely) add(&lds.likely, likely);
     }
 
     // What of N parts becomes that of the part and all before it. A barrier has to come
@@ -519,21 +564,19 @@ struct Picker {
             listed = {all ? 0 : b, b, all ? p.count_before + p.count : p.count};
             if (threadIdx.x == 0) lds.listed = 0;
             __syncthreads();
-            values.list(r, listed.first, listed.last, lds);
+            values.list(Bounds{r, listed.first, listed.last}, lds);
             __syncthreads();
             weigh_listed(values.s, r, listed.n, lds);
         }
         const bool from_list = listed.first <= b && b <= listed.last;
         const auto visit = [&](const auto& f) {  // (more than the list holds: they are read again)
             if (from_list) {
-                for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads) {
-                    const Turns t = turns_of(r, logit_at(lds.place[i]));
-                    if (bin_of(t) == b) f(lds.place[i], lds.weight[i]);
-                }
+                for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads)
+                    if (turns_of(r, logit_at(lds.place[i])).bin() == b) f(lds.place[i], lds.weight[i]);
             } else {
                 values.each([&](float l, uint32_t id) {
                     const Turns t = turns_of(r, l);
-                    if (t.candidate && bin_of(t) == b) f(place_of(l, id), weight_of(r, t, lds.table));
+                    if (t.candidate(r) && t.bin() == b) f(place_of(l, id), weight_of(r, t, lds.table));
                 });
             }
         };
@@ -623,7 +666,7 @@ struct Picker {
         uint32_t last = kBins - 1;
         if (o.top_k > 0 && static_cast<uint32_t>(o.top_k) <= kThreads) {
             const Turns t = turns_of(r, largest);
-            if (t.candidate) add(&lds.count[bin_of(t)], 1u);
+            if (t.candidate(r)) add(&lds.count[t.bin()], 1u);
             __syncthreads();
             sum_up<kBins, false>(lds.mass, lds.count, lds);
             const uint32_t most = lds.count[kBins - 1], k = static_cast<uint32_t>(o.top_k);
@@ -631,7 +674,7 @@ struct Picker {
             else __syncthreads();
             for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) lds.count[i] = 0;
         }
-        values.list(r, 0, last, lds);
+        values.list(Bounds{r, 0, last}, lds);
         __syncthreads();
     }
     // The n listed candidates, weighed: their mass within min_p, and where they are more
@@ -640,14 +683,14 @@ struct Picker {
         uint64_t likely = 0;
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
             const uint64_t w = lds.weight[i];
-            if (static_cast<double>(w) >= r.least) likely += w;
+            if (r.least != 0 && w >= r.least) likely += w;
             if (n > kFew) {
-                const uint32_t b = bin_of(turns_of(r, logit_at(lds.place[i])));
+                const uint32_t b = turns_of(r, logit_at(lds.place[i])).bin();
                 add(&lds.count[b], 1u);
                 add(&lds.mass[b], w);
             }
         }
-        if (r.least > 0.0 && likely) add(&lds.likely, likely);
+        if (likely) add(&lds.likely, likely);
         __syncthreads();
     }
 };
@@ -664,7 +707,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
     const typename P::Streamed again{source_of(a, row)};
     typename P::Held values;
     values.load(again.s, 0);
-    P::fill_table(lds);
+    P::fill_table(a.shift, lds);
     P::clear_bins(lds);
     const float largest = values.largest(), peak = P::peak_of(largest, lds);
     uint32_t id = ~0u;  // -1
@@ -673,7 +716,6 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
         id = P::first_with(values, peak, lds);
     } else {
         const Row r = row_of(peak, o, a.shift);
-        const double random = a.random[row];
         uint32_t n = kList + 1;
         if (P::lists_first(r, o)) {
             P::list_kept(values, largest, r, o, lds);
@@ -683,10 +725,10 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
             P::weigh_listed(again.s, r, n, lds);
             P::bin_listed(r, n, lds);
         } else {
-            P::fill_bins(values, r, lds);
+            P::fill_bins(values, r, o, lds);
             __syncthreads();
         }
-        id = n <= P::kFew ? P::pick_few(r, o, random, n, lds) : P::pick(again, r, o, random, n, lds);
+        id = n <= P::kFew ? P::pick_few(r, o, a.random[row], n, lds) : P::pick(again, r, o, a.random[row], n, lds);
     }
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
@@ -704,13 +746,57 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_peaks(Args a) {
     if (threadIdx.x == 0) stg(a.peaks + blockIdx.x, peak > -__builtin_inff() ? place_of(peak, id) : kNone);
 }
 
+// The place of a row's largest: the slices', a lane each.
 __device__ __forceinline__ uint64_t first_of(const Args& a, uint32_t row) {
     uint64_t first = kNone;
-    for (uint32_t i = 0; i < a.slices; ++i) {
+    for (uint32_t i = threadIdx.x % kWave; i < a.slices; i += kWave) {
         const uint64_t p = ldg(a.peaks + static_cast<uint64_t>(row) * a.slices + i);
         first = p < first ? p : first;
     }
-    return first;
+    return wave_min(first);
+}
+
+// The sums of a row's slices to the bins, two a thread, four slices' loads in flight.
+// Likely has to be 0.
+__device__ __forceinline__ void add_slices(const Slice* from, uint32_t slices, Wide::Scratch& lds) {
+    static_assert(2 * kWideThreads == kBins);
+    const uint32_t i = 2 * threadIdx.x;
+    uint64_t m0 = 0, m1 = 0;
+    uint32_t c0 = 0, c1 = 0;
+    for (uint32_t s = 0; s < slices; s += 4) {
+        uint4 m[4];
+        uint2 c[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            const Slice& of = from[min(s + k, slices - 1)];
+            m[k] = ldg(reinterpret_cast<const uint4*>(of.mass + i));
+            c[k] = ldg(reinterpret_cast<const uint2*>(of.count + i));
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) {
+            if (s + k >= slices) break;
+            m0 += static_cast<uint64_t>(m[k].y) << 32 | m[k].x, m1 += static_cast<uint64_t>(m[k].w) << 32 | m[k].z;
+            c0 += c[k].x, c1 += c[k].y;
+        }
+    }
+    lds.mass[i] = m0, lds.mass[i + 1] = m1, lds.count[i] = c0, lds.count[i + 1] = c1;
+    for (uint32_t s = threadIdx.x; s < slices; s += kWideThreads) add(&lds.likely, ldg(&from[s].likely));
+}
+
+// The lists of a row's slices one after another, each wave some of the slices': how
+// many are listed (more than kList where these are not all).
+__device__ __forceinline__ uint32_t join_lists(const Slice* from, uint32_t slices, Wide::Scratch& lds) {
+    uint32_t n = 0;
+    for (uint32_t s0 = 0; s0 < slices; s0 += kWave) {
+        const uint32_t l = threadIdx.x % kWave, of = s0 + l < slices ? min(ldg(&from[s0 + l].listed), kList + 1) : 0u;
+        const uint32_t upto = static_cast<uint32_t>(inclusive_sum(static_cast<int32_t>(of)));
+        for (uint32_t s = threadIdx.x / kWave; s < min(static_cast<uint32_t>(kWave), slices - s0); s += kWideThreads / kWave) {
+            const uint32_t mine = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(of), s)), to = n + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), s)) - mine;
+            for (uint32_t i = l; i < mine && to + i < kList; i += kWave) lds.id[to + i] = ldg(from[s0 + s].id + i);
+        }
+        n = min(n + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), kWave - 1)), kList + 1);
+    }
+    return n;
 }
 
 __global__ void __launch_bounds__(kWideThreads) k_sample_slices(Args a) {
@@ -733,9 +819,9 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_slices(Args a) {
         for (uint32_t i = threadIdx.x; i < n; i += kWideThreads) stg(to->id + i, lds.id[i]);
         return;
     }
-    Wide::fill_table(lds);
+    Wide::fill_table(a.shift, lds);
     __syncthreads();
-    Wide::fill_bins(values, r, lds);
+    Wide::fill_bins(values, r, o, lds);
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
     if (threadIdx.x == 0) stg(&to->likely, lds.likely);
@@ -752,43 +838,27 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_pick(Args a) {
         id = static_cast<uint32_t>(first);
     } else {
         const Row r = row_of(logit_at(first), o, a.shift);
-        const double random = a.random[row];
         Wide::Streamed values{source_of(a, row)};
         const Slice* from = a.parts + static_cast<uint64_t>(row) * a.slices;
-        Wide::fill_table(lds);
+        Wide::fill_table(a.shift, lds);
         Wide::clear_bins(lds);
         uint32_t n = kList + 1;
         const bool lists = Wide::lists_first(r, o);
         if (lists) {
-            n = 0;
-            for (uint32_t s = 0; s < a.slices; ++s) {
-                const uint32_t of = ldg(&from[s].listed);
-                for (uint32_t i = threadIdx.x; i < of && n + i < kList; i += kWideThreads) lds.id[n + i] = ldg(from[s].id + i);
-                n = min(n + of, kList + 1);
-            }
+            n = join_lists(from, a.slices, lds);
             __syncthreads();
         }
         if (n <= kList) {
             Wide::weigh_listed(values.s, r, n, lds);
             Wide::bin_listed(r, n, lds);
         } else if (lists) {
-            Wide::fill_bins(values, r, lds);
+            Wide::fill_bins(values, r, o, lds);
             __syncthreads();
         } else {
-            for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) {
-                uint64_t m = 0;
-                uint32_t c = 0;
-                for (uint32_t s = 0; s < a.slices; ++s) m += ldg(from[s].mass + i), c += ldg(from[s].count + i);
-                lds.mass[i] = m, lds.count[i] = c;
-            }
-            if (threadIdx.x == 0) {
-                uint64_t likely = 0;
-                for (uint32_t s = 0; s < a.slices; ++s) likely += ldg(&from[s].likely);
-                lds.likely = likely;
-            }
+            add_slices(from, a.slices, lds);
             __syncthreads();
         }
-        id = n <= Wide::kFew ? Wide::pick_few(r, o, random, n, lds) : Wide::pick(values, r, o, random, n, lds);
+        id = n <= Wide::kFew ? Wide::pick_few(r, o, a.random[row], n, lds) : Wide::pick(values, r, o, a.random[row], n, lds);
     }
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
