@@ -192,78 +192,105 @@ struct KeepArgs {
 };
 constexpr uint32_t kKeepVectors = 4;  // a thread has in flight
 
-// Workgroup (sequence, layer, pool). Wave 0 walks the tree: the first node after the
-// one it is at, of that parent, whose drafted token is the parent's pick, 64 nodes
-// looked at at once. (Every workgroup for itself: a walk of 6 of 13 nodes is some
-// 0.3 us, a launch of its own were 2.) Then the rows of the path move to the places
-// after one another that it takes. They are read and written by turns, 16 KB at
-// most, since a row may go to where another one comes from: never to where one of
-// a later turn does, as a path's k-th node is the k-th of the tree or a later one.
+// Workgroup (sequence, layer). It walks the tree: the first node after the one it is
+// at, of that parent, whose drafted token is the parent's pick, 64 nodes looked at at
+// once. (Every workgroup for itself: a walk is some 0.3 us, a launch of its own were
+// 2.) A tree of up to 64 nodes is in the lanes of each wave; a larger one in the LDS,
+// walked by the first. Then the rows of the path move to the places after one another
+// that it takes, both pools'. They are read and written by turns, 16 KB at most, since a
+// row may go to where another one comes from: never to where one of a later turn does, as
+// a path's k-th node is the k-th of the tree or a later one.
 template <typename V>
 __global__ void __launch_bounds__(kThreads) k_keep_drafts(KeepArgs a) {
-    __shared__ int32_t s_parent[vkml::pages::kMaxNodes], s_path[vkml::pages::kMaxNodes];
+    constexpr int32_t kNodes = static_cast<int32_t>(vkml::pages::kMaxNodes);
+    static_assert(kNodes <= 0x7FFF);
+    __shared__ int16_t s_parent[kNodes], s_path[kNodes];
     __shared__ int32_t s_count;
-    const int32_t s = static_cast<int32_t>(blockIdx.x), token0 = a.batch.start(s), n = min(a.batch.count(s), static_cast<int32_t>(vkml::pages::kMaxNodes));
-    const int32_t base = a.batch.length(s) - a.batch.count(s);
-    // The parent of each node that its parent's pick is the token of; of the others none.
-    for (int32_t i = static_cast<int32_t>(threadIdx.x); i < n; i += kThreads) {
-        const int32_t parent = ldg(a.parents + token0 + i);
-        s_parent[i] = parent >= 0 && parent < i && ldg(a.picked + token0 + parent) == ldg(a.drafted + token0 + i) ? parent : -1;
-    }
-    __syncthreads();
-    if (threadIdx.x < kWave) {
-        const int32_t l = static_cast<int32_t>(threadIdx.x);
-        int32_t at = 0, count = n > 0 ? 1 : 0;
-        if (l == 0 && n > 0) s_path[0] = 0;
-        for (int32_t i = 0; i < n;) {
-            const uint64_t found = __ballot(i + l > at && i + l < n && s_parent[min(i + l, n - 1)] == at);
-            if (found == 0) {
-                i += kWave;
-                continue;
-            }
-            at = i + static_cast<int32_t>(__builtin_ctzll(found));
-            i = at / kWave * kWave;
-            if (l == 0) s_path[count] = at;
+    const int32_t s = static_cast<int32_t>(blockIdx.x), token0 = a.batch.start(s), all = a.batch.count(s), n = min(all, kNodes);
+    const int32_t base = a.batch.length(s) - all, l = static_cast<int32_t>(threadIdx.x % kWave);
+    const bool small = n <= kWave;
+    const int32_t* table = a.table + static_cast<uint64_t>(s) * a.table_stride;
+    // The pages that the new tokens are in, from the first one's on, for a small tree
+    // (5 at most) a lane each, loaded beside the tree.
+    const auto page_at = [&](int32_t i) { return i >= 0 && i < static_cast<int32_t>(a.table_stride) ? static_cast<uint32_t>(ldg(table + i)) : ~0u; };
+    const int32_t first_page = base >> a.page_shift;
+    uint32_t held = ~0u;
+    if (small && l < 8) held = page_at(first_page + l);
+    int32_t count = n > 0 ? 1 : 0, path = 0;  // small: node l of the path
+    if (small) {
+        int32_t parent = -1, drafted = 0, picked = 0;
+        if (l < n) parent = ldg(a.parents + token0 + l), drafted = ldg(a.drafted + token0 + l), picked = ldg(a.picked + token0 + l);
+        // The parent of a node that its parent's pick is the token of; of the others none.
+        const bool earlier = parent >= 0 && parent < l;
+        const int32_t pick = __shfl(picked, earlier ? parent : 0);
+        if (!earlier || pick != drafted) parent = -1;
+        for (int32_t at = 0;;) {
+            const uint64_t found = __ballot(parent == at);
+            if (found == 0) break;
+            at = static_cast<int32_t>(__builtin_ctzll(found));
+            if (l == count) path = at;
             ++count;
         }
-        if (l == 0) s_count = count;
+    } else {
+        for (int32_t i = static_cast<int32_t>(threadIdx.x); i < n; i += kThreads) {
+            const int32_t parent = ldg(a.parents + token0 + i);
+            s_parent[i] = static_cast<int16_t>(parent >= 0 && parent < i && ldg(a.picked + token0 + parent) == ldg(a.drafted + token0 + i) ? parent : -1);
+        }
+        __syncthreads();
+        if (threadIdx.x < kWave) {
+            if (l == 0) s_path[0] = 0;
+            int32_t at = 0;
+            for (int32_t i = 0; i < n;) {
+                const uint64_t found = __ballot(i + l > at && i + l < n && s_parent[min(i + l, n - 1)] == at);
+                if (found == 0) {
+                    i += kWave;
+                    continue;
+                }
+                at = i + static_cast<int32_t>(__builtin_ctzll(found));
+                i = at / kWave * kWave;
+                if (l == 0) s_path[count] = static_cast<int16_t>(at);
+                ++count;
+            }
+            if (l == 0) s_count = count;
+        }
+        __syncthreads();
+        count = s_count;
     }
-    __syncthreads();
-    const int32_t count = s_count;
-    if (blockIdx.y == 0 && blockIdx.z == 0) {
-        const int32_t all = a.batch.count(s);
-        for (int32_t i = static_cast<int32_t>(threadIdx.x); i < all; i += kThreads) stg(a.path + token0 + i, i < count ? s_path[i] : -1);
+    // (by all of a wave's lanes at once)
+    const auto node_of = [&](int32_t j) { return small ? __shfl(path, min(j, kWave - 1)) : static_cast<int32_t>(s_path[min(j, kNodes - 1)]); };
+    if (blockIdx.y == 0) {
+        for (int32_t i0 = 0; i0 < all; i0 += kThreads) {
+            const int32_t i = i0 + static_cast<int32_t>(threadIdx.x), node = node_of(i);
+            if (i < all) stg(a.path + token0 + i, i < count ? node : -1);
+        }
+        const int32_t last = node_of(max(count, 1) - 1);
         if (threadIdx.x == 0) {
             stg(a.counts + s, count);
-            stg(a.next + s, count > 0 ? ldg(a.picked + token0 + s_path[count - 1]) : -1);
+            stg(a.next + s, count > 0 ? ldg(a.picked + token0 + last) : -1);
         }
     }
-    uint8_t* pool = a.pool[blockIdx.z] + blockIdx.y * a.layer_bytes;
-    const int32_t* table = a.table + static_cast<uint64_t>(s) * a.table_stride;
-    const uint32_t pieces = a.row_bytes / sizeof(V), per_node = a.kv_heads * pieces;
+    const uint32_t pieces = a.row_bytes / sizeof(V), per_pool = a.kv_heads * pieces, per_node = 2 * per_pool;
     const uint32_t head_bytes = a.row_bytes << a.page_shift;
-    const uint64_t units = static_cast<uint64_t>(count) * per_node;
-    const auto place = [&](int32_t pos, uint32_t unit) -> uint8_t* {  // null: in no page
-        if (pos < 0 || pos >= a.batch.table_keys) return nullptr;
-        const uint32_t page = static_cast<uint32_t>(ldg(table + (pos >> a.page_shift)));
-        if (page >= a.pages) return nullptr;
-        const uint32_t head = unit / pieces, row = static_cast<uint32_t>(pos) & ((1u << a.page_shift) - 1);
-        return pool + page * a.page_bytes + static_cast<uint64_t>(head) * head_bytes + row * a.row_bytes + unit % pieces * sizeof(V);
+    const uint64_t units = static_cast<uint64_t>(count) * per_node, layer = blockIdx.y * a.layer_bytes;
+    const auto page_of = [&](int32_t pos) {  // (as node_of; no page outside the table)
+        const int32_t i = pos >> a.page_shift;
+        return small ? static_cast<uint32_t>(__shfl(static_cast<int>(held), i - first_page)) : page_at(i);
     };
     for (uint64_t first = per_node; first < units; first += kKeepVectors * kThreads) {  // (node 0 stays)
         V v[kKeepVectors];
         uint8_t* to[kKeepVectors];
 #pragma unroll
         for (uint32_t i = 0; i < kKeepVectors; ++i) {
-            const uint64_t u = first + i * kThreads + threadIdx.x;
+            const uint64_t u = min(first + i * kThreads + threadIdx.x, units - 1);
+            const int32_t j = static_cast<int32_t>(u / per_node), node = node_of(j);
+            const uint32_t unit = static_cast<uint32_t>(u % per_node), in_pool = unit % per_pool;
+            const uint32_t from_page = page_of(base + node), to_page = page_of(base + j);
             to[i] = nullptr;
-            if (u >= units) continue;
-            const int32_t j = static_cast<int32_t>(u / per_node), node = s_path[j];
-            const uint32_t unit = static_cast<uint32_t>(u % per_node);
-            const uint8_t* from = node == j ? nullptr : place(base + node, unit);
-            if (!from) continue;
-            to[i] = place(base + j, unit);
-            v[i] = ldg(reinterpret_cast<const V*>(from));
+            if (node == j || first + i * kThreads + threadIdx.x >= units || from_page >= a.pages || to_page >= a.pages) continue;
+            uint8_t* pool = a.pool[unit / per_pool] + layer + static_cast<uint64_t>(in_pool / pieces) * head_bytes + in_pool % pieces * sizeof(V);
+            const uint32_t mask = (1u << a.page_shift) - 1;
+            to[i] = pool + to_page * a.page_bytes + (static_cast<uint32_t>(base + j) & mask) * a.row_bytes;
+            v[i] = ldg(reinterpret_cast<const V*>(pool + from_page * a.page_bytes + (static_cast<uint32_t>(base + node) & mask) * a.row_bytes));
         }
         // Every load of the turn has landed before the first store.
         __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
@@ -337,7 +364,7 @@ int vkml_keep_drafts(const vkml_keep_drafts_params* p, const int32_t* parents, c
     // (strides are multiples of 8 elements, so that rows start on 16 bytes as the pools and a row's bytes do)
     const bool wide = a.row_bytes % 16 == 0 && a.page_bytes % 16 == 0 && a.layer_bytes % 16 == 0 && aligned16(k_pages) && aligned16(v_pages);
     vkml::abi::ProfileScope prof("keep_drafts");
-    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(p->seqs, p->layers, 2), dim3(kThreads), 0, vkml::abi::stream(), a); };
+    const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(p->seqs, p->layers), dim3(kThreads), 0, vkml::abi::stream(), a); };
     wide ? go(k_keep_drafts<uint4>) : go(k_keep_drafts<uint32_t>);
     return vkml::abi::check_launch("keep_drafts");
 }
