@@ -130,6 +130,21 @@ def test_rows_of_any_size(vocab):
     check(like_a_model(rng, rows, vocab), *asked(rng, rows))
 
 
+@pytest.mark.parametrize("rows", [255, 256, 257, 300, 511, 1023, 1024, 1025])
+def test_many_rows(rows):
+    """Of every kind of request, in an order that changes (rows that take long come
+    first); the same row gives the same token wherever it stands."""
+    rng = np.random.default_rng(rows)
+    x, (o, u) = like_a_model(rng, rows, 8200), asked(rng, rows)
+    order = rng.permutation(rows)
+    o = [o[i] for i in order]
+    got = check(x, o, u)
+    back = np.argsort(order)
+    assert np.array_equal(Call(x[back], np.array(o, OPTIONS)[back], u[back]).run().result(), got[back])
+    # one kind alone
+    assert np.array_equal(Call(x, np.array([ASKED[1]] * rows, OPTIONS), u).run().result(), Call(x[::-1], np.array([ASKED[1]] * rows, OPTIONS), u[::-1]).run().result()[::-1])
+
+
 @pytest.mark.parametrize("vocab", [7, 1000, 32763, 32765, 40000])
 @pytest.mark.parametrize("offset,gap", [(0, 1), (1, 0), (2, 3), (3, 2), (3, 4)])
 def test_rows_that_start_anywhere(offset, gap, vocab):
