@@ -771,7 +771,8 @@ int vkml_attend_pages_window(const vkml_attend_pages_params* p, uint32_t window,
  * the pick after the last (-1). In every layer the keys and values of the path's
  * nodes move to the positions after one another that follow the sequence's earlier
  * keys, so that it goes on with d_lengths[s] - n + d_counts[s] keys (the caller's
- * to set); the rows behind them are unspecified, all others stay as they were. At
+ * to set); the rows behind them are unspecified, all others stay as they were (so
+ * the pages that hold a sequence's new tokens must be its own). At
  * most 4096 nodes a sequence: those past them are left out. layer_stride in
  * elements as page_stride (0: no gap). d_drafted, d_picked and the outputs [tokens]
  * and [seqs]; all but the pools may be any 32-bit values. */

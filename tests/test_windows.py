@@ -51,7 +51,8 @@ KEEP = dict(kv_heads=2, head_dim=128, kv_type=H.F16, page_size=16, pages=10, lay
     (dict(kv_heads=4097), "head layout"), (dict(kv_type=H.BF16), "f16 or f32"), (dict(page_size=24), "power of two"), (dict(pages=0), "pages"),
     (dict(layers=0), "layers"), (dict(layers=65536), "layers"), (dict(seqs=65537), "65536"), (dict(tokens=2 ** 22 + 1), "2^22"), (dict(table_stride=0), "table row"),
     (dict(page_stride=8), "pages overlap"), (dict(page_stride=4100), "multiple of 8"), (dict(layer_stride=4096 * 9), "layers overlap"),
-    (dict(layer_stride=4096 * 10 + 4), "multiple of 8"), (dict(layer_stride=2 ** 46 + 8), "too large")])
+    (dict(layer_stride=4096 * 10 + 4), "multiple of 8"), (dict(layer_stride=2 ** 46 + 8), "too large"), (dict(layer_stride=2 ** 46, layers=65535), "too large"),
+    (dict(pages=2 ** 31 - 1, page_stride=2 ** 33), "too large")])
 def test_keep_refuses(host, change, why):
     assert host.check_keep_c(C.byref(H.KeepDraftsParams(**KEEP))) is None
     assert why in said(host.check_keep_c(C.byref(H.KeepDraftsParams(**{**KEEP, **change}))))

@@ -403,6 +403,8 @@ inline const char* check(const vkml_keep_drafts_params& p) {
     if (p.layer_stride && p.layer_stride < (p.pages - 1) * stride + page) return "layers overlap";
     if (p.layer_stride % 8) return "layer_stride must be a multiple of 8";
     if (p.layer_stride > (1ull << 46)) return "layer_stride is too large";
+    // (a layer has less than 2^64 elements, if not bytes)
+    if (static_cast<double>(p.layer_stride ? p.layer_stride : p.pages * stride) * p.layers > 4611686018427387904.0 / 4) return "the pools are too large";
     return nullptr;
 }
 

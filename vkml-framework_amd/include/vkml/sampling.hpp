@@ -50,6 +50,9 @@ public:
 
     const SamplingOptions& options() const noexcept { return options_; }
 
+    // Throws for what options may not be (as the constructor).
+    static void check(const SamplingOptions& options);
+
 private:
     std::int32_t pick(std::span<const float> logits);
     // Counts a picked token for the frequency and presence penalties.

@@ -150,7 +150,7 @@ Tensor sample(const Tensor& logits, std::span<const SamplingOptions> options, st
     std::vector<vkml_sampling> each(r.rows);
     for (std::size_t i = 0; i < options.size(); ++i) {
         const SamplingOptions& o = options[i];
-        Sampler checked(o);  // (throws what its options may not be)
+        Sampler::check(o);
         if (o.repetition_penalty != 1.0f || o.frequency_penalty != 0.0f || o.presence_penalty != 0.0f) throw Error("sample: penalties change the logits before");
         if (i < each.size()) each[i] = {o.temperature, o.top_k, o.top_p, o.min_p};
     }

@@ -72,7 +72,9 @@ double log_partition(std::span<const float> logits) {
 
 }  // namespace
 
-Sampler::Sampler(SamplingOptions options) : options_(options), rng_(options.seed) {
+Sampler::Sampler(SamplingOptions options) : options_(options), rng_(options.seed) { check(options); }
+
+void Sampler::check(const SamplingOptions& options) {
     require(options.temperature >= 0.0f, "temperature must be 0 or more", options.temperature);
     require(options.top_p > 0.0f && options.top_p <= 1.0f, "top_p must be in (0, 1]", options.top_p);
     require(options.top_k >= 0, "top_k must be 0 (off) or more", float(options.top_k));
