@@ -807,7 +807,7 @@ int vkml_keep_drafts(const vkml_keep_drafts_params* p, const int32_t* d_parents,
  * the largest and summed exactly, so that the same row gives the same token in every
  * call. A row starts every row_stride floats; vocab at most 2^22. d_workspace:
  * vkml_sample_workspace_bytes(p) bytes of any content, 16-byte aligned (0, and NULL
- * taken, up to 32768 logits; 40 rows of 128256: 3.9 MB); calls that overlap need
+ * taken, up to 32768 logits; 40 rows of 128256: 6.2 MB); calls that overlap need
  * one each. */
 typedef struct vkml_sampling {
     float temperature;

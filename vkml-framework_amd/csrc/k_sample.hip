@@ -45,6 +45,7 @@ struct Args {
     const double* random;
     int32_t* tokens;
     uint64_t* peaks;  // [rows, slices]: the places of the slices' largest
+    Sums* totals;     // [rows]
     Slice* parts;     // [rows, slices]
     uint64_t row_stride;
     uint32_t rows, vocab, slices;
@@ -147,9 +148,10 @@ __device__ __forceinline__ float edge_of(const Row& r, double sum) {
     return value(hi);
 }
 
-// The logits of the candidates of bins first .. last.
+// The logits of the candidates of bins first .. last (or of none).
 struct Bounds {
-    float from, to;  // to: NaN for none
+    float from = __builtin_nanf(""), to = __builtin_nanf("");  // to: NaN for +infinity and beyond
+    Bounds() = default;
     __device__ __forceinline__ Bounds(const Row& r, uint32_t first, uint32_t last)
         : from(edge_of(r, fmin(r.limit, kMagic + static_cast<double>(last + 1) * kBinTurns))),
           to(first ? edge_of(r, kMagic + static_cast<double>(first) * kBinTurns) : __builtin_nanf("")) {}
@@ -300,11 +302,11 @@ struct Picker {
         }
         // The ids of the candidates in some bins to the list, lds.listed of them:
         // which they are as bits first, then one addition a wave for their places there.
-        __device__ __forceinline__ void list(const Bounds& of, Scratch& lds) {
+        __device__ __forceinline__ void list(const Bounds& some, const Bounds& others, Scratch& lds) {
             static_assert(4 * kVectors == 32);
             uint32_t bits = 0, k = 0, at_edge = 0;
             each([&](float l, uint32_t) {
-                const uint32_t hit = of.hold(l);
+                const uint32_t hit = some.hold(l) || others.hold(l);
                 if (k < 32) bits |= hit << k++;
                 else at_edge = hit;
             });
@@ -347,11 +349,11 @@ struct Picker {
             }
             if (threadIdx.x < s.edges()) f(s.value(s.edge(threadIdx.x)), s.edge(threadIdx.x));
         }
-        __device__ __forceinline__ void list(const Bounds& of, Scratch& lds) {
+        __device__ __forceinline__ void list(const Bounds& some, const Bounds& others, Scratch& lds) {
             for (uint32_t i = 0; i * kVectors * kThreads < s.vectors || i == 0; ++i) {
                 Held h;
                 h.load(s, i);
-                h.list(of, lds);
+                h.list(some, others, lds);
             }
         }
     };
@@ -570,8 +572,14 @@ struct Picker {
     }
 
     // Which bins' candidates the list in the LDS holds all of.
+    struct Range {
+        uint32_t first = 1, last = 0;
+        __device__ __forceinline__ bool holds(uint32_t b) const { return first <= b && b <= last; }
+    };
     struct Listed {
-        uint32_t first = 1, last = 0, n = 0;
+        Range some, others;
+        uint32_t n = 0;
+        __device__ __forceinline__ bool holds(uint32_t b) const { return some.holds(b) || others.holds(b); }
     };
 
     // The places and weights of the n listed ids. With a barrier after it.
@@ -585,22 +593,49 @@ struct Picker {
         __syncthreads();
     }
 
-    // The candidate with x before it, in the bins' sums and the row's values.
-    static __device__ __forceinline__ Found find(Streamed values, const Row& r, Wanted x, Listed& listed, Scratch& lds) {
+    // The bins that the draw may fall in once top_p has cut within part p.
+    static __device__ __forceinline__ Range drawn_after(const Part& p, const Row& r, double random, Scratch& lds) {
+        const uint64_t least = within(r, p.mass_before + 1, lds.likely), most = within(r, lds.mass[p.i], lds.likely);
+        const uint32_t first = part_with<kBins>(lds.mass, lds.count, {false, unit_of(random, least)}, lds).i;
+        return {first, part_with<kBins>(lds.mass, lds.count, {false, unit_of(random, most)}, lds).i};
+    }
+
+    // What to list of a row whose bins are summed up, for part p: its candidates, and all
+    // before them if they fit too; else those that the draw may ask for, if that comes
+    // next. None where its own are more than fit.
+    static __device__ __forceinline__ Listed to_list(const Part& p, bool cut, const Row& r, double random, Scratch& lds) {
+        Listed listed;
+        if (p.count > kList) return listed;
+        listed.n = p.count_before + p.count;
+        listed.some = {0, p.i};
+        if (listed.n <= kList) return listed;
+        listed.n = p.count;
+        listed.some.first = p.i;
+        if (cut) {
+            Range next = drawn_after(p, r, random, lds);
+            if (next.last == p.i) --next.last;  // (wraps where that is 0: then all before it fit)
+            const uint32_t n = next.holds(next.first) ? lds.count[next.last] - (next.first ? lds.count[next.first - 1] : 0) : 0;
+            if (n > 0 && n + listed.n <= kList) listed.others = next, listed.n += n;
+        }
+        return listed;
+    }
+    static __device__ __forceinline__ Bounds bounds_of(const Row& r, const Range& bins) { return bins.holds(bins.first) ? Bounds{r, bins.first, bins.last} : Bounds{}; }
+
+    // The candidate with x before it, in the bins' sums and the row's values; cut: the
+    // draw comes next.
+    static __device__ __forceinline__ Found find(Streamed values, const Row& r, Wanted x, bool cut, double random, Listed& listed, Scratch& lds) {
         const Part p = part_with<kBins>(lds.mass, lds.count, x, lds);
         x.before -= x.by_count ? p.count_before : p.mass_before;
         const uint32_t b = p.i;
-        if (p.count <= kList && !(listed.first <= b && b <= listed.last)) {
-            // The bin's candidates to the list, and all before them if they fit too.
-            const bool all = p.count_before + p.count <= kList;
-            listed = {all ? 0 : b, b, all ? p.count_before + p.count : p.count};
+        if (p.count <= kList && !listed.holds(b)) {
+            listed = to_list(p, cut, r, random, lds);
             if (threadIdx.x == 0) lds.listed = 0;
             __syncthreads();
-            values.list(Bounds{r, listed.first, listed.last}, lds);
+            values.list(bounds_of(r, listed.some), bounds_of(r, listed.others), lds);
             __syncthreads();
             weigh_listed(values.s, r, listed.n, lds);
         }
-        const bool from_list = listed.first <= b && b <= listed.last;
+        const bool from_list = listed.holds(b);
         const auto visit = [&](const auto& f) {  // (more than the list holds: they are read again)
             if (from_list) {
                 for (uint32_t i = threadIdx.x; i < listed.n; i += kThreads)
@@ -634,32 +669,38 @@ struct Picker {
         return among(visit, x, lo, hi, p.count, p.mass_before, lds);
     }
 
-    // The pick of a row whose bins are filled; n: of the candidates that are listed, more
-    // than kList where none are.
-    static __device__ __forceinline__ uint32_t pick(const Streamed& values, const Row& r, const vkml_sampling& o, double random, uint32_t n, Scratch& lds) {
-        sum_up<kBins, true>(lds.mass, lds.count, lds);
-        Listed listed;
-        if (n <= kList) listed = {0, kBins - 1, n};
+    // The steps of a pick, each looking for a candidate by what the one before leaves:
+    // top_k, top_p, the draw. Step `step`, or the next that there is; mass: what is kept.
+    static __device__ __forceinline__ Wanted wanted(int& step, uint64_t& mass, uint32_t count, const Row& r, const vkml_sampling& o, double random, const Scratch& lds) {
+        if (step == 0) {
+            if (o.top_k > 0 && static_cast<uint32_t>(o.top_k) < count) return {true, static_cast<uint64_t>(o.top_k - 1)};
+            ++step;
+        }
+        if (step == 1) {
+            if (o.top_p < 1.0f) return {false, reach_of(o.top_p, mass) - 1};  // the last unit that top_p asks for
+            ++step;
+        }
+        mass = within(r, mass, lds.likely);
+        return {false, unit_of(random, mass)};
+    }
+    // The pick of a row whose bins are summed up.
+    static __device__ __forceinline__ uint32_t pick(const Streamed& values, const Row& r, const vkml_sampling& o, double random, Listed listed, Scratch& lds) {
         uint64_t mass = lds.mass[kBins - 1];
         const uint32_t count = lds.count[kBins - 1];
-        // top_k, top_p, the draw: each looks for a candidate by what the one before leaves
 #pragma unroll 1
         for (int step = 0;; ++step) {
-            Wanted x{false, 0};
-            if (step == 0) {
-                if (o.top_k <= 0 || static_cast<uint32_t>(o.top_k) >= count) continue;
-                x = {true, static_cast<uint64_t>(o.top_k - 1)};
-            } else if (step == 1) {
-                if (!(o.top_p < 1.0f)) continue;
-                x.before = reach_of(o.top_p, mass) - 1;  // the last unit that top_p asks for
-            } else {
-                mass = within(r, mass, lds.likely);
-                x.before = unit_of(random, mass);
-            }
-            const Found f = find(values, r, x, listed, lds);
+            const Wanted x = wanted(step, mass, count, r, o, random, lds);
+            const Found f = find(values, r, x, step == 1, random, listed, lds);
             if (step == 2) return f.id;
             mass = f.mass;
         }
+    }
+    // What to list for the first of its steps.
+    static __device__ __forceinline__ Listed first_listed(const Row& r, const vkml_sampling& o, double random, Scratch& lds) {
+        uint64_t mass = lds.mass[kBins - 1];
+        int step = 0;
+        const Wanted x = wanted(step, mass, lds.count[kBins - 1], r, o, random, lds);
+        return to_list(part_with<kBins>(lds.mass, lds.count, x, lds), step == 1, r, random, lds);
     }
 
     // The same of n candidates that are listed, up to kFew: all ranked, then looked for
@@ -706,7 +747,7 @@ struct Picker {
             else __syncthreads();
             for (uint32_t i = threadIdx.x; i < kBins; i += kThreads) lds.count[i] = 0;
         }
-        values.list(Bounds{r, 0, last}, lds);
+        values.list(Bounds{r, 0, last}, Bounds{}, lds);
         __syncthreads();
     }
     // The n listed candidates, weighed: their mass within min_p, and where they are more
@@ -753,20 +794,30 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
             P::list_kept(values, largest, r, o, lds);
             n = lds.listed;
         }
+        typename P::Listed listed;
         if (n <= kList) {
             P::weigh_listed(again.s, r, n, lds);
             P::bin_listed(r, n, lds);
+            listed.some = {0, kBins - 1};
+            listed.n = n;
         } else {
             P::fill_bins(values, r, o, lds);
             __syncthreads();
         }
-        id = n <= P::kFew ? P::pick_few(r, o, a.random[row], n, lds) : P::pick(again, r, o, a.random[row], n, lds);
+        if (n <= P::kFew) {
+            id = P::pick_few(r, o, a.random[row], n, lds);
+        } else {
+            P::template sum_up<kBins, true>(lds.mass, lds.count, lds);
+            id = P::pick(again, r, o, a.random[row], listed, lds);
+        }
     }
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
 
-// Longer rows: their slices' largest, then what of the slices the picks need, then
-// the picks.
+// Longer rows, workgroups on slices of them: each slice's largest; then what top_k or
+// min_p keep of it, or its bins; for the latter rows then those candidates of each slice
+// that their picks begin with, found in all slices' bins (by each slice's workgroup for
+// itself: 98 KB of a row of 128256); then the picks.
 using Wide = Picker<kWideThreads>;
 
 __global__ void __launch_bounds__(kWideThreads) k_sample_peaks(Args a) {
@@ -800,7 +851,7 @@ __device__ __forceinline__ void add_slices(const Slice* from, uint32_t slices, W
         uint2 c[4];
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k) {
-            const Slice& of = from[min(s + k, slices - 1)];
+            const Sums& of = from[min(s + k, slices - 1)].sums;
             m[k] = ldg(reinterpret_cast<const uint4*>(of.mass + i));
             c[k] = ldg(reinterpret_cast<const uint2*>(of.count + i));
         }
@@ -812,7 +863,7 @@ __device__ __forceinline__ void add_slices(const Slice* from, uint32_t slices, W
         }
     }
     lds.mass[i] = m0, lds.mass[i + 1] = m1, lds.count[i] = c0, lds.count[i + 1] = c1;
-    for (uint32_t s = threadIdx.x; s < slices; s += kWideThreads) add(&lds.likely, ldg(&from[s].likely));
+    for (uint32_t s = threadIdx.x; s < slices; s += kWideThreads) add(&lds.likely, ldg(&from[s].sums.likely));
 }
 
 // The lists of a row's slices one after another, each wave some of the slices': how
@@ -855,8 +906,37 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_slices(Args a) {
     __syncthreads();
     Wide::fill_bins(values, r, o, lds);
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
-    if (threadIdx.x == 0) stg(&to->likely, lds.likely);
+    for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to->sums.mass + i, lds.mass[i]), stg(to->sums.count + i, lds.count[i]);
+    if (threadIdx.x == 0) stg(&to->sums.likely, lds.likely);
+}
+
+__global__ void __launch_bounds__(kWideThreads) k_sample_list(Args a) {
+    __shared__ Wide::Scratch lds;
+    const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
+    const vkml_sampling o = options_of(a, row);
+    if (greedy(o) || Wide::lists_first(o)) return;
+    const uint64_t first = first_of(a, row);
+    if (first == kNone) return;
+    Wide::Held values;
+    values.load(source_of(a, row), slice);
+    const Row r = row_of(logit_at(first), o, a.shift);
+    if (threadIdx.x == 0) lds.likely = 0, lds.listed = 0;
+    __syncthreads();
+    add_slices(a.parts + static_cast<uint64_t>(row) * a.slices, a.slices, lds);
+    __syncthreads();
+    Wide::sum_up<kBins, true>(lds.mass, lds.count, lds);
+    if (slice == 0) {
+        Sums* to = a.totals + row;
+        for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
+        if (threadIdx.x == 0) stg(&to->likely, lds.likely);
+    }
+    const Wide::Listed listed = Wide::first_listed(r, o, a.random[row], lds);
+    if (listed.n > 0) values.list(Wide::bounds_of(r, listed.some), Wide::bounds_of(r, listed.others), lds);
+    __syncthreads();
+    Slice* to = a.parts + blockIdx.x;
+    const uint32_t n = min(lds.listed, kList);
+    for (uint32_t i = threadIdx.x; i < n; i += kWideThreads) stg(to->id + i, lds.id[i]);
+    if (threadIdx.x == 0) stg(&to->listed, n);
 }
 
 __global__ void __launch_bounds__(kWideThreads) k_sample_pick(Args a) {
@@ -871,26 +951,35 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_pick(Args a) {
     } else {
         const Row r = row_of(logit_at(first), o, a.shift);
         Wide::Streamed values{source_of(a, row)};
-        const Slice* from = a.parts + static_cast<uint64_t>(row) * a.slices;
-        Wide::fill_table(a.shift, lds);
-        Wide::clear_bins(lds);
-        uint32_t n = kList + 1;
         const bool lists = Wide::lists_first(o);
+        Wide::fill_table(a.shift, lds);
         if (lists) {
-            n = join_lists(from, a.slices, lds);
-            __syncthreads();
+            Wide::clear_bins(lds);
+        } else {
+            const Sums* sums = a.totals + row;
+            for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) lds.mass[i] = ldg(sums->mass + i), lds.count[i] = ldg(sums->count + i);
+            if (threadIdx.x == 0) lds.likely = ldg(&sums->likely);
         }
-        if (n <= kList) {
-            Wide::weigh_listed(values.s, r, n, lds);
+        const uint32_t n = join_lists(a.parts + static_cast<uint64_t>(row) * a.slices, a.slices, lds);
+        __syncthreads();
+        Wide::Listed listed;
+        if (n <= kList) Wide::weigh_listed(values.s, r, n, lds);
+        if (!lists) {
+            if (n > 0) listed = Wide::first_listed(r, o, a.random[row], lds);
+        } else if (n <= kList) {
             Wide::bin_listed(r, n, lds);
-        } else if (lists) {
+            listed.some = {0, kBins - 1};
+            listed.n = n;
+        } else {
             Wide::fill_bins(values, r, o, lds);
             __syncthreads();
-        } else {
-            add_slices(from, a.slices, lds);
-            __syncthreads();
         }
-        id = n <= Wide::kFew ? Wide::pick_few(r, o, a.random[row], n, lds) : Wide::pick(values, r, o, a.random[row], n, lds);
+        if (lists && n <= Wide::kFew) {
+            id = Wide::pick_few(r, o, a.random[row], n, lds);
+        } else {
+            if (lists) Wide::sum_up<kBins, true>(lds.mass, lds.count, lds);
+            id = Wide::pick(values, r, o, a.random[row], listed, lds);
+        }
     }
     if (threadIdx.x == 0) stg(a.tokens + row, static_cast<int32_t>(id));
 }
@@ -922,7 +1011,8 @@ int vkml_sample(const vkml_sample_params* p, const float* logits, const vkml_sam
     a.slices = slices(p->vocab);
     if (a.slices > 1) {
         a.peaks = static_cast<uint64_t*>(workspace);
-        a.parts = reinterpret_cast<Slice*>(static_cast<uint8_t*>(workspace) + peaks_bytes(*p));
+        a.totals = reinterpret_cast<Sums*>(static_cast<uint8_t*>(workspace) + peaks_bytes(*p));
+        a.parts = reinterpret_cast<Slice*>(a.totals + p->rows);
     }
     // a row's weights fit 62 bits, one of them 51
     int32_t bits = 0;
@@ -940,6 +1030,7 @@ int vkml_sample(const vkml_sample_params* p, const float* logits, const vkml_sam
     if (a.slices == 1) return go(k_sample<kWideThreads>, p->rows, kWideThreads);
     if (const int r = go(k_sample_peaks, p->rows * a.slices, kWideThreads)) return r;
     if (const int r = go(k_sample_slices, p->rows * a.slices, kWideThreads)) return r;
+    if (const int r = go(k_sample_list, p->rows * a.slices, kWideThreads)) return r;
     return go(k_sample_pick, p->rows, kWideThreads);
 }
 

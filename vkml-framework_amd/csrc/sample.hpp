@@ -31,24 +31,25 @@ inline const char* check(const vkml_sample_params& p) {
     return nullptr;
 }
 
-// What a row of several slices keeps of one: its weights and counts by bin and its
-// mass within min_p; or the ids of the candidates that top_k or min_p leave of it,
-// more than kList where these are not all.
-struct Slice {
-    union {
-        uint64_t mass[kBins];
-        uint32_t id[kList];
-    };
-    union {
-        uint32_t count[kBins];
-        uint32_t listed;
-    };
+// Weights and counts by bin, and the mass within min_p: a slice's, or a row's up to
+// each bin.
+struct Sums {
+    uint64_t mass[kBins];
+    uint32_t count[kBins];
     uint64_t likely;
+    uint64_t unused;
+};
+// What a row of several slices keeps of one: its sums, and the ids of candidates, more
+// than kList where these are not all.
+struct Slice {
+    Sums sums;
+    uint32_t id[kList];
+    uint32_t listed, unused[3];
 };
 inline uint64_t peaks_bytes(const vkml_sample_params& p) { return (static_cast<uint64_t>(p.rows) * slices(p.vocab) * 8 + 15) / 16 * 16; }
 inline uint64_t workspace_bytes(const vkml_sample_params& p) {
     const uint64_t n = slices(p.vocab);
-    return n == 1 ? 0 : peaks_bytes(p) + static_cast<uint64_t>(p.rows) * n * sizeof(Slice);
+    return n == 1 ? 0 : peaks_bytes(p) + static_cast<uint64_t>(p.rows) * (sizeof(Sums) + n * sizeof(Slice));
 }
 
 }  // namespace vkml::sample
