@@ -289,6 +289,25 @@ int refusals(vkml::Context& ctx) {
     throws("not as the batch left it", [&] { c.cache.keep(batch, trees, ints, ints); });  // it has grown since
     if (c.cache.table().length(ids[0]) != 4 || c.cache.table().length(ids[1]) != 3) std::printf("a refused call changed a sequence\n"), ++wrong;
 
+    // Rows of a page that a fork reads, or that a page has left, are not moved.
+    for (const std::int64_t id : ids) c.cache.release(id);
+    const std::int64_t low = c.cache.create(), high = c.cache.create();
+    c.cache.batch(std::vector{low}, std::vector<std::int64_t>{1});
+    const PagedBatch drafts = c.cache.batch(std::vector{high}, std::vector<std::int64_t>{5});
+    const vkml::PagedTrees chain = c.cache.trees(drafts, std::vector<std::int32_t>{-1, 0, 1, 2, 3});
+    const std::int64_t fork = c.cache.fork(high);
+    throws("another's too", [&] { c.cache.keep(drafts, chain, ints, ints); });
+    c.cache.release(fork);
+    c.cache.release(low);
+    c.cache.compact();
+    throws("pages have moved", [&] { c.cache.keep(drafts, chain, ints, ints); });
+    if (c.cache.table().length(high) != 5) std::printf("a refused call changed a sequence\n"), ++wrong;
+    c.cache.truncate(high, 0);
+    const PagedBatch again = c.cache.batch(std::vector{high}, std::vector<std::int64_t>{5});
+    c.cache.release(c.cache.fork(high));
+    const vkml::KeptDrafts kept = c.cache.keep(again, chain, ints, ints);
+    if (kept.paths != std::vector<std::vector<std::int32_t>>{{0, 1, 2, 3, 4}} || c.cache.table().length(high) != 5) std::printf("not kept after a fork that is gone\n"), ++wrong;
+
     const Tensor logits = Tensor::zeros(ctx, {3, 10}, DType::F32);
     const std::vector<double> u = {0.1, 0.2, 0.3};
     vkml::SamplingOptions o;

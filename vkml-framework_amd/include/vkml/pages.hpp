@@ -54,6 +54,9 @@ public:
 
     std::int64_t length(std::int64_t id) const { return at(id).length; }
     const std::vector<std::int32_t>& row(std::int64_t id) const { return at(id).pages; }
+    // The pages that hold a sequence's keys from `first` on.
+    std::span<const std::int32_t> pages_from(std::int64_t id, std::int64_t first) const;
+    std::int64_t users(std::int32_t page) const { return users_.at(static_cast<std::size_t>(page)); }  // sequences that hold it
     std::int64_t pages() const noexcept { return static_cast<std::int64_t>(users_.size()); }
     std::int64_t page_size() const noexcept { return page_size_; }
     std::int64_t free_pages() const noexcept { return static_cast<std::int64_t>(free_.size()); }
@@ -82,6 +85,7 @@ struct PagedBatch {
     std::int64_t seqs = 0, tokens = 0, groups = 0;
     std::int64_t positions = 0;        // past the last position of a new token
     std::vector<std::int64_t> ids, before, added;  // the sequences, their earlier keys and their new tokens
+    std::vector<std::int32_t> new_pages;           // that hold these, sequence after sequence
 };
 
 // A batch's new tokens as trees, for speculative decoding: a sequence's first new
@@ -162,7 +166,7 @@ public:
     // Along each tree's path of tokens that are the pick after the one before, the keys
     // and values of every layer move to follow the sequence's earlier keys, and the
     // sequence ends there. Waits for the step. The sequences must be as the batch left
-    // them.
+    // them: not grown, moved by compact, or forked (but for forks that are gone).
     KeptDrafts keep(const PagedBatch& batch, const PagedTrees& trees, const Tensor& drafted, const Tensor& picked);
 
     const Tensor& k_pages() const noexcept { return k_; }  // [layers, pages, kv_heads, page_size, head_dim]

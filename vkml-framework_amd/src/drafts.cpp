@@ -80,8 +80,16 @@ KeptDrafts PagedCache::keep(const PagedBatch& batch, const PagedTrees& trees, co
             throw Error("PagedCache::keep: drafted and picked must be i32 " + to_string(want) + ", got " + std::string(to_string(t->dtype())) + " " + to_string(t->shape()));
         }
     }
+    // (Rows move within the new tokens' pages: they have to be the batch's still, and the
+    // sequence's own.)
+    auto page = batch.new_pages.begin();
     for (std::size_t i = 0; i < batch.ids.size(); ++i) {
-        if (table_.length(batch.ids[i]) != batch.before[i] + batch.added[i]) throw Error("PagedCache::keep: sequence " + std::to_string(batch.ids[i]) + " is not as the batch left it");
+        const std::string id = "PagedCache::keep: sequence " + std::to_string(batch.ids[i]);
+        if (table_.length(batch.ids[i]) != batch.before[i] + batch.added[i]) throw Error(id + " is not as the batch left it");
+        for (const std::int32_t now : table_.pages_from(batch.ids[i], batch.before[i])) {
+            if (page == batch.new_pages.end() || now != *page++) throw Error(id + " is not as the batch left it: its pages have moved");
+            if (table_.users(now) != 1) throw Error(id + "'s new keys are another's too");
+        }
     }
     KeptDrafts kept;
     kept.paths.resize(batch.ids.size());

@@ -24,6 +24,13 @@ const PageTable::Row& PageTable::at(std::int64_t id) const {
     return it->second;
 }
 
+std::span<const std::int32_t> PageTable::pages_from(std::int64_t id, std::int64_t first) const {
+    const Row& row = at(id);
+    if (first < 0 || first > row.length) throw Error("PageTable::pages_from: key " + std::to_string(first) + " of a sequence of " + std::to_string(row.length));
+    if (first == row.length) return {};
+    return std::span(row.pages).subspan(static_cast<std::size_t>(first / page_size_));
+}
+
 std::int32_t PageTable::take() {
     std::pop_heap(free_.begin(), free_.end(), std::greater<>());
     const std::int32_t page = free_.back();

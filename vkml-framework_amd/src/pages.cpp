@@ -115,6 +115,8 @@ PagedBatch PagedCache::batch(std::span<const std::int64_t> ids, std::span<const 
         for (std::size_t i = 0; i < ids.size(); ++i) {
             const auto& row = table_.row(ids[i]);
             std::copy(row.begin(), row.end(), table.begin() + static_cast<std::ptrdiff_t>(i * static_cast<std::size_t>(stride)));
+            const auto written = table_.pages_from(ids[i], b.before[i]);
+            b.new_pages.insert(b.new_pages.end(), written.begin(), written.end());
             lengths.push_back(static_cast<std::int32_t>(table_.length(ids[i])));
             starts.push_back(static_cast<std::int32_t>(starts.back() + tokens[i]));
         }
