@@ -44,9 +44,29 @@
 // reads the shared keys from memory); 2600 tokens of six prompts 147 us, 16 to join
 // (115 GFLOP).
 // What the three ways through a tile need at once is more than the scalar registers
-// hold: 155 to 198 are spilled to lanes of vector registers; of those none is.
+// hold: 161 to 195 are spilled to lanes of vector registers; of those none is.
 // Short ones are a chain of waits: 1.0 us for the batch's arrays, 0.8 to find the
 // part, 1.3 its first tile, 1.2 for pages and keys, 2 to 3 the block, 0.8 the end.
+//
+// The same kernel with another mask, as its own instances (MASK), so that the one above
+// keeps its registers. Trees (vkml_attend_pages_tree): the new tokens' keys are masked by
+// bits, up to three words a lane for 64 keys, read for blocks that hold new keys only;
+// the keys before these cost nothing more. Windows (vkml_attend_pages_window): a tile of
+// tokens whose window no longer begins at key 0 takes an axis of its own, the sinks and
+// then the keys from its first token's window on, as long as the longest such tile's
+// whatever the lengths (pages.hpp), so that the work is still cut without looking at
+// lengths; what is behind the window is neither read nor counted as cost.
+// Measured (a whole call, f16, 32 query and 8 KV heads of 128): 60 nodes over 8100 keys
+// 40 us, 31 of them the pieces (7.9 GFLOP: with the split counted twice 12.6 us at a
+// large product's rate) and 8.7 to join 512 pieces of 128 rows, 34 MB written and read;
+// 24 trees of 13 over 4100 shared keys 71 us, 8 to join (18.6 GFLOP: 29.7 us); 16 chats
+// of up to 30000 keys, windows of 4096, 56 us, 5 to join (245 MB: 4.3 TB/s); three prompts
+// of 1400 tokens, windows of 1024, 126 us, 15 to join (41 GFLOP: 65 us). Of many rows the
+// pieces are bound by the chain within a block (scores, weights, products; the next
+// block's loads run meanwhile): 17 us for four blocks of 64 keys with two workgroups a
+// compute unit, where the matrix units alone need 8. Of what is known from the start on,
+// 4 to 6 vector registers are in scratch memory with bits at f16 and head_dim 128, 3 with
+// a window and a soft cap.
 #include <hip/hip_runtime.h>
 
 #include <string>

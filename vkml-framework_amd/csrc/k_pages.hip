@@ -200,6 +200,9 @@ constexpr uint32_t kKeepVectors = 4;  // a thread has in flight
 // that it takes, both pools'. They are read and written by turns, 16 KB at most, since a
 // row may go to where another one comes from: never to where one of a later turn does, as
 // a path's k-th node is the k-th of the tree or a later one.
+// Bound by its waits (arrays, the walk, pages, rows: four in a chain) rather than by bytes:
+// one sequence's 16 layers 5.4 us, 24 sequences' 32 layers 9.2 (16 MB read and written, 3.2
+// us at a copy's rate; 11.2 with a workgroup a pool, which walks every tree twice).
 template <typename V>
 __global__ void __launch_bounds__(kThreads) k_keep_drafts(KeepArgs a) {
     constexpr int32_t kNodes = static_cast<int32_t>(vkml::pages::kMaxNodes);

@@ -19,6 +19,21 @@
 // so that the same row gives the same token whatever the atomics' order. e^x is
 // found in 64 bits, 2^(-n / 1024) from a table times a polynomial of degree 3, good to
 // 2^-50: the picks are those of sums in f64 unless a border is nearer than that.
+//
+// A row of up to 32768 logits is read once and stays in a workgroup's registers; a longer
+// one is cut into slices of as many, for a launch each of largest, weights, lists and
+// picks, since one workgroup for a row of 128256 would leave most of the GPU idle (40 rows)
+// and could not hold it.
+//
+// Measured (us): 1 row of 32768 9.8 (greedy, or top_k: 5 of it the launch and the load);
+// 40 24; 416 of requests that differ 32 (54 MB: 1.7 TB/s), 1024 74; 300 of 4096 15; 40
+// of 128256 48: 5 peaks, 14 weights, 14 lists, 14 picks. Not bound by bytes (10.6 us for
+// the 416, 4.0 for the 40 at a large copy's rate): a row whose candidates are all weighed
+// (top_p alone, or nothing) takes 18 by itself, 2 to load, 7 for 32 weights a thread, two
+// f64 products and polynomials and two LDS atomics each, 2 for the bins' sums, 2 to list, 4
+// for the rest, a chain of steps a few hundred clocks each between barriers; and a
+// workgroup of 1024 threads that holds a slice has a compute unit to itself (128 vector
+// registers a thread: with 64, so that two fit, they spill, and all rows got slower).
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -770,7 +785,9 @@ struct Picker {
 
 // ---------------------------------------------------------------- the launches
 
-// Rows of one slice: a workgroup a row, its values in registers.
+// Rows of one slice: a workgroup a row, its values in registers. (Of up to 8192 logits:
+// 256 threads, two workgroups a compute unit: 300 rows of 4096 15 us, 32 with 1024
+// threads.)
 template <uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
     using P = Picker<kThreads>;
@@ -817,7 +834,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
 // Longer rows, workgroups on slices of them: each slice's largest; then what top_k or
 // min_p keep of it, or its bins; for the latter rows then those candidates of each slice
 // that their picks begin with, found in all slices' bins (by each slice's workgroup for
-// itself: 98 KB of a row of 128256); then the picks.
+// itself: 98 KB of a row of 128256); then the picks. (40 rows of 128256: 48 us, 56 with
+// the picks' workgroups looking through their rows by themselves.)
 using Wide = Picker<kWideThreads>;
 
 __global__ void __launch_bounds__(kWideThreads) k_sample_peaks(Args a) {
