@@ -245,7 +245,7 @@ def test_draws_follow_the_weights():
     assert got.tolist() == ranked.tolist() * 3
 
 
-def test_a_million_rows_worth_of_small_rows():
+def test_twenty_thousand_small_rows():
     rng = np.random.default_rng(8)
     rows = 20000
     x = rng.standard_normal((rows, 6)).astype(np.float32)
