@@ -152,6 +152,16 @@ def test_rows_that_start_anywhere(offset, gap, vocab):
     check(like_a_model(rng, 13, vocab), *asked(rng, 13), stride=vocab + gap, offset=offset)
 
 
+@pytest.mark.parametrize("vocab", [192, 6000, 32768, 40000, 128256, 200000])
+def test_many_are_kept(vocab):
+    """By top_k on both sides of what is listed first, and by a min_p that leaves more
+    than a list holds."""
+    rng = np.random.default_rng(vocab + 1)
+    ks = [128, 191, 192, 193, 256, 257, 341, 512, 513, 768, 769, 1000, 1024, 1025, 5000]
+    o = [(1.0, k, p, 0.0) for k in ks for p in (0.9, 1.0)] + [(1.0, k, 1.0, m) for k in (0, 300, 2000) for m in (1e-5, 1e-3, 0.02)]
+    check(like_a_model(rng, len(o), vocab), o, rng.random(len(o)))
+
+
 @pytest.mark.parametrize("vocab", [1000, 32768, 128256])
 @pytest.mark.parametrize("step", [1 / 32, 1.0, 4.0])
 def test_equal_logits(step, vocab):

@@ -8,11 +8,11 @@
 // sorted: a candidate is found by its count or mass before it, in a histogram of the
 // weights' logarithms, then among its bin's candidates.
 //
-// Where top_k (of at most as many as a workgroup has threads) or min_p alone leave few,
-// these are listed first, and the rest is never weighed: the k-th largest of the
-// threads' own largest logits is a bound that at least k reach, and few more do. A list
-// of up to a quarter of the threads is ranked outright, every candidate against every
-// other; a longer one goes through a histogram of its own.
+// Where top_k (at most three quarters of a workgroup's threads, fewer in long rows) or
+// min_p alone leave few, these are listed first, and the rest is never weighed: the k-th
+// largest of the threads' own largest logits is a bound that at least k reach, and few
+// more do. A list of up to a quarter of the threads is ranked outright, every candidate
+// against every other; a longer one goes through a histogram of its own.
 //
 // Weights are whole numbers, units of 2^-shift of the largest (45 bits for 2^17
 // logits, so that all of a row's fit 62 bits): sums of them are exact in any order,
@@ -27,7 +27,7 @@
 //
 // Measured (us): 1 row of 32768 9.8 (greedy, or top_k: 5 of it the launch and the load);
 // 40 24; 416 of requests that differ 32 (54 MB: 1.7 TB/s), 1024 74; 300 of 4096 15; 40
-// of 128256 48: 5 peaks, 14 weights, 14 lists, 14 picks. Not bound by bytes (10.6 us for
+// of 128256 46 to 53: 5 peaks, 14 weights, 14 lists, 14 picks. Not bound by bytes (10.6 us for
 // the 416, 4.0 for the 40 at a large copy's rate): a row whose candidates are all weighed
 // (top_p alone, or nothing) takes 18 by itself, 2 to load, 7 for 32 weights a thread, two
 // f64 products and polynomials and two LDS atomics each, 2 for the bins' sums, 2 to list, 4
@@ -405,7 +405,7 @@ struct Picker {
         uint32_t kind = 3;
         if (t < a.rows) {
             const vkml_sampling o = options_of(a, t);
-            kind = greedy(o) ? 2 : lists_first(o) ? 1 : 0;
+            kind = greedy(o) ? 2 : lists_first(o, 1) ? 1 : 0;
         }
         uint32_t* counts = lds.sub_count;  // [3, kWaves]
         uint64_t mine = 0;
@@ -743,9 +743,13 @@ struct Picker {
         return lds.ranked_id[holds(unit_of(random, mass))];
     }
 
-    // Whether the candidates that top_k or min_p keep are listed first.
-    static __device__ __forceinline__ bool lists_first(const vkml_sampling& o) {
-        return (o.top_k > 0 && static_cast<uint32_t>(o.top_k) <= kThreads) || !weighs_all(o);
+    // Whether the candidates that top_k or min_p keep are listed first. (top_k: of values
+    // in no order the slices list about n (1 - (1 - top_k / kThreads)^(1 / 32)) of their n each:
+    // 1387 of one slice at three quarters of the threads, 1178 of four at a quarter. With more
+    // the list does not hold them all, and they are weighed after all: top_k 1000 of 40 rows
+    // of 128256 so 78 us, weighed at once 47.)
+    static __device__ __forceinline__ bool lists_first(const vkml_sampling& o, uint32_t slices) {
+        return (o.top_k > 0 && static_cast<uint32_t>(o.top_k) <= kThreads / 4 * 3 && static_cast<uint64_t>(o.top_k) * slices <= kThreads) || !weighs_all(o);
     }
     // Lists them, and what else is in their bins: the ids, lds.listed of them (more than
     // the list holds: some). Largest: of the thread's values. The counts are as they were,
@@ -807,7 +811,7 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
     } else {
         const Row r = row_of(peak, o, a.shift);
         uint32_t n = kList + 1;
-        if (P::lists_first(o)) {
+        if (P::lists_first(o, 1)) {
             P::list_kept(values, largest, r, o, lds);
             n = lds.listed;
         }
@@ -834,8 +838,9 @@ __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
 // Longer rows, workgroups on slices of them: each slice's largest; then what top_k or
 // min_p keep of it, or its bins; for the latter rows then those candidates of each slice
 // that their picks begin with, found in all slices' bins (by each slice's workgroup for
-// itself: 98 KB of a row of 128256); then the picks. (40 rows of 128256: 48 us, 56 with
-// the picks' workgroups looking through their rows by themselves.)
+// itself: 98 KB of a row of 128256), and the bins of those that listed too much; then the
+// picks. (40 rows of 128256: 48 us, 56 with the picks' workgroups looking through their
+// rows by themselves.)
 using Wide = Picker<kWideThreads>;
 
 __global__ void __launch_bounds__(kWideThreads) k_sample_peaks(Args a) {
@@ -884,8 +889,16 @@ __device__ __forceinline__ void add_slices(const Slice* from, uint32_t slices, W
     for (uint32_t s = threadIdx.x; s < slices; s += kWideThreads) add(&lds.likely, ldg(&from[s].sums.likely));
 }
 
-// The lists of a row's slices one after another, each wave some of the slices': how
-// many are listed (more than kList where these are not all).
+// How many a row's slices have listed (more than kList where these are not all).
+__device__ __forceinline__ uint32_t listed_in(const Slice* from, uint32_t slices) {
+    uint32_t n = 0;
+    for (uint32_t s0 = 0; s0 < slices; s0 += kWave) {
+        const uint32_t s = s0 + threadIdx.x % kWave, of = s < slices ? min(ldg(&from[s].listed), kList + 1) : 0u;
+        n = min(n + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(inclusive_sum(static_cast<int32_t>(of))), kWave - 1)), kList + 1);
+    }
+    return n;
+}
+// The lists, one after another, each wave some of the slices'; how many as above.
 __device__ __forceinline__ uint32_t join_lists(const Slice* from, uint32_t slices, Wide::Scratch& lds) {
     uint32_t n = 0;
     for (uint32_t s0 = 0; s0 < slices; s0 += kWave) {
@@ -900,6 +913,19 @@ __device__ __forceinline__ uint32_t join_lists(const Slice* from, uint32_t slice
     return n;
 }
 
+__device__ __forceinline__ void store_sums(Sums& to, const Wide::Scratch& lds) {
+    for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to.mass + i, lds.mass[i]), stg(to.count + i, lds.count[i]);
+    if (threadIdx.x == 0) stg(&to.likely, lds.likely);
+}
+// A slice's weights, by bins that are 0.
+__device__ __forceinline__ void sum_slice(const Args& a, Wide::Held& values, const Row& r, const vkml_sampling& o, Sums& to, Wide::Scratch& lds) {
+    Wide::fill_table(a.shift, lds);
+    __syncthreads();
+    Wide::fill_bins(values, r, o, lds);
+    __syncthreads();
+    store_sums(to, lds);
+}
+
 __global__ void __launch_bounds__(kWideThreads) k_sample_slices(Args a) {
     __shared__ Wide::Scratch lds;
     const uint32_t row = blockIdx.x / a.slices;
@@ -912,7 +938,7 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_slices(Args a) {
     const Row r = row_of(logit_at(first), o, a.shift);
     Wide::clear_bins(lds);
     Slice* to = a.parts + blockIdx.x;
-    if (Wide::lists_first(o)) {
+    if (Wide::lists_first(o, a.slices)) {
         Wide::list_kept(values, values.largest(), r, o, lds);
         const uint32_t n = lds.listed;
         if (threadIdx.x == 0) stg(&to->listed, n);
@@ -920,34 +946,31 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_slices(Args a) {
         for (uint32_t i = threadIdx.x; i < n; i += kWideThreads) stg(to->id + i, lds.id[i]);
         return;
     }
-    Wide::fill_table(a.shift, lds);
-    __syncthreads();
-    Wide::fill_bins(values, r, o, lds);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to->sums.mass + i, lds.mass[i]), stg(to->sums.count + i, lds.count[i]);
-    if (threadIdx.x == 0) stg(&to->sums.likely, lds.likely);
+    sum_slice(a, values, r, o, to->sums, lds);
 }
 
 __global__ void __launch_bounds__(kWideThreads) k_sample_list(Args a) {
     __shared__ Wide::Scratch lds;
     const uint32_t row = blockIdx.x / a.slices, slice = blockIdx.x % a.slices;
     const vkml_sampling o = options_of(a, row);
-    if (greedy(o) || Wide::lists_first(o)) return;
     const uint64_t first = first_of(a, row);
-    if (first == kNone) return;
+    if (greedy(o) || first == kNone) return;
+    const Slice* parts = a.parts + static_cast<uint64_t>(row) * a.slices;
+    const bool lists = Wide::lists_first(o, a.slices);
+    if (lists && listed_in(parts, a.slices) <= kList) return;
     Wide::Held values;
     values.load(source_of(a, row), slice);
     const Row r = row_of(logit_at(first), o, a.shift);
+    if (lists) {
+        Wide::clear_bins(lds);
+        return sum_slice(a, values, r, o, a.parts[blockIdx.x].sums, lds);
+    }
     if (threadIdx.x == 0) lds.likely = 0, lds.listed = 0;
     __syncthreads();
-    add_slices(a.parts + static_cast<uint64_t>(row) * a.slices, a.slices, lds);
+    add_slices(parts, a.slices, lds);
     __syncthreads();
     Wide::sum_up<kBins, true>(lds.mass, lds.count, lds);
-    if (slice == 0) {
-        Sums* to = a.totals + row;
-        for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) stg(to->mass + i, lds.mass[i]), stg(to->count + i, lds.count[i]);
-        if (threadIdx.x == 0) stg(&to->likely, lds.likely);
-    }
+    if (slice == 0) store_sums(a.totals[row], lds);
     const Wide::Listed listed = Wide::first_listed(r, o, a.random[row], lds);
     if (listed.n > 0) values.list(Wide::bounds_of(r, listed.some), Wide::bounds_of(r, listed.others), lds);
     __syncthreads();
@@ -969,7 +992,7 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_pick(Args a) {
     } else {
         const Row r = row_of(logit_at(first), o, a.shift);
         Wide::Streamed values{source_of(a, row)};
-        const bool lists = Wide::lists_first(o);
+        const bool lists = Wide::lists_first(o, a.slices);
         Wide::fill_table(a.shift, lds);
         if (lists) {
             Wide::clear_bins(lds);
@@ -978,7 +1001,8 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_pick(Args a) {
             for (uint32_t i = threadIdx.x; i < kBins; i += kWideThreads) lds.mass[i] = ldg(sums->mass + i), lds.count[i] = ldg(sums->count + i);
             if (threadIdx.x == 0) lds.likely = ldg(&sums->likely);
         }
-        const uint32_t n = join_lists(a.parts + static_cast<uint64_t>(row) * a.slices, a.slices, lds);
+        const Slice* parts = a.parts + static_cast<uint64_t>(row) * a.slices;
+        const uint32_t n = join_lists(parts, a.slices, lds);
         __syncthreads();
         Wide::Listed listed;
         if (n <= kList) Wide::weigh_listed(values.s, r, n, lds);
@@ -989,7 +1013,7 @@ __global__ void __launch_bounds__(kWideThreads) k_sample_pick(Args a) {
             listed.some = {0, kBins - 1};
             listed.n = n;
         } else {
-            Wide::fill_bins(values, r, o, lds);
+            add_slices(parts, a.slices, lds);
             __syncthreads();
         }
         if (lists && n <= Wide::kFew) {
