@@ -1,0 +1,163 @@
+// vkml::PagedCache's drafts without a device: the calls of the C ABI that it makes are
+// here, over host memory.
+// Usage: drafts_host_check PART. Prints a line a check ("ok" or what is wrong).
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+#include <functional>
+#include <string>
+#include <vector>
+
+#include "vkml/pages.hpp"
+#include "vkml_hip.h"
+
+extern "C" {
+const char* vkml_last_error(void) { return "made to fail"; }
+int vkml_is_initialized(void) { return 1; }
+int vkml_init(const char*) { return VKML_OK; }
+int vkml_shutdown(void) { return VKML_OK; }
+int vkml_synchronize(void) { return VKML_OK; }
+int vkml_get_device_info(vkml_device_info* info) { return *info = {}, VKML_OK; }
+int vkml_set_profiling(int) { return VKML_OK; }
+int vkml_get_profiling(void) { return 0; }
+int vkml_profile(vkml_kernel_time*, uint32_t, uint32_t* count) { return *count = 0, VKML_OK; }
+int vkml_reset_profile(void) { return VKML_OK; }
+int vkml_malloc(uint64_t bytes, void** out) {
+    *out = std::malloc(bytes);
+    return VKML_OK;
+}
+int vkml_free(void* p) { return std::free(p), VKML_OK; }
+int vkml_fill_u32(void* d, uint32_t v, uint64_t words) {
+    for (uint64_t i = 0; i < words; ++i) static_cast<uint32_t*>(d)[i] = v;
+    return VKML_OK;
+}
+int vkml_memcpy_h2d(void* d, const void* h, uint64_t n) { return std::memcpy(d, h, n), VKML_OK; }
+int vkml_memcpy_d2h(void* h, const void* d, uint64_t n) { return std::memcpy(h, d, n), VKML_OK; }
+int vkml_copy_pages(const vkml_copy_pages_params* p, const int32_t* src, const int32_t* dst, void* k, void* v) {
+    for (uint32_t layer = 0; layer < p->layers; ++layer)
+        for (uint32_t i = 0; i < p->count; ++i)
+            for (void* pool : {k, v}) {
+                char* base = static_cast<char*>(pool) + layer * p->pages * p->page_bytes;
+                std::memcpy(base + dst[i] * p->page_bytes, base + src[i] * p->page_bytes, p->page_bytes);
+            }
+    return VKML_OK;
+}
+int vkml_rope_kv_pages(const vkml_rope_kv_pages_params*, const float*, const float*, const int32_t*, const int32_t*, const int32_t*, const int32_t*, float*, void*,
+                       void*) {
+    return VKML_OK;
+}
+uint64_t vkml_attend_pages_workspace_bytes(const vkml_attend_pages_params*) { return 64; }
+int vkml_attend_pages(const vkml_attend_pages_params*, const float*, const void*, const void*, const int32_t*, const int32_t*, const int32_t*, const int32_t*,
+                      const int32_t*, void*, float*) {
+    return VKML_OK;
+}
+int vkml_attend_pages_tree(const vkml_attend_pages_params*, uint32_t, const float*, const void*, const void*, const int32_t*, const int32_t*, const int32_t*,
+                           const int32_t*, const int32_t*, const uint32_t*, void*, float*) {
+    return VKML_OK;
+}
+int vkml_attend_pages_window(const vkml_attend_pages_params*, uint32_t, uint32_t, const float*, const void*, const void*, const int32_t*, const int32_t*,
+                             const int32_t*, void*, float*) {
+    return VKML_OK;
+}
+// (one layer of keys of one head; row by row in the path's order)
+int vkml_keep_drafts(const vkml_keep_drafts_params* p, const int32_t* parents, const int32_t* drafted, const int32_t* picked, const int32_t* table,
+                     const int32_t* lengths, const int32_t* starts, int32_t* path, int32_t* counts, int32_t* next, void* k, void* v) {
+    const uint64_t bytes = p->head_dim * 4;
+    for (uint32_t s = 0; s < p->seqs; ++s) {
+        const int32_t first = starts[s], n = starts[s + 1] - first, base = lengths[s] - n;
+        int32_t at = -1, count = 0;
+        const auto row = [&](void* pool, int32_t pos) {
+            return static_cast<char*>(pool) + (static_cast<uint64_t>(table[s * p->table_stride + static_cast<uint32_t>(pos) / p->page_size]) * p->page_size + static_cast<uint32_t>(pos) % p->page_size) * bytes;
+        };
+        for (int32_t i = 0; i < n; ++i) path[first + i] = -1;
+        for (int32_t i = 0; i < n; ++i) {
+            if (i > 0 && (parents[first + i] != at || drafted[first + i] != picked[first + at])) continue;
+            for (void* pool : {k, v}) std::memmove(row(pool, base + count), row(pool, base + i), bytes);
+            path[first + count++] = at = i;
+        }
+        counts[s] = count;
+        next[s] = n > 0 ? picked[first + at] : -1;
+    }
+    return VKML_OK;
+}
+}
+
+namespace {
+
+using Ids = std::vector<std::int64_t>;
+using Ints = std::vector<std::int32_t>;
+using vkml::DType;
+using vkml::Tensor;
+constexpr std::int64_t kPages = 40, kPage = 16;
+
+int wrong = 0;
+void expect(bool ok, const std::string& what) {
+    if (!ok && wrong++ < 10) std::printf("%s\n", what.c_str());
+}
+void throws(const char* why, const char* what, const std::function<void()>& f) {
+    try {
+        f();
+    } catch (const vkml::Error& e) {
+        expect(std::string(e.what()).find(why) != std::string::npos, std::string(what) + ": \"" + e.what() + "\" for \"" + why + "\"");
+        return;
+    }
+    expect(false, std::string(what) + ": not refused: " + why);
+}
+
+// A cache of one layer, with keys of one head of two dims.
+struct Cache {
+    vkml::Context ctx;
+    vkml::PagedCache c{ctx, 1, 1, 2, kPages, kPage, DType::F32};
+
+    Tensor ints(const Ints& x) { return Tensor::from_data<std::int32_t>(ctx, x, {static_cast<std::int64_t>(x.size())}); }
+    Tensor qkv(const vkml::PagedBatch& b) { return Tensor::zeros(ctx, {b.tokens, 6}, DType::F32); }
+    Tensor q(const vkml::PagedBatch& b) { return Tensor::zeros(ctx, {b.tokens, 1, 2}, DType::F32); }
+};
+
+void trees() {
+    Cache x;
+    vkml::PagedCache& c = x.c;
+    const std::int64_t a = c.create(), b = c.create();
+    c.batch(Ids{a, b}, Ids{10, 3});
+    const Ints parents = {-1, 0, 0, -1, 0, 1};
+    const vkml::PagedBatch first = c.batch(Ids{a, b}, Ids{3, 3});
+    const vkml::PagedTrees of_first = c.trees(first, parents);
+    const Tensor none, drafted = x.ints({5, 6, 7, 8, 9, 4}), picked = x.ints({6, 0, 0, 9, 4, 1});
+    const auto refused = [&](const char* what, const vkml::PagedBatch& batch) {
+        const std::int64_t la = c.table().length(a), lb = c.table().length(b);
+        throws("another batch", what, [&] { c.append(0, batch, x.qkv(batch), none, vkml::RopeStyle::Interleaved, &of_first); });
+        throws("another batch", what, [&] { c.attention_tree(0, batch, of_first, x.q(batch)); });
+        throws("another batch", what, [&] { c.keep(batch, of_first, drafted, picked); });
+        expect(c.table().length(a) == la && c.table().length(b) == lb, std::string(what) + ": a refused call changed a sequence");
+    };
+    const auto back = [&] { c.truncate(a, 10), c.truncate(b, 3); };
+    back();
+    refused("the sequences in another order", c.batch(Ids{b, a}, Ids{3, 3}));
+    back();
+    refused("as many new tokens in all, not of each", c.batch(Ids{a, b}, Ids{2, 4}));
+    back();
+    refused("one sequence of as many", c.batch(Ids{a}, Ids{6}));
+    back();
+    refused("a third, without tokens", c.batch(Ids{a, b, c.create()}, Ids{3, 3, 0}));
+    back();
+    c.batch(Ids{a}, Ids{1});
+    refused("the next step's", c.batch(Ids{a, b}, Ids{3, 3}));
+    // What the trees say is as true of a batch of as many earlier keys and new tokens.
+    back();
+    const vkml::PagedBatch again = c.batch(Ids{a, b}, Ids{3, 3});
+    c.append(0, again, x.qkv(again), none, vkml::RopeStyle::Interleaved, &of_first);
+    c.attention_tree(0, again, of_first, x.q(again));
+    const vkml::KeptDrafts kept = c.keep(again, of_first, drafted, picked);
+    expect(kept.paths == std::vector<Ints>{{0, 1}, {0, 1, 2}} && kept.next == Ints{0, 1}, "another path");
+    expect(c.table().length(a) == 12 && c.table().length(b) == 6, "another length");
+}
+
+}  // namespace
+
+int main(int argc, char** argv) {
+    const std::string part = argc == 2 ? argv[1] : "";
+    if (part == "trees") trees();
+    else return 2;
+    std::printf("%s %s\n", wrong ? "WRONG" : "ok", part.c_str());
+    return wrong != 0;
+}

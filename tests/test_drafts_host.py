@@ -1,0 +1,30 @@
+"""vkml::PagedCache's trees of drafted tokens (vkml-framework_amd/src/drafts.cpp) on the
+CPU, over a C ABI in host memory (tests/cpp/drafts_host_check.cpp)."""
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.fixture(scope="module")
+def check(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("bin") / "drafts_host_check")
+    pkg = os.path.join(ROOT, "vkml-framework_amd")
+    subprocess.run(["g++", "-std=c++20", "-O1", "-g", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover", "-I" + os.path.join(pkg, "include"),
+                    "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(pkg, "src"), os.path.join(ROOT, "tests", "cpp", "drafts_host_check.cpp"),
+                    *(os.path.join(pkg, "src", f) for f in ("drafts.cpp", "pages.cpp", "page_table.cpp", "runtime.cpp")), "-o", out], check=True)
+
+    def run(part):
+        r = subprocess.run([out, part], capture_output=True, text=True, timeout=100)
+        print(r.stdout)
+        assert r.returncode == 0 and r.stdout.endswith("ok " + part + "\n"), r.stdout + r.stderr
+
+    return run
+
+
+def test_trees_of_another_batch_are_refused(check):
+    """Whose sequences have other earlier keys or get other numbers of new tokens, even
+    if these are as many in all; a refused call changes no sequence."""
+    check("trees")

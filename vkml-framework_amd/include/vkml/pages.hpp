@@ -94,6 +94,11 @@ struct PagedBatch {
 struct PagedTrees {
     Tensor parents, seen, positions;  // i32 [tokens], [tokens, words], [tokens]
     std::int64_t deepest = 0;         // past the last position
+    std::vector<std::int64_t> before, added;  // the batch's
+
+    // Whether they are of this batch, or of one whose sequences had as many keys and got
+    // as many new tokens, each: then its masks and positions are the same.
+    bool fit(const PagedBatch& batch) const { return before == batch.before && added == batch.added; }
 };
 
 // What a step of speculative decoding keeps of each of a batch's sequences: the
@@ -138,8 +143,8 @@ public:
     // sequence after sequence: q and k rotated at their positions by a table
     // from rope_table (for a part of the head: of that many dims; null: not
     // rotated) that holds them all, k and v into a layer's pages. Returns q
-    // [tokens, heads, head_dim]. With trees (of this batch) a token is rotated at its
-    // depth's position, not at its place in the sequence.
+    // [tokens, heads, head_dim]. With trees, which must fit the batch, a token is rotated
+    // at its depth's position, not at its place in the sequence.
     Tensor append(std::int64_t layer, const PagedBatch& batch, const Tensor& qkv, const Tensor& rope_table, RopeStyle style,
                   const PagedTrees* trees = nullptr);
 
@@ -153,7 +158,8 @@ public:
 
     // A step of speculative decoding: trees of a batch's new tokens; for each layer
     // append (with the trees) and attention_tree; the model's pick after
-    // every token (vkml::sample or argmax of its logits); then keep.
+    // every token (vkml::sample or argmax of its logits); then keep. Trees that do not
+    // fit the batch are refused.
     // parents [tokens], sequence after sequence: the index, among its sequence's new
     // tokens, of the one that a token was drafted after; -1 for a sequence's first (and
     // for a token that sees no other new one, which is never kept). At most 4096 new

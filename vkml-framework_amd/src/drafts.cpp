@@ -53,6 +53,8 @@ PagedTrees PagedCache::trees(const PagedBatch& batch, std::span<const std::int32
     }
     for (std::size_t i = 0; i < seen.size(); ++i) bits[i] = static_cast<std::int32_t>(seen[i]);
     detail::Runtime& runtime = TensorAccess::runtime(k_);
+    t.before = batch.before;
+    t.added = batch.added;
     t.parents = array(runtime, {batch.tokens});
     t.seen = array(runtime, {batch.tokens, static_cast<std::int64_t>(words)});
     t.positions = array(runtime, {batch.tokens});
@@ -63,8 +65,8 @@ PagedTrees PagedCache::trees(const PagedBatch& batch, std::span<const std::int32
 }
 
 Tensor PagedCache::attention_tree(std::int64_t layer, const PagedBatch& batch, const PagedTrees& trees, const Tensor& q, float softcap) const {
+    if (!trees.fit(batch)) throw Error("PagedCache::attention_tree: the trees are of another batch");
     const Shape& s = trees.seen.shape();
-    if (s.size() != 2 || s[0] != batch.tokens) throw Error("PagedCache::attention_tree: the trees are of another batch");
     return attend("PagedCache::attention_tree", batch, q, softcap, [&](const vkml_attend_pages_params& p, void* workspace, float* out) {
         return vkml_attend_pages_tree(&p, u32(s[1]), static_cast<const float*>(q.data()), pool(k_, layer), pool(v_, layer), ints(batch.table), ints(batch.lengths),
                                       ints(batch.starts), batch.groups > 0 ? ints(batch.group_starts) : nullptr,
@@ -74,7 +76,7 @@ Tensor PagedCache::attention_tree(std::int64_t layer, const PagedBatch& batch, c
 
 KeptDrafts PagedCache::keep(const PagedBatch& batch, const PagedTrees& trees, const Tensor& drafted, const Tensor& picked) {
     const Shape want = {batch.tokens};
-    if (trees.parents.shape() != want) throw Error("PagedCache::keep: the trees are of another batch");
+    if (!trees.fit(batch)) throw Error("PagedCache::keep: the trees are of another batch");
     for (const Tensor* t : {&drafted, &picked}) {
         if (t->dtype() != DType::I32 || t->shape() != want) {
             throw Error("PagedCache::keep: drafted and picked must be i32 " + to_string(want) + ", got " + std::string(to_string(t->dtype())) + " " + to_string(t->shape()));

@@ -154,7 +154,7 @@ Tensor PagedCache::append(std::int64_t layer, const PagedBatch& batch, const Ten
     if (rotated && (rope_table.dtype() != DType::F32 || t.size() != 3 || t[1] * 2 > head_dim_ || t[2] != 2)) {
         throw Error("PagedCache::append: heads of " + std::to_string(head_dim_) + " do not match the table " + to_string(t) + " from rope_table");
     }
-    if (trees && trees->positions.shape() != Shape{batch.tokens}) throw Error("PagedCache::append: the trees are of another batch");
+    if (trees && !trees->fit(batch)) throw Error("PagedCache::append: the trees are of another batch");
     const std::int64_t positions = trees ? trees->deepest : batch.positions;
     if (rotated && positions > t[0]) {
         throw Error("PagedCache::append: positions up to " + std::to_string(positions - 1) + " are outside the table's " + std::to_string(t[0]) + " positions");
