@@ -152,11 +152,49 @@ void trees() {
     expect(c.table().length(a) == 12 && c.table().length(b) == 6, "another length");
 }
 
+// A sequence that was cut and has as many keys again, in the same pages, holds others
+// than the batch's.
+void stale() {
+    Cache x;
+    vkml::PagedCache& c = x.c;
+    const std::int64_t a = c.create(), b = c.create();
+    c.batch(Ids{a, b}, Ids{10, 3});
+    const Tensor drafted = x.ints({5, 6, 7}), others = x.ints({4, 4, 4}), all = x.ints({6, 7, 0});
+    const Ints parents = {-1, 0, 1};
+    const auto refused = [&](const char* what, const vkml::PagedBatch& batch, const vkml::PagedTrees& trees) {
+        const std::int64_t length = c.table().length(a);
+        throws("not as the batch left it", what, [&] { c.keep(batch, trees, drafted, all); });
+        expect(c.table().length(a) == length, std::string(what) + ": a refused call changed a sequence");
+    };
+    const vkml::PagedBatch first = c.batch(Ids{a}, Ids{3});
+    const vkml::PagedTrees trees = c.trees(first, parents);
+    c.keep(first, trees, drafted, others);  // one stays
+    const vkml::PagedBatch second = c.batch(Ids{a}, Ids{2});
+    expect(c.table().length(a) == 13, "the test's own lengths");
+    refused("kept, and grown to as many", first, trees);
+    c.truncate(a, 10);
+    refused("cut", first, trees);
+    const vkml::PagedBatch third = c.batch(Ids{a}, Ids{3});
+    refused("cut, and grown to as many", first, trees);
+    throws("not as the batch left it", "cut, and grown past", [&] { c.keep(second, c.trees(second, Ints{-1, 0}), x.ints({7, 4}), x.ints({0, 0})); });
+    // What leaves a sequence's keys as they are does not matter.
+    c.release(c.fork(a));
+    c.batch(Ids{b, a}, Ids{20, 0});
+    c.truncate(a, 13);
+    c.truncate(b, 1);
+    try {
+        c.batch(Ids{a}, Ids{kPages * kPage});
+    } catch (const vkml::Error&) {
+    }
+    expect(c.keep(third, trees, drafted, all).paths == std::vector<Ints>{{0, 1, 2}}, "another path");
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
     const std::string part = argc == 2 ? argv[1] : "";
     if (part == "trees") trees();
+    else if (part == "stale") stale();
     else return 2;
     std::printf("%s %s\n", wrong ? "WRONG" : "ok", part.c_str());
     return wrong != 0;

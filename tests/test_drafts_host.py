@@ -28,3 +28,8 @@ def test_trees_of_another_batch_are_refused(check):
     """Whose sequences have other earlier keys or get other numbers of new tokens, even
     if these are as many in all; a refused call changes no sequence."""
     check("trees")
+
+
+def test_a_batch_whose_keys_have_gone_is_not_kept(check):
+    """Of a sequence that was cut and then grew to the batch's length again."""
+    check("stale")

@@ -56,6 +56,8 @@ public:
     const std::vector<std::int32_t>& row(std::int64_t id) const { return at(id).pages; }
     // The pages that hold a sequence's keys from `first` on.
     std::span<const std::int32_t> pages_from(std::int64_t id, std::int64_t first) const;
+    // How often a sequence has grown or was cut (an append taken back does not count).
+    std::int64_t changes(std::int64_t id) const { return at(id).changes; }
     std::int64_t users(std::int32_t page) const { return users_.at(static_cast<std::size_t>(page)); }  // sequences that hold it
     std::int64_t pages() const noexcept { return static_cast<std::int64_t>(users_.size()); }
     std::int64_t page_size() const noexcept { return page_size_; }
@@ -64,7 +66,7 @@ public:
 private:
     struct Row {
         std::vector<std::int32_t> pages;
-        std::int64_t length = 0;
+        std::int64_t length = 0, changes = 0;
     };
     const Row& at(std::int64_t id) const;
     std::int64_t pages_for(std::int64_t length) const { return (length + page_size_ - 1) / page_size_; }
@@ -86,6 +88,7 @@ struct PagedBatch {
     std::int64_t positions = 0;        // past the last position of a new token
     std::vector<std::int64_t> ids, before, added;  // the sequences, their earlier keys and their new tokens
     std::vector<std::int32_t> new_pages;           // that hold these, sequence after sequence
+    std::vector<std::int64_t> changes;             // of each sequence so far, in the table
 };
 
 // A batch's new tokens as trees, for speculative decoding: a sequence's first new
@@ -172,7 +175,7 @@ public:
     // Along each tree's path of tokens that are the pick after the one before, the keys
     // and values of every layer move to follow the sequence's earlier keys, and the
     // sequence ends there. Waits for the step. The sequences must be as the batch left
-    // them: not grown, moved by compact, or forked (but for forks that are gone).
+    // them: not grown or cut, moved by compact, or forked (but for forks that are gone).
     KeptDrafts keep(const PagedBatch& batch, const PagedTrees& trees, const Tensor& drafted, const Tensor& picked);
 
     const Tensor& k_pages() const noexcept { return k_; }  // [layers, pages, kv_heads, page_size, head_dim]

@@ -87,7 +87,7 @@ KeptDrafts PagedCache::keep(const PagedBatch& batch, const PagedTrees& trees, co
     auto page = batch.new_pages.begin();
     for (std::size_t i = 0; i < batch.ids.size(); ++i) {
         const std::string id = "PagedCache::keep: sequence " + std::to_string(batch.ids[i]);
-        if (table_.length(batch.ids[i]) != batch.before[i] + batch.added[i]) throw Error(id + " is not as the batch left it");
+        if (table_.changes(batch.ids[i]) != batch.changes[i]) throw Error(id + " is not as the batch left it");
         for (const std::int32_t now : table_.pages_from(batch.ids[i], batch.before[i])) {
             if (page == batch.new_pages.end() || now != *page++) throw Error(id + " is not as the batch left it: its pages have moved");
             if (table_.users(now) != 1) throw Error(id + "'s new keys are another's too");

@@ -73,6 +73,7 @@ void PageTable::truncate(std::int64_t id, std::int64_t length) {
         give(mine.pages.back());
         mine.pages.pop_back();
     }
+    if (mine.length != length) ++mine.changes;
     mine.length = length;
 }
 
@@ -113,6 +114,7 @@ std::vector<PageCopy> PageTable::append(std::span<const std::int64_t> ids, std::
             row.pages.back() = page;
         }
         row.length += tokens[i];
+        if (tokens[i] > 0) ++row.changes;
         while (static_cast<std::int64_t>(row.pages.size()) < pages_for(row.length)) row.pages.push_back(take());
     }
     return copies;
@@ -127,6 +129,7 @@ void PageTable::undo(std::span<const std::int64_t> ids, std::span<const std::int
     for (std::size_t i = 0; i < ids.size(); ++i) {
         Row& row = rows_.find(ids[i])->second;
         row.length -= tokens[i];
+        if (tokens[i] > 0) --row.changes;
         while (static_cast<std::int64_t>(row.pages.size()) > pages_for(row.length)) {
             give(row.pages.back());
             row.pages.pop_back();

@@ -117,6 +117,7 @@ PagedBatch PagedCache::batch(std::span<const std::int64_t> ids, std::span<const 
             std::copy(row.begin(), row.end(), table.begin() + static_cast<std::ptrdiff_t>(i * static_cast<std::size_t>(stride)));
             const auto written = table_.pages_from(ids[i], b.before[i]);
             b.new_pages.insert(b.new_pages.end(), written.begin(), written.end());
+            b.changes.push_back(table_.changes(ids[i]));
             lengths.push_back(static_cast<std::int32_t>(table_.length(ids[i])));
             starts.push_back(static_cast<std::int32_t>(starts.back() + tokens[i]));
         }
