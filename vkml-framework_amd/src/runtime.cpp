@@ -104,8 +104,12 @@ void* Runtime::acquire(std::uint64_t bytes, std::uint64_t& rounded) {
 
 void Runtime::release(void* ptr, std::uint64_t rounded) noexcept {
     if (!ptr) return;
-    free_.emplace(rounded, ptr);
-    pooled_bytes_ += rounded;
+    try {
+        free_.emplace(rounded, ptr);
+        pooled_bytes_ += rounded;
+    } catch (...) {  // no host memory to note it
+        (void)vkml_free(ptr);
+    }
 }
 
 void Runtime::synchronize() { check(vkml_synchronize(), "synchronize"); }
