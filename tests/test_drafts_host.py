@@ -33,3 +33,9 @@ def test_trees_of_another_batch_are_refused(check):
 def test_a_batch_whose_keys_have_gone_is_not_kept(check):
     """Of a sequence that was cut and then grew to the batch's length again."""
     check("stale")
+
+
+def test_a_keep_that_fails_leaves_no_keys_that_are_not_the_sequences_own(check):
+    """Whichever of its allocations fails, every sequence is as the batch left it and can
+    be kept still; where a call of the device fails, so, or it ends at its earlier keys."""
+    check("failures")

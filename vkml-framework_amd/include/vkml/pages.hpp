@@ -115,8 +115,8 @@ struct KeptDrafts {
 // The keys and values of several sequences, in up to 2^24 pages of `page_size`
 // (a power of two, 16 to 1024) and 2^30 bytes, f32 or f16, for every layer of a
 // model (up to 65535), of up to 4096 KV heads of up to 1024 dims. What
-// throws changes nothing: a batch that is refused, or for which there is no
-// memory, leaves every sequence with the keys that it had.
+// throws changes nothing (but see keep): a batch that is refused, or for which there
+// is no memory, leaves every sequence with the keys that it had.
 class PagedCache {
 public:
     PagedCache(Context& context, std::int64_t layers, std::int64_t kv_heads, std::int64_t head_dim, std::int64_t pages, std::int64_t page_size,
@@ -174,8 +174,10 @@ public:
     // drafted and picked, i32 [tokens]: each token, and the model's pick after it.
     // Along each tree's path of tokens that are the pick after the one before, the keys
     // and values of every layer move to follow the sequence's earlier keys, and the
-    // sequence ends there. Waits for the step. The sequences must be as the batch left
-    // them: not grown or cut, moved by compact, or forked (but for forks that are gone).
+    // sequence ends there. Waits for the step. Where the device fails in it, the batch's
+    // sequences end at their earlier keys (what else throws changes nothing). The
+    // sequences must be as the batch left them: not grown or cut, moved by compact, or
+    // forked (but for forks that are gone).
     KeptDrafts keep(const PagedBatch& batch, const PagedTrees& trees, const Tensor& drafted, const Tensor& picked);
 
     const Tensor& k_pages() const noexcept { return k_; }  // [layers, pages, kv_heads, page_size, head_dim]

@@ -96,6 +96,14 @@ KeptDrafts PagedCache::keep(const PagedBatch& batch, const PagedTrees& trees, co
     KeptDrafts kept;
     kept.paths.resize(batch.ids.size());
     if (batch.seqs == 0) return kept;
+    // All memory that the call takes comes before any row moves, that of the cuts among it
+    // (a cut that changes nothing makes its room).
+    std::vector<std::int32_t> nodes(static_cast<std::size_t>(batch.tokens)), many(batch.ids.size());
+    kept.next.resize(batch.ids.size());
+    for (std::size_t i = 0; i < batch.ids.size(); ++i) {
+        kept.paths[i].reserve(static_cast<std::size_t>(batch.added[i]));
+        table_.truncate(batch.ids[i], table_.length(batch.ids[i]));
+    }
     detail::Runtime& runtime = TensorAccess::runtime(k_);
     const Tensor path = array(runtime, want), counts = array(runtime, {batch.seqs}), next = array(runtime, {batch.seqs});
     vkml_keep_drafts_params p{};
@@ -108,13 +116,21 @@ KeptDrafts PagedCache::keep(const PagedBatch& batch, const PagedTrees& trees, co
     p.seqs = u32(batch.seqs);
     p.tokens = u32(batch.tokens);
     p.table_stride = u32(batch.table.shape().back());
-    check(vkml_keep_drafts(&p, ints(trees.parents), ints(drafted), ints(picked), ints(batch.table), ints(batch.lengths), ints(batch.starts),
-                           static_cast<std::int32_t*>(path.data()), static_cast<std::int32_t*>(counts.data()), static_cast<std::int32_t*>(next.data()), k_.data(),
-                           v_.data()),
-          "PagedCache::keep");
-    const std::vector<std::int32_t> nodes = batch.tokens > 0 ? path.to_vector<std::int32_t>() : std::vector<std::int32_t>{};
-    const std::vector<std::int32_t> many = counts.to_vector<std::int32_t>();
-    kept.next = next.to_vector<std::int32_t>();
+    const auto download = [](std::vector<std::int32_t>& to, const Tensor& from) {
+        if (!to.empty()) check(vkml_memcpy_d2h(to.data(), from.data(), to.size() * sizeof(std::int32_t)), "PagedCache::keep");
+    };
+    try {
+        check(vkml_keep_drafts(&p, ints(trees.parents), ints(drafted), ints(picked), ints(batch.table), ints(batch.lengths), ints(batch.starts),
+                               static_cast<std::int32_t*>(path.data()), static_cast<std::int32_t*>(counts.data()), static_cast<std::int32_t*>(next.data()), k_.data(),
+                               v_.data()),
+              "PagedCache::keep");
+        download(nodes, path);
+        download(many, counts);
+        download(kept.next, next);
+    } catch (...) {  // rows may have moved, and how is not known
+        for (std::size_t i = 0; i < batch.ids.size(); ++i) table_.truncate(batch.ids[i], batch.before[i]);
+        throw;
+    }
     auto first = nodes.begin();
     for (std::size_t i = 0; i < batch.ids.size(); ++i) {
         kept.paths[i].assign(first, first + many[i]);
