@@ -803,9 +803,11 @@ int vkml_keep_drafts(const vkml_keep_drafts_params* p, const int32_t* d_parents,
  * (in [0, 1); values outside count as its ends) times the kept weight. d_options
  * [rows], 16-byte aligned, device memory that the launch reads. Logits that are NaN
  * or -infinity are never picked, beside +infinity nothing else is; a row without a
- * candidate gives -1. Weights are rounded to 2^-min(51, 62 - ceil(log2(vocab))) of
- * the largest and summed exactly, so that the same row gives the same token in every
- * call. A row starts every row_stride floats; vocab at most 2^22. d_workspace:
+ * candidate gives -1. Weights are found to 2^-50 of the largest, rounded to
+ * 2^-min(51, 62 - ceil(log2(vocab))) of it (what is less than half of that is never
+ * picked) and summed exactly, so that the same row gives the same token in every
+ * call. A row starts every row_stride floats; vocab at most 2^22, rows times
+ * ceil(vocab / 32768) at most 2^21. d_workspace:
  * vkml_sample_workspace_bytes(p) bytes of any content, 16-byte aligned (0, and NULL
  * taken, up to 32768 logits; 40 rows of 128256: 6.2 MB); calls that overlap need
  * one each. */

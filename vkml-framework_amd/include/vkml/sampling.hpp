@@ -65,9 +65,12 @@ private:
 
 // A token for each row of logits, f32 [.., vocab], picked on the device as a Sampler
 // of that row's options would with its draw at random[row] (in [0, 1)) of the kept
-// weight; i32 [..]. options: one for every row, or one for all. Their penalties
-// must be off (they change the logits before), their seeds are not used. A row
-// without a token to pick (all NaN or -infinity) gives -1.
+// weight; i32 [..]. (A Sampler's weights are doubles; here each is rounded to
+// 2^-min(51, 62 - ceil(log2(vocab))) of the row's largest, 2^-45 for 2^17 logits: a draw
+// nearer to a border than the sum of these roundings may fall on its other side, and
+// tokens of less weight than half of that are never picked.) options: one for every row,
+// or one for all. Their penalties must be off (they change the logits before), their
+// seeds are not used. A row without a token to pick (all NaN or -infinity) gives -1.
 Tensor sample(const Tensor& logits, std::span<const SamplingOptions> options, std::span<const double> random);
 
 // A token's log probability under logits (their log-softmax, computed in
