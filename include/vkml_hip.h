@@ -754,8 +754,9 @@ int vkml_attend_pages_tree(const vkml_attend_pages_params* p, uint32_t seen_word
 
 /* vkml_attend_pages with a window: a token at position p sees the keys past p -
  * window up to its own, and its sequence's first `sinks` (0: none). Pages of which
- * no token sees a key are not read: their table entries may be -1. window at
- * least 1; no groups (p->groups 0). */
+ * no token sees a key need not be there: their table entries may be -1, so that a
+ * caller may give them back. Keys, the sinks' too, are taken as they were stored,
+ * rotated at their own positions. window at least 1; no groups (p->groups 0). */
 int vkml_attend_pages_window(const vkml_attend_pages_params* p, uint32_t window, uint32_t sinks, const float* d_q,
                              const void* d_k_pages, const void* d_v_pages, const int32_t* d_table,
                              const int32_t* d_lengths, const int32_t* d_starts, void* d_workspace, float* d_out);

@@ -26,9 +26,13 @@
 // picks, since one workgroup for a row of 128256 would leave most of the GPU idle (40 rows)
 // and could not hold it.
 //
-// Measured (us): 1 row of 32768 9.8 (greedy, or top_k: 5 of it the launch and the load);
-// 40 24; 416 of requests that differ 32 (54 MB: 1.7 TB/s), 1024 74; 300 of 4096 15; 40
-// of 128256 46 to 53: 5 peaks, 14 weights, 14 lists, 14 picks. Not bound by bytes (10.6 us for
+// Measured (us): 1 row of 32768 with top_k 40 9.8 (5 of it the launch and the load),
+// greedy 4.9, min_p 0.05 7.9, top_p 0.95 20.5, no cut 18.8; 40 24; 416 of requests that
+// differ 32 (54 MB: 1.7 TB/s), all with top_k 40 26, with top_p 0.95 56, without a cut 53;
+// 1024 74; 300 of 4096 15; 40 of 128256 46 to 53: 5 peaks, 14 weights, 14 lists, 14 picks.
+// Flat rows take longer, since a bin, 1/32 of a factor of two in weight, has more than the
+// list holds and the row is read again for it: normal logits at temperature 30, top_p
+// 0.95, 72 for 1 of 32768, 162 for 416, 241 for 40 of 128256. Not bound by bytes (10.6 us for
 // the 416, 4.0 for the 40 at a large copy's rate): a row whose candidates are all weighed
 // (top_p alone, or nothing) takes 18 by itself, 2 to load, 7 for 32 weights a thread, two
 // f64 products and polynomials and two LDS atomics each, 2 for the bins' sums, 2 to list, 4
@@ -795,8 +799,10 @@ struct Picker {
 // ---------------------------------------------------------------- the launches
 
 // Rows of one slice: a workgroup a row, its values in registers. (Of up to 8192 logits:
-// 256 threads, two workgroups a compute unit: 300 rows of 4096 15 us, 32 with 1024
-// threads.)
+// 256 threads, two workgroups a compute unit. Measured, us with 256 and 1024 threads, all
+// rows with top_p 0.95: 1 of 1000 12.0 and 13.3, of 4096 13.6 and 14.0, of 8192 15.7 and
+// 15.0; 256 of 8192 16.9 and 16.6; 300 of 4096 16.5 and 29.6; 1024 of 4096 31 and 58, of
+// 8192 37 and 64. With top_k 40 256 are ahead at all of these.)
 template <uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads) k_sample(Args a) {
     using P = Picker<kThreads>;

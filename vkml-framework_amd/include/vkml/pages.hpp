@@ -156,7 +156,10 @@ public:
     // head_dim 64 or 128.
     Tensor attention(std::int64_t layer, const PagedBatch& batch, const Tensor& q, float softcap = 0.0f) const;
     // The same over a window: a token sees the last `window` keys up to its own, and
-    // its sequence's first `sinks`. A batch without groups.
+    // its sequence's first `sinks`, each rotated at its own position. A batch without
+    // groups. The keys behind the window stay in their pages: a sequence gives pages back
+    // from its end alone (truncate, release). (vkml_attend_pages_window, over a caller's
+    // own tables, does without them.)
     Tensor attention_window(std::int64_t layer, const PagedBatch& batch, const Tensor& q, std::int64_t window, std::int64_t sinks = 0, float softcap = 0.0f) const;
 
     // A step of speculative decoding: trees of a batch's new tokens; for each layer
